@@ -356,6 +356,104 @@ int vte_decode_batch_setup(const vte_decode_model* m, const vte_decode_layer* la
 int vte_decode_batch_step(const vte_decode_model* m, void* workspace, int batch, long long kv_batch_stride,
                           const int* kv_offset, const void* x, void* h_out, void* stream);
 
+/* ---- 8-bit paged KV cache ----
+ * K and V as bytes; 16 consecutive tokens of one KV head (a block) share one
+ * scale 2^e, K and V apart: value = (byte - 128) * 2^e, e in -126..127; a block
+ * that received an Inf or a NaN has e = -128 and reads as NaN until its first
+ * place is written again.  A page holds page_tokens tokens (a power of two,
+ * 16..4096) of every KV head:
+ *   k            [n_pages][n_kv][page_tokens][head_dim]
+ *   v            [n_pages][n_kv][page_tokens / 16][head_dim][16]
+ *   k_exp, v_exp [n_pages][n_kv][page_tokens / 16]
+ * The memory needs no clearing.  head_dim 64 or 128; k and v 16-byte aligned.
+ * The struct is read by the host call only.  No counterpart in the reference
+ * (its cache is one fp16 range per sequence, kv_cache_append.hip.template:13-39). */
+typedef struct vte_kv_pages {
+    void *k, *v;         /* bytes */
+    void *k_exp, *v_exp; /* int8 */
+    int n_pages, page_tokens, n_kv, head_dim;
+} vte_kv_pages;
+
+/* The sequences of a call and their new rows.  Sequence b's rows of q, k and v
+ * are row_start[b] .. row_start[b + 1] - 1 (device int [batch + 1], not
+ * decreasing), the first of them at position kv_offset[b] (device int [batch];
+ * below 0: the sequence does not run), so the positions before it are in the
+ * cache.  row_start NULL: row b is sequence b's (rows = batch, max_rows = 1), or
+ * there are no new rows (rows = max_rows = 0).  rows: rows of q, k and v; those
+ * behind row_start[batch] belong to nobody.  max_rows: at least the most rows
+ * of one sequence; a sequence's rows past it are taken as not there.
+ * page_table: device int [batch][max_pages]; entry j holds the page of positions
+ * j * page_tokens ..; an entry outside [0, n_pages) is no page: rows for it are
+ * dropped, its tokens are not seen.  Positions past max_pages * page_tokens are
+ * dropped likewise.  A page that a call writes must belong to one sequence. */
+typedef struct vte_kv_rows {
+    int batch, rows, max_rows, max_pages;
+    const int *row_start, *kv_offset, *page_table;
+} vte_kv_rows;
+
+/* Write the new rows' k and v (dtype fp16 or fp32, [rows][n_kv][head_dim], rows
+ * k_stride / v_stride elements apart, 0: contiguous) into their pages, k rotated
+ * by its position on the way, and, with q, q_out [rows][n_q][head_dim] (dtype,
+ * contiguous; may be q) = q rotated (rows q_stride apart).  Rotation: rope_type
+ * and tables as vte_rope ([rope_rows][head_dim], type 2 [rope_rows][rotary_dim]);
+ * rows at positions from rope_rows on are dropped, their q_out left as it was.
+ * rope_cos and rope_sin NULL: no rotation, q must be NULL.  Each k and v value is
+ * rounded once, to its byte; a block's scale fits its largest value and never
+ * falls while tokens before the new rows live in it (when it grows by 2^d their
+ * bytes are shifted, rounded to nearest even).
+ * Replaces: rope_kernel (rope.hip.template:17-137) followed by
+ *           kv_cache_append_kernel (kv_cache_append.hip.template:13-39). */
+int vte_kv_pages_append(const vte_kv_pages* cache, const vte_kv_rows* rows, int dtype, const void* k, const void* v,
+                        long long k_stride, long long v_stride, const void* q, void* q_out, int n_q,
+                        long long q_stride, const void* rope_cos, const void* rope_sin, int rope_rows, int rope_type,
+                        int rotary_dim, void* stream);
+
+/* k_out and v_out [batch][out_rows][n_kv][head_dim] (dtype): the values at
+ * positions 0 .. kv_offset[b] + (b's new rows) - 1 of every sequence, each
+ * rounded once; rows past them (and past out_rows) are left as they were.  Tokens
+ * without a page give 0.  The layout is the fp16 cache's
+ * (vte/compiler/qwen_mapper.py:300-351). */
+int vte_kv_pages_read(const vte_kv_pages* cache, const vte_kv_rows* rows, int dtype, void* k_out, void* v_out,
+                      int out_rows, void* stream);
+
+/* Scratch bytes of vte_attn_pages (-1: rejected arguments). */
+long long vte_attn_pages_scratch_bytes(const vte_kv_pages* cache, const vte_kv_rows* rows, int n_q);
+
+/* Attention of the new rows over the paged cache (which holds them already):
+ * row i of sequence b sees positions 0 .. kv_offset[b] + i.  q and out
+ * [rows][n_q][head_dim] (dtype fp16 or fp32), n_q / n_kv <= 16.  A row that sees
+ * nothing (a sequence that does not run, no pages) gives 0; rows that belong to
+ * nobody are left as they were.  Sums and softmax statistics are fp32; with fp16
+ * the probabilities enter the products as fp16, with fp32 q and the probabilities
+ * enter as two fp16 parts each.  scratch: 16-byte aligned, need not be cleared;
+ * calls that may overlap (two streams, two graphs) need one each.  Capturable.
+ * Replaces: SplitKVAttentionDispatcher launches (vte/core/split_kv_attention.py:187-217)
+ *           for a cache in this form. */
+int vte_attn_pages(const vte_kv_pages* cache, const vte_kv_rows* rows, int dtype, const void* q, void* out, int n_q,
+                   float scale, void* scratch, long long scratch_bytes, void* stream);
+
+/* Scratch bytes of vte_sample for `rows` rows. */
+long long vte_sample_scratch_bytes(int rows);
+
+/* The next token of every row of fp32 logits [rows][vocab] (vocab <= 262144).
+ * Per row (device arrays of `rows`, NULL: off for every row): temperature (<= 0
+ * or NaN: greedy; NULL: 1), top_k (<= 0: off), top_p (off unless 0 < top_p < 1),
+ * min_p (<= 0: off, above 1 as 1) and u, the uniform in [0, 1).  Weights are
+ * exp((x - max) / temperature), the order is (value descending, index
+ * ascending): top-k keeps the first k, top-p those with a mass of at most top_p *
+ * (mass of the top-k) before them, min-p those of weight >= min_p; the token is
+ * the first kept one whose mass up to and with it exceeds u * (kept mass).
+ * Greedy: the largest logit, the lowest index among equal ones.  A NaN logit has
+ * no weight; a row of nothing but -Inf and NaN gives -1; +Inf entries share the
+ * draw.  Sums are exact (64-bit whole numbers; an entry below 2^-45 of the
+ * largest has no weight), so a token depends on its row and settings alone.
+ * scratch: 16-byte aligned, need not be cleared; calls that may overlap need one
+ * each.  Capturable.
+ * Replaces: Sampler.sample (vte/core/sampler.py:54-129) after the repetition
+ *           penalty, with the draw's random number given. */
+int vte_sample(const float* logits, int rows, int vocab, const float* temperature, const int* top_k,
+               const float* top_p, const float* min_p, const double* u, int* tokens, void* scratch, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

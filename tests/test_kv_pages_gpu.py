@@ -1,0 +1,383 @@
+"""The 8-bit paged KV cache on the GPU against the 64-bit oracle: bytes and exponents exactly, attention within
+bounds counted from the formats."""
+import math
+
+import numpy as np
+import pytest
+
+from oracle import kv_pages as okv
+from tests._dev import down, empty, up
+from vte_amd.core.rope_cache import build_rope_cache
+from vte_amd.kernels import KVPages, KVRows
+
+pytestmark = pytest.mark.gpu
+
+NP = {"f16": np.float16, "f32": np.float32}
+
+
+class Batch:
+    """Sequences with pages in random order, the oracle's cache beside the device's."""
+
+    def __init__(self, hip, K, rng, lens, n_kv, hd, page, spare=2, width=None, holes=()):
+        self.hip, self.K, self.rng, self.n_kv, self.hd, self.page = hip, K, rng, n_kv, hd, page
+        per = [max(1, -(-n // page)) for n in lens]
+        self.width = width or max(per)
+        self.n_pages = sum(per) + spare
+        order, at = rng.permutation(self.n_pages), 0
+        self.table = np.full((len(lens), self.width), -1, np.int32)
+        for b, p in enumerate(per):
+            m = min(p, self.width)
+            self.table[b, :m] = order[at:at + m]
+            at += p
+        for b, j, entry in holes:
+            self.table[b, j] = entry
+        self.ref = okv.Cache(len(lens), n_kv, hd, self.width, page)
+        self.d = {}
+        self.upload()
+
+    def upload(self):
+        for is_v, n in ((False, "k"), (True, "v")):
+            codes, exps = self.ref.pool(self.table, self.n_pages, is_v)
+            self.d[n], self.d[n + "e"] = up(self.hip, codes), up(self.hip, exps)
+        self.d["table"] = up(self.hip, self.table)
+        self.pages = KVPages.of(self.d["k"], self.d["v"], self.d["ke"], self.d["ve"], self.n_pages, self.page,
+                                self.n_kv, self.hd)
+
+    def rows(self, pos, new=None, pad=0, max_rows=None):
+        """New rows of each sequence from positions pos (new None: one each without row_start)."""
+        self.d["off"] = up(self.hip, np.asarray(pos, np.int32))
+        B = len(pos)
+        if new is None:
+            return KVRows.of(B, B, 1, None, self.d["off"], self.d["table"], self.width)
+        start = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+        self.d["start"] = up(self.hip, start)
+        return KVRows.of(B, int(start[-1]) + pad, max(new) if max_rows is None else max_rows, self.d["start"],
+                         self.d["off"], self.d["table"], self.width)
+
+    def drop(self, b, pos):
+        """Whether a row at pos has no place."""
+        return pos >= self.ref.cap or not 0 <= self.table[b, pos // self.page] < self.n_pages
+
+    def check(self, rows):
+        """The device's pages are the oracle's, byte for byte, where a sequence has live tokens."""
+        for is_v, n in ((False, "k"), (True, "v")):
+            codes, exps = down(self.d[n]), down(self.d[n + "e"])
+            for b, parts in enumerate(self.ref.v if is_v else self.ref.k):
+                c, e = okv.unpool(codes, exps, self.table[b], self.page, is_v)
+                live = np.array([not self.drop(b, t) for t in range(rows[b])], bool)
+                assert np.array_equal(c[:rows[b]][live], parts.c[:rows[b]][live]), (n, b)
+                el = live[::okv.BLOCK]
+                assert np.array_equal(e[:len(el)][el], parts.e[:len(el)][el]), (n, b)
+
+
+def append_ref(batch, b, pos, k, v):
+    """The oracle's append of rows whose places exist (a hole swallows whole blocks)."""
+    n = min(len(k), batch.ref.cap - pos)
+    t = 0
+    while t < n:
+        m = min(n - t, okv.BLOCK - (pos + t) % okv.BLOCK)
+        if not batch.drop(b, pos + t):
+            batch.ref.k[b].append(k[t:t + m], pos + t)
+            batch.ref.v[b].append(v[t:t + m], pos + t)
+        t += m
+
+
+def normal(rng, shape, dtype, scale=1.0):
+    return (scale * rng.standard_normal(shape)).astype(NP[dtype])
+
+
+@pytest.mark.parametrize("hd,dtype,rope", [(128, "f16", 0), (128, "f16", 1), (128, "f32", 0), (64, "f16", 0),
+                                           (64, "f32", 2), (128, "f16", 2), (128, "f16", None), (64, "f16", 1)])
+def test_append_token_by_token(hip, K, hd, dtype, rope):
+    """Three sequences from different places, magnitudes that climb by 2^12: the blocks' scales grow under tokens
+    that are already in, and shrink again with a new block."""
+    rng = np.random.default_rng(hd + 10 * (rope or 7))
+    n_kv, n_q, start = 2, 6, [0, 15, 37]
+    bt = Batch(hip, K, rng, [50, 66, 88], n_kv, hd, 32)
+    for b, n in enumerate(start):
+        for p in (bt.ref.k[b], bt.ref.v[b]):
+            p.append(normal(rng, (n, n_kv, hd), "f16"), 0)
+    bt.upload()
+    rd = {None: 0, 2: hd // 2 + 4}.get(rope, hd)
+    cos, sin = build_rope_cache(128, rd or hd, 1e4)
+    dc, ds = up(hip, cos), up(hip, sin)
+    for step in range(50):
+        pos = [s + step for s in start]
+        size = 2.0 ** rng.uniform(-6, 6)
+        q, k, v = (normal(rng, (3, h, hd), dtype, size) for h in (n_q, n_kv, n_kv))
+        dq, dk, dv, do = up(hip, q), up(hip, k), up(hip, v), empty(hip, q.shape, NP[dtype])
+        r = bt.rows(pos)
+        if rope is None:
+            K.kv_pages_append(bt.pages, r, dk, dv, dtype=dtype, stream=hip.stream)
+            kr = k.astype(np.float32)
+        else:
+            K.kv_pages_append(bt.pages, r, dk, dv, q=dq, q_out=do, n_q=n_q, rope_cos=dc, rope_sin=ds, rope_rows=128,
+                              rope_type=rope, rotary_dim=rd, dtype=dtype, stream=hip.stream)
+            kr = okv.rotate(k, pos, cos, sin, rope, rd)
+            assert np.array_equal(down(do), okv.rotate(q, pos, cos, sin, rope, rd).astype(NP[dtype]))
+        for b in range(3):
+            append_ref(bt, b, pos[b], kr[b:b + 1], v[b:b + 1])
+        if step % 7 == 0 or step == 49:
+            bt.check([p + 1 for p in pos])
+
+
+@pytest.mark.parametrize("page,hd,dtype", [(16, 128, "f16"), (64, 128, "f16"), (32, 64, "f32"), (256, 64, "f16")])
+def test_append_ragged_prompts(hip, K, page, hd, dtype):
+    """Chunks of 0 to 200 rows in one call, from places inside blocks, with a sequence that does not run, a table entry
+    that is no page, rows past the table, rows of nobody, strided k, v and q; other memory stays as it was."""
+    rng = np.random.default_rng(page + hd)
+    n_kv, n_q = 3, 6
+    pos, new = [0, 5, 31, -1, 16, 40, 3], [200, 0, 90, 4, 17, 60, 1]
+    lens = [p + n if p >= 0 else 0 for p, n in zip(pos, new)]
+    width = max(1, 208 // page)
+    holes = [(2, 64 // page, -1), (4, 0, 10 ** 6)] if page <= 64 else [(4, 0, -7)]
+    bt = Batch(hip, K, rng, lens, n_kv, hd, page, width=width, holes=holes)
+    for b, p in enumerate(pos):
+        if p > 0:
+            old = [normal(rng, (p, n_kv, hd), "f16", 0.3) for _ in "kv"]
+            append_ref(bt, b, 0, *old)
+    bt.upload()
+    before = {n: down(bt.d[n]).copy() for n in ("k", "v", "ke", "ve")}
+    R, pad = sum(new), 5
+    wide = normal(rng, (R + pad, n_q + 2 * n_kv, hd), dtype)  # q, k and v of one fused projection
+    dw = up(hip, wide)
+    size, ld = wide.itemsize, wide.shape[1] * hd
+    out = np.full((R + pad, n_q, hd), 9, NP[dtype])
+    do = up(hip, out)
+    limit = 205 if page <= 64 else 230  # the rotation's table ends inside sequence 0's last page or past the capacity
+    cos, sin = build_rope_cache(limit, hd, 1e4)
+    r = bt.rows(pos, new, pad)
+    K.kv_pages_append(bt.pages, r, dw.ptr + n_q * hd * size, dw.ptr + (n_q + n_kv) * hd * size, q=dw, q_out=do,
+                      n_q=n_q, rope_cos=up(hip, cos), rope_sin=up(hip, sin), rope_rows=limit, dtype=dtype,
+                      k_stride=ld, v_stride=ld, q_stride=ld, stream=hip.stream)
+    got, first = down(do), np.cumsum([0] + new)
+    written = set()
+    for b in range(len(pos)):
+        if pos[b] < 0:
+            continue
+        n = max(0, min(new[b], min(limit, bt.ref.cap) - pos[b]))
+        w = wide[first[b]:first[b] + n]
+        at = pos[b] + np.arange(n)
+        append_ref(bt, b, pos[b], okv.rotate(w[:, n_q:n_q + n_kv], at, cos, sin), w[:, n_q + n_kv:].astype(np.float32))
+        out[first[b]:first[b] + n] = okv.rotate(w[:, :n_q], at, cos, sin).astype(NP[dtype])
+        written |= {(int(bt.table[b, t // page]), t % page // 16) for t in at if not bt.drop(b, t)}
+    assert np.array_equal(got, out)
+    bt.check([min(max(n, 0), bt.ref.cap, max(p, limit)) for n, p in zip(lens, pos)])
+    for n, old in before.items():  # blocks that no new row fell into
+        now = down(bt.d[n])
+        for p in range(bt.n_pages):
+            for i in range(page // 16):
+                if (p, i) not in written:
+                    sl = (p, slice(None), slice(16 * i, 16 * i + 16)) if n == "k" else (p, slice(None), i)
+                    assert np.array_equal(now[sl], old[sl]), (n, p, i)
+
+
+def test_append_not_finite(hip, K):
+    """A block that receives an Inf or a NaN reads as NaN, and later ones of other heads and blocks do not."""
+    rng = np.random.default_rng(5)
+    bt = Batch(hip, K, rng, [40], 2, 64, 32)
+    k, v = (normal(rng, (40, 2, 64), "f16") for _ in "kv")
+    k[3, 0, 5], v[20, 1, 63], v[21, 0, 0] = np.inf, np.nan, -np.inf
+    for lo, hi in ((0, 25), (25, 40)):
+        K.kv_pages_append(bt.pages, bt.rows([lo], [hi - lo]), up(hip, k[lo:hi]), up(hip, v[lo:hi]), stream=hip.stream)
+        append_ref(bt, 0, lo, k[lo:hi], v[lo:hi])
+    bt.check([40])
+    ko, vo = empty(hip, (1, 40, 2, 64), np.float32), empty(hip, (1, 40, 2, 64), np.float32)
+    K.kv_pages_read(bt.pages, bt.rows([40], [0]), ko, vo, 40, dtype="f32", stream=hip.stream)
+    for got, part, bad in ((ko, bt.ref.k[0], [(0, 0)]), (vo, bt.ref.v[0], [(1, 1), (1, 0)])):
+        g = down(got)[0]
+        assert np.array_equal(g, part.values(40).astype(np.float32), equal_nan=True)
+        assert {(int(t) // 16, int(h)) for t, h, _ in zip(*np.nonzero(np.isnan(g)))} == set(bad)
+
+
+@pytest.mark.parametrize("dtype,size", [("f16", 6e4), ("f16", 1e-7), ("f32", 1e38), ("f32", 1e-44), ("f32", 0.0)])
+def test_append_and_read_extreme_magnitudes(hip, K, dtype, size):
+    rng = np.random.default_rng(6)
+    bt = Batch(hip, K, rng, [33], 1, 128, 16)
+    k, v = ((size * rng.uniform(-1, 1, (33, 1, 128))).astype(NP[dtype]) for _ in "kv")
+    K.kv_pages_append(bt.pages, bt.rows([0], [33]), up(hip, k), up(hip, v), dtype=dtype, stream=hip.stream)
+    append_ref(bt, 0, 0, k, v)
+    bt.check([33])
+    ko, vo = empty(hip, (1, 33, 1, 128), NP[dtype]), empty(hip, (1, 33, 1, 128), NP[dtype])
+    K.kv_pages_read(bt.pages, bt.rows([33], [0]), ko, vo, 33, dtype=dtype, stream=hip.stream)
+    assert np.array_equal(down(ko)[0], bt.ref.k[0].values(33).astype(NP[dtype]))
+    assert np.array_equal(down(vo)[0], bt.ref.v[0].values(33).astype(NP[dtype]))
+
+
+@pytest.mark.parametrize("hd,dtype,page,out_rows", [(128, "f16", 16, 100), (64, "f32", 64, 37), (128, "f32", 128, 300),
+                                                    (64, "f16", 32, 1)])
+def test_read(hip, K, hd, dtype, page, out_rows):
+    """Every sequence's rows, 0 where it has no page, the rest of the output as it was."""
+    rng = np.random.default_rng(hd + page)
+    lens, pos = [100, 1, 0, 64, 33], [100, 1, 0, 64, 30]
+    bt = Batch(hip, K, rng, lens, 2, hd, page, holes=[(3, 1, -1)] if page <= 32 else [])
+    for b, n in enumerate(lens):
+        append_ref(bt, b, 0, *(normal(rng, (n, 2, hd), "f16") for _ in "kv"))
+    bt.upload()
+    new = [0, 0, 0, 0, 3]
+    want = [np.full((5, out_rows, 2, hd), 7, NP[dtype]) for _ in "kv"]
+    ko, vo = up(hip, want[0]), up(hip, want[1])
+    pos[2] = -1
+    K.kv_pages_read(bt.pages, bt.rows(pos, new), ko, vo, out_rows, dtype=dtype, stream=hip.stream)
+    for w, parts in zip(want, (bt.ref.k, bt.ref.v)):
+        for b in range(5):
+            n = min(lens[b], out_rows) if pos[b] >= 0 else 0
+            x = parts[b].values(n)
+            for t in range(n):
+                w[b, t] = 0 if bt.drop(b, t) else x[t]
+    assert np.array_equal(down(ko), want[0]) and np.array_equal(down(vo), want[1])
+
+
+# ---------------------------------------------------------------------------- attention
+def attn_tolerance(dtype, hd, out, mag, big, vmax):
+    """|error| of one result.  fp16: the probabilities are rounded (2^-11 of each, so of the weighted |V|) and the
+    result is (2^-11); fp32: two fp16 parts of q and of the probabilities (2^-21 each: a rounded part and a rounded
+    rest of at most 2^-11 of it), the result 2^-24.  Both: scores are fp32 sums of hd + 3 roundings at most (2^-24 of
+    the sum of |q k| each), which e^x carries into both sums (twice); exponentials, sums and the rescaling by running
+    maxima add 2^-19 at most (2^-24 a rounding, below 32 of them in a chain); what is below the smallest fp16 after
+    scaling by 2^14 is 2^-38 of the largest weight for each of at most 2^16 tokens.  fp16 results below 2^-14 are
+    rounded to steps of 2^-24 (2^-25 at most)."""
+    p, r = (2.0 ** -11, 2.0 ** -11) if dtype == "f16" else (2.0 ** -20, 2.0 ** -24)
+    q = 0.0 if dtype == "f16" else 2.0 ** -21
+    score = big[:, None] * (q + (hd + 3) * 2.0 ** -24)
+    return (p + 2 * score + 2.0 ** -19) * mag + r * np.abs(out) + 2.0 ** -22 * vmax + (2.0 ** -25 if dtype == "f16" else 0)
+
+
+def matches(dtype, got, out, tol):
+    """Within the tolerance; an fp16 result from 65520 on (half a step past the largest, 65504) is Inf."""
+    with np.errstate(invalid="ignore"):
+        ok = np.isnan(out) | (np.abs(got - out) <= tol)
+        return ok | (np.isinf(got) & (np.abs(out) + tol >= 65520) & (got * out > 0)) if dtype == "f16" else ok
+
+
+def check_attention(hip, K, bt, pos, new, n_q, dtype, rng, pad=0, q_scale=1.0, row_start=True):
+    B, hd = len(pos), bt.hd
+    R = sum(new)
+    q = normal(rng, (R + pad, n_q, hd), dtype, q_scale)
+    out = np.full(q.shape, 5, NP[dtype])
+    do = up(hip, out)
+    r = bt.rows(pos, new if row_start else None, pad)
+    n = K.attn_pages_scratch_bytes(bt.pages, r, n_q)
+    scratch = up(hip, np.full(n, 0xFF, np.uint8))  # scratch holds NaNs: nothing reads what it did not write
+    scale = 1 / math.sqrt(hd)
+    K.attn_pages(bt.pages, r, up(hip, q), do, n_q, scale, scratch, n, dtype=dtype, stream=hip.stream)
+    got = down(do).astype(np.float64)
+    first = np.cumsum([0] + list(new))
+    for b in range(B):
+        kv = bt.ref.k[b].values(bt.ref.cap), bt.ref.v[b].values(bt.ref.cap)
+        present = np.array([not bt.drop(b, t) for t in range(bt.ref.cap)])
+        vmax = np.abs(kv[1][np.isfinite(kv[1])]).max(initial=0)
+        for i in range(new[b]):
+            o, mag, big = okv.attention(q[first[b] + i], *kv, pos[b] + i if pos[b] >= 0 else -1, scale, present)
+            g = got[first[b] + i]
+            assert np.array_equal(np.isnan(g), np.isnan(o)), (b, i)
+            tol = attn_tolerance(dtype, hd, o, mag, big, vmax)
+            ok = matches(dtype, g, o, tol)
+            if not ok.all():
+                pytest.fail(f"sequence {b} row {i}: {float(np.abs(g - o)[~ok].max())} off, {int((~ok).sum())} values")
+    assert (got[R:] == 5).all()
+    return got
+
+
+def filled(hip, K, rng, lens, n_kv, hd, page, v_sizes=None, **kw):
+    bt = Batch(hip, K, rng, lens, n_kv, hd, page, **kw)
+    for b, n in enumerate(lens):
+        n = min(n, bt.ref.cap)
+        v = rng.standard_normal((n, n_kv, hd))
+        if v_sizes is not None:
+            v *= 2.0 ** rng.uniform(*v_sizes, (n, n_kv, 1))
+        append_ref(bt, b, 0, rng.standard_normal((n, n_kv, hd)).astype(np.float16), v.astype(np.float32))
+    bt.upload()
+    return bt
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("n_q,n_kv", [(12, 2), (1, 1), (16, 1), (4, 4), (14, 2)])
+def test_attention_decode(hip, K, hd, dtype, n_q, n_kv):
+    """One row per sequence, lengths from one token on, across blocks, tiles and splits; one does not run."""
+    rng = np.random.default_rng(hd + n_q)
+    lens = [1, 2, 15, 16, 17, 63, 64, 65, 200, 257, 700, 0, 1025]
+    bt = filled(hip, K, rng, lens, n_kv, hd, 32)
+    check_attention(hip, K, bt, [n - 1 for n in lens], [1] * len(lens), n_q, dtype, rng, row_start=False)
+
+
+@pytest.mark.parametrize("page", [16, 64, 128, 1024])
+@pytest.mark.parametrize("dtype,n_q,n_kv,hd", [("f16", 6, 2, 128), ("f32", 7, 1, 64)])
+def test_attention_few_rows(hip, K, page, dtype, n_q, n_kv, hd):
+    """Several rows of a sequence at a time (0 to 5), one sequence alone, rows of nobody behind them."""
+    rng = np.random.default_rng(page + hd)
+    lens, new = [3, 70, 300, 5, 0, 1000], [3, 2, 5, 0, 1, 4]
+    bt = filled(hip, K, rng, lens, n_kv, hd, page)
+    check_attention(hip, K, bt, [n - m for n, m in zip(lens, new)], new, n_q, dtype, rng, pad=3)
+    bt = filled(hip, K, rng, [333], n_kv, hd, page)
+    check_attention(hip, K, bt, [332], [1], n_q, dtype, rng)
+
+
+@pytest.mark.parametrize("dtype,n_q,n_kv,hd,page", [("f16", 12, 2, 128, 64), ("f32", 12, 2, 128, 16),
+                                                    ("f16", 7, 1, 64, 256), ("f32", 4, 4, 64, 32),
+                                                    ("f16", 32, 2, 128, 32)])
+def test_attention_prompts(hip, K, dtype, n_q, n_kv, hd, page):
+    """Ragged prompt chunks in one call: from the first token, after cached ones, a single row, a long one."""
+    rng = np.random.default_rng(hd + n_q + page)
+    new = [130, 1, 0, 33, 64, 17]
+    old = [0, 500, 3, 90, 64, 1]
+    bt = filled(hip, K, rng, [a + b for a, b in zip(old, new)], n_kv, hd, page)
+    check_attention(hip, K, bt, old, new, n_q, dtype, rng, pad=2)
+
+
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_attention_holes_and_empty_rows(hip, K, dtype, new):
+    """Pages that are not there, all of a sequence's among them, and rows past the table's end."""
+    rng = np.random.default_rng(new)
+    lens = [300, 90, 64, 200]
+    bt = filled(hip, K, rng, lens, 2, 64, 32, width=6,
+                holes=[(0, 1, -1), (0, 2, 10 ** 6), (1, 0, -1), (1, 1, -5), (1, 2, -1), (2, 0, -1)])
+    check_attention(hip, K, bt, [n - new for n in lens], [new] * 4, 4, dtype, rng)
+
+
+@pytest.mark.parametrize("new", [1, 50])
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_attention_not_finite_blocks(hip, K, dtype, new):
+    """A NaN block makes NaN of the rows that see a token of it, and of no others; dead places hold anything."""
+    rng = np.random.default_rng(7)
+    lens = [200, 200, 200]
+    bt = filled(hip, K, rng, lens, 2, 128, 64)
+    bt.ref.k[0].e[2, 1] = okv.E_NAN
+    bt.ref.v[1].e[11, 0] = okv.E_NAN
+    bt.ref.k[2].e[13:] = okv.E_NAN  # behind the last token of sequence 2
+    bt.ref.v[2].e[13:] = okv.E_NAN
+    bt.upload()
+    got = check_attention(hip, K, bt, [n - new for n in lens], [new] * 3, 4, dtype, rng)
+    assert np.isnan(got).any() and not np.isnan(got[2 * new:]).any()
+
+
+@pytest.mark.parametrize("new", [1, 70])
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("v_sizes,q_scale", [((-20, 20), 1.0), ((0, 0), 30.0), ((-3, 3), 1e-3)])
+def test_attention_scales_and_peaks(hip, K, dtype, new, v_sizes, q_scale):
+    """V blocks of very different scales, sharply peaked scores, and small queries."""
+    rng = np.random.default_rng(8)
+    bt = filled(hip, K, rng, [900, 71], 1, 128, 64, v_sizes=v_sizes)
+    check_attention(hip, K, bt, [900 - new, 71 - new], [new, new], 6, dtype, rng, q_scale=q_scale)
+
+
+@pytest.mark.parametrize("new", [1, 30])
+def test_attention_does_not_depend_on_the_batch(hip, K, new):
+    """Equal bits for a sequence alone, in a batch and in other pages."""
+    rng = np.random.default_rng(9)
+    lens = [700, 40, 333]
+    bt = filled(hip, K, rng, lens, 2, 128, 64)
+    alone = Batch(hip, K, rng, [700], 2, 128, 64, spare=9)
+    alone.ref.k[0], alone.ref.v[0] = bt.ref.k[0], bt.ref.v[0]
+    alone.upload()
+    q = normal(rng, (3 * new, 4, 128), "f16")
+    res = []
+    for b, pos, n in ((bt, [x - new for x in lens], [new] * 3), (alone, [700 - new], [new])):
+        r = b.rows(pos, n)
+        need = K.attn_pages_scratch_bytes(b.pages, r, 4)
+        do = empty(hip, (sum(n), 4, 128), np.float16)
+        K.attn_pages(b.pages, r, up(hip, q[:sum(n)]), do, 4, 0.09, empty(hip, need, np.uint8), need, stream=hip.stream)
+        res.append(down(do)[:new].astype(np.float64))
+    assert np.abs(res[0] - res[1]).max() <= 2.0 ** -9 * np.abs(res[1]).max()

@@ -1,0 +1,117 @@
+"""The device draw against the sorted row in extended precision: the same token, always."""
+import numpy as np
+import pytest
+
+from oracle import sampling as osm
+from tests._dev import down, empty, up
+
+pytestmark = pytest.mark.gpu
+
+
+def draw(hip, K, logits, temperature=None, top_k=None, top_p=None, min_p=None, u=None):
+    R, V = logits.shape
+    f = lambda x, t: None if x is None else up(hip, np.broadcast_to(np.asarray(x, t), (R,)))
+    tok = up(hip, np.full(R, -7, np.int32))
+    need = K.sample_scratch_bytes(R)
+    scratch = up(hip, np.full(need, 0xFF, np.uint8))  # nothing relies on what scratch held
+    K.sample(up(hip, np.asarray(logits, np.float32)), R, V, tok, scratch, temperature=f(temperature, np.float32),
+             top_k=f(top_k, np.int32), top_p=f(top_p, np.float32), min_p=f(min_p, np.float32), u=f(u, np.float64),
+             stream=hip.stream)
+    return down(tok)
+
+
+def check(hip, K, logits, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, u=0.5):
+    """Every row's token; one whose u (or border) lies within 2^-44 * vocab of another token could be either."""
+    R, V = logits.shape
+    got = draw(hip, K, logits, temperature, top_k, top_p, min_p, u)
+    row = lambda x, t: np.broadcast_to(np.asarray(x, t), (R,))
+    s = [row(temperature, np.float32), row(top_k, np.int32), row(top_p, np.float32), row(min_p, np.float32),
+         row(u, np.float64)]
+    sure = 0
+    for r in range(R):
+        want, near = osm.sample(logits[r], float(s[0][r]), int(s[1][r]), float(s[2][r]), float(s[3][r]), float(s[4][r]))
+        assert got[r] == want or near < V * 2.0 ** -44, (r, got[r], want, near, [x[r] for x in s])
+        sure += near >= V * 2.0 ** -44
+    return sure
+
+
+@pytest.mark.parametrize("vocab", [1, 2, 63, 64, 65, 1000, 4096, 4097, 32003, 151936, 262144])
+def test_settings(hip, K, vocab):
+    """Rows of one call with all settings apart: greedy, top-k below and above the vocabulary, top-p, min-p."""
+    rng = np.random.default_rng(vocab)
+    R = 24 if vocab < 50000 else 8
+    x = (2.5 * rng.standard_normal((R, vocab))).astype(np.float32)
+    x[::2, rng.integers(0, vocab, 5)] += 12
+    for _ in range(3):
+        sure = check(hip, K, x, rng.choice([0.0, 0.3, 0.7, 1.0, 1.5, -1.0], R), rng.choice([0, 1, 2, 40, 500, 10 ** 6, -3], R),
+                     rng.choice([0.0, 0.1, 0.5, 0.9, 0.95, 1.0, 2.0], R), rng.choice([0.0, 0.02, 0.1, 1.0, 1.5], R),
+                     rng.random(R))
+        assert sure >= R - 1
+
+
+@pytest.mark.parametrize("sigma", [0.0, 0.01, 1.0, 4.0, 30.0])
+@pytest.mark.parametrize("top_k,top_p", [(0, 1.0), (0, 0.95), (40, 0.9), (5000, 0.99), (0, 0.999999)])
+def test_spreads(hip, K, sigma, top_k, top_p):
+    """From equal logits (every entry tied) to one that stands alone."""
+    rng = np.random.default_rng(int(sigma * 100) + top_k)
+    x = (sigma * rng.standard_normal((5, 20011))).astype(np.float32)
+    check(hip, K, x, 1.0, top_k, top_p, 0.0, [0.0, 0.25, 0.5, 0.9, 1 - 2.0 ** -53])
+
+
+def test_ties_go_to_the_lowest_index(hip, K):
+    """Levels of equal logits: the order inside a level is the index's, at top-k and top-p borders too."""
+    rng = np.random.default_rng(3)
+    x = rng.integers(-3, 4, (12, 3001)).astype(np.float32)
+    for top_k, top_p in ((0, 1.0), (7, 1.0), (700, 1.0), (0, 0.3), (1000, 0.7)):
+        check(hip, K, x, 1.0, top_k, top_p, 0.0, (np.arange(12) + 0.37) / 12)
+    z = np.zeros((1, 1000), np.float32)
+    z[0, ::2] = -0.0  # equal to 0
+    assert draw(hip, K, z, 1.0, 10, u=0.999)[0] == 9 and draw(hip, K, z, 0.0, u=0.5)[0] == 0
+
+
+def test_not_finite_logits(hip, K):
+    inf, nan = np.inf, np.nan
+    x = np.full((6, 300), -1.0, np.float32)
+    x[0, 5], x[0, 6] = nan, 3
+    x[1] = -inf
+    x[2] = nan
+    x[3, [7, 9]] = inf
+    x[4] = -inf
+    x[4, 250] = -1e30
+    x[5, :299] = nan
+    got = draw(hip, K, x, 1.0, u=[0.9, 0.5, 0.5, 0.6, 0.99, 0.99])
+    assert list(got[1:]) == [-1, -1, 9, 250, 299]
+    assert got[0] == osm.sample(x[0], u=0.9)[0]
+    assert list(draw(hip, K, x, 0.0, u=0.5)) == [6, -1, -1, 7, 250, 299]
+    assert list(draw(hip, K, x, np.nan, u=0.5)) == [6, -1, -1, 7, 250, 299]
+
+
+def test_uniforms_at_and_outside_the_ends(hip, K):
+    """u <= 0 and NaN: the first of the kept; u >= 1: the last one with weight."""
+    x = np.log(np.array([[2, 4, 1, 1, 0]] * 6, np.float32) + 1e-38)
+    got = draw(hip, K, x, 1.0, top_k=3, u=[0.0, -1.0, np.nan, 1.0, 7.0, np.inf])
+    assert list(got) == [1, 1, 1, 2, 2, 2]
+
+
+@pytest.mark.parametrize("temperature", [1e-30, 1e-3, 50.0, 1e30, np.inf])
+def test_extreme_temperatures(hip, K, temperature):
+    rng = np.random.default_rng(11)
+    x = (3 * rng.standard_normal((8, 5000))).astype(np.float32)
+    x[:, 77] = -np.inf
+    check(hip, K, x, temperature, [0, 0, 3, 40, 0, 0, 5, 0], [1, 0.5, 1, 0.9, 0.99, 1, 0.5, 1], 0.0, rng.random(8))
+
+
+def test_no_settings_is_the_plain_draw(hip, K):
+    rng = np.random.default_rng(12)
+    x = rng.standard_normal((4, 999)).astype(np.float32)
+    u = rng.random(4)
+    got = draw(hip, K, x, u=u)
+    assert [osm.sample(x[r], u=u[r])[0] for r in range(4)] == list(got)
+
+
+def test_frequencies(hip, K):
+    """4096 evenly spread uniforms fall on the tokens in their proportions, one apart at most."""
+    p = np.array([0.4, 0.3, 0.2, 0.1])
+    x = np.broadcast_to(np.log(p).astype(np.float32), (4096, 4))
+    got = draw(hip, K, np.ascontiguousarray(x), u=(np.arange(4096) + 0.5) / 4096)
+    assert (np.abs(np.bincount(got, minlength=4) - 4096 * p) <= 1).all()

@@ -13,6 +13,7 @@
 #include "vte_common.h"
 #include "fused_kernels.h"
 #include "decode_persistent.h"
+#include "kv_pages.h"
 #include <algorithm>
 #include <cmath>
 #include <cstdlib>
@@ -69,6 +70,19 @@ hipError_t gate_up_mm(const void* xn, const void* w_gate, const void* w_up, int 
                       hipStream_t st);
 hipError_t norm_mv(const void* x, const void* norm_w, float eps, const void* w, int fmt, void* out, bool out_f32,
                    const void* bias, const void* residual, float rs, int M, int K, int N, hipStream_t st);
+hipError_t kv_pages_append(const KvPages& c, const KvRows& r, int hd, bool f16, const void* k, const void* v,
+                           const void* q, void* q_out, int n_q, long long ks, long long vs, long long qs,
+                           const void* cosc, const void* sinc, int rope_rows, int rope_type, int rotary_dim,
+                           hipStream_t st);
+hipError_t kv_pages_read(const KvPages& c, const KvRows& r, int hd, bool f16, void* k_out, void* v_out, int out_rows,
+                         hipStream_t st);
+long long attn_pages_scratch_bytes(const KvPages& c, const KvRows& r, int hd, int n_q);
+hipError_t attn_pages(const KvPages& c, const KvRows& r, int hd, bool f16, const void* q, void* out, int n_q,
+                      float scale, void* scratch, hipStream_t st);
+long long sample_scratch_bytes(int rows);
+hipError_t sample(const float* logits, int rows, int vocab, const float* temperature, const int* top_k,
+                  const float* top_p, const float* min_p, const double* u, int* tokens, void* scratch,
+                  hipStream_t st);
 }  // namespace vte
 
 static thread_local char g_err[512] = "";
@@ -750,4 +764,136 @@ int vte_decode_batch_step(const vte_decode_model* m, void* ws, int batch, long l
     REQUIRE(occ >= 1, "decode_batch_step: the kernel does not fit on a CU (occupancy %d)", occ);
     e = vte::decode_persistent_mm_launch(P, blocks, lds, (hipStream_t)stream);
     return hip_status(e, "vte_decode_batch_step launch");
+}
+
+// ------------------------------------------------------------------ 8-bit paged KV cache, sampling
+
+static int check_pages(const char* who, const vte_kv_pages* c, const vte_kv_rows* r, KvPages* kc, KvRows* kr) {
+    REQUIRE(c && r, "%s: null cache or rows", who);
+    REQUIRE(c->head_dim == 64 || c->head_dim == 128, "%s: head_dim %d (64 or 128)", who, c->head_dim);
+    REQUIRE(c->n_kv >= 1 && c->n_kv <= 65535, "%s: n_kv %d", who, c->n_kv);
+    REQUIRE(c->n_pages >= 1, "%s: n_pages %d", who, c->n_pages);
+    REQUIRE(c->page_tokens >= 16 && c->page_tokens <= 4096 && (c->page_tokens & (c->page_tokens - 1)) == 0,
+            "%s: page_tokens %d is no power of two in 16..4096", who, c->page_tokens);
+    REQUIRE(r->batch >= 1 && r->batch <= 65535, "%s: batch %d outside 1..65535", who, r->batch);
+    REQUIRE(r->rows >= 0 && r->rows <= (1 << 24), "%s: rows %d outside 0..2^24", who, r->rows);
+    REQUIRE(r->max_rows >= 0 && r->max_rows <= r->rows, "%s: max_rows %d outside 0..rows (%d)", who, r->max_rows,
+            r->rows);
+    REQUIRE(r->max_pages >= 1 && (long long)r->max_pages * c->page_tokens <= (1 << 30),
+            "%s: max_pages %d: a table holds at least 1 page and at most 2^30 tokens", who, r->max_pages);
+    REQUIRE(r->row_start || (r->rows == r->batch && r->max_rows == 1) || (r->rows == 0 && r->max_rows == 0),
+            "%s: without row_start rows is the batch and max_rows 1 (or both 0)", who);
+    int log2 = 4;
+    while ((1 << log2) < c->page_tokens) ++log2;
+    *kc = KvPages{(uint8_t*)c->k, (uint8_t*)c->v, (int8_t*)c->k_exp, (int8_t*)c->v_exp, c->n_pages, log2, c->n_kv};
+    *kr = KvRows{r->row_start, r->kv_offset, r->page_table, r->batch, r->rows, r->max_rows, r->max_pages};
+    return 0;
+}
+static int check_pages_memory(const char* who, const vte_kv_pages* c, const vte_kv_rows* r, int dtype) {
+    REQUIRE(c->k && c->v && c->k_exp && c->v_exp && r->kv_offset && r->page_table, "%s: null pointer", who);
+    REQUIRE(aligned(c->k, 16) && aligned(c->v, 16), "%s: the pages must be 16-byte aligned", who);
+    REQUIRE(aligned(r->row_start, 4) && aligned(r->kv_offset, 4) && aligned(r->page_table, 4),
+            "%s: 4-byte alignment of the row description", who);
+    REQUIRE(dtype == VTE_F32 || dtype == VTE_F16, "%s: dtype must be 0 (f32) or 1 (f16)", who);
+    return 0;
+}
+
+int vte_kv_pages_append(const vte_kv_pages* cache, const vte_kv_rows* rows, int dtype, const void* k, const void* v,
+                        long long k_stride, long long v_stride, const void* q, void* q_out, int n_q,
+                        long long q_stride, const void* rope_cos, const void* rope_sin, int rope_rows, int rope_type,
+                        int rotary_dim, void* stream) {
+    KvPages c;
+    KvRows r;
+    int rc = check_pages("kv_pages_append", cache, rows, &c, &r);
+    if (!rc) rc = check_pages_memory("kv_pages_append", cache, rows, dtype);
+    if (rc) return rc;
+    const int hd = cache->head_dim;
+    const size_t size = dtype == VTE_F16 ? 2 : 4;
+    REQUIRE(r.rows >= 1 && r.max_rows >= 1, "kv_pages_append: no rows");
+    REQUIRE(k && v, "kv_pages_append: null k or v");
+    REQUIRE(aligned(k, size) && aligned(v, size) && aligned(q, size) && aligned(q_out, size),
+            "kv_pages_append: k, v and q must be aligned to their type");
+    const long long ks = k_stride ? k_stride : (long long)c.n_kv * hd, vs = v_stride ? v_stride : (long long)c.n_kv * hd;
+    REQUIRE(ks >= (long long)c.n_kv * hd && vs >= (long long)c.n_kv * hd && ks < (1LL << 31) && vs < (1LL << 31),
+            "kv_pages_append: k_stride %lld / v_stride %lld below a row of %d x %d", k_stride, v_stride, c.n_kv, hd);
+    REQUIRE((rope_cos == nullptr) == (rope_sin == nullptr), "kv_pages_append: one rotation table of two");
+    REQUIRE((q == nullptr) == (q_out == nullptr), "kv_pages_append: q and q_out go together");
+    REQUIRE(!q || rope_cos, "kv_pages_append: q without rotation tables");
+    const long long qs = q && !q_stride ? (long long)n_q * hd : q_stride;
+    if (q) {
+        REQUIRE(n_q >= 1 && n_q <= 65535 && qs >= (long long)n_q * hd && qs < (1LL << 31),
+                "kv_pages_append: n_q %d, q_stride %lld", n_q, q_stride);
+        REQUIRE(q != q_out || qs == (long long)n_q * hd, "kv_pages_append: in place q must be contiguous");
+    }
+    if (rope_cos) {
+        REQUIRE(rope_rows >= 1, "kv_pages_append: rope_rows %d", rope_rows);
+        REQUIRE(rope_type >= 0 && rope_type <= 2, "kv_pages_append: rope_type %d unknown", rope_type);
+        REQUIRE(rope_type != 2 || (rotary_dim > 0 && rotary_dim <= hd && rotary_dim % 2 == 0),
+                "kv_pages_append: bad rotary_dim %d", rotary_dim);
+        REQUIRE(aligned(rope_cos, 2) && aligned(rope_sin, 2), "kv_pages_append: tables must be 2-byte aligned");
+    }
+    return hip_status(vte::kv_pages_append(c, r, hd, dtype == VTE_F16, k, v, q, q_out, n_q, ks, vs, qs, rope_cos,
+                                           rope_sin, rope_rows, rope_type, rotary_dim, (hipStream_t)stream),
+                      "vte_kv_pages_append launch");
+}
+
+int vte_kv_pages_read(const vte_kv_pages* cache, const vte_kv_rows* rows, int dtype, void* k_out, void* v_out,
+                      int out_rows, void* stream) {
+    KvPages c;
+    KvRows r;
+    int rc = check_pages("kv_pages_read", cache, rows, &c, &r);
+    if (!rc) rc = check_pages_memory("kv_pages_read", cache, rows, dtype);
+    if (rc) return rc;
+    REQUIRE(k_out && v_out, "kv_pages_read: null output");
+    REQUIRE(out_rows >= 1, "kv_pages_read: out_rows %d", out_rows);
+    REQUIRE(aligned(k_out, 16) && aligned(v_out, 16), "kv_pages_read: outputs must be 16-byte aligned");
+    return hip_status(vte::kv_pages_read(c, r, cache->head_dim, dtype == VTE_F16, k_out, v_out, out_rows,
+                                         (hipStream_t)stream),
+                      "vte_kv_pages_read launch");
+}
+
+static int check_attn_pages(const vte_kv_pages* cache, const vte_kv_rows* rows, int n_q, KvPages* c, KvRows* r) {
+    int rc = check_pages("attn_pages", cache, rows, c, r);
+    if (rc) return rc;
+    REQUIRE(n_q >= c->n_kv && n_q <= 65535 && n_q % c->n_kv == 0 && n_q / c->n_kv <= 16,
+            "attn_pages: bad head counts %d/%d (groups of at most 16)", n_q, c->n_kv);
+    REQUIRE(r->rows >= 1 && r->max_rows >= 1, "attn_pages: no rows");
+    return 0;
+}
+
+long long vte_attn_pages_scratch_bytes(const vte_kv_pages* cache, const vte_kv_rows* rows, int n_q) {
+    KvPages c;
+    KvRows r;
+    if (check_attn_pages(cache, rows, n_q, &c, &r)) return -1;
+    return vte::attn_pages_scratch_bytes(c, r, cache->head_dim, n_q);
+}
+
+int vte_attn_pages(const vte_kv_pages* cache, const vte_kv_rows* rows, int dtype, const void* q, void* out, int n_q,
+                   float scale, void* scratch, long long scratch_bytes, void* stream) {
+    KvPages c;
+    KvRows r;
+    int rc = check_attn_pages(cache, rows, n_q, &c, &r);
+    if (!rc) rc = check_pages_memory("attn_pages", cache, rows, dtype);
+    if (rc) return rc;
+    REQUIRE(q && out && scratch, "attn_pages: null pointer");
+    REQUIRE(aligned(q, 16) && aligned(out, 16) && aligned(scratch, 16), "attn_pages: 16-byte alignment");
+    REQUIRE(scale > 0.f && scale <= 1e6f, "attn_pages: scale outside (0, 1e6]");
+    const long long need = vte::attn_pages_scratch_bytes(c, r, cache->head_dim, n_q);
+    REQUIRE(scratch_bytes >= need, "attn_pages: scratch of %lld bytes, %lld needed", scratch_bytes, need);
+    return hip_status(vte::attn_pages(c, r, cache->head_dim, dtype == VTE_F16, q, out, n_q, scale, scratch,
+                                      (hipStream_t)stream),
+                      "vte_attn_pages launch");
+}
+
+long long vte_sample_scratch_bytes(int rows) { return rows >= 1 ? vte::sample_scratch_bytes(rows) : 0; }
+
+int vte_sample(const float* logits, int rows, int vocab, const float* temperature, const int* top_k,
+               const float* top_p, const float* min_p, const double* u, int* tokens, void* scratch, void* stream) {
+    REQUIRE(logits && u && tokens && scratch, "sample: null pointer");
+    REQUIRE(rows >= 1 && rows <= 65535, "sample: rows %d outside 1..65535", rows);
+    REQUIRE(vocab >= 1 && vocab <= 262144, "sample: vocab %d outside 1..262144", vocab);
+    REQUIRE(aligned(logits, 4) && aligned(u, 8) && aligned(scratch, 16), "sample: alignment");
+    return hip_status(vte::sample(logits, rows, vocab, temperature, top_k, top_p, min_p, u, tokens, scratch,
+                                  (hipStream_t)stream),
+                      "vte_sample launch");
 }

@@ -59,10 +59,17 @@ SIGNATURES = {
     "vte_decode_batch_workspace_bytes": [_vp, _i],
     "vte_decode_batch_setup": [_vp, _vp, _i, _vp, _ll, _vp],
     "vte_decode_batch_step": [_vp, _vp, _i, _ll, _vp, _vp, _vp, _vp],
+    "vte_kv_pages_append": [_vp, _vp, _i, _vp, _vp, _ll, _ll, _vp, _vp, _i, _ll, _vp, _vp, _i, _i, _i, _vp],
+    "vte_kv_pages_read": [_vp, _vp, _i, _vp, _vp, _i, _vp],
+    "vte_attn_pages_scratch_bytes": [_vp, _vp, _i],
+    "vte_attn_pages": [_vp, _vp, _i, _vp, _vp, _i, _f, _vp, _ll, _vp],
+    "vte_sample_scratch_bytes": [_i],
+    "vte_sample": [_vp, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
     "vte_last_error": [],
 }
 RESTYPES = {"vte_last_error": ctypes.c_char_p, "vte_attn_scratch_floats": _ll, "vte_topk_scratch_bytes": _ll,
-            "vte_decode_workspace_bytes": _ll, "vte_decode_batch_workspace_bytes": _ll}
+            "vte_decode_workspace_bytes": _ll, "vte_decode_batch_workspace_bytes": _ll, "vte_attn_pages_scratch_bytes": _ll,
+            "vte_sample_scratch_bytes": _ll}
 
 
 class DecodeLayer(ctypes.Structure):
@@ -77,6 +84,28 @@ class DecodeModel(ctypes.Structure):
     _fields_ = [(n, _i) for n in ("n_layers", "hidden", "ffn", "n_q", "n_kv", "head_dim", "vocab", "max_seq")] + \
                [("eps", _f)] + [(n, _vp) for n in ("rope_cos", "rope_sin", "output_norm", "lm_head")] + \
                [("fmt_lm", _i)]
+
+
+class KVPages(ctypes.Structure):
+    """vte_kv_pages (include/vte_amd.h): an 8-bit paged KV cache."""
+    _fields_ = [(n, _vp) for n in ("k", "v", "k_exp", "v_exp")] + \
+               [(n, _i) for n in ("n_pages", "page_tokens", "n_kv", "head_dim")]
+
+    @classmethod
+    def of(cls, k, v, k_exp, v_exp, n_pages: int, page_tokens: int, n_kv: int, head_dim: int) -> "KVPages":
+        """From device pointers (ints or objects with ``.ptr``)."""
+        return cls(_p(k), _p(v), _p(k_exp), _p(v_exp), n_pages, page_tokens, n_kv, head_dim)
+
+
+class KVRows(ctypes.Structure):
+    """vte_kv_rows (include/vte_amd.h): the sequences of a call and their new rows."""
+    _fields_ = [(n, _i) for n in ("batch", "rows", "max_rows", "max_pages")] + \
+               [(n, _vp) for n in ("row_start", "kv_offset", "page_table")]
+
+    @classmethod
+    def of(cls, batch: int, rows: int, max_rows: int, row_start, kv_offset, page_table, max_pages: int) -> "KVRows":
+        """From device pointers; ``row_start`` None: one row per sequence, or none (rows = max_rows = 0)."""
+        return cls(batch, rows, max_rows, max_pages, _p(row_start), _p(kv_offset), _p(page_table))
 
 
 def _p(x) -> Optional[int]:
@@ -279,6 +308,43 @@ class VTEKernels:
         f = ctypes.c_int(0)
         self._check(self.lib.vte_decode_status(_p(ws), ctypes.byref(f)), "vte_decode_status")
         return f.value
+
+    def kv_pages_append(self, pages: KVPages, rows: KVRows, k, v, q=None, q_out=None, n_q=0, rope_cos=None,
+                        rope_sin=None, rope_rows=0, rope_type=0, rotary_dim=0, dtype="f16", k_stride=0, v_stride=0,
+                        q_stride=0, stream=None) -> None:
+        """The new rows' k (rotated by position where tables are given) and v into their 8-bit pages;
+        q_out = q rotated likewise.  Strides in elements between rows, 0: contiguous."""
+        self._check(self.lib.vte_kv_pages_append(ctypes.byref(pages), ctypes.byref(rows), DT[dtype], _p(k), _p(v),
+                                                 k_stride, v_stride, _p(q), _p(q_out), n_q, q_stride, _p(rope_cos),
+                                                 _p(rope_sin), rope_rows, rope_type, rotary_dim, self._st(stream)),
+                    "vte_kv_pages_append")
+
+    def kv_pages_read(self, pages: KVPages, rows: KVRows, k_out, v_out, out_rows: int, dtype="f16",
+                      stream=None) -> None:
+        """k_out, v_out [batch][out_rows][n_kv][head_dim] = every sequence's cached values."""
+        self._check(self.lib.vte_kv_pages_read(ctypes.byref(pages), ctypes.byref(rows), DT[dtype], _p(k_out),
+                                               _p(v_out), out_rows, self._st(stream)), "vte_kv_pages_read")
+
+    def attn_pages_scratch_bytes(self, pages: KVPages, rows: KVRows, n_q: int) -> int:
+        n = int(self.lib.vte_attn_pages_scratch_bytes(ctypes.byref(pages), ctypes.byref(rows), n_q))
+        if n < 0:
+            self._check(-1, "vte_attn_pages_scratch_bytes")
+        return n
+
+    def attn_pages(self, pages: KVPages, rows: KVRows, q, out, n_q: int, scale: float, scratch, scratch_bytes: int,
+                   dtype="f16", stream=None) -> None:
+        """Attention of the new rows (decoded tokens, prompt chunks) over the 8-bit paged cache."""
+        self._check(self.lib.vte_attn_pages(ctypes.byref(pages), ctypes.byref(rows), DT[dtype], _p(q), _p(out), n_q,
+                                            scale, _p(scratch), scratch_bytes, self._st(stream)), "vte_attn_pages")
+
+    def sample_scratch_bytes(self, rows: int) -> int:
+        return int(self.lib.vte_sample_scratch_bytes(rows))
+
+    def sample(self, logits, rows: int, vocab: int, tokens, scratch, temperature=None, top_k=None, top_p=None,
+               min_p=None, u=None, stream=None) -> None:
+        """tokens[r] drawn from row r of fp32 logits under the rows' settings and uniforms ``u`` (device arrays)."""
+        self._check(self.lib.vte_sample(_p(logits), rows, vocab, _p(temperature), _p(top_k), _p(top_p), _p(min_p),
+                                        _p(u), _p(tokens), _p(scratch), self._st(stream)), "vte_sample")
 
     def fill_normal_f16(self, dst, n, seed, scale=1.0, stream=None):
         self._check(self.lib.vte_fill_normal_f16(_p(dst), n, seed, scale, self._st(stream)), "vte_fill_normal_f16")
