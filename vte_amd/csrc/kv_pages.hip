@@ -1,4 +1,4 @@
-// Append, read and attention over the 8-bit paged KV cache (layout: kv_pages.h), gfx950.
+// Append and read of the 8-bit paged KV cache (layout: kv_pages.h), gfx950.
 // No counterpart in the reference, whose cache is one fp16 range per sequence
 // (vte/compiler/templates/rdna/kv_cache_append.hip.template:13-39).
 #include <algorithm>
@@ -180,56 +180,6 @@ __global__ __launch_bounds__(256) void kv_pages_read_kernel(KvPages c, KvRows r,
 }
 
 // ---------------------------------------------------------------------------
-// Attention, one wave per (row, query head): online softmax token by token,
-// dims over the lanes.
-// ---------------------------------------------------------------------------
-template <typename T, int HD>
-__global__ __launch_bounds__(64) void attn_pages_kernel(KvPages c, KvRows r, const T* __restrict__ q,
-                                                        T* __restrict__ out, int n_q, float scale) {
-    constexpr int PL = HD / 64;  // dims a lane holds: lane + 64 j
-    const int row = blockIdx.x, qh = blockIdx.y, lane = threadIdx.x;
-    const int b = kvp_row_seq(r, row);
-    if (b < 0) return;
-    const KvSeq s = kvp_seq(r, b);
-    const int i = row - s.first;
-    if (s.pos >= 0 && (i < 0 || i >= s.n)) return;
-    const int h = qh / (n_q / c.n_kv);
-    const int len = s.pos < 0 ? 0 : kvp_len(min(s.pos, 1 << 30) + i, kvp_capacity(c, r));
-    float qv[PL], o[PL], m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int j = 0; j < PL; ++j) {
-        qv[j] = ld_act<T>(q + ((size_t)row * n_q + qh) * HD + lane + 64 * j);
-        o[j] = 0.f;
-    }
-    for (int t = 0; t < len; ++t) {
-        const int page = kvp_page(c, r, b, t >> c.page_log2);
-        if (page < 0) {
-            t |= (1 << c.page_log2) - 1;
-            continue;
-        }
-        const int in_page = (t & ((1 << c.page_log2) - 1)) / KVP_BLOCK, p = t % KVP_BLOCK;
-        const size_t at = (((size_t)page * c.n_kv + h) << (c.page_log2 - 4)) + in_page;
-        float dot = 0.f;
-#pragma unroll
-        for (int j = 0; j < PL; ++j)
-            dot += qv[j] * (float)((int)c.k[at * (KVP_BLOCK * HD) + p * HD + lane + 64 * j] - KVP_ZERO);
-        const float sc = wave_sum(dot) * kvp_scale(c.k_exp[at]) * scale;
-        const float mn = sc > m || sc != sc ? sc : m;
-        const float corr = m == -INFINITY ? 0.f : expf(m - mn), w = expf(sc - mn);
-        l = l * corr + w;
-        const float wv = w * kvp_scale(c.v_exp[at]);
-#pragma unroll
-        for (int j = 0; j < PL; ++j)
-            o[j] = o[j] * corr +
-                   wv * (float)((int)c.v[at * (KVP_BLOCK * HD) + (lane + 64 * j) * KVP_BLOCK + p] - KVP_ZERO);
-        m = mn;
-    }
-#pragma unroll
-    for (int j = 0; j < PL; ++j)
-        st_act<T>(out + ((size_t)row * n_q + qh) * HD + lane + 64 * j, l == 0.f ? 0.f : o[j] / l);
-}
-
-// ---------------------------------------------------------------------------
 // Host launchers
 // ---------------------------------------------------------------------------
 namespace vte {
@@ -272,22 +222,6 @@ hipError_t kv_pages_read(const KvPages& c, const KvRows& r, int hd, bool f16, vo
                    : read_hd<float, 128>(c, r, k_out, v_out, out_rows, st);
     return f16 ? read_hd<__half, 64>(c, r, k_out, v_out, out_rows, st)
                : read_hd<float, 64>(c, r, k_out, v_out, out_rows, st);
-}
-
-long long attn_pages_scratch_bytes(const KvPages&, const KvRows&, int, int) { return 256; }
-
-template <typename T, int HD>
-static hipError_t attn_hd(const KvPages& c, const KvRows& r, const void* q, void* out, int n_q, float scale,
-                          hipStream_t st) {
-    hipLaunchKernelGGL((attn_pages_kernel<T, HD>), dim3(r.rows, n_q), dim3(64), 0, st, c, r, (const T*)q, (T*)out, n_q,
-                       scale);
-    return hipGetLastError();
-}
-hipError_t attn_pages(const KvPages& c, const KvRows& r, int hd, bool f16, const void* q, void* out, int n_q,
-                      float scale, void*, hipStream_t st) {
-    if (hd == 128)
-        return f16 ? attn_hd<__half, 128>(c, r, q, out, n_q, scale, st) : attn_hd<float, 128>(c, r, q, out, n_q, scale, st);
-    return f16 ? attn_hd<__half, 64>(c, r, q, out, n_q, scale, st) : attn_hd<float, 64>(c, r, q, out, n_q, scale, st);
 }
 
 }  // namespace vte
