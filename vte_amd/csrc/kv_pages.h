@@ -33,12 +33,12 @@ struct KvRows {
 
 __device__ __forceinline__ int kvp_capacity(const KvPages& c, const KvRows& r) { return r.max_pages << c.page_log2; }
 
-// Sequence b's new rows [first, first + n) and the position of the first; n = 0
+// Sequence b's new rows [first, first + n), and the position of the first; n = 0
 // for a sequence that is not running (kv_offset < 0).
 struct KvSeq {
     int first, n, pos;
 };
-__device__ __forceinline__ KvSeq kvp_seq(const KvRows& r, int b) {
+__device__ __forceinline__ KvSeq kvp_place(const KvRows& r, int b) {  // its rows, whether it runs or not
     KvSeq s;
     s.pos = r.kv_offset[b];
     if (r.row_start == nullptr) {
@@ -46,9 +46,13 @@ __device__ __forceinline__ KvSeq kvp_seq(const KvRows& r, int b) {
         s.n = r.max_rows;
     } else {
         s.first = max(r.row_start[b], 0);
-        s.n = min(min(r.row_start[b + 1], r.rows) - s.first, r.max_rows);
+        s.n = max(min(min(r.row_start[b + 1], r.rows) - s.first, r.max_rows), 0);
     }
-    if (s.n < 0 || s.pos < 0) s.n = 0;
+    return s;
+}
+__device__ __forceinline__ KvSeq kvp_seq(const KvRows& r, int b) {
+    KvSeq s = kvp_place(r, b);
+    if (s.pos < 0) s.n = 0;
     return s;
 }
 // The sequence of a row: the last one that starts at or before it, -1 behind the last sequence.
