@@ -9,31 +9,33 @@
 // mass).  T <= 0: the first of all.  Every filter keeps a prefix of the order, so
 // all that matters is at which mass each ends.
 //
-// The row is not sorted.  With y = 64 x / T, entries fall into bins floor(y); the
-// bin g below the largest entry's has weight e^(-g/64) times the sum of its
-// entries' e^(-(floor(y) + 1 - y) / 64), which are whole numbers of 2^-44 summed in
-// 64 bits: exact in any order and however the row is cut.  Sums over bins say in
+// The row is not sorted.  With y = 32 x / T, entries fall into bins round(y); the
+// bin g below the largest entry's has weight e^(-g/32) times the sum of its
+// entries' e^((y - round(y)) / 32), which are whole numbers of 2^-44 summed in 64
+// bits: exact in any order and however the row is cut.  Sums over bins say in
 // which bin each filter and the draw end, and only the entries of these few bins
-// are ordered.  2048 bins reach down to e^-32 of the largest weight; an entry
+// are ordered.  1024 bins reach down to e^-32 of the largest weight; an entry
 // below has none.
 //   1. sample_bins_kernel: blocks of a row each sum their part into bins.
-//   2. sample_draw_kernel: one block a row merges them, collects the entries of
-//      the bins in question and ends the filters and the draw in them.
+//   2. sample_draw_kernel: merges them, collects the entries of the bins in
+//      question and ends the filters and the draw in them.  One CU reads no more
+//      than some 30 GB/s, so while there are few rows several blocks share a row's
+//      reading: each merges for itself, and the last to be done (none waits) goes on.
 #include <algorithm>
 #include "vte_common.h"
 
 #define SMP_THREADS 1024
 #define SMP_WAVES (SMP_THREADS / 64)
 #define SMP_SUB 256         // entries whose largest one is kept (one wave's 16-byte load)
-#define SMP_BINS 2048
-#define SMP_PER_UNIT 64.0   // bins per unit of x / T
+#define SMP_BINS 1024       // one a thread
+#define SMP_PER_UNIT 32.0   // bins per unit of x / T
 #define SMP_ONE 17592186044416.0  // 2^44
 #define SMP_IDX_BITS 18
 #define SMP_DIGIT 10
 #define SMP_LEVELS 5        // 32 + 18 bits of (key, index) in digits of 10
-#define SMP_LIST 6144       // entries that are collected at most; more: the row is read again
+#define SMP_LIST 8192       // entries that are collected at most; more: the row is read again
 #define SMP_SMALL 1024      // entries of a bin that are ordered by counting
-#define SMP_SPLIT 16        // blocks of a row at most
+#define SMP_SPLIT 8         // blocks of a row at most
 
 // Scratch of a row.
 struct SmpScratch {
@@ -41,9 +43,11 @@ struct SmpScratch {
     uint32_t* count; // [blocks][SMP_BINS], rows with a top-k only
     float* sub;      // [entries / SMP_SUB] largest entry of each
     float* max;      // [blocks]
+    int* shared;     // entries collected, blocks of the draw that are done
+    uint32_t* list;  // [SMP_LIST] their indices
 };
 __host__ __device__ inline size_t smp_row_bytes(int blocks, int subs) {
-    return (size_t)blocks * SMP_BINS * 12 + ((size_t)subs * 4 + SMP_SPLIT * 4 + 15) / 16 * 16;
+    return (size_t)blocks * SMP_BINS * 12 + (SMP_SPLIT + 4 + SMP_LIST) * 4 + ((size_t)subs * 4 + 15) / 16 * 16;
 }
 __device__ __forceinline__ SmpScratch smp_scratch(uint8_t* base, int row, int blocks, int subs) {
     uint8_t* p = base + (size_t)row * smp_row_bytes(blocks, subs);
@@ -51,7 +55,9 @@ __device__ __forceinline__ SmpScratch smp_scratch(uint8_t* base, int row, int bl
     s.mass = reinterpret_cast<uint64_t*>(p);
     s.count = reinterpret_cast<uint32_t*>(p + (size_t)blocks * SMP_BINS * 8);
     s.max = reinterpret_cast<float*>(p + (size_t)blocks * SMP_BINS * 12);
-    s.sub = s.max + SMP_SPLIT;
+    s.shared = reinterpret_cast<int*>(s.max + SMP_SPLIT);
+    s.list = reinterpret_cast<uint32_t*>(s.shared + 4);
+    s.sub = reinterpret_cast<float*>(s.list + SMP_LIST);
     return s;
 }
 
@@ -64,68 +70,111 @@ __device__ __forceinline__ uint32_t smp_key(float x) {
 __device__ __forceinline__ uint64_t smp_place(float x, int i) {
     return ((uint64_t)smp_key(x) << SMP_IDX_BITS) | (uint64_t)(((1 << SMP_IDX_BITS) - 1) - i);
 }
+__device__ __forceinline__ float smp_value(uint64_t place) {
+    const uint32_t k = (uint32_t)(place >> SMP_IDX_BITS);
+    return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
+}
 __device__ __forceinline__ int smp_index(uint64_t place) {
     return ((1 << SMP_IDX_BITS) - 1) - (int)(place & ((1 << SMP_IDX_BITS) - 1));
 }
 
-// Where a row's bins lie: the largest value (of the row or of a part), 64 / T and floor(64 max / T).
+// Where a row's bins lie: the largest value (of the row or of a part), 32 / T, and the low word of round(32 max / T).
+// Rounding adds 1.5 2^52, whose low word then holds the whole number: differences of up to 2^31 bins are right, and
+// values that lie further down are raised to `low`, which is out of every bin.
+#define SMP_ROUND 6755399441055744.0
 struct SmpScale {
-    float max;
-    double s, top;
+    float max, low;
+    double s;
+    int top;
+    bool whole;  // 32 max / T is a place on this scale
+    bool flat;   // if not: every finite value weighs the same (T infinite); else the largest is alone
 };
 __device__ __forceinline__ SmpScale smp_scale(float max, float T) {
     SmpScale c;
     c.max = max;
     c.s = SMP_PER_UNIT / (double)T;
-    c.top = floor((double)max * c.s);
+    const double y = (double)max * c.s;
+    c.whole = fabs(y) < 35184372088832.0 && c.s > 0.0;  // 2^45: from 2^40 on neighbours are 2^16 bins apart
+    c.flat = !c.whole && !(c.s > 0.0) && max < INFINITY;
+    c.top = c.whole ? __double2loint(y + SMP_ROUND) : 0;
+    const double low = c.whole ? (y - 1.5 * SMP_BINS) / c.s : 0.0;
+    c.low = fmaxf(low < -3.4e38 ? -3.4e38f : (float)(low - 1.2e-7 * fabs(low) - 1e-45), -3.4028234664e38f);
     return c;
 }
-// Bin of x (false: no weight, NaN among them) and its weight in the bin, in units of 2^-44.
+// Bin of x (false: no weight, NaN among them) and its weight in the bin, in units of 2^-44: the series of e^(r / 32)
+// for y = round(y) + r (the next term is below 2^-45).
 __device__ __forceinline__ bool smp_bin(const SmpScale& c, float x, int& g, uint64_t& m) {
-    const double y = (double)x * c.s, a = floor(y);
-    double d = c.top - a, f = (a + 1.0 - y) * (1.0 / SMP_PER_UNIT);
-    if (x == c.max && !(fabs(d) < 1.0)) d = 0.0, f = 0.0;  // infinite or beyond whole numbers: itself alone
-    if (!(d < (double)SMP_BINS)) return false;
-    g = (int)d;
-    double p = fma(f, 1.0 / 720.0, -1.0 / 120.0);  // e^-f, f <= 1/64: the next term is below 2^-54
-    p = fma(f, p, 1.0 / 24.0);
-    p = fma(f, p, -1.0 / 6.0);
-    p = fma(f, p, 0.5);
-    p = fma(f, p, -1.0);
-    p = fma(f, p, 1.0);
+    constexpr double H = 1.0 / SMP_PER_UNIT;
+    double r = 0.0;
+    bool in = x > -INFINITY;
+    if (c.whole) {
+        const double v = (double)fmaxf(x, c.low);
+        const double t = fma(v, c.s, SMP_ROUND);
+        r = fma(v, c.s, SMP_ROUND - t);
+        g = c.top - __double2loint(t);
+        in = in && (unsigned)g < SMP_BINS;
+    } else {
+        in = in && (c.flat || x == c.max);
+        g = 0;
+    }
+    double p = fma(r, H * H * H * H * H / 120.0, H * H * H * H / 24.0);
+    p = fma(r, p, H * H * H / 6.0);
+    p = fma(r, p, H * H / 2.0);
+    p = fma(r, p, H);
+    p = fma(r, p, 1.0);
     // 2^52 + p 2^44 holds the whole number in its low bits
     m = (uint64_t)__double_as_longlong(fma(p, SMP_ONE, 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;
-    return true;
+    return in;
+}
+// Place of x inside its bin, from the largest value on, in 1024 steps.
+__device__ __forceinline__ int smp_inside(const SmpScale& c, float x) {
+    if (!c.whole) return 0;
+    const double t = fma((double)x, c.s, SMP_ROUND), r = fma((double)x, c.s, SMP_ROUND - t);
+    return min(max((int)((0.5 - r) * (double)SMP_THREADS), 0), SMP_THREADS - 1);
+}
+// Bins between the largest values of a part and of the row; SMP_BINS or more: none of the part's matter.
+__device__ __forceinline__ int smp_apart(const SmpScale& c, float part) {
+    if (part == c.max) return 0;
+    if (!c.whole) return c.flat ? 0 : SMP_BINS;
+    const int d = c.top - __double2loint(fma((double)fmaxf(part, c.low), c.s, SMP_ROUND));
+    return (unsigned)d < SMP_BINS ? d : SMP_BINS;
 }
 
-// Four entries of subset `sub` that lane holds: 16-byte loads where the row allows them.
+// Four entries of a subset: lane's 16 bytes where every row is 16-byte aligned and whole (WIDE), else one of each 64.
+// The load itself asks nothing of its values and takes no branch, so that several stay in flight; places behind the
+// row's end hold an entry of the row until smp_cut.
 struct SmpFour {
     float x[4];
-    int i[4];
 };
-__device__ __forceinline__ SmpFour smp_load(const float* row, int vocab, int sub, int lane, bool wide) {
+template <bool WIDE>
+__device__ __forceinline__ int smp_at(int sub, int lane, int e) {
+    return sub * SMP_SUB + (WIDE ? 4 * lane + e : 64 * e + lane);
+}
+template <bool WIDE>
+__device__ __forceinline__ SmpFour smp_load(const float* row, int vocab, int sub, int lane) {
     SmpFour r;
-    const int base = sub * SMP_SUB;
-    if (wide && base + SMP_SUB <= vocab) {
-        const float4 v = *reinterpret_cast<const float4*>(row + base + 4 * lane);
+    if constexpr (WIDE) {
+        const float4 v = *reinterpret_cast<const float4*>(row + min(smp_at<WIDE>(sub, lane, 0), vocab - 4));
         r.x[0] = v.x; r.x[1] = v.y; r.x[2] = v.z; r.x[3] = v.w;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) r.i[e] = base + 4 * lane + e;
     } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            r.i[e] = base + 64 * e + lane;
-            r.x[e] = r.i[e] < vocab ? row[r.i[e]] : -INFINITY;
-        }
+        for (int e = 0; e < 4; ++e) r.x[e] = row[min(smp_at<WIDE>(sub, lane, e), vocab - 1)];
     }
     return r;
+}
+template <bool WIDE>
+__device__ __forceinline__ void smp_cut(SmpFour& f, int vocab, int sub, int lane) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f.x[e] = smp_at<WIDE>(sub, lane, e) < vocab ? f.x[e] : -INFINITY;
 }
 __device__ __forceinline__ float smp_max4(const SmpFour& r) {  // NaN counts as nothing
     return fmaxf(fmaxf(fmaxf(r.x[0], -INFINITY), r.x[1]), fmaxf(r.x[2], r.x[3]));
 }
 
-// grid (blocks of a row, rows).  The block's first KEEP subsets a wave stay in registers between the two passes.
-#define SMP_KEEP 4
+// grid (blocks of a row, rows).  The block's first KEEP subsets a wave stay in registers between the two passes (all of
+// a part, for few rows); the others are read again, eight and then four in flight.
+#define SMP_KEEP 8
+template <bool WIDE>
 __global__ __launch_bounds__(SMP_THREADS) void sample_bins_kernel(const float* __restrict__ logits, int vocab,
                                                                   const float* __restrict__ temperature,
                                                                   const int* __restrict__ top_k, uint8_t* scratch,
@@ -133,40 +182,49 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_bins_kernel(const float* _
     __shared__ unsigned long long mass[SMP_BINS];
     __shared__ unsigned count[SMP_BINS];
     __shared__ float wmax[SMP_WAVES];
-    const int row = blockIdx.y, blocks = gridDim.x, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+    const int row = blockIdx.y, blocks = gridDim.x, tid = threadIdx.x, lane = tid & 63;
+    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const float* x = logits + (size_t)row * vocab;
-    const bool wide = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
     const SmpScratch sc = smp_scratch(scratch, row, blocks, subs);
     const int lo = (int)((long long)subs * blockIdx.x / blocks), hi = (int)((long long)subs * (blockIdx.x + 1) / blocks);
+    // subset j of this wave, one of the block's where there are fewer (lo < hi: no more blocks than subsets)
+    auto nth = [&](int j) { return lo + wv + SMP_WAVES * j; };
+    auto load = [&](int j) { return smp_load<WIDE>(x, vocab, min(nth(j), hi - 1), lane); };
+    SmpFour keep[SMP_KEEP];
+#pragma unroll
+    for (int j = 0; j < SMP_KEEP; ++j) keep[j] = load(j);
     const float T = temperature ? temperature[row] : 1.f;
     const bool counts = top_k != nullptr && top_k[row] > 0;
-    SmpFour keep[SMP_KEEP];
+    mass[tid] = 0;
+    count[tid] = 0;
     float best = -INFINITY;
-    auto first = [&](const SmpFour& f, int sub) {
+    auto first = [&](SmpFour& f, int j) {
+        smp_cut<WIDE>(f, vocab, min(nth(j), hi - 1), lane);
         const float m = wave_max(smp_max4(f));
-        if (lane == 0) sc.sub[sub] = m;
-        best = fmaxf(best, m);
+        if (lane == 0 && nth(j) < hi) sc.sub[nth(j)] = m;
+        best = fmaxf(best, m);  // (a subset twice changes nothing)
     };
+    const int n = (hi - lo + SMP_WAVES - 1) / SMP_WAVES;
 #pragma unroll
-    for (int j = 0; j < SMP_KEEP; ++j)
-        if (lo + wv + SMP_WAVES * j < hi) keep[j] = smp_load(x, vocab, lo + wv + SMP_WAVES * j, lane, wide);
-    for (int i = tid; i < SMP_BINS; i += SMP_THREADS) {
-        mass[i] = 0;
-        count[i] = 0;
+    for (int j = 0; j < SMP_KEEP; ++j) first(keep[j], j);
+    for (int j = SMP_KEEP; j < n; j += 8) {
+        SmpFour f[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = load(j + i);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) first(f[i], j + i);
     }
-#pragma unroll
-    for (int j = 0; j < SMP_KEEP; ++j)
-        if (lo + wv + SMP_WAVES * j < hi) first(keep[j], lo + wv + SMP_WAVES * j);
-    for (int sub = lo + wv + SMP_WAVES * SMP_KEEP; sub < hi; sub += SMP_WAVES) first(smp_load(x, vocab, sub, lane, wide), sub);
     if (lane == 0) wmax[wv] = best;
     __syncthreads();
     best = wmax[0];
 #pragma unroll
     for (int w = 1; w < SMP_WAVES; ++w) best = fmaxf(best, wmax[w]);
     if (tid == 0) sc.max[blockIdx.x] = best;
+    if (tid < 2 && blockIdx.x == 0) sc.shared[tid] = 0;
     if (!(best > -INFINITY) || !(T > 0.f)) return;  // nothing in it; greedy rows need the maxima only
     const SmpScale c = smp_scale(best, T);
-    auto second = [&](const SmpFour& f) {
+    auto second = [&](const SmpFour& f, int j) {
+        if (nth(j) >= hi) return;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             int g;
@@ -176,39 +234,61 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_bins_kernel(const float* _
             if (counts) atomicAdd(&count[g], 1u);
         }
     };
+    SmpFour f[4];
+    if (n > SMP_KEEP) {
 #pragma unroll
-    for (int j = 0; j < SMP_KEEP; ++j)
-        if (lo + wv + SMP_WAVES * j < hi) second(keep[j]);
-#pragma unroll 2
-    for (int sub = lo + wv + SMP_WAVES * SMP_KEEP; sub < hi; sub += SMP_WAVES) second(smp_load(x, vocab, sub, lane, wide));
-    __syncthreads();
-    for (int i = tid; i < SMP_BINS; i += SMP_THREADS) {
-        sc.mass[(size_t)blockIdx.x * SMP_BINS + i] = mass[i];
-        if (counts) sc.count[(size_t)blockIdx.x * SMP_BINS + i] = count[i];
+        for (int i = 0; i < 4; ++i) f[i] = load(SMP_KEEP + i);
     }
+#pragma unroll
+    for (int j = 0; j < SMP_KEEP; ++j) second(keep[j], j);
+    for (int j = SMP_KEEP; j < n; j += 4) {
+        SmpFour ahead[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ahead[i] = load(j + 4 + i);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            smp_cut<WIDE>(f[i], vocab, min(nth(j + i), hi - 1), lane);
+            second(f[i], j + i);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = ahead[i];
+    }
+    __syncthreads();
+    sc.mass[(size_t)blockIdx.x * SMP_BINS + tid] = mass[tid];
+    if (counts) sc.count[(size_t)blockIdx.x * SMP_BINS + tid] = count[tid];
 }
 
-// Sum over the threads up to and with this one; `sh` holds one value a wave.
+// Sum over the threads up to and with this one; `sh` holds one value a wave.  Inside a wave: shifts by 1, 2, 4 and 8
+// in rows of 16 lanes, then the rows' last lanes into the rows behind them.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t smp_from(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t smp_from(uint64_t v) {
+    return (uint64_t)smp_from<CTRL, ROWS>((uint32_t)v) | (uint64_t)smp_from<CTRL, ROWS>((uint32_t)(v >> 32)) << 32;
+}
 template <typename V>
 __device__ __forceinline__ V smp_scan(V v, V* sh) {
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const V up = __shfl_up(v, d, 64);
-        if (lane >= d) v += up;
-    }
+    v += smp_from<0x111, 0xF>(v);
+    v += smp_from<0x112, 0xF>(v);
+    v += smp_from<0x114, 0xF>(v);
+    v += smp_from<0x118, 0xF>(v);
+    v += smp_from<0x142, 0xA>(v);
+    v += smp_from<0x143, 0xC>(v);
     __syncthreads();
     if (lane == 63) sh[wv] = v;
     __syncthreads();
     V before = 0;
-    for (int w = 0; w < wv; ++w) before += sh[w];
+#pragma unroll
+    for (int w = 0; w < SMP_WAVES; ++w) before += w < wv ? sh[w] : 0;
     return before + v;
 }
 
 struct SmpRow {
     const float* x;
-    int vocab, subs;
-    bool wide;
+    int vocab;
     SmpScale c;
 };
 struct SmpShared {
@@ -219,25 +299,28 @@ struct SmpShared {
     uint64_t m[SMP_SMALL];
     uint32_t digit_n[SMP_SMALL];
     uint16_t need[1024];        // subsets that may hold wanted entries
-    uint32_t wanted[SMP_BINS / 32];
-    uint64_t wave[SMP_WAVES];
+    uint64_t wave[SMP_WAVES], before[2];
     uint64_t found, found_m;
-    int n, n_need, n_match, overflow;
+    int n, n_need, n_match, overflow, hit[2];
 };
 
-__device__ __forceinline__ double smp_edge(int g) { return exp(-(double)g / SMP_PER_UNIT); }  // weight at the bin's upper end
-// First bin whose running weight exceeds t (the last one with weight if none does): a bin with weight, whatever t is.
-__device__ __forceinline__ int smp_find(const SmpShared& S, double t) {
-    const double all = (double)S.mass[SMP_BINS - 1];
-    const bool none = !(all > t);
-    int lo = 0, hi = SMP_BINS - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        const double m = (double)S.mass[mid];
-        if (none ? m >= all : m > t) hi = mid;
-        else lo = mid + 1;
+__device__ __forceinline__ double smp_middle(int g) { return exp(-(double)g / SMP_PER_UNIT); }  // weight at the bin's middle
+// First bin whose running weight exceeds t0 (t1): the last one with weight if none does.  Thread t holds the running
+// weight with and before bin t, and that of all.
+struct SmpMine {
+    double before, with, all;
+};
+__device__ __forceinline__ void smp_find(SmpShared& S, const SmpMine& v, double t0, double t1, int& g0, int& g1) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const double t = i ? t1 : t0;
+        const bool none = !(v.all > t);
+        if (none ? v.before < v.all && v.with >= v.all : v.before <= t && v.with > t) S.hit[i] = threadIdx.x;
     }
-    return lo;
+    __syncthreads();
+    g0 = S.hit[0];
+    g1 = S.hit[1];
 }
 __device__ __forceinline__ double smp_before(const SmpShared& S, int g) { return g ? (double)S.mass[g - 1] : 0.0; }
 
@@ -248,9 +331,8 @@ __device__ __forceinline__ void smp_each(const SmpShared& S, const SmpRow& r, F 
     uint64_t m;
     if (!S.overflow) {
         for (int i = threadIdx.x; i < S.n; i += SMP_THREADS) {
-            const uint64_t c = S.list[i];
-            const uint32_t k = (uint32_t)(c >> SMP_IDX_BITS);
-            if (smp_bin(r.c, __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k), g, m)) f(c, g, m);
+            const uint64_t c = S.list[i];  // (0 has the value of a NaN)
+            if (smp_bin(r.c, smp_value(c), g, m)) f(c, g, m);
         }
         return;
     }
@@ -260,88 +342,109 @@ __device__ __forceinline__ void smp_each(const SmpShared& S, const SmpRow& r, F 
     }
 }
 
+// Ends in the n <= SMP_SMALL entries of S.place and S.m, `sum0` and `rank0` before them: as smp_end.
+template <bool COUNT>
+__device__ __forceinline__ void smp_end_few(SmpShared& S, int n, double t, uint64_t sum0, uint64_t rank0) {
+    if ((int)threadIdx.x >= n) return;
+    const uint64_t mine = S.place[threadIdx.x], w = S.m[threadIdx.x];
+    uint64_t sum = sum0, rank = rank0;
+    for (int i = 0; i < n; ++i) {
+        const bool before = S.place[i] >= mine;
+        sum += before ? S.m[i] : 0;
+        rank += before;
+    }
+    const bool passes = COUNT ? (double)rank >= t : (double)sum > t;
+    const bool passed = COUNT ? (double)(rank - 1) >= t : (double)(sum - w) > t;
+    if ((passes && !passed) || (!passes && rank == rank0 + n)) {
+        S.found = mine;
+        S.found_m = sum;
+    }
+}
+
 // In bin b (one with entries): the first entry in the order at which the running weight exceeds t (COUNT: the t-th
 // entry, from 1), the bin's last one if none does.  Its place, and the bin's weight up to and with it.  All threads.
+// Up to 64 entries count those before them; more are first split into 1024 steps of the bin; where one of these holds
+// more than SMP_SMALL (a flat row, ties), digit by digit over the places.
 template <bool COUNT>
 __device__ uint64_t smp_end(SmpShared& S, const SmpRow& r, int b, double t, uint64_t& upto) {
     const int tid = threadIdx.x;
     t = fmax(t, COUNT ? 1.0 : 0.0);
-    __syncthreads();
-    if (tid == 0) S.n_match = 0;
-    __syncthreads();
-    smp_each(S, r, [&](uint64_t c, int g, uint64_t m) {
-        if (g != b) return;
-        const int at = atomicAdd(&S.n_match, 1);
-        if (at < SMP_SMALL) {
-            S.place[at] = c;
-            S.m[at] = m;
-        }
-    });
-    __syncthreads();
-    const int n = S.n_match;
-    if (n <= SMP_SMALL) {  // every entry sums those before it
-        if (tid < n) {
-            const uint64_t mine = S.place[tid];
-            uint64_t sum = 0, rank = 0;
-            for (int i = 0; i < n; ++i) {
-                const bool before = S.place[i] >= mine;
-                sum += before ? S.m[i] : 0;
-                rank += before;
-            }
-            const bool passes = COUNT ? (double)rank >= t : (double)sum > t;
-            const bool passed = COUNT ? (double)(rank - 1) >= t : (double)(sum - S.m[tid]) > t;
-            if ((passes && !passed) || (!passes && rank == (uint64_t)n)) {
-                S.found = mine;
-                S.found_m = sum;
-            }
-        }
+    auto collect = [&](int step) {  // the bin's entries (of one step) into place and m, SMP_SMALL at most
         __syncthreads();
-        upto = S.found_m;
-        return S.found;
-    }
-    // many entries in one bin (a flat row, ties): digit by digit over the places
-    uint64_t prefix = 0, before = 0, before_n = 0;
-    for (int level = 0; level < SMP_LEVELS; ++level) {
-        const int shift = (SMP_LEVELS - 1 - level) * SMP_DIGIT;
+        if (tid == 0) S.n_match = 0;
+        __syncthreads();
+        smp_each(S, r, [&](uint64_t c, int g, uint64_t m) {
+            if (g != b || (step >= 0 && smp_inside(r.c, smp_value(c)) != step)) return;
+            const int at = atomicAdd(&S.n_match, 1);
+            if (at < SMP_SMALL) {
+                S.place[at] = c;
+                S.m[at] = m;
+            }
+        });
+        __syncthreads();
+        return S.n_match;
+    };
+    // sums over 1024 classes of entries, class `of` each (< 0: not in question): the class in which it ends
+    uint64_t sum0 = 0, rank0 = 0;
+    auto split = [&](auto of) {
         __syncthreads();
         S.m[tid] = 0;
         S.digit_n[tid] = 0;
+        if (tid == 0) S.hit[0] = -1;
         __syncthreads();
         smp_each(S, r, [&](uint64_t c, int g, uint64_t m) {
-            if (g != b || (level > 0 && (c >> (shift + SMP_DIGIT)) != prefix)) return;
-            const int d = SMP_THREADS - 1 - ((int)(c >> shift) & (SMP_THREADS - 1));  // largest first
+            const int d = g == b ? of(c) : -1;
+            if (d < 0) return;
             atomicAdd((unsigned long long*)&S.m[d], (unsigned long long)m);
             atomicAdd(&S.digit_n[d], 1u);
         });
         __syncthreads();
-        const uint64_t m = S.m[tid], c = S.digit_n[tid];
-        const uint64_t sum = before + smp_scan<unsigned long long>(m, (unsigned long long*)S.wave);
+        const uint64_t m = S.m[tid], n = S.digit_n[tid];
+        const uint64_t sum = sum0 + smp_scan<uint64_t>(m, S.wave);
         __syncthreads();
-        const uint64_t num = before_n + smp_scan<unsigned long long>(c, (unsigned long long*)S.wave);
-        const bool passes = COUNT ? (double)num >= t : (double)sum > t;
-        const bool passed = COUNT ? (double)(num - c) >= t : (double)(sum - m) > t;
+        const uint64_t rank = rank0 + smp_scan<uint32_t>((uint32_t)n, (uint32_t*)S.wave);
+        const bool passes = COUNT ? (double)rank >= t : (double)sum > t;
+        const bool passed = COUNT ? (double)(rank - n) >= t : (double)(sum - m) > t;
+        if (n && !passed) atomicMax(&S.hit[0], passes ? SMP_THREADS : tid);  // the last class, if none passes
         __syncthreads();
-        if (tid == 0) S.n_match = -1;
-        __syncthreads();
-        if (c && !passed) atomicMax(&S.n_match, passes ? SMP_THREADS : tid);  // the last digit, if none passes
-        __syncthreads();
-        const int last = S.n_match;
-        __syncthreads();
-        if (c && !passed && (last == SMP_THREADS ? passes : tid == last)) {
-            S.found = (uint64_t)(SMP_THREADS - 1 - tid);
-            S.place[0] = sum - m;
-            S.place[1] = num - c;
+        const int last = S.hit[0];
+        if (n && !passed && (last == SMP_THREADS ? passes : tid == last)) {
+            S.found = (uint64_t)tid;
             S.found_m = sum;
+            S.before[0] = sum - m;
+            S.before[1] = rank - n;
         }
         __syncthreads();
-        prefix = (prefix << SMP_DIGIT) | S.found;
-        before = S.place[0];
-        before_n = S.place[1];
+        sum0 = S.before[0];
+        rank0 = S.before[1];
+        return (int)S.found;
+    };
+    int n = collect(-1);
+    if (n > 64) {
+        const int step = split([&](uint64_t c) { return smp_inside(r.c, smp_value(c)); });
+        n = collect(step);
+        if (n > SMP_SMALL) {
+            uint64_t prefix = 0;
+            sum0 = rank0 = 0;
+            for (int level = 0; level < SMP_LEVELS; ++level) {
+                const int shift = (SMP_LEVELS - 1 - level) * SMP_DIGIT;
+                const int d = split([&](uint64_t c) {
+                    return level > 0 && (c >> (shift + SMP_DIGIT)) != prefix
+                               ? -1 : SMP_THREADS - 1 - ((int)(c >> shift) & (SMP_THREADS - 1));  // largest first
+                });
+                prefix = (prefix << SMP_DIGIT) | (uint64_t)(SMP_THREADS - 1 - d);
+            }
+            upto = S.found_m;
+            return prefix;
+        }
     }
+    smp_end_few<COUNT>(S, n, t, sum0, rank0);
+    __syncthreads();
     upto = S.found_m;
-    return prefix;
+    return S.found;
 }
 
+template <bool WIDE>
 __global__ __launch_bounds__(SMP_THREADS) void sample_draw_kernel(const float* __restrict__ logits, int vocab,
                                                                   const float* __restrict__ temperature,
                                                                   const int* __restrict__ top_k,
@@ -350,7 +453,8 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_draw_kernel(const float* _
                                                                   const double* __restrict__ u, int* __restrict__ tokens,
                                                                   uint8_t* scratch, int blocks, int subs) {
     __shared__ SmpShared S;
-    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+    const int row = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
+    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const SmpScratch sc = smp_scratch(scratch, row, blocks, subs);
     const float T = temperature ? temperature[row] : 1.f;
     float top = sc.max[0];
@@ -358,23 +462,23 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_draw_kernel(const float* _
     SmpRow r;
     r.x = logits + (size_t)row * vocab;
     r.vocab = vocab;
-    r.subs = subs;
-    r.wide = (reinterpret_cast<uintptr_t>(r.x) & 15) == 0;
     if (!(top > -INFINITY)) {  // nothing to draw from
-        if (tid == 0) tokens[row] = -1;
+        if (tid == 0 && blockIdx.x == 0) tokens[row] = -1;
         return;
     }
     if (!(T > 0.f)) {  // greedy: the first subset with the maximum, its first entry
+        if (blockIdx.x > 0) return;
         if (tid == 0) S.n = subs;
         __syncthreads();
         for (int s = tid; s < subs; s += SMP_THREADS)
             if (sc.sub[s] == top) atomicMin(&S.n, s);
         __syncthreads();
         if (wv == 0) {
-            const SmpFour f = smp_load(r.x, vocab, S.n, lane, r.wide);
+            SmpFour f = smp_load<WIDE>(r.x, vocab, S.n, lane);
+            smp_cut<WIDE>(f, vocab, S.n, lane);
             int at = vocab;
 #pragma unroll
-            for (int e = 3; e >= 0; --e) at = f.x[e] == top ? min(at, f.i[e]) : at;
+            for (int e = 3; e >= 0; --e) at = f.x[e] == top ? min(at, smp_at<WIDE>(S.n, lane, e)) : at;
             for (int d = 1; d < 64; d *= 2) at = min(at, __shfl_xor(at, d, 64));
             if (lane == 0) tokens[row] = at;
         }
@@ -382,40 +486,47 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_draw_kernel(const float* _
     }
     r.c = smp_scale(top, T);
     const int k = top_k ? top_k[row] : 0;
+    const double uu = fmin(fmax(u[row], 0.0), 1.0);  // NaN: 0
     const double p = top_p ? (double)top_p[row] : 1.0, mp = min_p ? (double)min_p[row] : 0.0;
     const bool has_k = k > 0, has_p = p > 0.0 && p < 1.0, has_m = mp > 0.0;
 
-    // ---- the row's bins: thread t sums bins 2 t and 2 t + 1 over the parts ----
-    uint64_t m[2] = {0, 0};
-    uint32_t n[2] = {0, 0};
-    for (int i = 0; i < blocks; ++i) {
-        const float part = sc.max[i];
-        if (!(part > -INFINITY)) continue;
-        const double d = part == top ? 0.0 : r.c.top - floor((double)part * r.c.s);  // bins between their first ones
-        if (!(d < (double)SMP_BINS)) continue;
+    // ---- the row's bins: thread t sums bin t over the parts, all of them requested together ----
+    uint64_t m = 0;
+    uint32_t n = 0;
+    {
+        uint64_t mm[SMP_SPLIT];
+        uint32_t nn[SMP_SPLIT];
+        int at[SMP_SPLIT];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int g = 2 * tid + e - (int)d;
-            if (g < 0) continue;
-            m[e] += sc.mass[(size_t)i * SMP_BINS + g];
-            if (has_k) n[e] += sc.count[(size_t)i * SMP_BINS + g];
+        for (int i = 0; i < SMP_SPLIT; ++i) {
+            const float part = i < blocks ? sc.max[i] : -INFINITY;
+            at[i] = part > -INFINITY ? tid - smp_apart(r.c, part) : -1;
+            const size_t o = (size_t)(i < blocks ? i : 0) * SMP_BINS + max(at[i], 0);
+            mm[i] = sc.mass[o];
+            nn[i] = has_k ? sc.count[o] : 0;
         }
+#pragma unroll
+        for (int i = 0; i < SMP_SPLIT; ++i)
+            if (at[i] >= 0) {
+                m += mm[i];
+                n += nn[i];
+            }
     }
+    SmpMine mine;
     {
         // whole numbers again, so that running sums do not fall and an empty bin adds nothing
-        const unsigned long long a = (unsigned long long)rint((double)m[0] * smp_edge(2 * tid));
-        const unsigned long long b = (unsigned long long)rint((double)m[1] * smp_edge(2 * tid + 1));
-        const unsigned long long s = smp_scan<unsigned long long>(a + b, (unsigned long long*)S.wave);
-        S.mass[2 * tid] = s - b;
-        S.mass[2 * tid + 1] = s;
+        const uint64_t w = (uint64_t)rint((double)m * smp_middle(tid));
+        const uint64_t sum = smp_scan<uint64_t>(w, S.wave);
+        mine.before = (double)(sum - w);
+        mine.with = (double)sum;
+        S.mass[tid] = sum;
         if (has_k) {
             __syncthreads();
-            const uint32_t c = smp_scan<uint32_t>(n[0] + n[1], (uint32_t*)S.wave);
-            S.count[2 * tid] = c - n[1];
-            S.count[2 * tid + 1] = c;
+            const uint32_t c = smp_scan<uint32_t>(n, (uint32_t*)S.wave);
+            S.count[tid] = c;
+            if (c - n < (uint32_t)k && c >= (uint32_t)k) S.hit[0] = tid;
         }
     }
-    for (int i = tid; i < SMP_BINS / 32; i += SMP_THREADS) S.wanted[i] = 0;
     if (tid == 0) {
         S.n = 0;
         S.n_need = 0;
@@ -424,28 +535,22 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_draw_kernel(const float* _
     __syncthreads();
 
     // ---- in which bins the filters and the draw may end ----
-    const double all = (double)S.mass[SMP_BINS - 1];
-    double z_lo = all, z_hi = all;  // mass of the top-k
+    mine.all = (double)S.mass[SMP_BINS - 1];
+    double z_lo = mine.all, z_hi = mine.all;  // mass of the top-k
     int kb = -1;
     if (has_k && (uint32_t)k < S.count[SMP_BINS - 1]) {
-        int lo = 0, hi = SMP_BINS - 1;  // first bin whose running count reaches k
-        while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            if (S.count[mid] >= (uint32_t)k) hi = mid;
-            else lo = mid + 1;
-        }
-        z_hi = (double)S.mass[lo];
+        const int g = S.hit[0];  // the first bin whose running count reaches k
+        z_hi = (double)S.mass[g];
         z_lo = z_hi;
-        if (S.count[lo] != (uint32_t)k) {
-            kb = lo;
-            z_lo = smp_before(S, lo);
+        if (S.count[g] != (uint32_t)k) {
+            kb = g;
+            z_lo = smp_before(S, g);
         }
     }
     int last = kb, p0 = 0, p1 = -1, m0 = 0, m1 = -1;
     double k_lo = z_lo, k_hi = z_hi;  // kept mass
     if (has_p) {
-        p0 = smp_find(S, p * z_lo);
-        p1 = z_lo == z_hi ? p0 : smp_find(S, p * z_hi);
+        smp_find(S, mine, p * z_lo, p * z_hi, p0, p1);
         k_lo = fmin(k_lo, smp_before(S, p0));
         k_hi = fmin(k_hi, (double)S.mass[p1]);
         last = max(last, p1);
@@ -455,55 +560,99 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_draw_kernel(const float* _
         int g = 0;
         uint64_t w = 0;
         smp_bin(r.c, top, g, w);
-        floor_w = fmin(mp, 1.0) * (double)w;  // in units of 2^-44 of bin 0's upper end
-        const double y = (log(SMP_ONE) - log(floor_w)) * SMP_PER_UNIT;
+        floor_w = fmin(mp, 1.0) * (double)w;  // in units of 2^-44 of bin 0's middle
+        const double y = (log(SMP_ONE) - log(floor_w)) * SMP_PER_UNIT + 0.5;
         m0 = (int)fmin(fmax(floor(y - 1e-6), 0.0), (double)(SMP_BINS - 1));
         m1 = (int)fmin(fmax(floor(y + 1e-6), 0.0), (double)(SMP_BINS - 1));
         k_lo = fmin(k_lo, smp_before(S, m0));
         k_hi = fmin(k_hi, (double)S.mass[m1]);
         last = max(last, m1);
     }
-    const double uu = fmin(fmax(u[row], 0.0), 1.0);  // NaN: 0
     // the draw lies before the end of the kept mass even where u is 1
     auto drawn = [&](double mass) { return fmin(uu * mass, mass * (1.0 - 1e-15)); };
-    const int u0 = smp_find(S, drawn(k_lo)), u1 = k_lo == k_hi ? u0 : smp_find(S, drawn(k_hi));
+    int u0, u1;
+    smp_find(S, mine, drawn(k_lo), drawn(k_hi), u0, u1);
     last = max(last, u1);
-    auto want = [&](int a, int b) {
-        for (int g = a + tid; g <= b; g += SMP_THREADS) atomicOr(&S.wanted[g >> 5], 1u << (g & 31));
+    // as ranges of values in fp32, wider than the bins by more than its roundings: what else they hold goes by bin later
+    const double y_top = rint((double)top * r.c.s), unit = (double)T / SMP_PER_UNIT;
+    struct Range {
+        float low, high;
     };
-    if (kb >= 0) want(kb, kb);
-    want(p0, p1);
-    want(m0, m1);
-    want(u0, u1);
+    auto want = [&](int a, int b) {
+        const double lo = (y_top - (double)b - 0.5) * unit, hi = (y_top - (double)a + 0.5) * unit;
+        Range w;
+        w.low = a > b ? INFINITY : r.c.whole ? (float)(lo - 1e-6 * fabs(lo)) : -INFINITY;
+        w.high = a > b ? -INFINITY : r.c.whole ? (float)(hi + 1e-6 * fabs(hi)) : INFINITY;
+        return w;
+    };
+    const Range wk = want(max(kb, 0), kb), wp = want(p0, p1), wm = want(m0, m1), wu = want(u0, u1);
     // ---- collect their entries, from the subsets whose largest one is not behind the last of these bins ----
-    for (int s = tid; s < subs; s += SMP_THREADS) {
+    const int s0 = (int)((long long)subs * blockIdx.x / gridDim.x), s1 = (int)((long long)subs * (blockIdx.x + 1) / gridDim.x);
+    for (int s = s0 + tid; s < s1; s += SMP_THREADS) {  // (at most one a thread)
         int g;
         uint64_t w;
         if (smp_bin(r.c, sc.sub[s], g, w) && g <= last) S.need[atomicAdd(&S.n_need, 1)] = (uint16_t)s;
     }
     __syncthreads();
-    auto take = [&](const SmpFour& f) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            int g = 0;
-            uint64_t w;
-            const bool in = smp_bin(r.c, f.x[e], g, w) && (S.wanted[g >> 5] >> (g & 31) & 1);
-            const uint64_t ask = __ballot(in);
-            if (ask == 0) continue;
-            int at = 0;
-            if (lane == 0) at = atomicAdd(&S.n, __popcll(ask));
-            at = __shfl(at, 0, 64) + __popcll(ask & ((1ull << lane) - 1));
-            if (in && at < SMP_LIST) S.list[at] = smp_place(f.x[e], f.i[e]);
-        }
+    const int n_need = S.n_need;
+    SmpFour f[4];  // four subsets a wave and round, the next round's requested ahead
+    auto fetch = [&](int i, int j) {
+        return smp_load<WIDE>(r.x, vocab, S.need[min(i + j * SMP_WAVES, n_need - 1)], lane);
     };
-    for (int i = wv; i < S.n_need; i += 4 * SMP_WAVES) {
-        SmpFour f[4];
+    if (n_need > 0) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[j] = fetch(wv, j);
+    }
+    for (int i = wv; i < n_need; i += 4 * SMP_WAVES) {
+        uint32_t in = 0;  // bit 4 j + e: entry e of subset j
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            if (i + j * SMP_WAVES < S.n_need) f[j] = smp_load(r.x, vocab, S.need[i + j * SMP_WAVES], lane, r.wide);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (i + j * SMP_WAVES < S.n_need) take(f[j]);
+            for (int e = 0; e < 4; ++e) {
+                const float x = f[j].x[e];
+                bool y = x >= wu.low && x <= wu.high;
+                if (has_p) y = y || (x >= wp.low && x <= wp.high);
+                if (kb >= 0) y = y || (x >= wk.low && x <= wk.high);
+                if (has_m) y = y || (x >= wm.low && x <= wm.high);
+                in |= y ? 1u << (4 * j + e) : 0u;
+            }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[j] = fetch(i + 4 * SMP_WAVES, j);
+#pragma unroll
+        for (int j = 1; j < 4; ++j)
+            if (i + j * SMP_WAVES >= n_need) in &= (1u << (4 * j)) - 1;  // the last subset again
+        int at = in ? atomicAdd(&S.n, __popc(in)) : 0;
+        while (in) {
+            const int b = __ffs(in) - 1, idx = smp_at<WIDE>(S.need[i + (b >> 2) * SMP_WAVES], lane, b & 3);
+            in &= in - 1;
+            if (at < SMP_LIST) S.list[at] = (uint64_t)min(idx, vocab);  // vocab: nothing
+            ++at;
+        }
+    }
+    __syncthreads();
+    if (gridDim.x > 1) {  // all blocks' entries together; the last one goes on with them
+        const int n = S.n;
+        if (tid == 0) S.hit[0] = atomicAdd(&sc.shared[0], n);
+        __syncthreads();
+        const int at = S.hit[0];
+        for (int i = tid; i < min(n, SMP_LIST); i += SMP_THREADS)
+            if (at + i < SMP_LIST)
+                __hip_atomic_store(&sc.list[at + i], (uint32_t)S.list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        // device-coherent stores, waited for by each wave before the block is counted, and device-coherent loads by the
+        // last block: no cache is written back (fences on both sides took 7 us more)
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (tid == 0) S.hit[1] = atomicAdd(&sc.shared[1], 1);
+        __syncthreads();
+        if (S.hit[1] != (int)gridDim.x - 1) return;
+        if (tid == 0) S.n = __hip_atomic_load(&sc.shared[0], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        for (int i = tid; i < min(S.n, SMP_LIST); i += SMP_THREADS)
+            S.list[i] = __hip_atomic_load(&sc.list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    for (int i = tid; i < min(S.n, SMP_LIST); i += SMP_THREADS) {
+        const int idx = (int)S.list[i];
+        S.list[i] = idx < vocab ? smp_place(r.x[idx], idx) : 0;
     }
     __syncthreads();
     if (tid == 0 && S.n > SMP_LIST) S.overflow = 1;
@@ -514,19 +663,20 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_draw_kernel(const float* _
     double z = z_hi;
     if (kb >= 0) {
         smp_end<true>(S, r, kb, (double)((uint32_t)k - (kb ? S.count[kb - 1] : 0)), upto);
-        z = fmin(fmax(smp_before(S, kb) + (double)upto * smp_edge(kb), z_lo), z_hi);  // roundings apart it lies there
+        z = fmin(fmax(smp_before(S, kb) + (double)upto * smp_middle(kb), z_lo), z_hi);  // roundings apart it lies there
     }
     double kept = z;
     if (has_p) {
-        const int b = smp_find(S, p * z);
-        smp_end<false>(S, r, b, (p * z - smp_before(S, b)) / smp_edge(b), upto);
-        kept = fmin(kept, smp_before(S, b) + (double)upto * smp_edge(b));
+        int b = p0, same;
+        if (p0 != p1) smp_find(S, mine, p * z, p * z, b, same);
+        smp_end<false>(S, r, b, (p * z - smp_before(S, b)) / smp_middle(b), upto);
+        kept = fmin(kept, smp_before(S, b) + (double)upto * smp_middle(b));
     }
     if (has_m) {  // the weights in bins m0 and m1 that reach the least one
         __syncthreads();
         if (tid < 2) S.m[tid] = 0;
         __syncthreads();
-        const double e0 = smp_edge(m0), e1 = smp_edge(m1);
+        const double e0 = smp_middle(m0), e1 = smp_middle(m1);
         smp_each(S, r, [&](uint64_t, int g, uint64_t w) {
             if ((g == m0 && (double)w * e0 >= floor_w) || (g == m1 && (double)w * e1 >= floor_w))
                 atomicAdd((unsigned long long*)&S.m[g == m0 ? 0 : 1], (unsigned long long)w);
@@ -535,14 +685,17 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_draw_kernel(const float* _
         kept = fmin(kept, smp_before(S, m0) + (double)S.m[0] * e0 + (double)S.m[1] * e1);
     }
     const double t = drawn(fmin(fmax(kept, k_lo), k_hi));
-    const int b = smp_find(S, t);
-    const uint64_t place = smp_end<false>(S, r, b, (t - smp_before(S, b)) / smp_edge(b), upto);
+    int b = u0, same;
+    if (u0 != u1) smp_find(S, mine, t, t, b, same);
+    const uint64_t place = smp_end<false>(S, r, b, (t - smp_before(S, b)) / smp_middle(b), upto);
     if (tid == 0) tokens[row] = smp_index(place);
 }
 
 namespace vte {
 // Blocks of a row: enough that two of 1024 threads lie on every CU.
 static int sample_blocks(int rows) { return std::max(1, std::min(SMP_SPLIT, 2 * device_cus() / rows)); }
+// Blocks that share the reading of a row, while they fit on the CUs at once.
+static int draw_blocks(int rows) { return std::max(1, std::min(16, device_cus() / rows)); }
 
 long long sample_scratch_bytes(int rows) {
     return (long long)rows * (long long)smp_row_bytes(sample_blocks(rows), (1 << SMP_IDX_BITS) / SMP_SUB);
@@ -551,12 +704,16 @@ hipError_t sample(const float* logits, int rows, int vocab, const float* tempera
                   const float* top_p, const float* min_p, const double* u, int* tokens, void* scratch,
                   hipStream_t st) {
     const int subs = (vocab + SMP_SUB - 1) / SMP_SUB, blocks = std::min(sample_blocks(rows), subs);
-    hipLaunchKernelGGL(sample_bins_kernel, dim3(blocks, rows), dim3(SMP_THREADS), 0, st, logits, vocab, temperature,
-                       top_k, (uint8_t*)scratch, subs);
+    const bool wide = vocab % 4 == 0 && (reinterpret_cast<uintptr_t>(logits) & 15) == 0;
+    auto bins = wide ? sample_bins_kernel<true> : sample_bins_kernel<false>;
+    auto draw = wide ? sample_draw_kernel<true> : sample_draw_kernel<false>;
+    hipLaunchKernelGGL(bins, dim3(blocks, rows), dim3(SMP_THREADS), 0, st, logits, vocab, temperature, top_k,
+                       (uint8_t*)scratch, subs);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(sample_draw_kernel, dim3(rows), dim3(SMP_THREADS), 0, st, logits, vocab, temperature, top_k,
-                       top_p, min_p, u, tokens, (uint8_t*)scratch, blocks, subs);
+    const int share = std::min(draw_blocks(rows), subs);
+    hipLaunchKernelGGL(draw, dim3(share, rows), dim3(SMP_THREADS), 0, st, logits, vocab, temperature, top_k, top_p, min_p, u,
+                       tokens, (uint8_t*)scratch, blocks, subs);
     return hipGetLastError();
 }
 }  // namespace vte
