@@ -110,8 +110,8 @@ class KVRows(ctypes.Structure):
 
 def _p(x) -> Optional[int]:
     """Device pointer argument: int, c_void_p, an object with ``.ptr`` or None."""
-    if x is None:
-        return None
+    if x is None or type(x) is int:  # (first: most calls of a step pass plain addresses)
+        return x
     if isinstance(x, ctypes.c_void_p):
         return x.value
     if hasattr(x, "ptr"):
