@@ -326,6 +326,20 @@ def test_attention_prompts(hip, K, dtype, n_q, n_kv, hd, page):
     check_attention(hip, K, bt, old, new, n_q, dtype, rng, pad=2)
 
 
+@pytest.mark.parametrize("dtype,n_q,n_kv,hd", [("f16", 16, 4, 128), ("f32", 24, 4, 64), ("f16", 8, 4, 64),
+                                               ("f32", 12, 4, 128)])
+def test_attention_many_prompts(hip, K, dtype, n_q, n_kv, hd):
+    """140 sequences with 0 to 90 new rows each: more row blocks than two a CU, so the wider ones."""
+    rng = np.random.default_rng(hd + n_q)
+    new = [int(x) for x in rng.integers(0, 6, 140)]
+    new[3], new[77] = 90, 33
+    old = [int(x) for x in rng.integers(0, 30, 140)]
+    old[50], old[77] = 400, 131
+    bt = filled(hip, K, rng, [a + b for a, b in zip(old, new)], n_kv, hd, 32)
+    old[9] = -1
+    check_attention(hip, K, bt, old, new, n_q, dtype, rng, pad=1)
+
+
 @pytest.mark.parametrize("new", [1, 40])
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
 def test_attention_holes_and_empty_rows(hip, K, dtype, new):

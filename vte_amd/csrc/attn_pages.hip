@@ -12,8 +12,6 @@
 // byte 0..255 of a masked token times probability 0 is the only thing a place that
 // nobody sees can add: its exponent, which may be anything, is never used.
 #include <algorithm>
-#include <type_traits>
-
 #include "attn_tile.h"
 #include "kv_pages.h"
 
@@ -24,7 +22,24 @@
 typedef _Float16 pa_h2 __attribute__((ext_vector_type(2)));
 typedef unsigned pa_u2 __attribute__((ext_vector_type(2)));
 
-// 8 bytes as 8 fp16 whole numbers (byte - 128).
+// 8 bytes as 8 fp16 whole numbers (byte - 128), or `by` times them (one rounded operation; exact for a power of two
+// from 2^-24 on).
+__device__ __forceinline__ half8_t pa_half8(uint32_t a, uint32_t b, _Float16 by) {
+    union {
+        uint32_t u[4];
+        pa_h2 h[4];
+        half8_t v;
+    } r;
+    r.u[0] = __builtin_amdgcn_perm(0x64646464u, a, 0x04010400u);
+    r.u[1] = __builtin_amdgcn_perm(0x64646464u, a, 0x04030402u);
+    r.u[2] = __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u);
+    r.u[3] = __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u);
+    const _Float16 z = (_Float16)-1152.f * by;
+    const pa_h2 f = {by, by}, m = {z, z};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.h[i] = __builtin_elementwise_fma(r.h[i], f, m);
+    return r.v;
+}
 __device__ __forceinline__ half8_t pa_half8(uint32_t a, uint32_t b) {
     union {
         uint32_t u[4];
@@ -432,419 +447,449 @@ __global__ __launch_bounds__(256) void attn_pages_combine_kernel(KvPages c, KvRo
 
 // ---------------------------------------------------------------------------
 // Many rows.  Rows of a KV head are numbered (new row, query head of the group),
-// so a group of any size fills 32-row MFMA tiles; 128 of them are a row block and
-// see tokens up to their last row's position.  A segment is (KV head, row block);
-// shares of 64-token steps are cut as above, from a plan that a first launch
-// writes (row blocks of a ragged batch and the steps before each).
+// so a group of any size fills 32-row MFMA tiles; 256 or 128 of them are a row
+// block and see tokens up to their last row's position, in steps of 64.  One block
+// of threads takes a row block, or while these are fewer than the CUs one of nsp
+// equal shares of its steps (joined by a second launch).
 //
-// A block's four waves own 32 rows each and walk the same steps.  The bytes of a
-// step become fp16 once per block on their way into LDS, times 2^(e - ref) with
-// ref the largest exponent so far (exact down to 2^-24 of the largest block's
+// The block's eight waves hold 32 rows each (GROUPS = 1), or are two groups of
+// four that take every other step and whose sums meet in LDS at the end (GROUPS =
+// 2: half as many rows, so twice as many blocks or half as many shares).  The bytes
+// of a step become fp16 once per group on their way into LDS, times 2^(e - ref)
+// with ref the largest exponent so far (exact down to 2^-24 of the largest block's
 // step), so a step's scores and sums have one scale.  Scores are K.Q^T, sums are
 // V^T.P^T (a lane is a row in both), K rows are read with token bits 2 and 3
 // swapped so that a lane's scores are its operand of the second product as they
 // stand.
 // ---------------------------------------------------------------------------
-#define PA_ROWS 128  // rows of a row block
+#define PA_SHARES 16
 
 typedef float floatx16_t __attribute__((ext_vector_type(16)));
 
+// Row block `slot` of all sequences' in their order: its sequence (-1: there are not so many) and number there.
+// One wave, sequences over its lanes.
 struct PaRowBlock {
-    int b, rb;      // sequence, row block of it
-    int steps;      // 64-token steps that its rows see
-    int before;     // steps of the row blocks before it
+    int b, rb;
+    KvSeq s;  // with n the rows of a sequence that does not run, too
 };
-struct PaStart {
-    int block, h, at, pad;  // row block, KV head and step of it that a share starts with
-};
-struct PaPrompt {
-    PaRowBlock* rb;  // [row blocks]
-    PaStart* start;  // [blocks]
-    int* total;      // row blocks, steps of one KV head, steps of a share
-};
-
-// One block: row blocks of every sequence, their steps, and where each share starts.
-__global__ __launch_bounds__(1024) void attn_pages_plan_kernel(KvPages c, KvRows r, PaPlan pl, PaPrompt pp, int n_q) {
-    __shared__ int wsum[16];
-    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-    const int G = n_q / c.n_kv, cap = kvp_capacity(c, r);
-    auto scan = [&](int mine, int& total) {  // sum over the threads before this one
-        int incl = mine;
+template <int ROWS>
+__device__ __forceinline__ PaRowBlock pa_row_block(const KvRows& r, int G, int slot) {
+    const int lane = threadIdx.x & 63;
+    PaRowBlock R;
+    R.b = -1;
+    for (int b0 = 0; b0 < r.batch; b0 += 64) {
+        const KvSeq s = kvp_place(r, min(b0 + lane, r.batch - 1));
+        const int n = b0 + lane < r.batch ? (s.n * G + ROWS - 1) / ROWS : 0;
+        int incl = n;
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) {
             const int up = __shfl_up(incl, d, 64);
             if (lane >= d) incl += up;
         }
-        __syncthreads();
-        if (lane == 63) wsum[wv] = incl;
-        __syncthreads();
-        int before = 0;
-        total = 0;
-        for (int w = 0; w < 16; ++w) {
-            before += w < wv ? wsum[w] : 0;
-            total += wsum[w];
+        const uint64_t here = __ballot(slot < incl);
+        if (here != 0) {
+            const int l = __ffsll((unsigned long long)here) - 1;
+            R.b = b0 + l;
+            R.rb = slot - __builtin_amdgcn_readlane(incl - n, l);
+            R.s.first = __builtin_amdgcn_readlane(s.first, l);
+            R.s.n = __builtin_amdgcn_readlane(s.n, l);
+            R.s.pos = __builtin_amdgcn_readlane(s.pos, l);
+            return R;
         }
-        return before + incl - mine;
-    };
-    // row blocks, in the sequences' order
-    const int per = (r.batch + 1023) / 1024;
-    int mine = 0, n_rb, steps;
-    for (int b = tid * per; b < min(r.batch, tid * per + per); ++b) mine += (kvp_place(r, b).n * G + PA_ROWS - 1) / PA_ROWS;
-    int at = scan(mine, n_rb);
-    for (int b = tid * per; b < min(r.batch, tid * per + per); ++b) {
-        const int n = (kvp_place(r, b).n * G + PA_ROWS - 1) / PA_ROWS;
-        for (int i = 0; i < n; ++i) pp.rb[at++] = PaRowBlock{b, i, 0, 0};
+        slot -= __builtin_amdgcn_readlane(incl, 63);
     }
-    __threadfence_block();
-    __syncthreads();
-    // steps of each
-    const int per2 = (n_rb + 1023) / 1024, lo = min(n_rb, tid * per2), hi = min(n_rb, lo + per2);
-    mine = 0;
-    for (int i = lo; i < hi; ++i) {
-        const int b = pp.rb[i].b;
-        const KvSeq s = kvp_place(r, b);
-        const int last = min((pp.rb[i].rb * PA_ROWS + PA_ROWS - 1) / G, s.n - 1);
-        const int n = s.pos < 0 ? 0 : ((s.pos < cap - last ? s.pos + last + 1 : cap) + PA_TILE - 1) / PA_TILE;
-        pp.rb[i].steps = n;
-        mine += n;
-    }
-    int before = scan(mine, steps);
-    const int share = max(1, (int)(((long long)steps * c.n_kv + pl.blocks - 1) / pl.blocks));
-    for (int i = lo; i < hi; ++i) {
-        const int n = pp.rb[i].steps;
-        pp.rb[i].before = before;
-        for (int h = 0; h < c.n_kv; ++h) {  // shares that start in this segment
-            const long long t0 = (long long)h * steps + before;
-            for (long long k = (t0 + share - 1) / share; k * share < t0 + n; ++k)
-                pp.start[k] = PaStart{i, h, (int)(k * share - t0), 0};
-        }
-        before += n;
-    }
-    if (tid == 0) {
-        pp.total[0] = n_rb;
-        pp.total[1] = steps;
-        pp.total[2] = share;
-    }
+    return R;
+}
+// Steps of a row block, and the steps of one of its nsp shares (even: both groups get as many).
+template <int ROWS>
+__device__ __forceinline__ int pa_steps(const PaRowBlock& R, int G, int cap) {
+    if (R.s.pos < 0) return 0;
+    const int last = min((R.rb * ROWS + ROWS - 1) / G, R.s.n - 1);
+    return ((R.s.pos < cap - last ? R.s.pos + last + 1 : cap) + PA_TILE - 1) / PA_TILE;
+}
+__device__ __forceinline__ int pa_share_of(int steps, int nsp) {
+    return nsp == 1 ? steps : ((steps + nsp - 1) / nsp + 1) / 2 * 2;
 }
 
-template <typename T, int HD>
-__global__ __launch_bounds__(256, 2) void attn_pages_prompt_kernel(KvPages c, KvRows r, PaPlan pl, PaPrompt pp,
+struct PaPrompt {
+    int nsp;    // shares of a row block
+    float* ml;  // [row blocks][n_kv][nsp][128][2]: maximum (log2), sum
+    int* ev;    // [row blocks][n_kv][nsp][4]: exponent the record's sums are relative to, per 32 rows
+    float* o;   // [row blocks][n_kv][nsp][128][HD]
+};
+
+// A row's results: dims 32 i + 8 (j / 4) + j % 4 from dst on.
+template <typename T, int N>
+__device__ __forceinline__ void pa_store(T* dst, const floatx16_t (&o)[N], float l, int ref) {
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            union {
+                T t[4];
+                uint2 u2;
+                uint4 u4[sizeof(T) / 4 < 1 ? 1 : sizeof(T) / 4];
+            } r;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) st_act<T>(&r.t[e], l == 0.f ? 0.f : ldexpf(o[i][4 * j + e] * inv, ref));
+            if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(dst + 32 * i + 8 * j) = r.u2;
+            else *reinterpret_cast<uint4*>(dst + 32 * i + 8 * j) = r.u4[0];
+        }
+}
+
+// grid (row blocks, n_kv, nsp), the last row blocks (which see most) first; nsp > 1 with two groups only.
+template <typename T, int HD, int GROUPS>
+__global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, KvRows r, PaPrompt pp,
                                                                    const T* __restrict__ q, T* __restrict__ out,
                                                                    int n_q, float scale) {
     constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;
-    constexpr int KS = HD / 16, DT = HD / 32, U = HD / 64;  // 16-dim steps of a score, 32-dim tiles, staged pieces a thread
-    constexpr int KROW = PA_TILE * 16 + 8;                  // halves of a 16-dim column of K, 16 bytes apart in banks
+    constexpr int WAVES = 8 / GROUPS, ROWS = 32 * WAVES;  // of a group
+    constexpr int KS = HD / 16, DT = HD / 32;              // 16-dim steps of a score, 32-dim tiles
+    constexpr int NP = 8 * HD / (64 * WAVES);              // 16-byte pieces of K and V a thread stages (1: waves 0..3 K, 4..7 V)
+    // A lane's operand is 16 bytes of one token (K) or dim (V); those of neighbouring tokens or dims lie side by side, so
+    // that reads touch every bank once (with a token's two pieces side by side they took twice as long).
+    constexpr int KROW = PA_TILE * 8 + 8;  // halves of 8 dims of K, 64 tokens; rows of neighbouring dims 16 bytes apart in banks
     struct alignas(16) Tile {
-        _Float16 k[KS * KROW];
-        _Float16 v[4 * HD * 16];
+        _Float16 k[2 * KS * KROW];     // [dims 8 half .. of 16][16-dim step][token][8 dims]
+        _Float16 v[4 * 2 * HD * 8];    // [block][its 8 tokens][dim][8 tokens]
     };
-    __shared__ Tile tiles[2];
-    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    union Shared {
+        Tile tiles[GROUPS][2];         // [group][buffer]
+        float o[GROUPS][GROUPS == 2 ? DT / 2 * 16 : 1][64 * WAVES];  // what a group leaves to the other
+    };
+    __shared__ Shared S;
+    __shared__ float m_sh[GROUPS][ROWS], l_sh[GROUPS][ROWS];
+    __shared__ int ev_sh[GROUPS][WAVES];
+    const int tid = threadIdx.x & (64 * WAVES - 1), lane = threadIdx.x & 63;
+    const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & (WAVES - 1);
+    const int grp = GROUPS == 2 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 8) : 0;
     const int row = lane & 31, half = lane >> 5;
     const int G = n_q / c.n_kv, cap = kvp_capacity(c, r), bl = c.page_log2 - 4;
-    const int steps = pp.total[1], share = pp.total[2];
-    const long long all = (long long)steps * c.n_kv;
-    long long t = (long long)blockIdx.x * share;
-    const long long t_end = min(all, t + share);
-    if (t >= t_end) return;
-    const PaStart st = pp.start[blockIdx.x];
-    int rbi = __builtin_amdgcn_readfirstlane(st.block), h = __builtin_amdgcn_readfirstlane(st.h);
-    int a = __builtin_amdgcn_readfirstlane(st.at);
+    const int slot = gridDim.x - 1 - blockIdx.x, h = blockIdx.y;
+    const PaRowBlock R = pa_row_block<ROWS>(r, G, slot);
+    if (R.b < 0) return;
+    const KvSeq s = R.s;
+    const int steps = pa_steps<ROWS>(R, G, cap), share = pa_share_of(steps, pp.nsp);
+    const int a = blockIdx.z * share, z = min(steps, a + share), pieces = steps ? (steps + share - 1) / share : 1;
+    if (a >= z && !(steps == 0 && blockIdx.z == 0)) return;
+    const int* table = r.page_table + (size_t)R.b * r.max_pages;
 
-    while (t < t_end) {
-        const PaRowBlock R = pp.rb[rbi];
-        const int b = __builtin_amdgcn_readfirstlane(R.b), nt = __builtin_amdgcn_readfirstlane(R.steps);
-        if (a >= nt) {  // a row block that sees nothing, or the end of this one
-            a = 0;
-            if (++rbi == pp.total[0]) {
-                rbi = 0;
-                ++h;
-            }
-            continue;
+    // ---- this lane's row ----
+    const int r0 = R.rb * ROWS + wv * 32, rows = s.n * G;
+    const int ri = min(r0 + row, rows - 1), qi = ri / G, qh = h * G + ri - qi * G;
+    T* dst = out + ((size_t)(s.first + qi) * n_q + qh) * HD;
+    if (steps == 0) {  // a sequence that does not run
+        if (r0 + row < rows && grp == 0)
+            for (int d = half * (HD / 2); d < (half + 1) * (HD / 2); ++d) st_act<T>(dst + d, 0.f);
+        return;
+    }
+    const int end = r0 + row < rows ? kvp_len(s.pos + qi, cap) : 0;
+    const int seg_end = kvp_len(s.pos + min((R.rb * ROWS + ROWS - 1) / G, s.n - 1), cap);  // of the row block
+    const int longest = r0 < rows ? kvp_len(s.pos + min(r0 + 31, rows - 1) / G, cap) : 0;       // of the wave
+    const int shortest = r0 + 31 < rows ? kvp_len(s.pos + r0 / G, cap) : 0;
+
+    // Staging: registers, then LDS.  Lane j & 3 knows block j's page and exponents; a wave's pieces lie in one block.
+    uint4 stage[NP];
+    // u: its part of K or V, the block and the first piece of it (of HD) that the wave's lanes take
+    auto is_v = [&](int u) { return NP >= 2 ? u >= NP / 2 : wv >= WAVES / 2; };
+    auto first = [&](int u) { return (NP >= 2 ? u % (NP / 2) * WAVES + wv : wv % (WAVES / 2)) * 64; };
+    int ek, ev, page;
+    bool used;
+    auto find = [&](int step) {
+        const int blk = 4 * step + (lane & 3);
+        used = step < z && blk * KVP_BLOCK < seg_end;
+        page = used ? table[blk >> bl] : -1;
+        used = used && (unsigned)page < (unsigned)c.n_pages;
+    };
+    auto load = [&](int step) {
+        const int blk = 4 * step + (lane & 3);
+        const size_t i = (((size_t)(used ? page : 0) * c.n_kv + h) << bl) + (blk & ((1 << bl) - 1));
+        ek = c.k_exp[i];
+        ev = c.v_exp[i];
+#pragma unroll
+        for (int u = 0; u < NP; ++u) {
+            const int j = first(u) / HD, p = __builtin_amdgcn_readlane(used ? page : 0, j);
+            const size_t at = (((size_t)p * c.n_kv + h) << bl) + ((4 * step + j) & ((1 << bl) - 1));
+            stage[u] = ldg_g16((is_v(u) ? c.v : c.k) + at * (KVP_BLOCK * HD) + (first(u) % HD + lane) * 16);
         }
-        const int z = (int)min((long long)nt, a + (t_end - t));
-        const KvSeq s = kvp_seq(r, b);
-        const int* table = r.page_table + (size_t)b * r.max_pages;
+    };
+    find(a + grp);
+    load(a + grp);
 
-        // ---- this lane's row ----
-        const int r0 = R.rb * PA_ROWS + wv * 32, rows = s.n * G;
-        const int ri = min(r0 + row, rows - 1), qi = ri / G, qh = h * G + ri - qi * G;
-        const int end = r0 + row < rows ? kvp_len(s.pos + qi, cap) : 0;
-        const int seg_end = kvp_len(s.pos + min((R.rb * PA_ROWS + PA_ROWS - 1) / G, s.n - 1), cap);  // of the row block
-        const int longest = r0 < rows ? kvp_len(s.pos + min(r0 + 31, rows - 1) / G, cap) : 0;       // of the wave
-        const int shortest = r0 + 31 < rows ? kvp_len(s.pos + r0 / G, cap) : 0;
-        half8_t qb[PARTS][KS];
-        float q_unit = 1.f;
+    half8_t qb[PARTS][KS];
+    float q_unit = 1.f;
+    {
+        const T* qp = q + ((size_t)(s.first + qi) * n_q + qh) * HD + 8 * half;
+        if constexpr (PARTS == 1) {
+#pragma unroll
+            for (int i = 0; i < KS; ++i) qb[0][i] = *reinterpret_cast<const half8_t*>(qp + 16 * i);
+        } else {  // scaled by a power of two so that the second part keeps its bits too
+            float amax = 0.f;
+#pragma unroll
+            for (int i = 0; i < KS; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(qp[16 * i + j]));
+            amax = fmaxf(amax, __shfl_xor(amax, 32, 64));
+            const int e = min(max((int)(__float_as_uint(amax) >> 23) - 127, -110), 126);  // 2^e <= amax
+            const float up = __uint_as_float((uint32_t)(127 + 13 - e) << 23);
+            q_unit = __uint_as_float((uint32_t)(127 - 13 + e) << 23);
+#pragma unroll
+            for (int i = 0; i < KS; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float y = qp[16 * i + j] * up;
+                    qb[0][i][j] = (_Float16)y;
+                    qb[1][i][j] = (_Float16)(y - (float)qb[0][i][j]);
+                }
+        }
+    }
+    const float c2 = scale * 1.44269504088896340736f * q_unit;
+
+    float m_run = PA_NONE, l_run = 0.f;
+    floatx16_t o[DT];  // lane: row, dims 32 dt + 8 (i / 4) + 4 half + i % 4
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
+    int o_ref = KVP_E_MIN;                              // exponent that o is relative to
+    int k_ref = KVP_E_MIN, v_ref = KVP_E_MIN;           // of the step staged last
+    int cur_k = KVP_E_MIN, cur_v = KVP_E_MIN, cur_odd = 0;  // of the step in work; its blocks without a page, NaN in V
+    int next_odd = 0;
+    auto put = [&](Tile& D) {
+        next_odd = 0;
+        int e[4], f[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const bool in = __builtin_amdgcn_readlane((int)used, j);
+            e[j] = in ? __builtin_amdgcn_readlane(ek, j) : -1000;
+            f[j] = in ? __builtin_amdgcn_readlane(ev, j) : -1000;
+            if (!in) next_odd |= 1 << j;
+            if (f[j] == KVP_E_NAN) next_odd |= 16 << j;
+            k_ref = max(k_ref, e[j]);
+            v_ref = max(v_ref, f[j]);
+        }
+#pragma unroll
+        for (int u = 0; u < NP; ++u) {
+            const int j = first(u) / HD, piece = first(u) % HD + lane;
+            int x = is_v(u) ? f[0] : e[0];
+#pragma unroll
+            for (int i = 1; i < 4; ++i) x = i == j ? (is_v(u) ? f[i] : e[i]) : x;
+            // (NaN in V is dealt with where its rows are: 0 times it would reach rows that do not see it)
+            const _Float16 by = x == KVP_E_NAN ? (_Float16)(is_v(u) ? 0.f : NAN)
+                                               : (_Float16)pa_pow2(x - (is_v(u) ? v_ref : k_ref));
+            // K piece: token piece / KS of the block, dims 16 (piece % KS) ..; V piece: dim `piece`
+            _Float16* to = is_v(u) ? D.v + (2 * j * HD + piece) * 8
+                                   : D.k + (piece % KS) * KROW + (16 * j + piece / KS) * 8;
+            *reinterpret_cast<half8_t*>(to) = pa_half8(stage[u].x, stage[u].y, by);
+            *reinterpret_cast<half8_t*>(to + (is_v(u) ? HD * 8 : KS * KROW)) = pa_half8(stage[u].z, stage[u].w, by);
+        }
+    };
+
+    // K row of 32-token tile tt: token with bits 2 and 3 of the lane's row swapped
+    const int kt = (row & 0x13) | (row & 4) << 1 | (row & 8) >> 1;
+    // `ends`: some of the wave's rows do not see all of the step, or a block of it has no page or NaN in V
+    auto work = [&](const Tile& D, int step, bool ends) {
+        floatx16_t sc[2];
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) sc[tt][j] = 0.f;
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+                const half8_t k = *reinterpret_cast<const half8_t*>(D.k + (half * KS + i) * KROW + (32 * tt + kt) * 8);
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p)
+                    sc[tt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qb[p][i], sc[tt], 0, 0, 0);
+            }
+        }
+        // lane: its row's scores of tokens 32 tt + 16 (j / 8) + 8 half + j % 8
+        const int live = end - step * PA_TILE - 8 * half;
+        if (ends) {
+#pragma unroll
+            for (int kb = 0; kb < 4; ++kb) {
+                const int n = cur_odd >> kb & 1 ? 0 : live - 16 * kb;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int i = 8 * (kb & 1) + j;
+                    sc[kb >> 1][i] = j < n ? sc[kb >> 1][i] : -INFINITY;
+                }
+            }
+        }
+        float mx = sc[0][0];
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) mx = fmaxf(mx, sc[tt][j]);
         {
-            const T* qp = q + ((size_t)(s.first + qi) * n_q + qh) * HD + 8 * half;
-            if constexpr (PARTS == 1) {
-#pragma unroll
-                for (int i = 0; i < KS; ++i) qb[0][i] = *reinterpret_cast<const half8_t*>(qp + 16 * i);
-            } else {  // scaled by a power of two so that the second part keeps its bits too
-                float amax = 0.f;
-#pragma unroll
-                for (int i = 0; i < KS; ++i)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(qp[16 * i + j]));
-                amax = fmaxf(amax, __shfl_xor(amax, 32, 64));
-                const int e = min(max((int)(__float_as_uint(amax) >> 23) - 127, -110), 126);  // 2^e <= amax
-                const float up = __uint_as_float((uint32_t)(127 + 13 - e) << 23);
-                q_unit = __uint_as_float((uint32_t)(127 - 13 + e) << 23);
-#pragma unroll
-                for (int i = 0; i < KS; ++i)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const float y = qp[16 * i + j] * up;
-                        qb[0][i][j] = (_Float16)y;
-                        qb[1][i][j] = (_Float16)(y - (float)qb[0][i][j]);
-                    }
-            }
+            const pa_u2 w = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+            mx = fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1]));
         }
-        const float c2 = scale * 1.44269504088896340736f * q_unit;
-
-        float m_run = PA_NONE, l_run = 0.f;
-        floatx16_t o[DT];  // lane: row, dims 32 dt + 8 (i / 4) + 4 half + i % 4
+        const float kf = kvp_scale(cur_k) * c2;
+        mx = fmaxf(m_run, mx * kf);
+        if (__any(mx > m_run) || cur_v > o_ref) {
+            const float corr = __builtin_amdgcn_exp2f(m_run - mx);
+            l_run *= corr;
+            const float both = corr * pa_pow2(o_ref - cur_v);
 #pragma unroll
-        for (int i = 0; i < DT; ++i)
-#pragma unroll
-            for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
-        int o_ref = KVP_E_MIN;                              // exponent that o is relative to
-        int k_ref = KVP_E_MIN, v_ref = KVP_E_MIN;           // of the step staged last
-        int cur_k = KVP_E_MIN, cur_v = KVP_E_MIN, cur_odd = 0;  // of the step in work; its blocks without a page, NaN in V
-
-        // Staging: registers, then LDS.  Lane j & 3 knows block j's page and exponents; a wave's pieces lie in one block.
-        uint4 kx[U], vx[U];
-        int ek, ev, page;
-        bool used;
-        auto find = [&](int step) {
-            const int blk = 4 * step + (lane & 3);
-            used = blk * KVP_BLOCK < seg_end;
-            page = used ? table[blk >> bl] : -1;
-            used = used && (unsigned)page < (unsigned)c.n_pages;
-        };
-        auto load = [&](int step) {
-            const int blk = 4 * step + (lane & 3);
-            const size_t i = (((size_t)(used ? page : 0) * c.n_kv + h) << bl) + (blk & ((1 << bl) - 1));
-            ek = c.k_exp[i];
-            ev = c.v_exp[i];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int j = U == 2 ? 2 * u + (wv >> 1) : wv;  // the block of this wave's pieces
-                const int p = __builtin_amdgcn_readlane(used ? page : 0, j);
-                const size_t at = (((size_t)p * c.n_kv + h) << bl) + ((4 * step + j) & ((1 << bl) - 1));
-                const int piece = U == 2 ? (wv & 1) * 64 + lane : lane;  // of the block's HD pieces
-                kx[u] = ldg_g16(c.k + at * (KVP_BLOCK * HD) + piece * 16);
-                vx[u] = ldg_g16(c.v + at * (KVP_BLOCK * HD) + piece * 16);
-            }
-        };
-        auto scaled = [&](const uint4& x, _Float16 f, _Float16* dst) {
-            const half8_t lo = pa_half8(x.x, x.y) * f, hi = pa_half8(x.z, x.w) * f;
-            *reinterpret_cast<half8_t*>(dst) = lo;
-            *reinterpret_cast<half8_t*>(dst + 8) = hi;
-        };
-        int next_odd = 0;
-        auto put = [&](Tile& D) {
-            next_odd = 0;
-            int e[4], f[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const bool in = __builtin_amdgcn_readlane((int)used, j);
-                e[j] = in ? __builtin_amdgcn_readlane(ek, j) : -1000;
-                f[j] = in ? __builtin_amdgcn_readlane(ev, j) : -1000;
-                if (!in) next_odd |= 1 << j;
-                if (f[j] == KVP_E_NAN) next_odd |= 16 << j;
-                k_ref = max(k_ref, e[j]);
-                v_ref = max(v_ref, f[j]);
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int j = U == 2 ? 2 * u + (wv >> 1) : wv;
-                int ej = e[0], fj = f[0];
-#pragma unroll
-                for (int i = 1; i < 4; ++i) {
-                    ej = i == j ? e[i] : ej;
-                    fj = i == j ? f[i] : fj;
-                }
-                const _Float16 kf = ej == KVP_E_NAN ? (_Float16)NAN : (_Float16)pa_pow2(ej - k_ref);
-                const _Float16 vf = fj == KVP_E_NAN ? (_Float16)0.f : (_Float16)pa_pow2(fj - v_ref);
-                const int piece = U == 2 ? (wv & 1) * 64 + lane : lane;
-                // K piece: token piece / KS of the block, dims 16 (piece % KS) ..; V piece: dim `piece`
-                scaled(kx[u], kf, D.k + (piece % KS) * KROW + (16 * j + piece / KS) * 16);
-                scaled(vx[u], vf, D.v + (j * HD + piece) * 16);
-            }
-        };
-
-        // K row of 32-token tile tt: token with bits 2 and 3 of the lane's row swapped
-        const int kt = (row & 0x13) | (row & 4) << 1 | (row & 8) >> 1;
-        auto work = [&](const Tile& S, int step, auto ends) {
-            constexpr bool ENDS = decltype(ends)::value;
-            floatx16_t sc[2];
-#pragma unroll
-            for (int tt = 0; tt < 2; ++tt) {
-#pragma unroll
-                for (int j = 0; j < 16; ++j) sc[tt][j] = 0.f;
-#pragma unroll
-                for (int i = 0; i < KS; ++i) {
-                    const half8_t k = *reinterpret_cast<const half8_t*>(S.k + i * KROW + (32 * tt + kt) * 16 + 8 * half);
-#pragma unroll
-                    for (int p = 0; p < PARTS; ++p)
-                        sc[tt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qb[p][i], sc[tt], 0, 0, 0);
-                }
-            }
-            // lane: its row's scores of tokens 32 tt + 16 (j / 8) + 8 half + j % 8
-            const int live = end - step * PA_TILE - 8 * half;
-            if constexpr (ENDS) {
-#pragma unroll
-                for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const bool in = 32 * tt + 16 * (j >> 3) + (j & 7) < live && !(cur_odd >> (2 * tt + (j >> 3)) & 1);
-                        sc[tt][j] = in ? sc[tt][j] : -INFINITY;
-                    }
-            }
-            float mx = sc[0][0];
-#pragma unroll
-            for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-                for (int j = 0; j < 16; ++j) mx = fmaxf(mx, sc[tt][j]);
-            {
-                const pa_u2 w = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
-                mx = fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1]));
-            }
-            const float kf = kvp_scale(cur_k) * c2;
-            mx = fmaxf(m_run, mx * kf);
-            if (__any(mx > m_run) || cur_v > o_ref) {
-                const float corr = __builtin_amdgcn_exp2f(m_run - mx);
-                l_run *= corr;
-                const float both = corr * pa_pow2(o_ref - cur_v);
-#pragma unroll
-                for (int dt = 0; dt < DT; ++dt) o[dt] *= both;
-                m_run = mx;
-                o_ref = cur_v;
-            }
-            const float shift = (float)PA_P_LOG2 - mx;
-            half8_t pf[PARTS][4];
-#pragma unroll
-            for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const float p = __builtin_amdgcn_exp2f(fmaf(sc[tt][j], kf, shift));
-                    l_run += p;
-                    const int kb = 2 * tt + (j >> 3);
-                    float w = p;
-                    if constexpr (ENDS) w = (cur_odd >> (4 + kb) & 1) && !(sc[tt][j] == -INFINITY) ? NAN : p;
-                    pf[0][kb][j & 7] = (_Float16)w;
-                    if constexpr (PARTS == 2) pf[1][kb][j & 7] = (_Float16)(w - (float)pf[0][kb][j & 7]);
-                }
+            for (int dt = 0; dt < DT; ++dt) o[dt] *= both;
+            m_run = mx;
+            o_ref = cur_v;
+        }
+        if (cur_odd >> 4) {  // NaN in V: the sums of the rows that see a token of its block
 #pragma unroll
             for (int kb = 0; kb < 4; ++kb)
+                if ((cur_odd >> (4 + kb) & 1) && end - step * PA_TILE > 16 * kb) {
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt) {
-                    const half8_t v = *reinterpret_cast<const half8_t*>(S.v + (kb * HD + 32 * dt + row) * 16 + 8 * half);
+                    for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-                    for (int p = 0; p < PARTS; ++p)
-                        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pf[p][kb], o[dt], 0, 0, 0);
+                        for (int j = 0; j < 16; ++j) o[dt][j] = NAN;
                 }
-        };
-
-        find(a);
-        load(a);
-        put(tiles[0]);
-        cur_k = k_ref;
-        cur_v = v_ref;
-        cur_odd = next_odd;
-        if (a + 1 < z) find(a + 1);
-        __syncthreads();
-        int buf = 0;
-        for (int step = a; step < z; ++step) {
-            const bool more = step + 1 < z;
-            if (more) load(step + 1);
-            if (step * PA_TILE < longest) {
-                if (step * PA_TILE + PA_TILE <= shortest && cur_odd == 0) work(tiles[buf], step, std::false_type{});
-                else work(tiles[buf], step, std::true_type{});
-            }
-            if (more) {
-                put(tiles[buf ^ 1]);
-                cur_k = k_ref;
-                cur_v = v_ref;
-                cur_odd = next_odd;
-                if (step + 2 < z) find(step + 2);
-            }
-            __syncthreads();
-            buf ^= 1;
         }
-
-        // ---- results ----
-        const long long seg_t = (long long)h * steps + R.before;
-        const int first = (int)(seg_t / share), pieces = (int)((seg_t + nt - 1) / share) - first + 1;
-        {
-            const pa_u2 w = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_run), __float_as_uint(l_run), false, false);
-            l_run = __uint_as_float(w[0]) + __uint_as_float(w[1]);
-        }
-        const size_t rec = pa_rec(first, blockIdx.x - first);
-        if (pieces > 1) {
-            float* po = pl.o + (rec * PA_ROWS + wv * 32 + row) * HD + 4 * half;
+        const float shift = (float)PA_P_LOG2 - mx;
+        union {
+            half8_t v[4];
+            pa_h2 h[16];
+        } pf[PARTS];
+        const pa_h2 ones = {(_Float16)1.f, (_Float16)1.f};
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt)
+        for (int i = 0; i < 16; ++i) {  // the sum of the probabilities as the products have them
+            const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[i >> 3][2 * (i & 7)], kf, shift));
+            const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[i >> 3][2 * (i & 7) + 1], kf, shift));
+            pf[0].h[i] = pa_h2{(_Float16)p0, (_Float16)p1};
+            l_run = __builtin_amdgcn_fdot2(pf[0].h[i], ones, l_run, false);
+            if constexpr (PARTS == 2) {
+                pf[1].h[i] = pa_h2{(_Float16)(p0 - (float)pf[0].h[i][0]), (_Float16)(p1 - (float)pf[0].h[i][1])};
+                l_run = __builtin_amdgcn_fdot2(pf[1].h[i], ones, l_run, false);
+            }
+        }
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                const half8_t v = *reinterpret_cast<const half8_t*>(D.v + ((2 * kb + half) * HD + 32 * dt + row) * 8);
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p)
+                    o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pf[p].v[kb], o[dt], 0, 0, 0);
+            }
+    };
+
+    put(S.tiles[grp][0]);
+    cur_k = k_ref;
+    cur_v = v_ref;
+    cur_odd = next_odd;
+    find(a + grp + GROUPS);
+    __syncthreads();
+    int buf = 0;
+    for (int step = a + grp; step < z + grp; step += GROUPS) {  // (a group without a last step takes part in the barriers)
+        const bool more = step + GROUPS < z;
+        if (more) load(step + GROUPS);
+        if (step < z && step * PA_TILE < longest)
+            work(S.tiles[grp][buf], step, step * PA_TILE + PA_TILE > shortest || cur_odd != 0);
+        if (more) {
+            put(S.tiles[grp][buf ^ 1]);
+            cur_k = k_ref;
+            cur_v = v_ref;
+            cur_odd = next_odd;
+            find(step + 2 * GROUPS);
+        }
+        __syncthreads();
+        buf ^= 1;
+    }
+
+    // ---- results ----
+    {
+        const pa_u2 w = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_run), __float_as_uint(l_run), false, false);
+        l_run = __uint_as_float(w[0]) + __uint_as_float(w[1]);
+    }
+    if constexpr (GROUPS == 1) {
+        if (r0 + row < rows) pa_store<T, DT>(dst + 4 * half, o, l_run, o_ref);
+    } else {  // each group leaves half of the dims to the other
+        if (half == 0) {
+            m_sh[grp][wv * 32 + row] = m_run;
+            l_sh[grp][wv * 32 + row] = l_run;
+        }
+        if (lane == 0) ev_sh[grp][wv] = o_ref;
+        floatx16_t mine[DT / 2];
+#pragma unroll
+        for (int i = 0; i < DT / 2; ++i) {
+            mine[i] = grp ? o[DT / 2 + i] : o[i];
+            const floatx16_t other = grp ? o[i] : o[DT / 2 + i];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) S.o[grp][16 * i + j][tid] = other[j];
+        }
+        __syncthreads();
+        const float m2 = m_sh[grp ^ 1][wv * 32 + row], M = fmaxf(m_run, m2);
+        const int e2 = ev_sh[grp ^ 1][wv], EV = max(o_ref, e2);
+        const float f1 = __builtin_amdgcn_exp2f(m_run - M), f2 = __builtin_amdgcn_exp2f(m2 - M);
+        const float L = l_run * f1 + l_sh[grp ^ 1][wv * 32 + row] * f2;
+        const float g1 = f1 * pa_pow2(o_ref - EV), g2 = f2 * pa_pow2(e2 - EV);
+#pragma unroll
+        for (int i = 0; i < DT / 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) mine[i][j] = mine[i][j] * g1 + S.o[grp ^ 1][16 * i + j][tid] * g2;
+        const int d0 = grp * (HD / 2) + 4 * half;  // first dim of mine
+        if (pieces > 1) {
+            const size_t rec = ((size_t)slot * c.n_kv + h) * pp.nsp + blockIdx.z;
+            float* po = pp.o + (rec * ROWS + wv * 32 + row) * HD + d0;
+#pragma unroll
+            for (int i = 0; i < DT / 2; ++i)
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    *reinterpret_cast<floatx4_t*>(po + 32 * dt + 8 * j) =
-                        floatx4_t{o[dt][4 * j], o[dt][4 * j + 1], o[dt][4 * j + 2], o[dt][4 * j + 3]};
-            if (half == 0) {
-                pl.ml[(rec * PA_ROWS + wv * 32 + row) * 2] = m_run;
-                pl.ml[(rec * PA_ROWS + wv * 32 + row) * 2 + 1] = l_run;
+                    *reinterpret_cast<floatx4_t*>(po + 32 * i + 8 * j) =
+                        floatx4_t{mine[i][4 * j], mine[i][4 * j + 1], mine[i][4 * j + 2], mine[i][4 * j + 3]};
+            if (half == 0 && grp == 0) {
+                pp.ml[(rec * ROWS + wv * 32 + row) * 2] = M;
+                pp.ml[(rec * ROWS + wv * 32 + row) * 2 + 1] = L;
             }
-            if (lane == 0) pl.ev[4 * rec + wv] = o_ref;
+            if (lane == 0 && grp == 0) pp.ev[4 * rec + wv] = EV;
         } else if (r0 + row < rows) {
-            T* po = out + ((size_t)(s.first + qi) * n_q + qh) * HD + 4 * half;
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                for (int j = 0; j < 16; ++j)
-                    st_act<T>(po + 32 * dt + 8 * (j >> 2) + (j & 3), l_run == 0.f ? 0.f : ldexpf(o[dt][j] / l_run, o_ref));
+            pa_store<T, DT / 2>(dst + d0, mine, L, EV);
         }
-        t += z - a;
-        a = z;
     }
 }
 
-// Combine of the cut row blocks, and zeros for the rows that see nothing: grid (row blocks, n_kv, PA_ROWS / rows of a
-// block), HD / 4 threads a row.
+// Joins the shares of the row blocks: grid (row blocks, n_kv, 128 / rows of a block), HD / 4 threads a row.
 template <typename T, int HD>
-__global__ __launch_bounds__(256) void attn_pages_prompt_combine_kernel(KvPages c, KvRows r, PaPlan pl, PaPrompt pp,
+__global__ __launch_bounds__(256) void attn_pages_prompt_combine_kernel(KvPages c, KvRows r, PaPrompt pp,
                                                                         T* __restrict__ out, int n_q) {
-    constexpr int TD = HD / 4;
-    if ((int)blockIdx.x >= pp.total[0]) return;
-    const PaRowBlock R = pp.rb[blockIdx.x];
-    const int h = blockIdx.y, G = n_q / c.n_kv, share = pp.total[2];
-    const int rr = blockIdx.z * (256 / TD) + threadIdx.x / TD, d = threadIdx.x % TD * 4;
-    const KvSeq s = kvp_place(r, R.b);
-    const int ri = R.rb * PA_ROWS + rr;
-    if (ri >= s.n * G) return;
-    T* dst = out + ((size_t)(s.first + ri / G) * n_q + h * G + ri % G) * HD + d;
-    if (R.steps == 0) {
-        for (int e = 0; e < 4; ++e) st_act<T>(dst + e, 0.f);
-        return;
-    }
-    const long long seg_t = (long long)h * pp.total[1] + R.before;
-    const int first = (int)(seg_t / share), pieces = (int)((seg_t + R.steps - 1) / share) - first + 1;
-    if (pieces == 1) return;
+    constexpr int TD = HD / 4, ROWS = 128;
+    const int slot = blockIdx.x, h = blockIdx.y, G = n_q / c.n_kv;
+    const PaRowBlock R = pa_row_block<ROWS>(r, G, slot);
+    if (R.b < 0) return;
+    const int rr = blockIdx.z * (256 / TD) + threadIdx.x / TD, d = threadIdx.x % TD * 4, ri = R.rb * ROWS + rr;
+    const int steps = pa_steps<ROWS>(R, G, kvp_capacity(c, r)), share = pa_share_of(steps, pp.nsp);
+    if (steps <= share || ri >= R.s.n * G) return;
+    const int pieces = (steps + share - 1) / share;
+    const size_t rec0 = ((size_t)slot * c.n_kv + h) * pp.nsp;
     float M = PA_NONE, L = 0.f;
     int EV = KVP_E_MIN;
     for (int i = 0; i < pieces; ++i) {
-        const size_t rec = pa_rec(first, i);
-        M = fmaxf(M, pl.ml[(rec * PA_ROWS + rr) * 2]);
-        EV = max(EV, pl.ev[4 * rec + rr / 32]);
+        M = fmaxf(M, pp.ml[((rec0 + i) * ROWS + rr) * 2]);
+        EV = max(EV, pp.ev[4 * (rec0 + i) + rr / 32]);
     }
     floatx4_t O = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int i = 0; i < pieces; ++i) {
-        const size_t rec = pa_rec(first, i);
-        const float f = __builtin_amdgcn_exp2f(pl.ml[(rec * PA_ROWS + rr) * 2] - M);
-        L = fmaf(pl.ml[(rec * PA_ROWS + rr) * 2 + 1], f, L);
-        O += *reinterpret_cast<const floatx4_t*>(pl.o + (rec * PA_ROWS + rr) * HD + d) *
-             (f * pa_pow2(pl.ev[4 * rec + rr / 32] - EV));
+    for (int i0 = 0; i0 < pieces; i0 += 4) {  // four requested together (past the last one: the last again)
+        floatx4_t o[4];
+        float m[4], l[4];
+        int ev[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const size_t rec = rec0 + min(i0 + i, pieces - 1);
+            o[i] = *reinterpret_cast<const floatx4_t*>(pp.o + (rec * ROWS + rr) * HD + d);
+            m[i] = pp.ml[(rec * ROWS + rr) * 2];
+            l[i] = pp.ml[(rec * ROWS + rr) * 2 + 1];
+            ev[i] = pp.ev[4 * rec + rr / 32];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (i0 + i >= pieces) continue;
+            const float f = __builtin_amdgcn_exp2f(m[i] - M);
+            L = fmaf(l[i], f, L);
+            O += o[i] * (f * pa_pow2(ev[i] - EV));
+        }
     }
+    T* dst = out + ((size_t)(R.s.first + ri / G) * n_q + h * G + ri % G) * HD + d;
 #pragma unroll
     for (int e = 0; e < 4; ++e) st_act<T>(dst + e, L == 0.f ? 0.f : ldexpf(O[e] / L, EV));
 }
@@ -878,41 +923,40 @@ static PaPlan rows_plan(const KvPages& c, const KvRows& r, int hd, int G, void* 
     *bytes = n;
     return p;
 }
-// Blocks of the many-rows form, likewise; at most `rbs` row blocks.
-static PaPlan prompt_plan(const KvPages& c, const KvRows& r, int hd, int G, void* scratch, PaPrompt* pp, long long* rbs,
-                          long long* bytes) {
-    *rbs = ((long long)r.rows * G + PA_ROWS - 1) / PA_ROWS + r.batch;
-    const long long steps = *rbs * c.n_kv * ((((long long)r.max_pages << c.page_log2) + PA_TILE - 1) / PA_TILE);
-    PaPlan p;
-    p.blocks = (int)std::min<long long>(2 * device_cus(), steps);
-    p.ncol = PA_ROWS;
-    p.seg = nullptr;
-    const long long recs = 2LL * p.blocks;
+// The many-rows form: rows of a block, row blocks at most (each sequence may end one early), and shares of each, as many
+// as fill the CUs.
+struct PromptForm {
+    int groups;
+    long long rbs;
+    PaPrompt p;
+    long long bytes;
+};
+static PromptForm prompt_form(const KvPages& c, const KvRows& r, int hd, int G, void* scratch) {
+    PromptForm f;
+    auto blocks = [&](int rows) { return ((long long)r.rows * G + rows - 1) / rows + r.batch - 1; };
+    f.groups = blocks(256) * c.n_kv >= 2 * device_cus() ? 1 : 2;
+    f.rbs = blocks(f.groups == 1 ? 256 : 128);
+    const long long steps = (((long long)r.max_pages << c.page_log2) + PA_TILE - 1) / PA_TILE;
+    f.p.nsp = (int)std::max<long long>(1, std::min<long long>({PA_SHARES, steps / 2, device_cus() / (f.rbs * c.n_kv)}));
+    const long long recs = f.p.nsp == 1 ? 0 : f.rbs * c.n_kv * f.p.nsp;
     uint8_t* at = static_cast<uint8_t*>(scratch);
-    long long n = 0;
-    p.o = reinterpret_cast<float*>(at);
-    n += pa_up(recs * PA_ROWS * hd * 4);
-    p.ml = reinterpret_cast<float*>(at + n);
-    n += pa_up(recs * PA_ROWS * 8);
-    p.ev = reinterpret_cast<int*>(at + n);
+    long long n = 16;
+    f.p.o = reinterpret_cast<float*>(at + n);
+    n += pa_up(recs * 128 * hd * 4);
+    f.p.ml = reinterpret_cast<float*>(at + n);
+    n += pa_up(recs * 128 * 8);
+    f.p.ev = reinterpret_cast<int*>(at + n);
     n += pa_up(recs * 16);
-    pp->rb = reinterpret_cast<PaRowBlock*>(at + n);
-    n += pa_up(*rbs * sizeof(PaRowBlock));
-    pp->start = reinterpret_cast<PaStart*>(at + n);
-    n += pa_up(p.blocks * sizeof(PaStart));
-    pp->total = reinterpret_cast<int*>(at + n);
-    n += 16;
-    *bytes = n;
-    return p;
+    f.bytes = n;
+    return f;
 }
 static bool rows_form(const KvRows& r, int G) { return r.max_rows * G <= 16; }
 
 long long attn_pages_scratch_bytes(const KvPages& c, const KvRows& r, int hd, int n_q) {
     const int G = n_q / c.n_kv;
-    long long n, rbs;
-    PaPrompt pp;
-    if (rows_form(r, G)) rows_plan(c, r, hd, G, nullptr, &n);
-    else prompt_plan(c, r, hd, G, nullptr, &pp, &rbs, &n);
+    if (!rows_form(r, G)) return prompt_form(c, r, hd, G, nullptr).bytes;
+    long long n;
+    rows_plan(c, r, hd, G, nullptr, &n);
     return n;
 }
 
@@ -931,18 +975,14 @@ static hipError_t attn_hd(const KvPages& c, const KvRows& r, const void* q, void
                            p, (T*)out, n_q);
         return hipGetLastError();
     }
-    long long rbs;
-    PaPrompt pp;
-    const PaPlan p = prompt_plan(c, r, HD, G, scratch, &pp, &rbs, &bytes);
-    hipLaunchKernelGGL(attn_pages_plan_kernel, dim3(1), dim3(1024), 0, st, c, r, p, pp, n_q);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((attn_pages_prompt_kernel<T, HD>), dim3(p.blocks), dim3(256), 0, st, c, r, p, pp, (const T*)q,
-                       (T*)out, n_q, scale);
-    e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((attn_pages_prompt_combine_kernel<T, HD>), dim3((unsigned)rbs, c.n_kv, PA_ROWS * HD / 1024),
-                       dim3(256), 0, st, c, r, p, pp, (T*)out, n_q);
+    const PromptForm f = prompt_form(c, r, HD, G, scratch);
+    auto kernel = f.groups == 1 ? attn_pages_prompt_kernel<T, HD, 1> : attn_pages_prompt_kernel<T, HD, 2>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)f.rbs, c.n_kv, f.p.nsp), dim3(512), 0, st, c, r, f.p, (const T*)q, (T*)out,
+                       n_q, scale);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || f.p.nsp == 1) return e;
+    hipLaunchKernelGGL((attn_pages_prompt_combine_kernel<T, HD>), dim3((unsigned)f.rbs, c.n_kv, 128 * HD / 1024),
+                       dim3(256), 0, st, c, r, f.p, (T*)out, n_q);
     return hipGetLastError();
 }
 hipError_t attn_pages(const KvPages& c, const KvRows& r, int hd, bool f16, const void* q, void* out, int n_q,
