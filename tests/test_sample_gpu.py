@@ -115,3 +115,20 @@ def test_frequencies(hip, K):
     x = np.broadcast_to(np.log(p).astype(np.float32), (4096, 4))
     got = draw(hip, K, np.ascontiguousarray(x), u=(np.arange(4096) + 0.5) / 4096)
     assert (np.abs(np.bincount(got, minlength=4) - 4096 * p) <= 1).all()
+
+
+@pytest.mark.parametrize("vocab", [100003, 100004])
+def test_long_parts_of_many_rows(hip, K, vocab):
+    """172 rows: two parts each, longer than what stays in registers; a much larger entry late in a part, parts of
+    nothing but -Inf, an infinite temperature."""
+    rng = np.random.default_rng(vocab)
+    x = (2 * rng.standard_normal((172, vocab))).astype(np.float32)
+    x[1, 49000] = x[2, 99999] = 60
+    x[3, :50000] = x[4, 49000:] = -np.inf
+    x[5, 40000:] += 200
+    x[6, 48000:49000] = np.nan
+    x[7, 49999] = np.inf
+    T = rng.choice([0.2, 0.7, 1.0, 1.5], 172)
+    T[8], T[9] = np.inf, 0
+    check(hip, K, x, T, rng.choice([0, 0, 40, 3000], 172), rng.choice([1.0, 0.95, 0.5], 172),
+          rng.choice([0.0, 0.0, 0.05], 172), rng.random(172))

@@ -595,7 +595,7 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
     auto is_v = [&](int u) { return NP >= 2 ? u >= NP / 2 : wv >= WAVES / 2; };
     auto first = [&](int u) { return (NP >= 2 ? u % (NP / 2) * WAVES + wv : wv % (WAVES / 2)) * 64; };
     int ek, ev, page;
-    bool used;
+    bool used, got;  // block j is of use: in the step that is looked for, in the one in the registers
     auto find = [&](int step) {
         const int blk = 4 * step + (lane & 3);
         used = step < z && blk * KVP_BLOCK < seg_end;
@@ -613,6 +613,8 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
             const size_t at = (((size_t)p * c.n_kv + h) << bl) + ((4 * step + j) & ((1 << bl) - 1));
             stage[u] = ldg_g16((is_v(u) ? c.v : c.k) + at * (KVP_BLOCK * HD) + (first(u) % HD + lane) * 16);
         }
+        got = used;
+        find(step + GROUPS);
     };
     find(a + grp);
     load(a + grp);
@@ -661,7 +663,7 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
         int e[4], f[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const bool in = __builtin_amdgcn_readlane((int)used, j);
+            const bool in = __builtin_amdgcn_readlane((int)got, j);
             e[j] = in ? __builtin_amdgcn_readlane(ek, j) : -1000;
             f[j] = in ? __builtin_amdgcn_readlane(ev, j) : -1000;
             if (!in) next_odd |= 1 << j;
@@ -774,25 +776,29 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
             }
     };
 
+    // Of the two waves on a SIMD one stages the next step before its work and one after it, so that the bytes' conversion
+    // and the softmax of one fall on the other's matrix products.
+    const bool early = GROUPS == 2 ? grp : wv >= WAVES / 2;
     put(S.tiles[grp][0]);
     cur_k = k_ref;
     cur_v = v_ref;
     cur_odd = next_odd;
-    find(a + grp + GROUPS);
+    if (early && a + grp + GROUPS < z) load(a + grp + GROUPS);
     __syncthreads();
     int buf = 0;
     for (int step = a + grp; step < z + grp; step += GROUPS) {  // (a group without a last step takes part in the barriers)
         const bool more = step + GROUPS < z;
-        if (more) load(step + GROUPS);
+        if (early && more) {
+            put(S.tiles[grp][buf ^ 1]);
+            if (step + 2 * GROUPS < z) load(step + 2 * GROUPS);
+        }
+        if (!early && more) load(step + GROUPS);
         if (step < z && step * PA_TILE < longest)
             work(S.tiles[grp][buf], step, step * PA_TILE + PA_TILE > shortest || cur_odd != 0);
-        if (more) {
-            put(S.tiles[grp][buf ^ 1]);
-            cur_k = k_ref;
-            cur_v = v_ref;
-            cur_odd = next_odd;
-            find(step + 2 * GROUPS);
-        }
+        if (!early && more) put(S.tiles[grp][buf ^ 1]);
+        cur_k = k_ref;
+        cur_v = v_ref;
+        cur_odd = next_odd;
         __syncthreads();
         buf ^= 1;
     }

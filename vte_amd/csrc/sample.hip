@@ -35,6 +35,7 @@
 #define SMP_LEVELS 5        // 32 + 18 bits of (key, index) in digits of 10
 #define SMP_LIST 8192       // entries that are collected at most; more: the row is read again
 #define SMP_SMALL 1024      // entries of a bin that are ordered by counting
+#define SMP_AHEAD 4         // subsets a wave of the draw has in flight (8: one row 16.1 -> 18.6 us, 256 rows the same)
 #define SMP_SPLIT 8         // blocks of a row at most
 
 // Scratch of a row.
@@ -103,6 +104,8 @@ __device__ __forceinline__ SmpScale smp_scale(float max, float T) {
 }
 // Bin of x (false: no weight, NaN among them) and its weight in the bin, in units of 2^-44: the series of e^(r / 32)
 // for y = round(y) + r (the next term is below 2^-45).
+// ABOVE: bins above the scale's largest value that count too (g is below 0 there).
+template <int ABOVE = 0>
 __device__ __forceinline__ bool smp_bin(const SmpScale& c, float x, int& g, uint64_t& m) {
     constexpr double H = 1.0 / SMP_PER_UNIT;
     double r = 0.0;
@@ -112,7 +115,7 @@ __device__ __forceinline__ bool smp_bin(const SmpScale& c, float x, int& g, uint
         const double t = fma(v, c.s, SMP_ROUND);
         r = fma(v, c.s, SMP_ROUND - t);
         g = c.top - __double2loint(t);
-        in = in && (unsigned)g < SMP_BINS;
+        in = in && (unsigned)(g + ABOVE) < SMP_BINS + ABOVE;
     } else {
         in = in && (c.flat || x == c.max);
         g = 0;
@@ -131,6 +134,11 @@ __device__ __forceinline__ int smp_inside(const SmpScale& c, float x) {
     if (!c.whole) return 0;
     const double t = fma((double)x, c.s, SMP_ROUND), r = fma((double)x, c.s, SMP_ROUND - t);
     return min(max((int)((0.5 - r) * (double)SMP_THREADS), 0), SMP_THREADS - 1);
+}
+// Bins from the scale's largest value up to a larger one; SMP_ROOM + 1 where that is more than SMP_ROOM.
+__device__ __forceinline__ int smp_above(const SmpScale& c, float top) {
+    const double d = rint((double)top * c.s) - rint((double)c.max * c.s);
+    return d <= (double)SMP_BINS ? (int)d : SMP_BINS + 1;
 }
 // Bins between the largest values of a part and of the row; SMP_BINS or more: none of the part's matter.
 __device__ __forceinline__ int smp_apart(const SmpScale& c, float part) {
@@ -171,17 +179,19 @@ __device__ __forceinline__ float smp_max4(const SmpFour& r) {  // NaN counts as 
     return fmaxf(fmaxf(fmaxf(r.x[0], -INFINITY), r.x[1]), fmaxf(r.x[2], r.x[3]));
 }
 
-// grid (blocks of a row, rows).  The block's first KEEP subsets a wave stay in registers between the two passes (all of
-// a part, for few rows); the others are read again, eight and then four in flight.
+// grid (blocks of a row, rows).  A part of at most KEEP subsets a wave (few rows) stays in registers while its largest
+// entry is found.  A longer one is read once: its bins are laid from the largest entry of those first subsets on, with
+// SMP_ROOM bins above it for what follows; if that is not enough (a much larger entry comes later) it is read again.
 #define SMP_KEEP 8
+#define SMP_ROOM SMP_BINS
 template <bool WIDE>
 __global__ __launch_bounds__(SMP_THREADS) void sample_bins_kernel(const float* __restrict__ logits, int vocab,
                                                                   const float* __restrict__ temperature,
                                                                   const int* __restrict__ top_k, uint8_t* scratch,
                                                                   int subs) {
-    __shared__ unsigned long long mass[SMP_BINS];
-    __shared__ unsigned count[SMP_BINS];
-    __shared__ float wmax[SMP_WAVES];
+    __shared__ unsigned long long mass[SMP_ROOM + SMP_BINS];
+    __shared__ unsigned count[SMP_ROOM + SMP_BINS];
+    __shared__ float wmax[2][SMP_WAVES];
     const int row = blockIdx.y, blocks = gridDim.x, tid = threadIdx.x, lane = tid & 63;
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const float* x = logits + (size_t)row * vocab;
@@ -195,8 +205,10 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_bins_kernel(const float* _
     for (int j = 0; j < SMP_KEEP; ++j) keep[j] = load(j);
     const float T = temperature ? temperature[row] : 1.f;
     const bool counts = top_k != nullptr && top_k[row] > 0;
-    mass[tid] = 0;
-    count[tid] = 0;
+    for (int i = tid; i < SMP_ROOM + SMP_BINS; i += SMP_THREADS) {
+        mass[i] = 0;
+        count[i] = 0;
+    }
     float best = -INFINITY;
     auto first = [&](SmpFour& f, int j) {
         smp_cut<WIDE>(f, vocab, min(nth(j), hi - 1), lane);
@@ -204,58 +216,86 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_bins_kernel(const float* _
         if (lane == 0 && nth(j) < hi) sc.sub[nth(j)] = m;
         best = fmaxf(best, m);  // (a subset twice changes nothing)
     };
+    auto largest = [&](int i) {  // of all waves'
+        if (lane == 0) wmax[i][wv] = best;
+        __syncthreads();
+        float m = wmax[i][0];
+#pragma unroll
+        for (int w = 1; w < SMP_WAVES; ++w) m = fmaxf(m, wmax[i][w]);
+        return m;
+    };
     const int n = (hi - lo + SMP_WAVES - 1) / SMP_WAVES;
 #pragma unroll
     for (int j = 0; j < SMP_KEEP; ++j) first(keep[j], j);
-    for (int j = SMP_KEEP; j < n; j += 8) {
-        SmpFour f[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = load(j + i);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) first(f[i], j + i);
-    }
-    if (lane == 0) wmax[wv] = best;
-    __syncthreads();
-    best = wmax[0];
-#pragma unroll
-    for (int w = 1; w < SMP_WAVES; ++w) best = fmaxf(best, wmax[w]);
-    if (tid == 0) sc.max[blockIdx.x] = best;
-    if (tid < 2 && blockIdx.x == 0) sc.shared[tid] = 0;
-    if (!(best > -INFINITY) || !(T > 0.f)) return;  // nothing in it; greedy rows need the maxima only
-    const SmpScale c = smp_scale(best, T);
-    auto second = [&](const SmpFour& f, int j) {
+    const float ref = largest(0);
+    const bool draws = T > 0.f;  // greedy rows need the maxima only
+    const SmpScale c = smp_scale(ref, T);
+    auto add = [&](const SmpScale& s, const SmpFour& f, int j) {
         if (nth(j) >= hi) return;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             int g;
             uint64_t m;
-            if (!smp_bin(c, f.x[e], g, m)) continue;
-            atomicAdd(&mass[g], (unsigned long long)m);
-            if (counts) atomicAdd(&count[g], 1u);
+            if (!smp_bin<SMP_ROOM>(s, f.x[e], g, m)) continue;
+            atomicAdd(&mass[SMP_ROOM + g], (unsigned long long)m);
+            if (counts) atomicAdd(&count[SMP_ROOM + g], 1u);
         }
     };
-    SmpFour f[4];
-    if (n > SMP_KEEP) {
+    float top = ref;
+    int shift = 0;
+    if (n <= SMP_KEEP) {
+        if (draws && ref > -INFINITY) {
+#pragma unroll
+            for (int j = 0; j < SMP_KEEP; ++j) add(c, keep[j], j);
+        }
+    } else {
+        const bool lay = draws && c.whole;
+        SmpFour f[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) f[i] = load(SMP_KEEP + i);
-    }
+        if (lay) {
 #pragma unroll
-    for (int j = 0; j < SMP_KEEP; ++j) second(keep[j], j);
-    for (int j = SMP_KEEP; j < n; j += 4) {
-        SmpFour ahead[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) ahead[i] = load(j + 4 + i);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            smp_cut<WIDE>(f[i], vocab, min(nth(j + i), hi - 1), lane);
-            second(f[i], j + i);
+            for (int j = 0; j < SMP_KEEP; ++j) add(c, keep[j], j);
         }
+        for (int j = SMP_KEEP; j < n; j += 4) {
+            SmpFour ahead[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) f[i] = ahead[i];
+            for (int i = 0; i < 4; ++i) ahead[i] = load(j + 4 + i);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                first(f[i], j + i);
+                if (lay) add(c, f[i], j + i);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[i] = ahead[i];
+        }
+        top = largest(1);
+        shift = lay ? smp_above(c, top) : SMP_ROOM + 1;
+        if (shift > SMP_ROOM && draws && top > -INFINITY) {  // once more, from the largest entry on
+            for (int i = tid; i < SMP_ROOM + SMP_BINS; i += SMP_THREADS) {
+                mass[i] = 0;
+                count[i] = 0;
+            }
+            __syncthreads();
+            const SmpScale t = smp_scale(top, T);
+            for (int j = 0; j < n; j += 4) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) f[i] = load(j + i);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    smp_cut<WIDE>(f[i], vocab, min(nth(j + i), hi - 1), lane);
+                    add(t, f[i], j + i);
+                }
+            }
+            shift = 0;
+        }
     }
+    if (tid == 0) sc.max[blockIdx.x] = top;
+    if (tid < 2 && blockIdx.x == 0) sc.shared[tid] = 0;
+    if (!draws || !(top > -INFINITY)) return;
     __syncthreads();
-    sc.mass[(size_t)blockIdx.x * SMP_BINS + tid] = mass[tid];
-    if (counts) sc.count[(size_t)blockIdx.x * SMP_BINS + tid] = count[tid];
+    sc.mass[(size_t)blockIdx.x * SMP_BINS + tid] = mass[SMP_ROOM - shift + tid];
+    if (counts) sc.count[(size_t)blockIdx.x * SMP_BINS + tid] = count[SMP_ROOM - shift + tid];
 }
 
 // Sum over the threads up to and with this one; `sh` holds one value a wave.  Inside a wave: shifts by 1, 2, 4 and 8
@@ -595,18 +635,18 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_draw_kernel(const float* _
     }
     __syncthreads();
     const int n_need = S.n_need;
-    SmpFour f[4];  // four subsets a wave and round, the next round's requested ahead
+    SmpFour f[SMP_AHEAD];  // subsets a wave and round, the next round's requested ahead
     auto fetch = [&](int i, int j) {
         return smp_load<WIDE>(r.x, vocab, S.need[min(i + j * SMP_WAVES, n_need - 1)], lane);
     };
     if (n_need > 0) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) f[j] = fetch(wv, j);
+        for (int j = 0; j < SMP_AHEAD; ++j) f[j] = fetch(wv, j);
     }
-    for (int i = wv; i < n_need; i += 4 * SMP_WAVES) {
+    for (int i = wv; i < n_need; i += SMP_AHEAD * SMP_WAVES) {
         uint32_t in = 0;  // bit 4 j + e: entry e of subset j
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < SMP_AHEAD; ++j)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const float x = f[j].x[e];
@@ -617,9 +657,9 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_draw_kernel(const float* _
                 in |= y ? 1u << (4 * j + e) : 0u;
             }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) f[j] = fetch(i + 4 * SMP_WAVES, j);
+        for (int j = 0; j < SMP_AHEAD; ++j) f[j] = fetch(i + SMP_AHEAD * SMP_WAVES, j);
 #pragma unroll
-        for (int j = 1; j < 4; ++j)
+        for (int j = 1; j < SMP_AHEAD; ++j)
             if (i + j * SMP_WAVES >= n_need) in &= (1u << (4 * j)) - 1;  // the last subset again
         int at = in ? atomicAdd(&S.n, __popc(in)) : 0;
         while (in) {
