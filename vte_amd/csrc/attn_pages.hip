@@ -586,24 +586,21 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
     }
     const int end = r0 + row < rows ? kvp_len(s.pos + qi, cap) : 0;
     const int seg_end = kvp_len(s.pos + min((R.rb * ROWS + ROWS - 1) / G, s.n - 1), cap);  // of the row block
-    const int longest = r0 < rows ? kvp_len(s.pos + min(r0 + 31, rows - 1) / G, cap) : 0;       // of the wave
-    const int shortest = r0 + 31 < rows ? kvp_len(s.pos + r0 / G, cap) : 0;
+    const int shortest = r0 + 31 < rows ? kvp_len(s.pos + r0 / G, cap) : 0;  // of the wave
 
     // Staging: registers, then LDS.  Lane j & 3 knows block j's page and exponents; a wave's pieces lie in one block.
     uint4 stage[NP];
     // u: its part of K or V, the block and the first piece of it (of HD) that the wave's lanes take
     auto is_v = [&](int u) { return NP >= 2 ? u >= NP / 2 : wv >= WAVES / 2; };
     auto first = [&](int u) { return (NP >= 2 ? u % (NP / 2) * WAVES + wv : wv % (WAVES / 2)) * 64; };
+    // (No branches here and in put, which stand in one run with the products; a page number is not looked at until
+    // the step after the one in which it is asked for.)
     int ek, ev, page;
-    bool used, got;  // block j is of use: in the step that is looked for, in the one in the registers
-    auto find = [&](int step) {
-        const int blk = 4 * step + (lane & 3);
-        used = step < z && blk * KVP_BLOCK < seg_end;
-        page = used ? table[blk >> bl] : -1;
-        used = used && (unsigned)page < (unsigned)c.n_pages;
-    };
+    bool got;  // block j of the step in the registers is of use
+    auto find = [&](int step) { page = table[min((4 * step + (lane & 3)) >> bl, r.max_pages - 1)]; };
     auto load = [&](int step) {
         const int blk = 4 * step + (lane & 3);
+        const bool used = (step < z) & (blk * KVP_BLOCK < seg_end) & ((unsigned)page < (unsigned)c.n_pages);
         const size_t i = (((size_t)(used ? page : 0) * c.n_kv + h) << bl) + (blk & ((1 << bl) - 1));
         ek = c.k_exp[i];
         ev = c.v_exp[i];
@@ -656,18 +653,16 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
         for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
     int o_ref = KVP_E_MIN;                              // exponent that o is relative to
     int k_ref = KVP_E_MIN, v_ref = KVP_E_MIN;           // of the step staged last
-    int cur_k = KVP_E_MIN, cur_v = KVP_E_MIN, cur_odd = 0;  // of the step in work; its blocks without a page, NaN in V
-    int next_odd = 0;
+    int next_odd = 0;                                   // its blocks without a page, and with NaN in V
     auto put = [&](Tile& D) {
         next_odd = 0;
         int e[4], f[4];
+        const int my_k = got ? ek : -1000, my_v = got ? ev : -1000;  // -1000: times 0
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const bool in = __builtin_amdgcn_readlane((int)got, j);
-            e[j] = in ? __builtin_amdgcn_readlane(ek, j) : -1000;
-            f[j] = in ? __builtin_amdgcn_readlane(ev, j) : -1000;
-            if (!in) next_odd |= 1 << j;
-            if (f[j] == KVP_E_NAN) next_odd |= 16 << j;
+            e[j] = __builtin_amdgcn_readlane(my_k, j);
+            f[j] = __builtin_amdgcn_readlane(my_v, j);
+            next_odd |= (e[j] == -1000 ? 1 << j : 0) | (f[j] == KVP_E_NAN ? 16 << j : 0);
             k_ref = max(k_ref, e[j]);
             v_ref = max(v_ref, f[j]);
         }
@@ -691,7 +686,10 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
     // K row of 32-token tile tt: token with bits 2 and 3 of the lane's row swapped
     const int kt = (row & 0x13) | (row & 4) << 1 | (row & 8) >> 1;
     // `ends`: some of the wave's rows do not see all of the step, or a block of it has no page or NaN in V
-    auto work = [&](const Tile& D, int step, bool ends) {
+    auto work = [&](const Tile& D, Tile& next, int step, bool ends) {
+        const int cur_k = k_ref, cur_v = v_ref, cur_odd = next_odd;
+        put(next);
+        load(step + 2 * GROUPS);
         floatx16_t sc[2];
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt) {
@@ -704,6 +702,15 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
                 for (int p = 0; p < PARTS; ++p)
                     sc[tt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qb[p][i], sc[tt], 0, 0, 0);
             }
+        }
+        // the next step's bytes are turned under these products: two reads ahead, then a product, a read and six
+        // vector operations in turn
+        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+        for (int i = 0; i < 2 * KS * PARTS; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);
         }
         // lane: its row's scores of tokens 32 tt + 16 (j / 8) + 8 half + j % 8
         const int live = end - step * PA_TILE - 8 * half;
@@ -727,7 +734,7 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
             const pa_u2 w = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
             mx = fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1]));
         }
-        const float kf = kvp_scale(cur_k) * c2;
+        const float kf = fmaxf(kvp_scale(cur_k) * c2, 1e-38f);  // (not 0: masked scores are -Inf)
         mx = fmaxf(m_run, mx * kf);
         if (__any(mx > m_run) || cur_v > o_ref) {
             const float corr = __builtin_amdgcn_exp2f(m_run - mx);
@@ -776,29 +783,13 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
             }
     };
 
-    // Of the two waves on a SIMD one stages the next step before its work and one after it, so that the bytes' conversion
-    // and the softmax of one fall on the other's matrix products.
-    const bool early = GROUPS == 2 ? grp : wv >= WAVES / 2;
     put(S.tiles[grp][0]);
-    cur_k = k_ref;
-    cur_v = v_ref;
-    cur_odd = next_odd;
-    if (early && a + grp + GROUPS < z) load(a + grp + GROUPS);
+    load(a + grp + GROUPS);
     __syncthreads();
     int buf = 0;
-    for (int step = a + grp; step < z + grp; step += GROUPS) {  // (a group without a last step takes part in the barriers)
-        const bool more = step + GROUPS < z;
-        if (early && more) {
-            put(S.tiles[grp][buf ^ 1]);
-            if (step + 2 * GROUPS < z) load(step + 2 * GROUPS);
-        }
-        if (!early && more) load(step + GROUPS);
-        if (step < z && step * PA_TILE < longest)
-            work(S.tiles[grp][buf], step, step * PA_TILE + PA_TILE > shortest || cur_odd != 0);
-        if (!early && more) put(S.tiles[grp][buf ^ 1]);
-        cur_k = k_ref;
-        cur_v = v_ref;
-        cur_odd = next_odd;
+    // (A group without a last step, and a wave whose rows end before the block's, go along with everything masked.)
+    for (int step = a + grp; step < z + grp; step += GROUPS) {
+        work(S.tiles[grp][buf], S.tiles[grp][buf ^ 1], step, step * PA_TILE + PA_TILE > shortest || next_odd != 0);
         __syncthreads();
         buf ^= 1;
     }
