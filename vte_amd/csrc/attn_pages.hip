@@ -109,25 +109,46 @@ struct PaShare {
     long long t, t_end, before;
     long long share;
     int b;
+    KvSeq s;
 };
+// Sum over the lanes up to and with this one: shifts by 1, 2, 4 and 8 in rows of 16 lanes, then the rows' last lanes into
+// the rows behind them.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ long long pa_from(long long v) {
+    const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+    const int hi = __builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, ROWS, 0xF, false);
+    return (long long)((unsigned long long)(unsigned)hi << 32 | lo);
+}
+__device__ __forceinline__ long long pa_uniform(long long v) {  // the same in every lane: a scalar
+    const unsigned lo = __builtin_amdgcn_readfirstlane((int)v);
+    return (long long)((unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 | lo);
+}
+__device__ __forceinline__ long long pa_scan(long long v) {
+    v += pa_from<0x111, 0xF>(v);
+    v += pa_from<0x112, 0xF>(v);
+    v += pa_from<0x114, 0xF>(v);
+    v += pa_from<0x118, 0xF>(v);
+    v += pa_from<0x142, 0xA>(v);
+    v += pa_from<0x143, 0xC>(v);
+    return v;
+}
 __device__ __forceinline__ PaShare pa_share(const KvPages& c, const KvRows& r, int cap, int block, int blocks) {
     __shared__ long long wsum[4];
-    __shared__ long long found[2];
+    __shared__ long long found[5];
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
     const int per = (r.batch + 255) / 256;
     long long mine = 0;
-    for (int b = tid * per; b < min(r.batch, tid * per + per); ++b)
-        mine += (long long)c.n_kv * ((pa_tokens(kvp_seq(r, b), cap) + PA_TILE - 1) / PA_TILE);
-    long long incl = mine;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const long long up = __shfl_up(incl, d, 64);
-        if (lane >= d) incl += up;
+    KvSeq mine_last = {0, 0, 0};
+    for (int b = tid * per; b < min(r.batch, tid * per + per); ++b) {
+        mine_last = kvp_seq(r, b);
+        mine += (long long)c.n_kv * ((pa_tokens(mine_last, cap) + PA_TILE - 1) / PA_TILE);
     }
+    long long incl = pa_scan(mine);
     if (lane == 63) wsum[wv] = incl;
     __syncthreads();
-    for (int w = 0; w < wv; ++w) incl += wsum[w];
-    const long long total = wsum[0] + wsum[1] + wsum[2] + wsum[3];
+    const long long w4[4] = {wsum[0], wsum[1], wsum[2], wsum[3]};
+    incl += wv > 2 ? w4[0] + w4[1] + w4[2] : wv > 1 ? w4[0] + w4[1] : wv > 0 ? w4[0] : 0;
+    const long long total = pa_uniform(w4[0] + w4[1] + w4[2] + w4[3]);
     PaShare s;
     s.share = ((total + blocks - 1) / blocks + 3) / 4 * 4;
     s.t = s.share * block;
@@ -135,17 +156,26 @@ __device__ __forceinline__ PaShare pa_share(const KvPages& c, const KvRows& r, i
     if (mine > 0 && s.t >= incl - mine && s.t < incl) {
         long long before = incl - mine;
         int b = tid * per;
-        for (;; ++b) {
-            const long long n = (long long)c.n_kv * ((pa_tokens(kvp_seq(r, b), cap) + PA_TILE - 1) / PA_TILE);
-            if (s.t < before + n) break;
-            before += n;
-        }
+        KvSeq q = mine_last;
+        if (per > 1)
+            for (;; ++b) {
+                q = kvp_seq(r, b);
+                const long long n = (long long)c.n_kv * ((pa_tokens(q, cap) + PA_TILE - 1) / PA_TILE);
+                if (s.t < before + n) break;
+                before += n;
+            }
         found[0] = b;
         found[1] = before;
+        found[2] = q.first;
+        found[3] = q.n;
+        found[4] = q.pos;
     }
     __syncthreads();
-    s.b = (int)found[0];
-    s.before = found[1];
+    s.b = __builtin_amdgcn_readfirstlane((int)found[0]);
+    s.before = pa_uniform(found[1]);
+    s.s.first = __builtin_amdgcn_readfirstlane((int)found[2]);
+    s.s.n = __builtin_amdgcn_readfirstlane((int)found[3]);
+    s.s.pos = __builtin_amdgcn_readfirstlane((int)found[4]);
     return s;
 }
 
@@ -174,13 +204,16 @@ __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(KvPages c, KvRo
     PaShare sh = pa_share(c, r, cap, blockIdx.x, pl.blocks);
     int b = sh.b;
     long long t = sh.t, before = sh.before;
+    KvSeq s = sh.s;
 
     while (t < sh.t_end) {
-        const KvSeq s = kvp_seq(r, b);
         const int len = pa_tokens(s, cap), nt = (len + PA_TILE - 1) / PA_TILE;
         if (t - before >= (long long)nt * c.n_kv) {  // the next sequence
             before += (long long)nt * c.n_kv;
-            ++b;
+            s = kvp_seq(r, ++b);
+            s.first = __builtin_amdgcn_readfirstlane(s.first);
+            s.n = __builtin_amdgcn_readfirstlane(s.n);
+            s.pos = __builtin_amdgcn_readfirstlane(s.pos);
             continue;
         }
         const int h = (int)((t - before) / nt), a = (int)((t - before) - (long long)h * nt);
