@@ -203,9 +203,9 @@ int vte_topk_noalloc(const float* logits, int rows, int vocab, int k, float* out
 
 /* Greedy decoding on the device (temperature 0, no repetition penalty): for
  * each row b, tok = top_idx[b*k] (the top-1 candidate of vte_topk: the
- * largest logit, lowest id among equal ones), tokens[b] = tok, kv_offset[b] =
- * min(kv_offset[b] + 1, max_pos), history[*step][b] = tok while *step <
- * history_steps; then *step += 1.  Appended to a captured decode step, the
+ * largest logit, lowest id among equal ones; or vte_sample's tokens with k =
+ * 1), tokens[b] = max(tok, 0), kv_offset[b] = min(kv_offset[b] + 1, max_pos),
+ * history[*step][b] = tok while *step < history_steps; then *step += 1.  Appended to a captured decode step, the
  * next replay decodes the next token with no host round trip.
  * Replaces: the greedy pick of topk_reduce_greedy_kernel
  *           (topk_reduce_greedy.hip.template:52-83) and the host loop that feeds

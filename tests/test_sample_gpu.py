@@ -132,3 +132,82 @@ def test_long_parts_of_many_rows(hip, K, vocab):
     T[8], T[9] = np.inf, 0
     check(hip, K, x, T, rng.choice([0, 0, 40, 3000], 172), rng.choice([1.0, 0.95, 0.5], 172),
           rng.choice([0.0, 0.0, 0.05], 172), rng.random(172))
+
+
+# ---------------------------------------------------------------------------- in the decode step
+@pytest.fixture(scope="module")
+def tiny():
+    from vte_amd.core.model_config import TINY
+    from vte_amd.core.weights import SyntheticQwen2
+    return SyntheticQwen2(TINY, seed=3)
+
+
+@pytest.mark.parametrize("B", [1, 3])
+def test_generate_sampled_matches_host_loop(hip, K, tiny, B):
+    """The draws of the captured loop are those of a loop that reads each step's logits, for the settings of each
+    sequence; a second call with other settings replays the same graph; temperature 0 is generate_greedy."""
+    from vte_amd.core.hip_graph_executor import HIPGraphExecutor
+    ex = HIPGraphExecutor(hip, tiny, batch_size=B, max_seq=256, top_k=40)
+    rng = np.random.default_rng(B)
+    try:
+        toks0, pos0 = [5 + 7 * b for b in range(B)], [60 + 17 * b for b in range(B)]
+        for n, T, k, p, m in ((12, [0.7, 1.5, 0.0][:B], 0, 0.95, 0.0), (7, 1.0, [40, 0, 5][:B], 1.0, [0.0, 0.1, 0.0][:B])):
+            u = rng.random((n, B))
+            ex.fill_kv_prefix(seed=12)
+            host, toks, pos = [], list(toks0), list(pos0)
+            row = lambda v, b: v[b] if isinstance(v, list) else v
+            for i in range(n):
+                ex.execute_decode_batch(toks, pos)
+                x = ex.read_logits()
+                toks = [osm.sample(x[b], float(np.float32(row(T, b))), row(k, b), float(np.float32(row(p, b))),
+                                   float(np.float32(row(m, b))), u[i, b])[0] for b in range(B)]
+                pos = [q + 1 for q in pos]
+                host.append(toks)
+            ex.fill_kv_prefix(seed=12)
+            assert np.array_equal(ex.generate_sampled(toks0, pos0, n, u, T, k, p, m), np.array(host))
+        ex.fill_kv_prefix(seed=12)
+        greedy = ex.generate_greedy(toks0, pos0, 6)
+        ex.fill_kv_prefix(seed=12)
+        assert np.array_equal(ex.generate_sampled(toks0, pos0, 6, np.zeros((6, B)), temperature=0.0), greedy)
+        from vte_amd.bridge.hip_runtime import HIPSafetyError
+        for bad in (lambda: ex.generate_sampled(toks0, pos0, 0, np.zeros((0, B))),
+                    lambda: ex.generate_sampled(toks0, [255] * B, 2, np.zeros((2, B))),
+                    lambda: ex.generate_sampled(toks0, pos0, 2, np.zeros((3, B)))):
+            with pytest.raises(HIPSafetyError):
+                bad()
+    finally:
+        ex.close()
+
+
+def test_advance_keeps_a_row_without_a_draw_inside_the_vocabulary(hip, K):
+    tok, off, hist, step = (up(hip, np.array(a, np.int32)) for a in ([4, 4], [7, 9], [0] * 4, [0]))
+    K.greedy_advance(up(hip, np.array([-1, 12], np.int32)), 1, 2, tok, off, 9, hist, 2, step, stream=hip.stream)
+    assert list(down(tok)) == [0, 12] and list(down(off)) == [8, 9] and list(down(hist)) == [-1, 12, 0, 0]
+
+
+def test_captured_draws(hip, K):
+    """Replays of a captured draw see the logits, settings and uniforms staged before each, with eager draws of another
+    size (and scratch of their own) in between."""
+    rng = np.random.default_rng(21)
+    R, V = 5, 50001
+    need = K.sample_scratch_bytes(R)
+    x, u = empty(hip, (R, V), np.float32), empty(hip, R, np.float64)
+    T, k, tok, scratch = empty(hip, R, np.float32), empty(hip, R, np.int32), empty(hip, R, np.int32), empty(hip, need, np.uint8)
+    hip.stream_synchronize()
+    hip.stream_begin_capture()
+    K.sample(x, R, V, tok, scratch, temperature=T, top_k=k, u=u, stream=hip.stream)
+    g = hip.stream_end_capture()
+    ge = hip.graph_instantiate(g)
+    try:
+        for i in range(5):
+            logits = (rng.choice([0.5, 2.5]) * rng.standard_normal((R, V))).astype(np.float32)
+            st = rng.choice([0.0, 0.8, 1.2], R).astype(np.float32), rng.choice([0, 3, 400], R).astype(np.int32), rng.random(R)
+            x.upload(logits), T.upload(st[0]), k.upload(st[1]), u.upload(st[2])
+            hip.graph_launch(ge)
+            hip.synchronize()
+            want = [osm.sample(logits[r], float(st[0][r]), int(st[1][r]), u=float(st[2][r])) for r in range(R)]
+            assert all(a == b or near < V * 2.0 ** -44 for a, (b, near) in zip(down(tok), want))
+            check(hip, K, (3 * rng.standard_normal((2, 777))).astype(np.float32), 1.0, 0, 0.9, 0.0, rng.random(2))
+    finally:
+        hip.graph_exec_destroy(ge)
+        hip.graph_destroy(g)

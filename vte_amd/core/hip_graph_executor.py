@@ -635,6 +635,83 @@ class HIPGraphExecutor:
         self.hip.safe_memcpy_device_to_host(out, ctypes.c_void_p(hist.ptr), "sampler_greedy_tokens")
         return out[:n_steps].copy()
 
+    def generate_sampled(self, tokens: Sequence[int], kv_offsets: Sequence[int], n_steps: int, uniforms,
+                         temperature=0.7, top_k=0, top_p=1.0, min_p=0.0) -> np.ndarray:
+        """Sampled decoding of ``n_steps`` tokens per sequence with no host
+        round trip: a captured graph of the step, ``vte_sample`` over its
+        logits and ``vte_greedy_advance`` feeding the drawn token back, replayed
+        back to back.  ``uniforms`` [n_steps, B]: the draws' random numbers in
+        [0, 1).  Settings are one value or one per sequence (temperature <= 0:
+        greedy; no repetition penalty).  Returns the tokens, [n_steps, B]; each
+        is what ``vte_sample`` draws from the step's logits (the host sampler's
+        draw, vte/core/sampler.py:54-129, for the same random number)."""
+        if self.prefill_of is not None:
+            raise HIPSafetyError("a prefill executor's columns are one sequence's tokens; decode through the owner")
+        if n_steps < 1 or max(kv_offsets) + n_steps > self.max_seq:
+            raise HIPSafetyError(f"{n_steps} steps from position {int(max(kv_offsets))} exceed max_seq {self.max_seq}")
+        u = np.ascontiguousarray(uniforms, np.float64)
+        if u.shape != (n_steps, self.B):
+            raise HIPSafetyError(f"uniforms of shape {u.shape}, expected {(n_steps, self.B)}")
+        per_row = [np.array(np.broadcast_to(np.asarray(v, t), (self.B,)))
+                   for v, t in ((temperature, np.float32), (top_k, np.int32), (top_p, np.float32), (min_p, np.float32))]
+        if self._exclude() is not None:
+            self.excl_cnt.zero()  # no repetition window
+        sm = getattr(self, "_sampled", None)
+        if sm is None or sm["cap"] < n_steps:
+            self._free_sampled()
+            sm = self._sampled = self._capture_sampled(max(n_steps, 256))
+        for name, v in zip(("temperature", "top_k", "top_p", "min_p"), per_row):
+            sm[name].upload(v)
+        all_u = np.zeros((sm["cap"], self.B), np.float64)
+        all_u[:n_steps] = u
+        sm["all_u"].upload(all_u)
+        self._update_staging_buffers(tokens, kv_offsets)
+        self._pin_fresh = False
+        sm["step"].zero()
+        for i in range(n_steps):
+            self.hip.memcpy_device_to_device(sm["u"].ptr, sm["all_u"].ptr + 8 * self.B * i, 8 * self.B)
+            self.hip.graph_launch(sm["exec"])
+        self.hip.synchronize()
+        self._check_persistent()
+        out = np.empty((sm["cap"], self.B), np.int32)
+        self.hip.safe_memcpy_device_to_host(out, ctypes.c_void_p(sm["history"].ptr), "sampler_drawn_tokens")
+        out = out[:n_steps].copy()
+        if out.min() < 0:
+            raise HIPRuntimeError("a step's logits hold nothing to draw from (only -Inf and NaN)")
+        return out
+
+    def _capture_sampled(self, cap: int) -> dict:
+        """The captured sampled step, its settings and history buffers."""
+        A = lambda shape, dt, tag: DeviceArray(self.hip, shape, dt, tag)
+        B, K = self.B, self.K
+        sm = {"cap": cap, "temperature": A(B, np.float32, "sample_temperature"), "top_k": A(B, np.int32, "sample_top_k"),
+              "top_p": A(B, np.float32, "sample_top_p"), "min_p": A(B, np.float32, "sample_min_p"),
+              "u": A(B, np.float64, "sample_u"), "all_u": A((cap, B), np.float64, "sample_all_u"),
+              "tokens": A(B, np.int32, "sample_tokens"), "history": A((cap, B), np.int32, "sample_history"),
+              "step": A(1, np.int32, "sample_step"),
+              "scratch": A(K.sample_scratch_bytes(B), np.uint8, "sample_scratch")}
+        self.hip.stream_synchronize()
+        self.hip.stream_begin_capture()
+        try:
+            self.enqueue_step()
+            K.sample(self.logits, B, self.cfg.vocab, sm["tokens"], sm["scratch"], temperature=sm["temperature"],
+                     top_k=sm["top_k"], top_p=sm["top_p"], min_p=sm["min_p"], u=sm["u"], stream=self.hip.stream)
+            K.greedy_advance(sm["tokens"], 1, B, self.staging_input, self.staging_kv_offset, self.max_seq - 1,
+                             sm["history"], cap, sm["step"], stream=self.hip.stream)
+        finally:
+            sm["graph"] = self.hip.stream_end_capture()
+        sm["exec"] = self.hip.graph_instantiate(sm["graph"])
+        return sm
+
+    def _free_sampled(self) -> None:
+        sm, self._sampled = getattr(self, "_sampled", None), None
+        if sm is not None:
+            self.hip.graph_exec_destroy(sm["exec"])
+            self.hip.graph_destroy(sm["graph"])
+            for v in sm.values():
+                if isinstance(v, DeviceArray):
+                    v.free()
+
     def _free_greedy(self) -> None:
         gr = getattr(self, "_greedy", None)
         if gr is not None:
@@ -720,6 +797,7 @@ class HIPGraphExecutor:
         self._dependents = []
         self.closed = True
         self._free_greedy()
+        self._free_sampled()
         if self.graph_exec is not None:
             self.hip.graph_exec_destroy(self.graph_exec)
             self.hip.graph_destroy(self.graph)

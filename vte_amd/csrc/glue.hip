@@ -810,7 +810,7 @@ __global__ void greedy_advance_kernel(const int* __restrict__ top_idx, int k, in
     const int s = s_step;
     for (int b = threadIdx.x; b < rows; b += blockDim.x) {
         const int tok = top_idx[(size_t)b * k];
-        tokens[b] = tok;
+        tokens[b] = max(tok, 0);  // (-1: nothing was drawn; recorded, and no row of the embedding)
         kv_offset[b] = min(kv_offset[b] + 1, max_pos);
         if (s < hist_steps) history[(size_t)s * rows + b] = tok;
     }
