@@ -395,3 +395,198 @@ def test_attention_does_not_depend_on_the_batch(hip, K, new):
         K.attn_pages(b.pages, r, up(hip, q[:sum(n)]), do, 4, 0.09, empty(hip, need, np.uint8), need, stream=hip.stream)
         res.append(down(do)[:new].astype(np.float64))
     assert np.abs(res[0] - res[1]).max() <= 2.0 ** -9 * np.abs(res[1]).max()
+
+
+# ---------------------------------------------------------------------------- together, captured, on other streams
+def test_captured_decode_loop(hip, K):
+    """Embedding (q, k and v rows of a token), append, attention, LM head, draw and feedback as one captured graph,
+    replayed 30 times over ragged sequences that cross blocks and pages: every replay's cache is the oracle's, its
+    logits within the attention's bounds of the oracle's, its tokens the draws from these logits."""
+    from oracle import sampling as osm
+    from oracle.dequant import dequantize_matrix
+    from vte_amd import synthetic as syn
+    rng = np.random.default_rng(31)
+    n_q, n_kv, hd, V, start = 6, 2, 64, 1000, [0, 13, 30, 47]
+    B, width, qd = 4, (n_q + 2 * n_kv) * hd, n_q * hd
+    bt = Batch(hip, K, rng, [s + 31 for s in start], n_kv, hd, 16)
+    for b, n in enumerate(start):
+        append_ref(bt, b, 0, *(normal(rng, (n, n_kv, hd), "f16") for _ in "kv"))
+    bt.upload()
+    table, head = syn.random_matrix("q8_0", rng, V, width), syn.random_matrix("q8_0", rng, V, qd)
+    rows_f = dequantize_matrix("q8_0", table, V, width).astype(np.float16)
+    head_f = dequantize_matrix("q8_0", head, V, qd).astype(np.float64)
+    cos, sin = build_rope_cache(96, hd, 1e4)
+    steps = 30
+    us = rng.random((steps, B))
+    d = {n: up(hip, v) for n, v in dict(table=table, head=head, cos=cos, sin=sin, tok=np.arange(B, dtype=np.int32),
+                                        step=np.zeros(1, np.int32), T=np.full(B, 0.8, np.float32),
+                                        p=np.full(B, 0.9, np.float32), u=us[0]).items()}
+    x, att, logits = empty(hip, (B, width), np.float16), empty(hip, (B, n_q, hd), np.float16), empty(hip, (B, V), np.float32)
+    nxt, hist = empty(hip, B, np.int32), empty(hip, (steps, B), np.int32)
+    r = bt.rows(start)
+    off = bt.d["off"]
+    need, sneed = K.attn_pages_scratch_bytes(bt.pages, r, n_q), K.sample_scratch_bytes(B)
+    scratch, sscratch = empty(hip, need, np.uint8), empty(hip, sneed, np.uint8)
+    st, scale = hip.stream, 1 / math.sqrt(hd)
+
+    def step():
+        K.embedding("q8_0", d["tok"], d["table"], x, B, width, stream=st)
+        K.kv_pages_append(bt.pages, r, x.ptr + 2 * qd, x.ptr + 2 * (qd + n_kv * hd), q=x, q_out=att, n_q=n_q,
+                          rope_cos=d["cos"], rope_sin=d["sin"], rope_rows=96, k_stride=width, v_stride=width,
+                          q_stride=width, stream=st)
+        K.attn_pages(bt.pages, r, att, att, n_q, scale, scratch, need, stream=st)  # in place
+        K.gemv("q8_0", att, d["head"], logits, B, qd, V, in_dtype="f16", out_dtype="f32", stream=st)
+        K.sample(logits, B, V, nxt, sscratch, temperature=d["T"], top_p=d["p"], u=d["u"], stream=st)
+        K.greedy_advance(nxt, 1, B, d["tok"], off, 95, hist, steps, d["step"], stream=st)
+
+    hip.stream_synchronize()
+    hip.stream_begin_capture()
+    try:
+        step()
+    finally:
+        g = hip.stream_end_capture()
+    ge = hip.graph_instantiate(g)
+    toks, pos = np.arange(B), list(start)
+    try:
+        for i in range(steps):
+            d["u"].upload(us[i])
+            hip.graph_launch(ge)
+            hip.synchronize()
+            got = down(logits).astype(np.float64)
+            w = rows_f[toks].astype(np.float32).reshape(B, n_q + 2 * n_kv, hd)
+            for b in range(B):
+                q = okv.rotate(w[b:b + 1, :n_q], [pos[b]], cos, sin).astype(np.float16)[0]
+                append_ref(bt, b, pos[b], okv.rotate(w[b:b + 1, n_q:n_q + n_kv], [pos[b]], cos, sin), w[b:b + 1, n_q + n_kv:])
+                kv = bt.ref.k[b].values(pos[b] + 1), bt.ref.v[b].values(pos[b] + 1)
+                o, mag, big = okv.attention(q, *kv, pos[b], scale)
+                tol = attn_tolerance("f16", hd, o, mag, big, np.abs(kv[1]).max()).reshape(-1)
+                want = head_f @ o.reshape(-1)
+                # the head's products and sums in fp32: 2^-24 of the sum of |products| for each of qd + 8 roundings
+                slack = np.abs(head_f) @ tol + (qd + 8) * 2.0 ** -24 * (np.abs(head_f) @ (np.abs(o.reshape(-1)) + tol))
+                assert (np.abs(got[b] - want) <= slack).all(), (i, b)
+                t, near = osm.sample(got[b], float(np.float32(0.8)), 0, float(np.float32(0.9)), 0.0, us[i, b])
+                drawn = int(down(d["tok"])[b])
+                assert drawn == t or near < V * 2.0 ** -44
+            toks, pos = down(d["tok"]).copy(), [p + 1 for p in pos]
+            if i % 10 == 0:
+                bt.check(pos)
+                check_attention(hip, K, bt, [p - 3 for p in pos], [2] * B, n_q, "f32", rng)  # eager work in between
+                off.upload(np.array(pos, np.int32))
+                r.kv_offset = off.ptr  # (the check staged its own offsets elsewhere)
+                bt.d["off"] = off
+        bt.check(pos)
+        assert (down(hist) >= 0).all()
+    finally:
+        hip.graph_exec_destroy(ge)
+        hip.graph_destroy(g)
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_captured_attention_follows_staged_lengths(hip, K, new):
+    """Lengths, rows and pages are read on the device: one captured launch serves other lengths and tables."""
+    rng = np.random.default_rng(new)
+    bt = filled(hip, K, rng, [300, 170, 64], 2, 128, 32)
+    q = normal(rng, (3 * new, 4, 128), "f16")
+    dq, do = up(hip, q), empty(hip, q.shape, np.float16)
+    r = bt.rows([0, 0, 0], [new] * 3)
+    off = bt.d["off"]
+    n = K.attn_pages_scratch_bytes(bt.pages, r, 4)
+    scratch = empty(hip, n, np.uint8)
+    hip.stream_synchronize()
+    hip.stream_begin_capture()
+    K.attn_pages(bt.pages, r, dq, do, 4, 0.09, scratch, n, stream=hip.stream)
+    g = hip.stream_end_capture()
+    ge = hip.graph_instantiate(g)
+    try:
+        for pos in ([300 - new, 170 - new, 64 - new], [0, 0, 0], [17, -1, 5], [300 - new, 3, 0]):
+            off.upload(np.array(pos, np.int32))
+            hip.graph_launch(ge)
+            got = down(do).astype(np.float64)
+            for b in range(3):
+                kv = bt.ref.k[b].values(bt.ref.cap), bt.ref.v[b].values(bt.ref.cap)
+                for i in range(new):
+                    o, mag, big = okv.attention(q[b * new + i], *kv, pos[b] + i if pos[b] >= 0 else -1, 0.09,
+                                                np.array([not bt.drop(b, t) for t in range(bt.ref.cap)]))
+                    tol = attn_tolerance("f16", 128, o, mag, big, 8.0)
+                    assert matches("f16", got[b * new + i], o, tol).all(), (pos, b, i)
+    finally:
+        hip.graph_exec_destroy(ge)
+        hip.graph_destroy(g)
+
+
+def test_two_streams_at_once(hip, K):
+    """Prompt and decode attention on two streams that are not the runtime's, each with its own scratch, in turn and
+    together: the results of each alone."""
+    import ctypes
+    rng = np.random.default_rng(41)
+    streams = []
+    for _ in range(2):
+        s = ctypes.c_void_p()
+        hip._check_error(hip._lib.hipStreamCreate(ctypes.byref(s)), "hipStreamCreate")
+        streams.append(s)
+    jobs = []
+    for new in (1, 150):
+        bt = filled(hip, K, rng, [900, 333], 2, 128, 64)
+        q = up(hip, normal(rng, (2 * new, 8, 128), "f16"))
+        r = bt.rows([900 - new, 333 - new], [new, new])
+        n = K.attn_pages_scratch_bytes(bt.pages, r, 8)
+        jobs.append((bt, r, q, empty(hip, (2 * new, 8, 128), np.float16), empty(hip, n, np.uint8), n))
+    try:
+        alone = []
+        for (bt, r, q, o, sc, n), s in zip(jobs, streams):
+            K.attn_pages(bt.pages, r, q, o, 8, 0.1, sc, n, stream=s)
+            hip.synchronize()
+            alone.append(down(o).copy())
+        for _ in range(10):
+            for (bt, r, q, o, sc, n), s in zip(jobs, streams):
+                K.attn_pages(bt.pages, r, q, o, 8, 0.1, sc, n, stream=s)
+        hip.synchronize()
+        for (_, _, _, o, _, _), a in zip(jobs, alone):
+            assert np.array_equal(down(o), a)
+    finally:
+        for s in streams:
+            hip._lib.hipStreamDestroy(s)
+
+
+def test_offsets_past_32_bits(hip, K):
+    """A pool of 5 GiB of K: pages beyond 2^32 bytes are written and read in their places."""
+    rng = np.random.default_rng(51)
+    page, n_kv, hd = 4096, 2, 128
+    n_pages = 5 * 2 ** 30 // (page * n_kv * hd)
+    size, blocks = n_pages * page * n_kv * hd, n_pages * n_kv * page // 16
+    d = {n: empty_raw(hip, s) for n, s in (("k", size), ("v", size), ("ke", blocks), ("ve", blocks))}
+    table = np.array([[n_pages - 1], [1], [n_pages - 2]], np.int32)
+    lens = [70, 33, 20]
+    ref = okv.Cache(3, n_kv, hd, 1, page)
+    new = [up(hip, normal(rng, (sum(lens), n_kv, hd), "f16")) for _ in "kv"]
+    k, v = (down(x).astype(np.float32) for x in new)
+    first = np.cumsum([0] + lens)
+    for b, n in enumerate(lens):
+        ref.k[b].append(k[first[b]:first[b + 1]], 0)
+        ref.v[b].append(v[first[b]:first[b + 1]], 0)
+    dt, off, start = up(hip, table), up(hip, np.zeros(3, np.int32)), up(hip, first.astype(np.int32))
+    pages = KVPages.of(d["k"], d["v"], d["ke"], d["ve"], n_pages, page, n_kv, hd)
+    rows = KVRows.of(3, sum(lens), max(lens), start, off, dt, 1)
+    K.kv_pages_append(pages, rows, *new, stream=hip.stream)
+    ko, vo = empty(hip, (3, 80, n_kv, hd), np.float16), empty(hip, (3, 80, n_kv, hd), np.float16)
+    K.kv_pages_read(pages, rows, ko, vo, 80, stream=hip.stream)
+    for got, parts in ((down(ko), ref.k), (down(vo), ref.v)):
+        for b, n in enumerate(lens):
+            assert np.array_equal(got[b, :n], parts[b].values(n).astype(np.float16))
+    one = KVRows.of(3, 3, 1, None, up(hip, np.array([n - 1 for n in lens], np.int32)), dt, 1)
+    for r, q in ((one, normal(rng, (3, 4, hd), "f16")), (rows, normal(rng, (sum(lens), 4, hd), "f16"))):
+        n = K.attn_pages_scratch_bytes(pages, r, 4)
+        do = empty(hip, q.shape, np.float16)
+        K.attn_pages(pages, r, up(hip, q), do, 4, 0.1, empty(hip, n, np.uint8), n, stream=hip.stream)
+        got = down(do).astype(np.float64)
+        for b, m in enumerate(lens):
+            for i in ([m - 1] if r is one else range(m)):
+                row = b if r is one else first[b] + i
+                o, mag, big = okv.attention(q[row], ref.k[b].values(m), ref.v[b].values(m), i, 0.1)
+                assert matches("f16", got[row], o, attn_tolerance("f16", hd, o, mag, big, 8.0)).all()
+    for p in d.values():
+        hip.safe_free(p)
+
+
+def empty_raw(hip, nbytes):
+    return hip.safe_malloc(nbytes, "pool")

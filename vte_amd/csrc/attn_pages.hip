@@ -189,7 +189,7 @@ struct PaTile {
 
 template <typename T, int HD>
 __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(KvPages c, KvRows r, PaPlan pl,
-                                                                 const T* __restrict__ q, T* __restrict__ out, int n_q,
+                                                                 const T* q, T* out, int n_q,
                                                                  float scale) {
     constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;  // fp16 parts of q and of the probabilities
     constexpr int KC = HD / 64;                    // 16-byte pieces of a K row that a lane holds
@@ -574,7 +574,7 @@ __device__ __forceinline__ void pa_store(T* dst, const floatx16_t (&o)[N], float
 // grid (row blocks, n_kv, nsp), the last row blocks (which see most) first; nsp > 1 with two groups only.
 template <typename T, int HD, int GROUPS>
 __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, KvRows r, PaPrompt pp,
-                                                                   const T* __restrict__ q, T* __restrict__ out,
+                                                                   const T* q, T* out,
                                                                    int n_q, float scale) {
     constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;
     constexpr int WAVES = 8 / GROUPS, ROWS = 32 * WAVES;  // of a group
