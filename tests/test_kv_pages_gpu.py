@@ -250,10 +250,11 @@ def matches(dtype, got, out, tol):
         return ok | (np.isinf(got) & (np.abs(out) + tol >= 65520) & (got * out > 0)) if dtype == "f16" else ok
 
 
-def check_attention(hip, K, bt, pos, new, n_q, dtype, rng, pad=0, q_scale=1.0, row_start=True):
+def check_attention(hip, K, bt, pos, new, n_q, dtype, rng, pad=0, q_scale=1.0, row_start=True, zero_dims=0, before=None):
     B, hd = len(pos), bt.hd
     R = sum(new)
     q = normal(rng, (R + pad, n_q, hd), dtype, q_scale)
+    q[:, :, :zero_dims] = 0
     out = np.full(q.shape, 5, NP[dtype])
     do = up(hip, out)
     r = bt.rows(pos, new if row_start else None, pad)
@@ -266,8 +267,11 @@ def check_attention(hip, K, bt, pos, new, n_q, dtype, rng, pad=0, q_scale=1.0, r
     for b in range(B):
         kv = bt.ref.k[b].values(bt.ref.cap), bt.ref.v[b].values(bt.ref.cap)
         present = np.array([not bt.drop(b, t) for t in range(bt.ref.cap)])
-        vmax = np.abs(kv[1][np.isfinite(kv[1])]).max(initial=0)
         for i in range(new[b]):
+            if before is not None and pos[b] + i >= before:
+                continue
+            seen = kv[1][:max(pos[b] + i + 1, 0)]
+            vmax = np.abs(seen[np.isfinite(seen)]).max(initial=0)
             o, mag, big = okv.attention(q[first[b] + i], *kv, pos[b] + i if pos[b] >= 0 else -1, scale, present)
             g = got[first[b] + i]
             assert np.array_equal(np.isnan(g), np.isnan(o)), (b, i)
@@ -375,6 +379,36 @@ def test_attention_scales_and_peaks(hip, K, dtype, new, v_sizes, q_scale):
     rng = np.random.default_rng(8)
     bt = filled(hip, K, rng, [900, 71], 1, 128, 64, v_sizes=v_sizes)
     check_attention(hip, K, bt, [900 - new, 71 - new], [new, new], 6, dtype, rng, q_scale=q_scale)
+
+
+@pytest.mark.parametrize("power", [20, 40, 100])
+@pytest.mark.parametrize("new,n_q,hd", [(4, 4, 128), (70, 2, 128), (150, 4, 64), (600, 16, 128)])
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_attention_of_rows_before_huge_tokens(hip, K, dtype, new, n_q, hd, power):
+    """Tokens that a row does not see leave its result alone, however large they are (those of blocks of their own: a
+    block has one scale)."""
+    rng = np.random.default_rng(new + power)
+    n, at = 800, 800 - new // 2 - (800 - new // 2) % 16
+    bt = Batch(hip, K, rng, [n], 1, hd, 64)
+    k, v = rng.standard_normal((2, n, 1, hd)).astype(np.float32)
+    k[at:] *= 2.0 ** power
+    v[at:] *= 2.0 ** power
+    append_ref(bt, 0, 0, k, v)
+    bt.upload()
+    check_attention(hip, K, bt, [n - new], [new], n_q, dtype, rng, before=at)
+
+
+@pytest.mark.parametrize("new", [1, 70])
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_attention_beside_huge_keys_in_other_dims(hip, K, dtype, new):
+    """Keys of one block are 2^60 times the others', in dims that no query has: scores of both are ordinary."""
+    rng = np.random.default_rng(12)
+    bt = Batch(hip, K, rng, [300], 2, 128, 64)
+    k, v = rng.standard_normal((2, 300, 2, 128)).astype(np.float32)
+    k[112:128, :, :4] *= 2.0 ** 60
+    append_ref(bt, 0, 0, k, v)
+    bt.upload()
+    check_attention(hip, K, bt, [300 - new], [new], 6, dtype, rng, zero_dims=4)
 
 
 @pytest.mark.parametrize("new", [1, 30])

@@ -91,7 +91,7 @@ struct PaPlan {
     int blocks;  // grid of the main launch
     int ncol;    // columns (rows of the second form) of a record
     float* ml;   // [2 blocks][ncol][2]: maximum (log2), sum
-    int* ev;     // [2 blocks]: exponent the record's sums are relative to
+    int* ev;     // [2 blocks][ncol]: exponent that the sums are relative to
     float* o;    // [2 blocks][ncol][HD]
     int2* seg;   // [segments]: first block, pieces
 };
@@ -195,7 +195,7 @@ __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(KvPages c, KvRo
     constexpr int KC = HD / 64;                    // 16-byte pieces of a K row that a lane holds
     constexpr int DT = HD / 16;
     __shared__ float m_sh[4][16], l_sh[4][16];
-    __shared__ int ev_sh[4];
+    __shared__ int ev_sh[4][16];
     __shared__ __align__(16) float o_sh[4][16][HD + 4];
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, grp = lane >> 4;
@@ -260,7 +260,7 @@ __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(KvPages c, KvRo
         const float c2 = scale * 1.44269504088896340736f * q_unit;  // exp(scale s) = 2^(c2 s)
 
         float m_run = PA_NONE, l_run = 0.f;
-        int ev_ref = KVP_E_MIN;
+        int ev_ref = KVP_E_MIN;  // largest V exponent that the column has seen
         floatx4_t o[DT];  // lane: column col, dims 16 dt + 4 grp + i
 #pragma unroll
         for (int i = 0; i < DT; ++i) o[i] = floatx4_t{0.f, 0.f, 0.f, 0.f};
@@ -314,9 +314,8 @@ __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(KvPages c, KvRo
                     mx = fmaxf(mx, sc[tt][i]);
                 }
             mx = pa_max4(mx);
-            const bool in_use = x.has && p0 < len;
-            const int evm = max(ev_ref, pa_max4(in_use ? x.ev : KVP_E_MIN));
-            if (__any(mx > m_run) || evm > ev_ref) {
+            const int evm = max(ev_ref, pa_max4(live > 0 ? x.ev : KVP_E_MIN));
+            if (__any((mx > m_run) | (evm > ev_ref))) {
                 const float corr = __builtin_amdgcn_exp2f(m_run - mx);
                 l_run *= corr;
                 const float both = corr * pa_pow2(ev_ref - evm);
@@ -369,25 +368,25 @@ __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(KvPages c, KvRo
         if (grp == 0) {
             m_sh[wv][col] = m_run;
             l_sh[wv][col] = l_run;
+            ev_sh[wv][col] = ev_ref;
         }
-        if (lane == 0) ev_sh[wv] = ev_ref;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<floatx4_t*>(&o_sh[wv][col][16 * dt + 4 * grp]) = o[dt];
         __syncthreads();
         const int seg = b * c.n_kv + h;
         const int first = (int)(seg_t / sh.share), pieces = (int)((seg_t + nt - 1) / sh.share) - first + 1;
         const size_t rec = pa_rec(first, blockIdx.x - first);
-        const int EV = max(max(ev_sh[0], ev_sh[1]), max(ev_sh[2], ev_sh[3]));
         for (int i = tid; i < ncol * (HD / 4); i += 256) {
             const int cc = i / (HD / 4), d = i % (HD / 4) * 4;
             const float M = fmaxf(fmaxf(m_sh[0][cc], m_sh[1][cc]), fmaxf(m_sh[2][cc], m_sh[3][cc]));
+            const int EV = max(max(ev_sh[0][cc], ev_sh[1][cc]), max(ev_sh[2][cc], ev_sh[3][cc]));
             float L = 0.f;
             floatx4_t O = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
                 const float f = __builtin_amdgcn_exp2f(m_sh[w][cc] - M);
                 L = fmaf(l_sh[w][cc], f, L);
-                O += *reinterpret_cast<const floatx4_t*>(&o_sh[w][cc][d]) * (f * pa_pow2(ev_sh[w] - EV));
+                O += *reinterpret_cast<const floatx4_t*>(&o_sh[w][cc][d]) * (f * pa_pow2(ev_sh[w][cc] - EV));
             }
             if (pieces == 1) {
                 const int i_row = cc / G;
@@ -399,13 +398,11 @@ __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(KvPages c, KvRo
                 if (d == 0) {
                     pl.ml[(rec * pl.ncol + cc) * 2] = M;
                     pl.ml[(rec * pl.ncol + cc) * 2 + 1] = L;
+                    pl.ev[rec * pl.ncol + cc] = EV;
                 }
             }
         }
-        if (tid == 0) {
-            if (pieces > 1) pl.ev[rec] = EV;
-            if (a == 0) pl.seg[seg] = make_int2(first, pieces);
-        }
+        if (tid == 0 && a == 0) pl.seg[seg] = make_int2(first, pieces);
         __syncthreads();
         t += z - a;
     }
@@ -438,7 +435,7 @@ __global__ __launch_bounds__(256) void attn_pages_combine_kernel(KvPages c, KvRo
     for (int i = tid; i < sg.y; i += 256) {
         const size_t rec = pa_rec(sg.x, i);
         M = fmaxf(M, pl.ml[(rec * pl.ncol + cc) * 2]);
-        EV = max(EV, pl.ev[rec]);
+        EV = max(EV, pl.ev[rec * pl.ncol + cc]);
     }
     M = wave_max(M);
     for (int x = 1; x < 64; x *= 2) EV = max(EV, __shfl_xor(EV, x, 64));
@@ -457,7 +454,7 @@ __global__ __launch_bounds__(256) void attn_pages_combine_kernel(KvPages c, KvRo
             const size_t rec = pa_rec(sg.x, i0 + tid);
             const float f = __builtin_amdgcn_exp2f(pl.ml[(rec * pl.ncol + cc) * 2] - M);
             l = fmaf(pl.ml[(rec * pl.ncol + cc) * 2 + 1], f, l);
-            w_sh[tid] = f * pa_pow2(pl.ev[rec] - EV);
+            w_sh[tid] = f * pa_pow2(pl.ev[rec * pl.ncol + cc] - EV);
         }
         __syncthreads();
 #pragma unroll 4
@@ -489,13 +486,17 @@ __global__ __launch_bounds__(256) void attn_pages_combine_kernel(KvPages c, KvRo
 // four that take every other step and whose sums meet in LDS at the end (GROUPS =
 // 2: half as many rows, so twice as many blocks or half as many shares).  The bytes
 // of a step become fp16 once per group on their way into LDS, times 2^(e - ref)
-// with ref the largest exponent so far (exact down to 2^-24 of the largest block's
-// step), so a step's scores and sums have one scale.  Scores are K.Q^T, sums are
+// with ref the largest exponent of the step (K) or so far (V), so a step's scores
+// and sums have one scale.  That is exact while no block lies below 2^-24 of ref
+// (PA_APART); a row's result must not depend on how large tokens are that it does
+// not see, so a wave that met such a block does its rows over, block by block
+// (pa_apart, some ten times as long).  Scores are K.Q^T, sums are
 // V^T.P^T (a lane is a row in both), K rows are read with token bits 2 and 3
 // swapped so that a lane's scores are its operand of the second product as they
 // stand.
 // ---------------------------------------------------------------------------
 #define PA_SHARES 16
+#define PA_APART 24
 
 typedef float floatx16_t __attribute__((ext_vector_type(16)));
 
@@ -547,7 +548,7 @@ __device__ __forceinline__ int pa_share_of(int steps, int nsp) {
 struct PaPrompt {
     int nsp;    // shares of a row block
     float* ml;  // [row blocks][n_kv][nsp][128][2]: maximum (log2), sum
-    int* ev;    // [row blocks][n_kv][nsp][4]: exponent the record's sums are relative to, per 32 rows
+    int* ev;    // [row blocks][n_kv][nsp][128]: exponent that the row's sums are relative to
     float* o;   // [row blocks][n_kv][nsp][128][HD]
 };
 
@@ -569,6 +570,81 @@ __device__ __forceinline__ void pa_store(T* dst, const floatx16_t (&o)[N], float
             if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(dst + 32 * i + 8 * j) = r.u2;
             else *reinterpret_cast<uint4*>(dst + 32 * i + 8 * j) = r.u4[0];
         }
+}
+
+// The sums of a wave's rows over steps first, first + GROUPS, .. below z with one scale per block and row: K and V as
+// whole numbers, scores in fp32 by two-element products, each row's sums relative to the largest exponent it sees.
+// Blocks of the least exponent hold zeros, or values below 2^-119 that count as zeros beside larger ones: they alone do
+// not lead here.
+template <typename T, int HD, int GROUPS, int PARTS, int KS, int DT>
+__device__ __forceinline__ void pa_apart(const KvPages& c, const int* table, int max_pages, int h, int first, int z,
+                                         int seg_end, int end, int half, const half8_t (&qb)[PARTS][KS], float c2,
+                                         float& m_run, float& l_run, int& ev_row, floatx16_t (&o)[DT]) {
+    const int bl = c.page_log2 - 4;
+    m_run = PA_NONE;
+    l_run = 0.f;
+    ev_row = KVP_E_MIN;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
+    for (int blk = 4 * first; blk < 4 * z && blk * KVP_BLOCK < seg_end;
+         blk += blk % 4 == 3 ? 4 * GROUPS - 3 : 1) {
+        const int page = table[min(blk >> bl, max_pages - 1)];
+        if ((unsigned)page >= (unsigned)c.n_pages) continue;
+        const size_t at = (((size_t)page * c.n_kv + h) << bl) + (blk & ((1 << bl) - 1));
+        const int ek = c.k_exp[at], ev = c.v_exp[at], n = end - blk * KVP_BLOCK;  // places that the row sees
+        const uint8_t* kr = c.k + at * (KVP_BLOCK * HD) + 8 * half;
+        const uint8_t* vr = c.v + at * (KVP_BLOCK * HD) + 4 * half * KVP_BLOCK;
+        float w[KVP_BLOCK], mx = m_run;
+        const float kf = kvp_scale(ek) * c2;
+#pragma unroll
+        for (int t = 0; t < KVP_BLOCK; ++t) {
+            float s = 0.f;
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+                const uint2 b = *reinterpret_cast<const uint2*>(kr + t * HD + 16 * i);
+                union {
+                    half8_t v;
+                    pa_h2 h[4];
+                } k, x;
+                k.v = pa_half8(b.x, b.y);
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p) {
+                    x.v = qb[p][i];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) s = __builtin_amdgcn_fdot2(k.h[j], x.h[j], s, false);
+                }
+            }
+            const pa_u2 u = __builtin_amdgcn_permlane32_swap(__float_as_uint(s), __float_as_uint(s), false, false);
+            w[t] = t < n ? (__uint_as_float(u[0]) + __uint_as_float(u[1])) * kf : -INFINITY;
+            mx = fmaxf(mx, w[t]);
+        }
+        const int evm = n > 0 ? max(ev_row, ev) : ev_row;
+        const float corr = __builtin_amdgcn_exp2f(m_run - mx), both = corr * pa_pow2(ev_row - evm);
+        const float vf = ev == KVP_E_NAN ? NAN : pa_pow2(min(ev - evm, 0));
+        l_run *= corr;
+#pragma unroll
+        for (int t = 0; t < KVP_BLOCK; ++t) {
+            const float p = __builtin_amdgcn_exp2f(w[t] - mx + (float)PA_P_LOG2);
+            l_run += p;
+            w[t] = t < n ? p * vf : 0.f;
+        }
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const uint4 b = ldg_g16(vr + (32 * dt + 8 * (i / 4) + i % 4) * KVP_BLOCK);
+                const half8_t v0 = pa_half8(b.x, b.y), v1 = pa_half8(b.z, b.w);
+                float x = o[dt][i] * both;
+#pragma unroll
+                for (int t = 0; t < 8; ++t) x = fmaf((float)v0[t], w[t], fmaf((float)v1[t], w[8 + t], x));
+                o[dt][i] = x;
+            }
+        m_run = mx;
+        ev_row = evm;
+    }
+    if (half) l_run = 0.f;  // (both halves hold the whole sum)
 }
 
 // grid (row blocks, n_kv, nsp), the last row blocks (which see most) first; nsp > 1 with two groups only.
@@ -593,7 +669,7 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
     };
     __shared__ Shared S;
     __shared__ float m_sh[GROUPS][ROWS], l_sh[GROUPS][ROWS];
-    __shared__ int ev_sh[GROUPS][WAVES];
+    __shared__ int ev_sh[GROUPS][ROWS];
     const int tid = threadIdx.x & (64 * WAVES - 1), lane = threadIdx.x & 63;
     const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & (WAVES - 1);
     const int grp = GROUPS == 2 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 8) : 0;
@@ -685,12 +761,15 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
 #pragma unroll
         for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
     int o_ref = KVP_E_MIN;                              // exponent that o is relative to
-    int k_ref = KVP_E_MIN, v_ref = KVP_E_MIN;           // of the step staged last
+    int k_ref = KVP_E_MIN, v_ref = KVP_E_MIN;           // of the step staged last: its largest, the largest so far
     int next_odd = 0;                                   // its blocks without a page, and with NaN in V
+    int apart = 0;                                      // some blocks' scales lie too far apart for all this
     auto put = [&](Tile& D) {
         next_odd = 0;
         int e[4], f[4];
         const int my_k = got ? ek : -1000, my_v = got ? ev : -1000;  // -1000: times 0
+        const int v_old = v_ref;
+        k_ref = KVP_E_MIN;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             e[j] = __builtin_amdgcn_readlane(my_k, j);
@@ -699,6 +778,9 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
             k_ref = max(k_ref, e[j]);
             v_ref = max(v_ref, f[j]);
         }
+        // (lane j & 3: of block j; the last one: sums that vanish in fp32 beside larger ones)
+        apart |= ((my_k > KVP_E_MIN) & (my_k < k_ref - PA_APART)) | ((my_v > KVP_E_MIN) & (my_v < v_ref - PA_APART)) |
+                 ((v_old > KVP_E_MIN) & (v_ref - v_old > 96));
 #pragma unroll
         for (int u = 0; u < NP; ++u) {
             const int j = first(u) / HD, piece = first(u) % HD + lane;
@@ -827,19 +909,23 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
         buf ^= 1;
     }
 
+    int ev_row = o_ref;  // of this lane's row
+    if (__any(apart))
+        pa_apart<T, HD, GROUPS>(c, table, r.max_pages, h, a + grp, z, seg_end, end, half, qb, c2, m_run, l_run, ev_row, o);
+
     // ---- results ----
     {
         const pa_u2 w = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_run), __float_as_uint(l_run), false, false);
         l_run = __uint_as_float(w[0]) + __uint_as_float(w[1]);
     }
     if constexpr (GROUPS == 1) {
-        if (r0 + row < rows) pa_store<T, DT>(dst + 4 * half, o, l_run, o_ref);
+        if (r0 + row < rows) pa_store<T, DT>(dst + 4 * half, o, l_run, ev_row);
     } else {  // each group leaves half of the dims to the other
         if (half == 0) {
             m_sh[grp][wv * 32 + row] = m_run;
             l_sh[grp][wv * 32 + row] = l_run;
+            ev_sh[grp][wv * 32 + row] = ev_row;
         }
-        if (lane == 0) ev_sh[grp][wv] = o_ref;
         floatx16_t mine[DT / 2];
 #pragma unroll
         for (int i = 0; i < DT / 2; ++i) {
@@ -850,10 +936,10 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
         }
         __syncthreads();
         const float m2 = m_sh[grp ^ 1][wv * 32 + row], M = fmaxf(m_run, m2);
-        const int e2 = ev_sh[grp ^ 1][wv], EV = max(o_ref, e2);
+        const int e2 = ev_sh[grp ^ 1][wv * 32 + row], EV = max(ev_row, e2);
         const float f1 = __builtin_amdgcn_exp2f(m_run - M), f2 = __builtin_amdgcn_exp2f(m2 - M);
         const float L = l_run * f1 + l_sh[grp ^ 1][wv * 32 + row] * f2;
-        const float g1 = f1 * pa_pow2(o_ref - EV), g2 = f2 * pa_pow2(e2 - EV);
+        const float g1 = f1 * pa_pow2(ev_row - EV), g2 = f2 * pa_pow2(e2 - EV);
 #pragma unroll
         for (int i = 0; i < DT / 2; ++i)
 #pragma unroll
@@ -871,8 +957,8 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
             if (half == 0 && grp == 0) {
                 pp.ml[(rec * ROWS + wv * 32 + row) * 2] = M;
                 pp.ml[(rec * ROWS + wv * 32 + row) * 2 + 1] = L;
+                pp.ev[rec * ROWS + wv * 32 + row] = EV;
             }
-            if (lane == 0 && grp == 0) pp.ev[4 * rec + wv] = EV;
         } else if (r0 + row < rows) {
             pa_store<T, DT / 2>(dst + d0, mine, L, EV);
         }
@@ -896,7 +982,7 @@ __global__ __launch_bounds__(256) void attn_pages_prompt_combine_kernel(KvPages 
     int EV = KVP_E_MIN;
     for (int i = 0; i < pieces; ++i) {
         M = fmaxf(M, pp.ml[((rec0 + i) * ROWS + rr) * 2]);
-        EV = max(EV, pp.ev[4 * (rec0 + i) + rr / 32]);
+        EV = max(EV, pp.ev[(rec0 + i) * ROWS + rr]);
     }
     floatx4_t O = {0.f, 0.f, 0.f, 0.f};
     for (int i0 = 0; i0 < pieces; i0 += 4) {  // four requested together (past the last one: the last again)
@@ -909,7 +995,7 @@ __global__ __launch_bounds__(256) void attn_pages_prompt_combine_kernel(KvPages 
             o[i] = *reinterpret_cast<const floatx4_t*>(pp.o + (rec * ROWS + rr) * HD + d);
             m[i] = pp.ml[(rec * ROWS + rr) * 2];
             l[i] = pp.ml[(rec * ROWS + rr) * 2 + 1];
-            ev[i] = pp.ev[4 * rec + rr / 32];
+            ev[i] = pp.ev[rec * ROWS + rr];
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -947,7 +1033,7 @@ static PaPlan rows_plan(const KvPages& c, const KvRows& r, int hd, int G, void* 
     p.ml = reinterpret_cast<float*>(at + n);
     n += pa_up(recs * p.ncol * 8);
     p.ev = reinterpret_cast<int*>(at + n);
-    n += pa_up(recs * 4);
+    n += pa_up(recs * p.ncol * 4);
     p.seg = reinterpret_cast<int2*>(at + n);
     n += pa_up(segments * 8);
     *bytes = n;
@@ -976,7 +1062,7 @@ static PromptForm prompt_form(const KvPages& c, const KvRows& r, int hd, int G, 
     f.p.ml = reinterpret_cast<float*>(at + n);
     n += pa_up(recs * 128 * 8);
     f.p.ev = reinterpret_cast<int*>(at + n);
-    n += pa_up(recs * 16);
+    n += pa_up(recs * 128 * 4);
     f.bytes = n;
     return f;
 }
