@@ -411,6 +411,22 @@ def test_attention_beside_huge_keys_in_other_dims(hip, K, dtype, new):
     check_attention(hip, K, bt, [300 - new], [new], 6, dtype, rng, zero_dims=4)
 
 
+@pytest.mark.parametrize("new", [2, 70])
+def test_attention_of_positions_at_the_end_of_int(hip, K, new):
+    """Positions behind the table see all of it, up to the largest int; what they append has no place."""
+    rng = np.random.default_rng(13)
+    bt = filled(hip, K, rng, [128, 128], 2, 64, 64)
+    check_attention(hip, K, bt, [2 ** 31 - 1, 2 ** 31 - new], [new, new], 4, "f32", rng)
+    r = bt.rows([2 ** 31 - 1, 2 ** 31 - new], [new, new])
+    x = up(hip, normal(rng, (2 * new, 2, 64), "f16"))
+    K.kv_pages_append(bt.pages, r, x, x, stream=hip.stream)
+    bt.check([128, 128])
+    ko, vo = empty(hip, (2, 128, 2, 64), np.float32), empty(hip, (2, 128, 2, 64), np.float32)
+    K.kv_pages_read(bt.pages, r, ko, vo, 128, dtype="f32", stream=hip.stream)
+    for b in range(2):
+        assert np.array_equal(down(ko)[b], bt.ref.k[b].values(128)) and np.array_equal(down(vo)[b], bt.ref.v[b].values(128))
+
+
 @pytest.mark.parametrize("new", [1, 30])
 def test_attention_does_not_depend_on_the_batch(hip, K, new):
     """Equal bits for a sequence alone, in a batch and in other pages."""

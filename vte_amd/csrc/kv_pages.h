@@ -40,13 +40,13 @@ struct KvSeq {
 };
 __device__ __forceinline__ KvSeq kvp_place(const KvRows& r, int b) {  // its rows, whether it runs or not
     KvSeq s;
-    s.pos = r.kv_offset[b];
+    s.pos = min(r.kv_offset[b], 1 << 30);  // (no table reaches further; pos + row stays an int)
     if (r.row_start == nullptr) {
         s.first = b;
         s.n = r.max_rows;
     } else {
-        s.first = max(r.row_start[b], 0);
-        s.n = max(min(min(r.row_start[b + 1], r.rows) - s.first, r.max_rows), 0);
+        s.first = min(max(r.row_start[b], 0), r.rows);
+        s.n = max(min(min(max(r.row_start[b + 1], 0), r.rows) - s.first, r.max_rows), 0);
     }
     return s;
 }
