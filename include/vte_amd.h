@@ -394,10 +394,13 @@ typedef struct vte_kv_rows {
 /* Write the new rows' k and v (dtype fp16 or fp32, [rows][n_kv][head_dim], rows
  * k_stride / v_stride elements apart, 0: contiguous) into their pages, k rotated
  * by its position on the way, and, with q, q_out [rows][n_q][head_dim] (dtype,
- * contiguous; may be q) = q rotated (rows q_stride apart).  Rotation: rope_type
- * and tables as vte_rope ([rope_rows][head_dim], type 2 [rope_rows][rotary_dim]);
+ * contiguous; may be q) = q rotated (rows q_stride apart).  Rotation: tables as
+ * vte_rope ([rope_rows][head_dim], type 2 [rope_rows][rotary_dim]; pair i takes
+ * entry i), rope_type 0: dims i and i + head_dim / 2 are a pair, 1: 2 i and 2 i + 1,
+ * 2: i and i + rotary_dim / 2 of the first rotary_dim, the others as they are;
  * rows at positions from rope_rows on are dropped, their q_out left as it was.
- * rope_cos and rope_sin NULL: no rotation, q must be NULL.  Each k and v value is
+ * rope_cos and rope_sin NULL: no rotation, q must be NULL.  rows * n_q <= 2^25.
+ * Each k and v value is
  * rounded once, to its byte; a block's scale fits its largest value and never
  * falls while tokens before the new rows live in it (when it grows by 2^d their
  * bytes are shifted, rounded to nearest even).
@@ -411,7 +414,7 @@ int vte_kv_pages_append(const vte_kv_pages* cache, const vte_kv_rows* rows, int 
 /* k_out and v_out [batch][out_rows][n_kv][head_dim] (dtype): the values at
  * positions 0 .. kv_offset[b] + (b's new rows) - 1 of every sequence, each
  * rounded once; rows past them (and past out_rows) are left as they were.  Tokens
- * without a page give 0.  The layout is the fp16 cache's
+ * without a page give 0.  At most 2^27 rows x n_kv a sequence.  The layout is the fp16 cache's
  * (vte/compiler/qwen_mapper.py:300-351). */
 int vte_kv_pages_read(const vte_kv_pages* cache, const vte_kv_rows* rows, int dtype, void* k_out, void* v_out,
                       int out_rows, void* stream);

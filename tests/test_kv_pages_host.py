@@ -62,13 +62,15 @@ def test_no_rows_read_but_neither_append_nor_attend():
                                  dict(rope_cos=P, rope_sin=P, rope_rows=0), dict(q=P, q_out=P, n_q=0, rope=1),
                                  dict(rope=1, rope_type=3), dict(rope=1, rope_type=2, rotary_dim=3),
                                  dict(rope=1, rope_type=2, rotary_dim=130), dict(q=P, q_out=P, n_q=4, q_stride=511, rope=1),
-                                 dict(q=P, q_out=P, n_q=4, q_stride=1024, rope=1)], ids=str)
+                                 dict(q=P, q_out=P, n_q=4, q_stride=1024, rope=1),
+                                 dict(q=P, q_out=P + 8, n_q=65535, r=dict(batch=1, rows=1 << 10, row_start=P), rope=1)], ids=str)
 def test_append_refusals(bad):
     a = dict(k=P, v=P) | bad
+    r = a.pop("r", {})
     if a.pop("rope", 0):
         a = dict(rope_cos=P, rope_sin=P, rope_rows=10) | a
     with pytest.raises(HIPSafetyError):
-        kernels().kv_pages_append(pages(), rows(), **a)
+        kernels().kv_pages_append(pages(), rows(**r), **a)
 
 
 def test_read_and_attention_refusals():
@@ -77,6 +79,7 @@ def test_read_and_attention_refusals():
     assert need > 0
     for call in (lambda: K.kv_pages_read(c, r, None, P, 64), lambda: K.kv_pages_read(c, r, P, P, 0),
                  lambda: K.kv_pages_read(c, r, P + 2, P, 64),
+                 lambda: K.kv_pages_read(pages(n_kv=4, page_tokens=4096), rows(max_pages=1 << 14), P, P, (1 << 25) + 1),
                  lambda: K.attn_pages(c, r, P, P, 12, 0.1, P, need - 1),
                  lambda: K.attn_pages(c, r, P, P, 12, 0.1, None, need),
                  lambda: K.attn_pages(c, r, P, P, 12, 0.1, P + 4, need),
@@ -96,7 +99,8 @@ def test_read_and_attention_refusals():
 
 @pytest.mark.parametrize("bad", [dict(logits=None), dict(u=None), dict(tokens=None), dict(scratch=None), dict(rows=0),
                                  dict(rows=65536), dict(vocab=0), dict(vocab=262145), dict(logits=P + 2),
-                                 dict(u=P + 4), dict(scratch=P + 8)], ids=str)
+                                 dict(u=P + 4), dict(scratch=P + 8), dict(tokens=P + 2), dict(temperature=P + 1),
+                                 dict(top_k=P + 2), dict(top_p=P + 3), dict(min_p=P + 2)], ids=str)
 def test_sample_refusals(bad):
     a = dict(logits=P, rows=2, vocab=100, tokens=P, scratch=P, u=P) | bad
     with pytest.raises(HIPSafetyError):

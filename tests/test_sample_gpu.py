@@ -172,7 +172,9 @@ def test_generate_sampled_matches_host_loop(hip, K, tiny, B):
         from vte_amd.bridge.hip_runtime import HIPSafetyError
         for bad in (lambda: ex.generate_sampled(toks0, pos0, 0, np.zeros((0, B))),
                     lambda: ex.generate_sampled(toks0, [255] * B, 2, np.zeros((2, B))),
-                    lambda: ex.generate_sampled(toks0, pos0, 2, np.zeros((3, B)))):
+                    lambda: ex.generate_sampled(toks0, pos0, 2, np.zeros((3, B))),
+                    lambda: ex.generate_sampled(toks0, pos0, 2, np.ones((2, B))),
+                    lambda: ex.generate_sampled(toks0, pos0, 2, np.full((2, B), np.nan))):
             with pytest.raises(HIPSafetyError):
                 bad()
     finally:

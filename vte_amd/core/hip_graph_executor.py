@@ -652,6 +652,8 @@ class HIPGraphExecutor:
         u = np.ascontiguousarray(uniforms, np.float64)
         if u.shape != (n_steps, self.B):
             raise HIPSafetyError(f"uniforms of shape {u.shape}, expected {(n_steps, self.B)}")
+        if not ((u >= 0) & (u < 1)).all():
+            raise HIPSafetyError("uniforms outside [0, 1)")
         per_row = [np.array(np.broadcast_to(np.asarray(v, t), (self.B,)))
                    for v, t in ((temperature, np.float32), (top_k, np.int32), (top_p, np.float32), (min_p, np.float32))]
         if self._exclude() is not None:

@@ -824,6 +824,7 @@ int vte_kv_pages_append(const vte_kv_pages* cache, const vte_kv_rows* rows, int 
         REQUIRE(n_q >= 1 && n_q <= 65535 && qs >= (long long)n_q * hd && qs < (1LL << 31),
                 "kv_pages_append: n_q %d, q_stride %lld", n_q, q_stride);
         REQUIRE(q != q_out || qs == (long long)n_q * hd, "kv_pages_append: in place q must be contiguous");
+        REQUIRE((long long)r.rows * n_q <= (1 << 25), "kv_pages_append: rows %d x n_q %d above 2^25", r.rows, n_q);
     }
     if (rope_cos) {
         REQUIRE(rope_rows >= 1, "kv_pages_append: rope_rows %d", rope_rows);
@@ -847,6 +848,8 @@ int vte_kv_pages_read(const vte_kv_pages* cache, const vte_kv_rows* rows, int dt
     REQUIRE(k_out && v_out, "kv_pages_read: null output");
     REQUIRE(out_rows >= 1, "kv_pages_read: out_rows %d", out_rows);
     REQUIRE(aligned(k_out, 16) && aligned(v_out, 16), "kv_pages_read: outputs must be 16-byte aligned");
+    REQUIRE(std::min<long long>(out_rows, (long long)r.max_pages * cache->page_tokens) * c.n_kv <= (1 << 27),
+            "kv_pages_read: %d rows of %d heads: above 2^27", out_rows, c.n_kv);
     return hip_status(vte::kv_pages_read(c, r, cache->head_dim, dtype == VTE_F16, k_out, v_out, out_rows,
                                          (hipStream_t)stream),
                       "vte_kv_pages_read launch");
@@ -893,7 +896,8 @@ int vte_sample(const float* logits, int rows, int vocab, const float* temperatur
     REQUIRE(logits && u && tokens && scratch, "sample: null pointer");
     REQUIRE(rows >= 1 && rows <= 65535, "sample: rows %d outside 1..65535", rows);
     REQUIRE(vocab >= 1 && vocab <= 262144, "sample: vocab %d outside 1..262144", vocab);
-    REQUIRE(aligned(logits, 4) && aligned(u, 8) && aligned(scratch, 16), "sample: alignment");
+    REQUIRE(aligned(logits, 4) && aligned(temperature, 4) && aligned(top_k, 4) && aligned(top_p, 4) &&
+                aligned(min_p, 4) && aligned(tokens, 4) && aligned(u, 8) && aligned(scratch, 16), "sample: alignment");
     return hip_status(vte::sample(logits, rows, vocab, temperature, top_k, top_p, min_p, u, tokens, scratch,
                                   (hipStream_t)stream),
                       "vte_sample launch");
