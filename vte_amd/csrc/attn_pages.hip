@@ -12,6 +12,7 @@
 // byte 0..255 of a masked token times probability 0 is the only thing a place that
 // nobody sees can add: its exponent, which may be anything, is never used.
 #include <algorithm>
+#include <type_traits>
 #include "attn_tile.h"
 #include "kv_pages.h"
 
@@ -114,16 +115,20 @@ struct PaShare {
 // Sum over the lanes up to and with this one: shifts by 1, 2, 4 and 8 in rows of 16 lanes, then the rows' last lanes into
 // the rows behind them.
 template <int CTRL, int ROWS>
+__device__ __forceinline__ int pa_from(int v) {
+    return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
+}
+template <int CTRL, int ROWS>
 __device__ __forceinline__ long long pa_from(long long v) {
-    const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
-    const int hi = __builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, ROWS, 0xF, false);
-    return (long long)((unsigned long long)(unsigned)hi << 32 | lo);
+    const unsigned lo = (unsigned)pa_from<CTRL, ROWS>((int)v);
+    return (long long)((unsigned long long)(unsigned)pa_from<CTRL, ROWS>((int)(v >> 32)) << 32 | lo);
 }
 __device__ __forceinline__ long long pa_uniform(long long v) {  // the same in every lane: a scalar
     const unsigned lo = __builtin_amdgcn_readfirstlane((int)v);
     return (long long)((unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 | lo);
 }
-__device__ __forceinline__ long long pa_scan(long long v) {
+template <typename V>
+__device__ __forceinline__ V pa_scan(V v) {
     v += pa_from<0x111, 0xF>(v);
     v += pa_from<0x112, 0xF>(v);
     v += pa_from<0x114, 0xF>(v);
@@ -499,6 +504,7 @@ __global__ __launch_bounds__(256) void attn_pages_combine_kernel(KvPages c, KvRo
 #define PA_APART 24
 
 typedef float floatx16_t __attribute__((ext_vector_type(16)));
+typedef float floatx8_t __attribute__((ext_vector_type(8), aligned(16)));
 
 // Row block `slot` of all sequences' in their order: its sequence (-1: there are not so many) and number there.
 // One wave, sequences over its lanes.
@@ -514,12 +520,7 @@ __device__ __forceinline__ PaRowBlock pa_row_block(const KvRows& r, int G, int s
     for (int b0 = 0; b0 < r.batch; b0 += 64) {
         const KvSeq s = kvp_place(r, min(b0 + lane, r.batch - 1));
         const int n = b0 + lane < r.batch ? (s.n * G + ROWS - 1) / ROWS : 0;
-        int incl = n;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const int up = __shfl_up(incl, d, 64);
-            if (lane >= d) incl += up;
-        }
+        const int incl = pa_scan(n);
         const uint64_t here = __ballot(slot < incl);
         if (here != 0) {
             const int l = __ffsll((unsigned long long)here) - 1;
@@ -647,7 +648,8 @@ __device__ __forceinline__ void pa_apart(const KvPages& c, const int* table, int
     if (half) l_run = 0.f;  // (both halves hold the whole sum)
 }
 
-// grid (row blocks, n_kv, nsp), the last row blocks (which see most) first; nsp > 1 with two groups only.
+// grid (row blocks * n_kv, nsp), the last row blocks (which see most) first, whatever their head: with the heads one after
+// the other some started long ones late (four ragged fp32 prompts 65 -> 53 us).  nsp > 1 with two groups only.
 template <typename T, int HD, int GROUPS>
 __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, KvRows r, PaPrompt pp,
                                                                    const T* q, T* out,
@@ -675,13 +677,13 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
     const int grp = GROUPS == 2 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 8) : 0;
     const int row = lane & 31, half = lane >> 5;
     const int G = n_q / c.n_kv, cap = kvp_capacity(c, r), bl = c.page_log2 - 4;
-    const int slot = gridDim.x - 1 - blockIdx.x, h = blockIdx.y;
+    const int slot = (gridDim.x - 1 - blockIdx.x) / c.n_kv, h = blockIdx.x % c.n_kv;
     const PaRowBlock R = pa_row_block<ROWS>(r, G, slot);
     if (R.b < 0) return;
     const KvSeq s = R.s;
     const int steps = pa_steps<ROWS>(R, G, cap), share = pa_share_of(steps, pp.nsp);
-    const int a = blockIdx.z * share, z = min(steps, a + share), pieces = steps ? (steps + share - 1) / share : 1;
-    if (a >= z && !(steps == 0 && blockIdx.z == 0)) return;
+    const int a = blockIdx.y * share, z = min(steps, a + share), pieces = steps ? (steps + share - 1) / share : 1;
+    if (a >= z && !(steps == 0 && blockIdx.y == 0)) return;
     const int* table = r.page_table + (size_t)R.b * r.max_pages;
 
     // ---- this lane's row ----
@@ -723,34 +725,40 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
         find(step + GROUPS);
     };
     find(a + grp);
+    // (q is asked for while the page number is on its way)
+    typedef typename std::conditional<PARTS == 1, half8_t, floatx8_t>::type q8_t;
+    q8_t q_raw[KS];
+    {
+        const T* qp = q + ((size_t)(s.first + qi) * n_q + qh) * HD + 8 * half;
+#pragma unroll
+        for (int i = 0; i < KS; ++i) q_raw[i] = *reinterpret_cast<const q8_t*>(qp + 16 * i);
+    }
+    __builtin_amdgcn_sched_barrier(0);
     load(a + grp);
 
     half8_t qb[PARTS][KS];
     float q_unit = 1.f;
-    {
-        const T* qp = q + ((size_t)(s.first + qi) * n_q + qh) * HD + 8 * half;
-        if constexpr (PARTS == 1) {
+    if constexpr (PARTS == 1) {
 #pragma unroll
-            for (int i = 0; i < KS; ++i) qb[0][i] = *reinterpret_cast<const half8_t*>(qp + 16 * i);
-        } else {  // scaled by a power of two so that the second part keeps its bits too
-            float amax = 0.f;
+        for (int i = 0; i < KS; ++i) qb[0][i] = q_raw[i];
+    } else {  // scaled by a power of two so that the second part keeps its bits too
+        float amax = 0.f;
 #pragma unroll
-            for (int i = 0; i < KS; ++i)
+        for (int i = 0; i < KS; ++i)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(qp[16 * i + j]));
-            amax = fmaxf(amax, __shfl_xor(amax, 32, 64));
-            const int e = min(max((int)(__float_as_uint(amax) >> 23) - 127, -110), 126);  // 2^e <= amax
-            const float up = __uint_as_float((uint32_t)(127 + 13 - e) << 23);
-            q_unit = __uint_as_float((uint32_t)(127 - 13 + e) << 23);
+            for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(q_raw[i][j]));
+        amax = fmaxf(amax, __shfl_xor(amax, 32, 64));
+        const int e = min(max((int)(__float_as_uint(amax) >> 23) - 127, -110), 126);  // 2^e <= amax
+        const float up = __uint_as_float((uint32_t)(127 + 13 - e) << 23);
+        q_unit = __uint_as_float((uint32_t)(127 - 13 + e) << 23);
 #pragma unroll
-            for (int i = 0; i < KS; ++i)
+        for (int i = 0; i < KS; ++i)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float y = qp[16 * i + j] * up;
-                    qb[0][i][j] = (_Float16)y;
-                    qb[1][i][j] = (_Float16)(y - (float)qb[0][i][j]);
-                }
-        }
+            for (int j = 0; j < 8; ++j) {
+                const float y = q_raw[i][j] * up;
+                qb[0][i][j] = (_Float16)y;
+                qb[1][i][j] = (_Float16)(y - (float)qb[0][i][j]);
+            }
     }
     const float c2 = scale * 1.44269504088896340736f * q_unit;
 
@@ -803,9 +811,8 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
     // `ends`: some of the wave's rows do not see all of the step, or a block of it has no page or NaN in V
     auto work = [&](const Tile& D, Tile& next, int step, bool ends) {
         const int cur_k = k_ref, cur_v = v_ref, cur_odd = next_odd;
-        put(next);
-        load(step + 2 * GROUPS);
         floatx16_t sc[2];
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt) {
 #pragma unroll
@@ -818,15 +825,18 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
                     sc[tt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qb[p][i], sc[tt], 0, 0, 0);
             }
         }
-        // the next step's bytes are turned under these products: two reads ahead, then a product, a read and six
-        // vector operations in turn
-        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+        // The next step's bytes are turned under these products (written behind them: their reads stand before).
+        put(next);
+        load(step + 2 * GROUPS);
+        constexpr int QM = 2 * KS * PARTS, AHEAD = 4;
+        __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
 #pragma unroll
-        for (int i = 0; i < 2 * KS * PARTS; ++i) {
+        for (int i = 0; i < QM; ++i) {
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            if (i % PARTS == 0) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);
         }
+        __builtin_amdgcn_sched_barrier(0);
         // lane: its row's scores of tokens 32 tt + 16 (j / 8) + 8 half + j % 8
         const int live = end - step * PA_TILE - 8 * half;
         if (ends) {
@@ -870,32 +880,56 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
                         for (int j = 0; j < 16; ++j) o[dt][j] = NAN;
                 }
         }
+        // Sums: a block's probabilities are formed, and the one's V behind it read, under its products.
         const float shift = (float)PA_P_LOG2 - mx;
-        union {
-            half8_t v[4];
-            pa_h2 h[16];
-        } pf[PARTS];
         const pa_h2 ones = {(_Float16)1.f, (_Float16)1.f};
+        union Probs {
+            half8_t v;
+            pa_h2 h[4];
+        } pf[2][PARTS];
+        half8_t vb[2][DT];
+        auto probs = [&](int kb) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {  // the sum of the probabilities as the products have them
-            const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[i >> 3][2 * (i & 7)], kf, shift));
-            const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[i >> 3][2 * (i & 7) + 1], kf, shift));
-            pf[0].h[i] = pa_h2{(_Float16)p0, (_Float16)p1};
-            l_run = __builtin_amdgcn_fdot2(pf[0].h[i], ones, l_run, false);
-            if constexpr (PARTS == 2) {
-                pf[1].h[i] = pa_h2{(_Float16)(p0 - (float)pf[0].h[i][0]), (_Float16)(p1 - (float)pf[0].h[i][1])};
-                l_run = __builtin_amdgcn_fdot2(pf[1].h[i], ones, l_run, false);
+            for (int i = 0; i < 4; ++i) {  // the sum of the probabilities as the products have them
+                const int j = 8 * (kb & 1) + 2 * i;
+                const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[kb >> 1][j], kf, shift));
+                const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[kb >> 1][j + 1], kf, shift));
+                Probs(&f)[PARTS] = pf[kb & 1];
+                f[0].h[i] = pa_h2{(_Float16)p0, (_Float16)p1};
+                l_run = __builtin_amdgcn_fdot2(f[0].h[i], ones, l_run, false);
+                if constexpr (PARTS == 2) {
+                    f[1].h[i] = pa_h2{(_Float16)(p0 - (float)f[0].h[i][0]), (_Float16)(p1 - (float)f[0].h[i][1])};
+                    l_run = __builtin_amdgcn_fdot2(f[1].h[i], ones, l_run, false);
+                }
             }
-        }
+        };
+        auto read_v = [&](int kb) {
 #pragma unroll
-        for (int kb = 0; kb < 4; ++kb)
+            for (int dt = 0; dt < DT; ++dt)
+                vb[kb & 1][dt] = *reinterpret_cast<const half8_t*>(D.v + ((2 * kb + half) * HD + 32 * dt + row) * 8);
+        };
+        read_v(0);
+        probs(0);
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt) {
-                const half8_t v = *reinterpret_cast<const half8_t*>(D.v + ((2 * kb + half) * HD + 32 * dt + row) * 8);
+        for (int kb = 0; kb < 4; ++kb) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (kb < 3) read_v(kb + 1);
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
                 for (int p = 0; p < PARTS; ++p)
-                    o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pf[p].v[kb], o[dt], 0, 0, 0);
+                    o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vb[kb & 1][dt], pf[kb & 1][p].v, o[dt], 0, 0, 0);
+            if (kb < 3) {
+                probs(kb + 1);
+                __builtin_amdgcn_sched_group_barrier(0x100, DT, 0);
+#pragma unroll
+                for (int i = 0; i < DT * PARTS; ++i) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x402, PARTS == 1 ? 24 / DT + 1 : 52 / (2 * DT) + 1, 0);
+                }
             }
+        }
+        __builtin_amdgcn_sched_barrier(0);
     };
 
     put(S.tiles[grp][0]);
@@ -946,7 +980,7 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
             for (int j = 0; j < 16; ++j) mine[i][j] = mine[i][j] * g1 + S.o[grp ^ 1][16 * i + j][tid] * g2;
         const int d0 = grp * (HD / 2) + 4 * half;  // first dim of mine
         if (pieces > 1) {
-            const size_t rec = ((size_t)slot * c.n_kv + h) * pp.nsp + blockIdx.z;
+            const size_t rec = ((size_t)slot * c.n_kv + h) * pp.nsp + blockIdx.y;
             float* po = pp.o + (rec * ROWS + wv * 32 + row) * HD + d0;
 #pragma unroll
             for (int i = 0; i < DT / 2; ++i)
@@ -1093,7 +1127,7 @@ static hipError_t attn_hd(const KvPages& c, const KvRows& r, const void* q, void
     }
     const PromptForm f = prompt_form(c, r, HD, G, scratch);
     auto kernel = f.groups == 1 ? attn_pages_prompt_kernel<T, HD, 1> : attn_pages_prompt_kernel<T, HD, 2>;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)f.rbs, c.n_kv, f.p.nsp), dim3(512), 0, st, c, r, f.p, (const T*)q, (T*)out,
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(f.rbs * c.n_kv), f.p.nsp), dim3(512), 0, st, c, r, f.p, (const T*)q, (T*)out,
                        n_q, scale);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || f.p.nsp == 1) return e;
