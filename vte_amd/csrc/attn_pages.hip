@@ -772,38 +772,33 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
     int k_ref = KVP_E_MIN, v_ref = KVP_E_MIN;           // of the step staged last: its largest, the largest so far
     int next_odd = 0;                                   // its blocks without a page, and with NaN in V
     int apart = 0;                                      // some blocks' scales lie too far apart for all this
-    auto put = [&](Tile& D) {
-        next_odd = 0;
-        int e[4], f[4];
+    int by_k = 0, by_v = 0;                             // lane j & 3: block j's factors, fp16
+    auto scales = [&] {
         const int my_k = got ? ek : -1000, my_v = got ? ev : -1000;  // -1000: times 0
+        auto max4 = [](int x) {                                      // of the four blocks
+            x = max(x, __builtin_amdgcn_update_dpp(0, x, 0xB1, 0xF, 0xF, false));
+            return __builtin_amdgcn_readfirstlane(max(x, __builtin_amdgcn_update_dpp(0, x, 0x4E, 0xF, 0xF, false)));
+        };
         const int v_old = v_ref;
-        k_ref = KVP_E_MIN;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            e[j] = __builtin_amdgcn_readlane(my_k, j);
-            f[j] = __builtin_amdgcn_readlane(my_v, j);
-            next_odd |= (e[j] == -1000 ? 1 << j : 0) | (f[j] == KVP_E_NAN ? 16 << j : 0);
-            k_ref = max(k_ref, e[j]);
-            v_ref = max(v_ref, f[j]);
-        }
-        // (lane j & 3: of block j; the last one: sums that vanish in fp32 beside larger ones)
+        k_ref = max(max4(my_k), KVP_E_MIN);
+        v_ref = max(max4(my_v), v_old);
+        next_odd = (int)(__ballot(!got) & 15) | (int)(__ballot(my_v == KVP_E_NAN) & 15) << 4;
+        // (the last one: sums that vanish in fp32 beside larger ones)
         apart |= ((my_k > KVP_E_MIN) & (my_k < k_ref - PA_APART)) | ((my_v > KVP_E_MIN) & (my_v < v_ref - PA_APART)) |
                  ((v_old > KVP_E_MIN) & (v_ref - v_old > 96));
-#pragma unroll
-        for (int u = 0; u < NP; ++u) {
-            const int j = first(u) / HD, piece = first(u) % HD + lane;
-            int x = is_v(u) ? f[0] : e[0];
-#pragma unroll
-            for (int i = 1; i < 4; ++i) x = i == j ? (is_v(u) ? f[i] : e[i]) : x;
-            // (NaN in V is dealt with where its rows are: 0 times it would reach rows that do not see it)
-            const _Float16 by = x == KVP_E_NAN ? (_Float16)(is_v(u) ? 0.f : NAN)
-                                               : (_Float16)pa_pow2(x - (is_v(u) ? v_ref : k_ref));
-            // K piece: token piece / KS of the block, dims 16 (piece % KS) ..; V piece: dim `piece`
-            _Float16* to = is_v(u) ? D.v + (2 * j * HD + piece) * 8
-                                   : D.k + (piece % KS) * KROW + (16 * j + piece / KS) * 8;
-            *reinterpret_cast<half8_t*>(to) = pa_half8(stage[u].x, stage[u].y, by);
-            *reinterpret_cast<half8_t*>(to + (is_v(u) ? HD * 8 : KS * KROW)) = pa_half8(stage[u].z, stage[u].w, by);
-        }
+        // (NaN in V is dealt with where its rows are: 0 times it would reach rows that do not see it)
+        by_k = my_k == KVP_E_NAN ? 0x7E00 : (int)__builtin_bit_cast(unsigned short, (_Float16)pa_pow2(my_k - k_ref));
+        by_v = my_v == KVP_E_NAN ? 0 : (int)__builtin_bit_cast(unsigned short, (_Float16)pa_pow2(my_v - v_ref));
+    };
+    auto put = [&](Tile& D, int u) {
+        const int j = first(u) / HD, piece = first(u) % HD + lane;
+        const int by16 = __builtin_amdgcn_readlane(is_v(u) ? by_v : by_k, j);
+        const _Float16 by = __builtin_bit_cast(_Float16, (unsigned short)by16);
+        // K piece: token piece / KS of the block, dims 16 (piece % KS) ..; V piece: dim `piece`
+        _Float16* to = is_v(u) ? D.v + (2 * j * HD + piece) * 8
+                               : D.k + (piece % KS) * KROW + (16 * j + piece / KS) * 8;
+        *reinterpret_cast<half8_t*>(to) = pa_half8(stage[u].x, stage[u].y, by);
+        *reinterpret_cast<half8_t*>(to + (is_v(u) ? HD * 8 : KS * KROW)) = pa_half8(stage[u].z, stage[u].w, by);
     };
 
     // K row of 32-token tile tt: token with bits 2 and 3 of the lane's row swapped
@@ -811,32 +806,42 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
     // `ends`: some of the wave's rows do not see all of the step, or a block of it has no page or NaN in V
     auto work = [&](const Tile& D, Tile& next, int step, bool ends) {
         const int cur_k = k_ref, cur_v = v_ref, cur_odd = next_odd;
+        // Scores: under every four products the next four operands are read and a part of the next step's bytes is turned.
+        constexpr int RUN = 4, RUNS = 2 * KS / RUN;
         floatx16_t sc[2];
-        __builtin_amdgcn_sched_barrier(0);
+        half8_t kb[2][RUN];
+        auto read_k = [&](int u) {  // tile u / KS, 16-dim step u % KS
+            return *reinterpret_cast<const half8_t*>(D.k + (half * KS + u % KS) * KROW + (32 * (u / KS) + kt) * 8);
+        };
 #pragma unroll
-        for (int tt = 0; tt < 2; ++tt) {
+        for (int u = 0; u < RUN; ++u) kb[0][u] = read_k(u);
+        scales();
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
             for (int j = 0; j < 16; ++j) sc[tt][j] = 0.f;
 #pragma unroll
-            for (int i = 0; i < KS; ++i) {
-                const half8_t k = *reinterpret_cast<const half8_t*>(D.k + (half * KS + i) * KROW + (32 * tt + kt) * 8);
+        for (int n = 0; n < RUNS; ++n) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (n + 1 < RUNS)
+#pragma unroll
+                for (int u = 0; u < RUN; ++u) kb[n + 1 & 1][u] = read_k((n + 1) * RUN + u);
+#pragma unroll
+            for (int u = n * RUN; u < (n + 1) * RUN; ++u)
 #pragma unroll
                 for (int p = 0; p < PARTS; ++p)
-                    sc[tt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qb[p][i], sc[tt], 0, 0, 0);
+                    sc[u / KS] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kb[n & 1][u % RUN], qb[p][u % KS], sc[u / KS], 0, 0, 0);
+#pragma unroll
+            for (int u = n * NP / RUNS; u < (n + 1) * NP / RUNS; ++u) put(next, u);
+            __builtin_amdgcn_sched_group_barrier(0x100, RUN, 0);
+#pragma unroll
+            for (int i = 0; i < RUN * PARTS; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, 6 / PARTS, 0);
             }
         }
-        // The next step's bytes are turned under these products (written behind them: their reads stand before).
-        put(next);
-        load(step + 2 * GROUPS);
-        constexpr int QM = 2 * KS * PARTS, AHEAD = 4;
-        __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
-#pragma unroll
-        for (int i = 0; i < QM; ++i) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            if (i % PARTS == 0) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);
-        }
         __builtin_amdgcn_sched_barrier(0);
+        load(step + 2 * GROUPS);
         // lane: its row's scores of tokens 32 tt + 16 (j / 8) + 8 half + j % 8
         const int live = end - step * PA_TILE - 8 * half;
         if (ends) {
@@ -932,7 +937,9 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
         __builtin_amdgcn_sched_barrier(0);
     };
 
-    put(S.tiles[grp][0]);
+    scales();
+#pragma unroll
+    for (int u = 0; u < NP; ++u) put(S.tiles[grp][0], u);
     load(a + grp + GROUPS);
     __syncthreads();
     int buf = 0;
