@@ -234,8 +234,9 @@ def attn_tolerance(dtype, hd, out, mag, big, vmax):
     result is (2^-11); fp32: two fp16 parts of q and of the probabilities (2^-21 each: a rounded part and a rounded
     rest of at most 2^-11 of it), the result 2^-24.  Both: scores are fp32 sums of hd + 3 roundings at most (2^-24 of
     the sum of |q k| each), which e^x carries into both sums (twice); exponentials, sums and the rescaling by running
-    maxima add 2^-19 at most (2^-24 a rounding, below 32 of them in a chain); what is below the smallest fp16 after
-    scaling by 2^14 is 2^-38 of the largest weight for each of at most 2^16 tokens.  fp16 results below 2^-14 are
+    maxima add 2^-19 at most (2^-24 a rounding, below 32 of them in a chain); half the smallest fp16 is 2^-25, of
+    probabilities scaled by 2^14 2^-39 of the largest for each of at most 2^16 tokens, of a prompt's scaled by 2^9 2^-34
+    for each of at most 2^12.  fp16 results below 2^-14 are
     rounded to steps of 2^-24 (2^-25 at most)."""
     p, r = (2.0 ** -11, 2.0 ** -11) if dtype == "f16" else (2.0 ** -20, 2.0 ** -24)
     q = 0.0 if dtype == "f16" else 2.0 ** -21

@@ -502,6 +502,8 @@ __global__ __launch_bounds__(256) void attn_pages_combine_kernel(KvPages c, KvRo
 // ---------------------------------------------------------------------------
 #define PA_SHARES 16
 #define PA_APART 24
+#define PA_LAG 6    // sums are rescaled when a maximum has grown by more than 2^6 ..
+#define PA_Q_LOG2 9 // .. so probabilities are held as 2^9 p, at most 2^15
 
 typedef float floatx16_t __attribute__((ext_vector_type(16)));
 typedef float floatx8_t __attribute__((ext_vector_type(8), aligned(16)));
@@ -627,7 +629,7 @@ __device__ __forceinline__ void pa_apart(const KvPages& c, const int* table, int
         l_run *= corr;
 #pragma unroll
         for (int t = 0; t < KVP_BLOCK; ++t) {
-            const float p = __builtin_amdgcn_exp2f(w[t] - mx + (float)PA_P_LOG2);
+            const float p = __builtin_amdgcn_exp2f(w[t] - mx + (float)PA_Q_LOG2);
             l_run += p;
             w[t] = t < n ? p * vf : 0.f;
         }
@@ -866,7 +868,7 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
         }
         const float kf = fmaxf(kvp_scale(cur_k) * c2, 1e-38f);  // (not 0: masked scores are -Inf)
         mx = fmaxf(m_run, mx * kf);
-        if (__any(mx > m_run) || cur_v > o_ref) {
+        if (__any(mx > m_run + (float)PA_LAG) || cur_v > o_ref) {
             const float corr = __builtin_amdgcn_exp2f(m_run - mx);
             l_run *= corr;
             const float both = corr * pa_pow2(o_ref - cur_v);
@@ -886,7 +888,7 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
                 }
         }
         // Sums: a block's probabilities are formed, and the one's V behind it read, under its products.
-        const float shift = (float)PA_P_LOG2 - mx;
+        const float shift = (float)PA_Q_LOG2 - m_run;
         const pa_h2 ones = {(_Float16)1.f, (_Float16)1.f};
         union Probs {
             half8_t v;
