@@ -1023,28 +1023,35 @@ __global__ __launch_bounds__(256) void attn_pages_prompt_combine_kernel(KvPages 
     const size_t rec0 = ((size_t)slot * c.n_kv + h) * pp.nsp;
     float M = PA_NONE, L = 0.f;
     int EV = KVP_E_MIN;
-    for (int i = 0; i < pieces; ++i) {
-        M = fmaxf(M, pp.ml[((rec0 + i) * ROWS + rr) * 2]);
-        EV = max(EV, pp.ev[(rec0 + i) * ROWS + rr]);
-    }
     floatx4_t O = {0.f, 0.f, 0.f, 0.f};
-    for (int i0 = 0; i0 < pieces; i0 += 4) {  // four requested together (past the last one: the last again)
-        floatx4_t o[4];
-        float m[4], l[4];
-        int ev[4];
+    constexpr int AT_ONCE = 8;
+    for (int i0 = 0; i0 < pieces; i0 += AT_ONCE) {  // requested together (past the last one: the last again)
+        floatx4_t o[AT_ONCE];
+        float2 ml[AT_ONCE];
+        int ev[AT_ONCE];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const size_t rec = rec0 + min(i0 + i, pieces - 1);
-            o[i] = *reinterpret_cast<const floatx4_t*>(pp.o + (rec * ROWS + rr) * HD + d);
-            m[i] = pp.ml[(rec * ROWS + rr) * 2];
-            l[i] = pp.ml[(rec * ROWS + rr) * 2 + 1];
-            ev[i] = pp.ev[rec * ROWS + rr];
+        for (int i = 0; i < AT_ONCE; ++i) {
+            const size_t rec = (rec0 + min(i0 + i, pieces - 1)) * ROWS + rr;
+            o[i] = *reinterpret_cast<const floatx4_t*>(pp.o + rec * HD + d);
+            ml[i] = *reinterpret_cast<const float2*>(pp.ml + rec * 2);
+            ev[i] = pp.ev[rec];
         }
+        float m = M;
+        int x = EV;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (i0 + i >= pieces) continue;
-            const float f = __builtin_amdgcn_exp2f(m[i] - M);
-            L = fmaf(l[i], f, L);
+        for (int i = 0; i < AT_ONCE; ++i) {
+            m = fmaxf(m, ml[i].x);
+            x = max(x, ev[i]);
+        }
+        const float old = __builtin_amdgcn_exp2f(M - m);
+        L *= old;
+        O *= old * pa_pow2(EV - x);
+        M = m;
+        EV = x;
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+            const float f = i0 + i < pieces ? __builtin_amdgcn_exp2f(ml[i].x - M) : 0.f;
+            L = fmaf(ml[i].y, f, L);
             O += o[i] * (f * pa_pow2(ev[i] - EV));
         }
     }
