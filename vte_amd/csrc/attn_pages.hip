@@ -230,6 +230,32 @@ __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(KvPages c, KvRo
         const int ncol = s.n * G, ci = min(col, ncol - 1);
         const int qi = ci / G, qh = h * G + ci - qi * G;
         const int end = col < ncol ? kvp_len(s.pos + qi, cap) : 0;
+        // K row of 16-row tile tt: token 16 (col / 4) + 4 tt + col % 4, so that the scores a lane gets from the four
+        // tiles are those of block grp in order, which is the order V's 16 bytes hold its tokens in.
+        auto load = [&](PaTile<HD>& x, int tile) {
+            const int t0 = tile * PA_TILE;
+            const int last = (len - 1) >> 4;  // blocks past the end read the last one (their tokens are masked)
+            const int kb = min((t0 >> 4) + (col >> 2), last), vb = min((t0 >> 4) + grp, last);
+            const int kp = table[kb >> bl], vp = table[vb >> bl];
+            x.has = (unsigned)vp < (unsigned)c.n_pages;
+            const size_t ka = ((((size_t)((unsigned)kp < (unsigned)c.n_pages ? kp : 0) * c.n_kv + h) << bl) +
+                               (kb & ((1 << bl) - 1))) * (KVP_BLOCK * HD);
+            const size_t vi = (((size_t)(x.has ? vp : 0) * c.n_kv + h) << bl) + (vb & ((1 << bl) - 1));
+            const uint8_t* kr = c.k + ka + (col & 3) * HD + 16 * grp;
+#pragma unroll
+            for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+                for (int j = 0; j < KC; ++j) x.k[tt][j] = ldg_g16(kr + 4 * tt * HD + 64 * j);
+            x.ek = c.k_exp[vi];
+            x.ev = c.v_exp[vi];
+            const uint8_t* vr = c.v + vi * (KVP_BLOCK * HD) + col * KVP_BLOCK;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) x.v[dt] = ldg_g16(vr + 256 * dt);
+        };
+        PaTile<HD> A, B;
+        int tile = a + wv;
+        if (tile < z) load(A, tile);  // (asked for before q, whose turning into fp16 would hold it up)
+
         half8_t qb[PARTS][2 * KC];
         float q_unit = 1.f;  // of the values in qb
         {
@@ -270,28 +296,6 @@ __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(KvPages c, KvRo
 #pragma unroll
         for (int i = 0; i < DT; ++i) o[i] = floatx4_t{0.f, 0.f, 0.f, 0.f};
 
-        // K row of 16-row tile tt: token 16 (col / 4) + 4 tt + col % 4, so that the scores a lane gets from the four
-        // tiles are those of block grp in order, which is the order V's 16 bytes hold its tokens in.
-        auto load = [&](PaTile<HD>& x, int tile) {
-            const int t0 = tile * PA_TILE;
-            const int last = (len - 1) >> 4;  // blocks past the end read the last one (their tokens are masked)
-            const int kb = min((t0 >> 4) + (col >> 2), last), vb = min((t0 >> 4) + grp, last);
-            const int kp = table[kb >> bl], vp = table[vb >> bl];
-            x.has = (unsigned)vp < (unsigned)c.n_pages;
-            const size_t ka = ((((size_t)((unsigned)kp < (unsigned)c.n_pages ? kp : 0) * c.n_kv + h) << bl) +
-                               (kb & ((1 << bl) - 1))) * (KVP_BLOCK * HD);
-            const size_t vi = (((size_t)(x.has ? vp : 0) * c.n_kv + h) << bl) + (vb & ((1 << bl) - 1));
-            const uint8_t* kr = c.k + ka + (col & 3) * HD + 16 * grp;
-#pragma unroll
-            for (int tt = 0; tt < 4; ++tt)
-#pragma unroll
-                for (int j = 0; j < KC; ++j) x.k[tt][j] = ldg_g16(kr + 4 * tt * HD + 64 * j);
-            x.ek = c.k_exp[vi];
-            x.ev = c.v_exp[vi];
-            const uint8_t* vr = c.v + vi * (KVP_BLOCK * HD) + col * KVP_BLOCK;
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt) x.v[dt] = ldg_g16(vr + 256 * dt);
-        };
         auto step = [&](const PaTile<HD>& x, int tile) {
             const int p0 = tile * PA_TILE + 16 * grp;  // this lane group's block
             floatx4_t sc[4];
@@ -355,9 +359,6 @@ __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(KvPages c, KvRo
         };
 
         // ---- the wave's tiles, the next one's loads under this one's work ----
-        PaTile<HD> A, B;
-        int tile = a + wv;
-        if (tile < z) load(A, tile);
         while (tile < z) {
             if (tile + 4 < z) load(B, tile + 4);
             step(A, tile);
