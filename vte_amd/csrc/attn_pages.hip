@@ -436,6 +436,12 @@ __global__ __launch_bounds__(256) void attn_pages_combine_kernel(KvPages c, KvRo
     }
     const int2 sg = pl.seg[seg];
     if (sg.y == 1) return;
+    auto sums = [&](int i) {
+        return *reinterpret_cast<const floatx4_t*>(pl.o + (pa_rec(sg.x, i) * pl.ncol + cc) * HD + d);
+    };
+    floatx4_t early[2];  // the group's first pieces, under the way to their weights
+#pragma unroll
+    for (int u = 0; u < 2; ++u) early[u] = sums(min(g + u * GR, sg.y - 1));
     float M = PA_NONE;
     int EV = KVP_E_MIN;
     for (int i = tid; i < sg.y; i += 256) {
@@ -463,9 +469,13 @@ __global__ __launch_bounds__(256) void attn_pages_combine_kernel(KvPages c, KvRo
             w_sh[tid] = f * pa_pow2(pl.ev[rec * pl.ncol + cc] - EV);
         }
         __syncthreads();
+        if (i0 == 0) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+                if (g + u * GR < n) O += early[u] * w_sh[g + u * GR];
+        }
 #pragma unroll 4
-        for (int i = g; i < n; i += GR)
-            O += *reinterpret_cast<const floatx4_t*>(pl.o + (pa_rec(sg.x, i0 + i) * pl.ncol + cc) * HD + d) * w_sh[i];
+        for (int i = g + (i0 == 0 ? 2 * GR : 0); i < n; i += GR) O += sums(i0 + i) * w_sh[i];
         __syncthreads();
     }
     l = wave_sum(l);
