@@ -155,7 +155,9 @@ __device__ __forceinline__ PaShare pa_share(const KvPages& c, const KvRows& r, i
     incl += wv > 2 ? w4[0] + w4[1] + w4[2] : wv > 1 ? w4[0] + w4[1] : wv > 0 ? w4[0] : 0;
     const long long total = pa_uniform(w4[0] + w4[1] + w4[2] + w4[3]);
     PaShare s;
-    s.share = ((total + blocks - 1) / blocks + 3) / 4 * 4;
+    // (a tile for each wave at least; whole rounds of four beyond that left CUs idle: eight documents of 16384 to 65536
+    // tokens 44.0 -> 41.3 us without, 16 ragged sequences 19.7 -> 18.3 us)
+    s.share = max((total + blocks - 1) / blocks, 4LL);
     s.t = s.share * block;
     s.t_end = min(total, s.t + s.share);
     if (mine > 0 && s.t >= incl - mine && s.t < incl) {
