@@ -35,6 +35,7 @@
 #define SMP_LEVELS 5        // 32 + 18 bits of (key, index) in digits of 10
 #define SMP_LIST 8192       // entries that are collected at most; more: the row is read again
 #define SMP_SMALL 1024      // entries of a bin that are ordered by counting
+#define SMP_FEW 128         // .. without a split first
 #define SMP_AHEAD 4         // subsets a wave of the draw has in flight (8: one row 16.1 -> 18.6 us, 256 rows the same)
 #define SMP_SPLIT 8         // blocks of a row at most
 
@@ -102,6 +103,12 @@ __device__ __forceinline__ SmpScale smp_scale(float max, float T) {
     c.low = fmaxf(low < -3.4e38 ? -3.4e38f : (float)(low - 1.2e-7 * fabs(low) - 1e-45), -3.4028234664e38f);
     return c;
 }
+// fma with its constants in registers: the two-operand form that the compiler takes moves one there each time.
+__device__ __forceinline__ double smp_fma(double a, double b, double c) {
+    double d;
+    asm("v_fma_f64 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
+    return d;
+}
 // Bin of x (false: no weight, NaN among them) and its weight in the bin, in units of 2^-44: the series of e^(r / 32)
 // for y = round(y) + r (the next term is below 2^-45).
 // ABOVE: bins above the scale's largest value that count too (g is below 0 there).
@@ -120,13 +127,13 @@ __device__ __forceinline__ bool smp_bin(const SmpScale& c, float x, int& g, uint
         in = in && (c.flat || x == c.max);
         g = 0;
     }
-    double p = fma(r, H * H * H * H * H / 120.0, H * H * H * H / 24.0);
-    p = fma(r, p, H * H * H / 6.0);
+    double p = smp_fma(r, H * H * H * H * H / 120.0, H * H * H * H / 24.0);
+    p = smp_fma(r, p, H * H * H / 6.0);
     p = fma(r, p, H * H / 2.0);
     p = fma(r, p, H);
     p = fma(r, p, 1.0);
     // 2^52 + p 2^44 holds the whole number in its low bits
-    m = (uint64_t)__double_as_longlong(fma(p, SMP_ONE, 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;
+    m = (uint64_t)__double_as_longlong(smp_fma(p, SMP_ONE, 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;
     return in;
 }
 // Place of x inside its bin, from the largest value on, in 1024 steps.
@@ -172,11 +179,29 @@ __device__ __forceinline__ SmpFour smp_load(const float* row, int vocab, int sub
 }
 template <bool WIDE>
 __device__ __forceinline__ void smp_cut(SmpFour& f, int vocab, int sub, int lane) {
+    if ((sub + 1) * SMP_SUB <= vocab) return;  // (the same for a wave)
 #pragma unroll
     for (int e = 0; e < 4; ++e) f.x[e] = smp_at<WIDE>(sub, lane, e) < vocab ? f.x[e] : -INFINITY;
 }
 __device__ __forceinline__ float smp_max4(const SmpFour& r) {  // NaN counts as nothing
     return fmaxf(fmaxf(fmaxf(r.x[0], -INFINITY), r.x[1]), fmaxf(r.x[2], r.x[3]));
+}
+
+// Largest of the wave's values of four subsets at once: lane 16 i has subset i's (halves, then rows of 16 lanes change
+// places and carry two subsets each on; inside a row as whole numbers in the same order, which need no quieting).
+typedef unsigned smp_u2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ float smp_max_of_four(float a, float b, float c, float d) {
+    auto two = [](smp_u2 w) { return fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1])); };
+    const float ac = two(__builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(c), false, false));
+    const float bd = two(__builtin_amdgcn_permlane32_swap(__float_as_uint(b), __float_as_uint(d), false, false));
+    const float x = two(__builtin_amdgcn_permlane16_swap(__float_as_uint(ac), __float_as_uint(bd), false, false));
+    int i = (int)__float_as_uint(x);
+    i ^= (i >> 31) & 0x7FFFFFFF;
+    i = max(i, __builtin_amdgcn_update_dpp(i, i, 0xB1, 0xF, 0xF, false));
+    i = max(i, __builtin_amdgcn_update_dpp(i, i, 0x4E, 0xF, 0xF, false));
+    i = max(i, __builtin_amdgcn_update_dpp(i, i, 0x141, 0xF, 0xF, false));
+    i = max(i, __builtin_amdgcn_update_dpp(i, i, 0x140, 0xF, 0xF, false));
+    return __uint_as_float((uint32_t)(i ^ ((i >> 31) & 0x7FFFFFFF)));
 }
 
 // grid (blocks of a row, rows).  A part of at most KEEP subsets a wave (few rows) stays in registers while its largest
@@ -210,23 +235,30 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_bins_kernel(const float* _
         count[i] = 0;
     }
     float best = -INFINITY;
-    auto first = [&](SmpFour& f, int j) {
-        smp_cut<WIDE>(f, vocab, min(nth(j), hi - 1), lane);
-        const float m = wave_max(smp_max4(f));
-        if (lane == 0 && nth(j) < hi) sc.sub[nth(j)] = m;
-        best = fmaxf(best, m);  // (a subset twice changes nothing)
+    auto first = [&](SmpFour* f, int j) {  // subsets j .. j + 3
+        float m[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            smp_cut<WIDE>(f[i], vocab, min(nth(j + i), hi - 1), lane);
+            m[i] = smp_max4(f[i]);
+        }
+        const float x = smp_max_of_four(m[0], m[1], m[2], m[3]);
+        const int at = nth(j + (lane >> 4));
+        if ((lane & 15) == 0 && at < hi) sc.sub[at] = x;
+        best = fmaxf(best, x);  // (a subset twice changes nothing)
     };
     auto largest = [&](int i) {  // of all waves'
-        if (lane == 0) wmax[i][wv] = best;
+        const float m = fmaxf(fmaxf(wave_rows4(best, 0), wave_rows4(best, 1)), fmaxf(wave_rows4(best, 2), wave_rows4(best, 3)));
+        if (lane == 0) wmax[i][wv] = m;
         __syncthreads();
-        float m = wmax[i][0];
+        float x = wmax[i][0];
 #pragma unroll
-        for (int w = 1; w < SMP_WAVES; ++w) m = fmaxf(m, wmax[i][w]);
-        return m;
+        for (int w = 1; w < SMP_WAVES; ++w) x = fmaxf(x, wmax[i][w]);
+        return x;
     };
     const int n = (hi - lo + SMP_WAVES - 1) / SMP_WAVES;
 #pragma unroll
-    for (int j = 0; j < SMP_KEEP; ++j) first(keep[j], j);
+    for (int j = 0; j < SMP_KEEP; j += 4) first(keep + j, j);
     const float ref = largest(0);
     const bool draws = T > 0.f;  // greedy rows need the maxima only
     const SmpScale c = smp_scale(ref, T);
@@ -261,10 +293,10 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_bins_kernel(const float* _
             SmpFour ahead[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) ahead[i] = load(j + 4 + i);
+            first(f, j);
+            if (lay) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                first(f[i], j + i);
-                if (lay) add(c, f[i], j + i);
+                for (int i = 0; i < 4; ++i) add(c, f[i], j + i);
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) f[i] = ahead[i];
@@ -382,28 +414,43 @@ __device__ __forceinline__ void smp_each(const SmpShared& S, const SmpRow& r, F 
     }
 }
 
-// Ends in the n <= SMP_SMALL entries of S.place and S.m, `sum0` and `rank0` before them: as smp_end.
+// Sum over the 16 lanes of a row: every lane gets it.
+template <typename V>
+__device__ __forceinline__ V smp_row_sum(V v) {
+    v += smp_from<0xB1, 0xF>(v);
+    v += smp_from<0x4E, 0xF>(v);
+    v += smp_from<0x141, 0xF>(v);
+    v += smp_from<0x140, 0xF>(v);
+    return v;
+}
+// Ends in the n <= SMP_SMALL entries of S.place and S.m, `sum0` and `rank0` before them: as smp_end.  16 lanes count
+// what is before an entry.
 template <bool COUNT>
 __device__ __forceinline__ void smp_end_few(SmpShared& S, int n, double t, uint64_t sum0, uint64_t rank0) {
-    if ((int)threadIdx.x >= n) return;
-    const uint64_t mine = S.place[threadIdx.x], w = S.m[threadIdx.x];
-    uint64_t sum = sum0, rank = rank0;
-    for (int i = 0; i < n; ++i) {
-        const bool before = S.place[i] >= mine;
-        sum += before ? S.m[i] : 0;
-        rank += before;
-    }
-    const bool passes = COUNT ? (double)rank >= t : (double)sum > t;
-    const bool passed = COUNT ? (double)(rank - 1) >= t : (double)(sum - w) > t;
-    if ((passes && !passed) || (!passes && rank == rank0 + n)) {
-        S.found = mine;
-        S.found_m = sum;
+    const int part = threadIdx.x & 15;
+    for (int at = threadIdx.x >> 4; at < n; at += SMP_THREADS / 16) {
+        const uint64_t mine = S.place[at], w = S.m[at];
+        uint64_t sum = 0;
+        uint32_t r = 0;
+        for (int i = part; i < n; i += 16) {
+            const bool before = S.place[i] >= mine;
+            sum += before ? S.m[i] : 0;
+            r += before;
+        }
+        sum = sum0 + smp_row_sum(sum);
+        const uint64_t rank = rank0 + smp_row_sum(r);
+        const bool passes = COUNT ? (double)rank >= t : (double)sum > t;
+        const bool passed = COUNT ? (double)(rank - 1) >= t : (double)(sum - w) > t;
+        if (part == 0 && ((passes && !passed) || (!passes && rank == rank0 + n))) {
+            S.found = mine;
+            S.found_m = sum;
+        }
     }
 }
 
 // In bin b (one with entries): the first entry in the order at which the running weight exceeds t (COUNT: the t-th
 // entry, from 1), the bin's last one if none does.  Its place, and the bin's weight up to and with it.  All threads.
-// Up to 64 entries count those before them; more are first split into 1024 steps of the bin; where one of these holds
+// Up to 128 entries count those before them; more are first split into 1024 steps of the bin; where one of these holds
 // more than SMP_SMALL (a flat row, ties), digit by digit over the places.
 template <bool COUNT>
 __device__ uint64_t smp_end(SmpShared& S, const SmpRow& r, int b, double t, uint64_t& upto) {
@@ -460,7 +507,7 @@ __device__ uint64_t smp_end(SmpShared& S, const SmpRow& r, int b, double t, uint
         return (int)S.found;
     };
     int n = collect(-1);
-    if (n > 64) {
+    if (n > SMP_FEW) {
         const int step = split([&](uint64_t c) { return smp_inside(r.c, smp_value(c)); });
         n = collect(step);
         if (n > SMP_SMALL) {
