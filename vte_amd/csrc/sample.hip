@@ -345,23 +345,35 @@ __device__ __forceinline__ uint64_t smp_lane(uint64_t v, int l) {
     return (uint64_t)smp_lane((uint32_t)v, l) | (uint64_t)smp_lane((uint32_t)(v >> 32), l) << 32;
 }
 template <typename V>
-__device__ __forceinline__ V smp_scan(V v, V* sh) {
-    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+__device__ __forceinline__ V smp_rows_scan(V v) {  // in rows of 16 lanes
     v += smp_from<0x111, 0xF>(v);
     v += smp_from<0x112, 0xF>(v);
     v += smp_from<0x114, 0xF>(v);
     v += smp_from<0x118, 0xF>(v);
+    return v;
+}
+template <typename V>
+__device__ __forceinline__ V smp_wave_scan(V v) {
+    v = smp_rows_scan(v);
     v += smp_from<0x142, 0xA>(v);
     v += smp_from<0x143, 0xC>(v);
-    __syncthreads();
-    if (lane == 63) sh[wv] = v;
-    __syncthreads();
-    V w = sh[lane & 15];  // running sums of the waves', in rows of 16 lanes
-    w += smp_from<0x111, 0xF>(w);
-    w += smp_from<0x112, 0xF>(w);
-    w += smp_from<0x114, 0xF>(w);
-    w += smp_from<0x118, 0xF>(w);
+    return v;
+}
+template <typename V>
+__device__ __forceinline__ V smp_join(V v, const V* sh, V& all) {  // with the waves' sums
+    const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const V w = smp_rows_scan(sh[threadIdx.x & 15]);
+    all = smp_lane(w, 15);
     return v + (wv > 0 ? smp_lane(w, wv - 1) : 0);
+}
+template <typename V>
+__device__ __forceinline__ V smp_scan(V v, V* sh) {
+    V all;
+    v = smp_wave_scan(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 63) sh[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return smp_join(v, sh, all);
 }
 
 struct SmpRow {
@@ -378,6 +390,7 @@ struct SmpShared {
     uint32_t digit_n[SMP_SMALL];
     uint16_t need[1024];        // subsets that may hold wanted entries
     uint64_t wave[SMP_WAVES], before[2];
+    uint32_t wave_n[SMP_WAVES];
     uint64_t found, found_m;
     int n, n_need, n_match, overflow, hit[2];
 };
@@ -483,7 +496,6 @@ __device__ uint64_t smp_end(SmpShared& S, const SmpRow& r, int b, double t, uint
         __syncthreads();
         S.m[tid] = 0;
         S.digit_n[tid] = 0;
-        if (tid == 0) S.hit[0] = -1;
         __syncthreads();
         smp_each(S, r, [&](uint64_t c, int g, uint64_t m) {
             const int d = g == b ? of(c) : -1;
@@ -492,16 +504,22 @@ __device__ uint64_t smp_end(SmpShared& S, const SmpRow& r, int b, double t, uint
             atomicAdd(&S.digit_n[d], 1u);
         });
         __syncthreads();
-        const uint64_t m = S.m[tid], n = S.digit_n[tid];
-        const uint64_t sum = sum0 + smp_scan<uint64_t>(m, S.wave);
+        const uint64_t m = S.m[tid];
+        const uint32_t n = S.digit_n[tid];
+        uint64_t sum = smp_wave_scan(m), all;
+        uint32_t rank32 = smp_wave_scan(n), all_n;
+        if ((tid & 63) == 63) {
+            S.wave[tid >> 6] = sum;
+            S.wave_n[tid >> 6] = rank32;
+        }
         __syncthreads();
-        const uint64_t rank = rank0 + smp_scan<uint32_t>((uint32_t)n, (uint32_t*)S.wave);
+        sum = sum0 + smp_join(sum, S.wave, all);
+        rank32 = smp_join(rank32, S.wave_n, all_n);
+        const uint64_t rank = rank0 + rank32;
         const bool passes = COUNT ? (double)rank >= t : (double)sum > t;
         const bool passed = COUNT ? (double)(rank - n) >= t : (double)(sum - m) > t;
-        if (n && !passed) atomicMax(&S.hit[0], passes ? SMP_THREADS : tid);  // the last class, if none passes
-        __syncthreads();
-        const int last = S.hit[0];
-        if (n && !passed && (last == SMP_THREADS ? passes : tid == last)) {
+        const bool none = COUNT ? !((double)(rank0 + all_n) >= t) : !((double)(sum0 + all) > t);
+        if (n && (none ? rank32 == all_n : passes && !passed)) {  // none passes: the last class
             S.found = (uint64_t)tid;
             S.found_m = sum;
             S.before[0] = sum - m;
@@ -512,7 +530,7 @@ __device__ uint64_t smp_end(SmpShared& S, const SmpRow& r, int b, double t, uint
         rank0 = S.before[1];
         return (int)S.found;
     };
-    int n = collect(-1);
+    int n = S.n > 4 * SMP_FEW ? SMP_SMALL + 1 : collect(-1);  // (of many collected ones most bins have more)
     if (n > SMP_FEW) {
         const int step = split([&](uint64_t c) { return smp_inside(r.c, smp_value(c)); });
         n = collect(step);
