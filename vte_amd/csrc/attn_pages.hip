@@ -87,6 +87,14 @@ __device__ __forceinline__ float pa_pow2(int d) { return d < -126 ? 0.f : __uint
 // segment that lies in one share is done there; one that is cut leaves a record in
 // each: it is its first block's last piece and the first piece of the others, so
 // two records a block are enough.
+//
+// Bound by the cache's bytes where contexts are long: eight documents of 16384 to
+// 65536 tokens, 168 MB, 41 us in all, 4.1 TB/s (a sum over as many bytes reads 4.0,
+// a copy moves 5.0); by latencies where they are short: 2049 tokens 12.2 us, two
+// launches, in the first four loads one after the other (positions, page, bytes, q) and a
+// tile's work.  Bytes go from memory to registers, where a lane's 16 are its operand
+// once permuted: no LDS, each is used once, and a wave has the next tile's under way
+// (two blocks of 256 threads a CU is all that those registers leave).
 // ---------------------------------------------------------------------------
 struct PaPlan {
     int blocks;  // grid of the main launch
@@ -512,8 +520,17 @@ __global__ __launch_bounds__(256) void attn_pages_combine_kernel(KvPages c, KvRo
 // V^T.P^T (a lane is a row in both), K rows are read with token bits 2 and 3
 // swapped so that a lane's scores are its operand of the second product as they
 // stand.
+//
+// Bound by issue: a group's step is 32 products a wave (1000 cycles) beside as many
+// cycles of turning bytes and some 800 of softmax, which overlap in part: 2.4 us for
+// two groups' steps.  The runs below fix what stands between two products (left to
+// itself the compiler read an operand right before each).  Beside that a block starts
+// (4 us: sequence, page, bytes, the first tile) and ends (3 us), which weighs on short
+// ones: four sequences of 2048 new tokens, 32 query and 8 KV heads of 128, 202 us, 680
+// TFLOP/s (a large fp16 matrix product: 1100 to 1200); a chunk of 512 after 1536 tokens,
+// in shares of 8 steps, 24 us, 231.
 // ---------------------------------------------------------------------------
-#define PA_SHARES 16
+#define PA_SHARES 64
 #define PA_APART 24
 #define PA_LAG 6    // sums are rescaled when a maximum has grown by more than 2^6 ..
 #define PA_Q_LOG2 9 // .. so probabilities are held as 2^9 p, at most 2^15
@@ -1104,6 +1121,11 @@ static PaPlan rows_plan(const KvPages& c, const KvRows& r, int hd, int G, void* 
 }
 // The many-rows form: rows of a block, row blocks at most (each sequence may end one early), and shares of each, as many
 // as fill the CUs.
+// Rows of a block: 256 (one group) from 7/4 blocks a CU on, else 128 (two groups).  256 / 128, us, 2048 new tokens a
+// sequence: 1.5 blocks a CU 107.9 / 103.3, 1.75 140 / 156, 2 100.8 / 119.1, 4 202 / 233.
+// Shares: of four steps at least, or of two while there are no more than 16; no more than 64.  Three new tokens, 16 query
+// heads, 16 / 32 / 64 / 128 shares, us: after 8192 tokens 22.4 / 20.6 / 23.1 / 23.0, after 32768 51 / 35 / 30 / 35; after
+// 2048 8 / 16 shares 16.5 / 15.6.
 struct PromptForm {
     int groups;
     long long rbs;
@@ -1113,10 +1135,11 @@ struct PromptForm {
 static PromptForm prompt_form(const KvPages& c, const KvRows& r, int hd, int G, void* scratch) {
     PromptForm f;
     auto blocks = [&](int rows) { return ((long long)r.rows * G + rows - 1) / rows + r.batch - 1; };
-    f.groups = blocks(256) * c.n_kv >= 2 * device_cus() ? 1 : 2;
+    f.groups = blocks(256) * c.n_kv * 4 >= 7 * device_cus() ? 1 : 2;
     f.rbs = blocks(f.groups == 1 ? 256 : 128);
     const long long steps = (((long long)r.max_pages << c.page_log2) + PA_TILE - 1) / PA_TILE;
-    f.p.nsp = (int)std::max<long long>(1, std::min<long long>({PA_SHARES, steps / 2, device_cus() / (f.rbs * c.n_kv)}));
+    const long long most = std::max(std::min(16LL, steps / 2), std::min<long long>(PA_SHARES, steps / 4));
+    f.p.nsp = (int)std::max(1LL, std::min(most, device_cus() / (f.rbs * c.n_kv)));
     const long long recs = f.p.nsp == 1 ? 0 : f.rbs * c.n_kv * f.p.nsp;
     uint8_t* at = static_cast<uint8_t*>(scratch);
     long long n = 16;
@@ -1129,6 +1152,8 @@ static PromptForm prompt_form(const KvPages& c, const KvRows& r, int hd, int G, 
     f.bytes = n;
     return f;
 }
+// One tile's columns hold them all.  (Few-rows / many-rows form, us: one sequence of 2049 tokens 12.2 / 16.4, 16 ragged ones
+// of up to 8192 18.3 / 32.5, eight of up to 65536 41.2 / 90.5.)
 static bool rows_form(const KvRows& r, int G) { return r.max_rows * G <= 16; }
 
 long long attn_pages_scratch_bytes(const KvPages& c, const KvRows& r, int hd, int n_q) {

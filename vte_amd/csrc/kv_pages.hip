@@ -15,7 +15,15 @@
 // none).  HD threads take K, each 8 rotation pairs of one token, HD threads V,
 // each 16 dims of one token, whose bytes change places in LDS.  Otherwise one wave
 // takes K and one V, a lane holding one pair of dims for all 16 tokens (heads of
-// 64: 8 tokens, the upper 32 lanes the later ones).
+// 64: 8 tokens, the upper 32 lanes the later ones): 2-byte loads and single bytes
+// stored, but any alignment and the partial rotation.
+//
+// A value is read once and a byte written once; a block of the cache is whole in
+// its block of threads because the scale needs its largest value first.  Few tokens:
+// a launch and four loads in a row (position, page, old exponent and bytes), 3.7 us
+// for one token.  Prompts: bytes, 41 MB of four chunks of 700 to 2048 tokens with
+// their q in 10.7 us, 3.9 TB/s (a large copy reaches 5.0).  With the read-back of the
+// chunks, us: 14.8 WIDE, 44.1 otherwise; one token each of 64 sequences 13.6 / 15.3.
 // ---------------------------------------------------------------------------
 struct KvRope {
     const __half *cosc, *sinc;
@@ -332,7 +340,10 @@ __global__ __launch_bounds__(WIDE ? 2 * HD : 128) void kv_pages_append_kernel(Kv
 // ---------------------------------------------------------------------------
 // Read: rows 0 .. end - 1 of every sequence as T [batch][out_rows][n_kv][HD].
 // HD threads turn one block of one head of K (16 dims of a token each), HD threads
-// the same of V (4 dims of 4 tokens each, whose bytes change places by permutes).
+// the same of V (4 dims of 4 tokens each, whose bytes change places by permutes: a
+// row's stores are then 8 or 16 bytes, as K's; with single values they took twice as
+// long, 48 us for what now takes 23).  Bound by bytes: 102 MB of a ragged batch of 16
+// sequences of up to 8192 tokens, 23 us, 4.4 TB/s (a copy: 5.0).
 // ---------------------------------------------------------------------------
 template <typename T, int N>
 __device__ __forceinline__ void kvp_put(T* dst, const uint32_t (&w)[N], float f) {  // 4 N bytes as values

@@ -21,6 +21,13 @@
 //      question and ends the filters and the draw in them.  One CU reads no more
 //      than some 30 GB/s, so while there are few rows several blocks share a row's
 //      reading: each merges for itself, and the last to be done (none waits) goes on.
+//
+// Bound by the two readings where there are many rows: 256 rows of 151936, 156 MB,
+// bins 41 us (3.8 TB/s; some 25 vector operations and an LDS addition an entry take
+// nearly as long), draw 60 us, of which reading 36 (a broad distribution's ends lie in
+// bins that nearly all subsets reach into; of a peaked one it reads a few).  Few rows:
+// by latencies, one row 8 + 14 us: merging 4, scans and ends of the filters 7.
+// With unaligned rows (not WIDE) / WIDE, us: one row 24.0 / 22.5, 256 107.2 / 100.6.
 #include <algorithm>
 #include "vte_common.h"
 
@@ -37,7 +44,7 @@
 #define SMP_SMALL 1024      // entries of a bin that are ordered by counting
 #define SMP_FEW 128         // .. without a split first
 #define SMP_AHEAD 4         // subsets a wave of the draw has in flight (8: one row 16.1 -> 18.6 us, 256 rows the same)
-#define SMP_SPLIT 8         // blocks of a row at most
+#define SMP_SPLIT 8         // blocks of a row at most (2: one row 30.6 us, 16 rows 37.8; 8: 22.5, 30.9; 16 as 8)
 
 // Scratch of a row.
 struct SmpScratch {
@@ -879,7 +886,8 @@ namespace vte {
 // Blocks of a row: as many as find a CU each (their registers let one lie on a CU; 256 rows in 512 blocks 47.5 us, in 256
 // 41.2 us).
 static int sample_blocks(int rows) { return std::max(1, std::min(SMP_SPLIT, device_cus() / rows)); }
-// Blocks that share the reading of a row, while they fit on the CUs at once.
+// Blocks that share the reading of a row, while they fit on the CUs at once: one / 16, us: 16 rows 55.6 / 30.9, one peaked
+// row, of which little is read, 21.8 / 22.5.
 static int draw_blocks(int rows) { return std::max(1, std::min(16, device_cus() / rows)); }
 
 long long sample_scratch_bytes(int rows) {
