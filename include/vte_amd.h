@@ -424,7 +424,8 @@ long long vte_attn_pages_scratch_bytes(const vte_kv_pages* cache, const vte_kv_r
 
 /* Attention of the new rows over the paged cache (which holds them already):
  * row i of sequence b sees positions 0 .. kv_offset[b] + i.  q and out
- * [rows][n_q][head_dim] (dtype fp16 or fp32; out may be q), n_q / n_kv <= 16.  A row that sees
+ * [rows][n_q][head_dim] (dtype fp16 or fp32; out may be q), n_q / n_kv <= 16,
+ * rows * n_q <= 2^25, batch * n_kv <= 2^20.  A row that sees
  * nothing (a sequence that does not run, no pages) gives 0; rows that belong to
  * nobody are left as they were.  Sums and softmax statistics are fp32; with fp16
  * the probabilities enter the products as fp16, with fp32 q and the probabilities

@@ -420,6 +420,24 @@ def test_attention_beside_huge_keys_in_other_dims(hip, K, dtype, new):
     check_attention(hip, K, bt, [300 - new], [new], 6, dtype, rng, zero_dims=4)
 
 
+@pytest.mark.parametrize("new", [1, 70])
+def test_attention_of_scores_far_below_zero(hip, K, new):
+    """Equal keys, so equal weights, at scores of -6e32: the mean of V."""
+    rng = np.random.default_rng(15)
+    bt = Batch(hip, K, rng, [200], 1, 64, 64)
+    v = rng.standard_normal((200, 1, 64)).astype(np.float32)
+    append_ref(bt, 0, 0, np.full((200, 1, 64), 1e14, np.float32), v)
+    bt.upload()
+    r = bt.rows([200 - new], [new])
+    q, out = up(hip, np.full((new, 4, 64), -1e18, np.float32)), empty(hip, (new, 4, 64), np.float32)
+    need = K.attn_pages_scratch_bytes(bt.pages, r, 4)
+    K.attn_pages(bt.pages, r, q, out, 4, 0.1, empty(hip, need, np.uint8), need, dtype="f32", stream=hip.stream)
+    got, v = down(out), bt.ref.v[0].values(200)[:, 0]
+    for i in range(new):
+        # weights of 1 and sums of up to 200 of them: 200 roundings of 2^-24 of the largest |V| at most
+        assert np.abs(got[i] - v[:201 - new + i].mean(0)).max() <= 200 * 2.0 ** -24 * np.abs(v).max()
+
+
 @pytest.mark.parametrize("new", [2, 70])
 def test_attention_of_positions_at_the_end_of_int(hip, K, new):
     """Positions behind the table see all of it, up to the largest int; what they append has no place."""

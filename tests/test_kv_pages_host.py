@@ -88,7 +88,9 @@ def test_read_and_attention_refusals():
                  lambda: K.attn_pages(c, r, P, P, 12, float("nan"), P, need),
                  lambda: K.attn_pages(c, r, P, P, 13, 0.1, P, need),   # no multiple of n_kv
                  lambda: K.attn_pages(c, r, P, P, 34, 0.1, P, 1 << 40),  # 17 heads of one KV head
-                 lambda: K.attn_pages_scratch_bytes(c, r, 34)):
+                 lambda: K.attn_pages_scratch_bytes(c, r, 34),
+                 lambda: K.attn_pages_scratch_bytes(pages(n_kv=16), rows(rows=(1 << 21) + 1, max_rows=9, row_start=P), 16),
+                 lambda: K.attn_pages_scratch_bytes(pages(n_kv=32), rows(batch=32769, rows=32769), 32)):
         with pytest.raises(HIPSafetyError):
             call()
     lib, ref = K.lib, ctypes.byref

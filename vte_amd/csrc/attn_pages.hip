@@ -18,7 +18,7 @@
 
 #define PA_TILE 64       // tokens of a wave's step: a lane group of 16 holds one block of 16
 #define PA_P_LOG2 14     // probabilities are held as 2^14 p
-#define PA_NONE (-1e30f) // running maximum before anything is seen
+#define PA_NONE (-3e38f) // running maximum before anything is seen
 
 typedef _Float16 pa_h2 __attribute__((ext_vector_type(2)));
 typedef unsigned pa_u2 __attribute__((ext_vector_type(2)));
@@ -515,8 +515,8 @@ __global__ __launch_bounds__(256) void attn_pages_combine_kernel(KvPages c, KvRo
 // with ref the largest exponent of the step (K) or so far (V), so a step's scores
 // and sums have one scale.  That is exact while no block lies below 2^-24 of ref
 // (PA_APART); a row's result must not depend on how large tokens are that it does
-// not see, so a wave that met such a block does its rows over, block by block
-// (pa_apart, some ten times as long).  Scores are K.Q^T, sums are
+// not see, so a wave that met such a block, or a score beyond 2^20, does its rows over,
+// block by block (pa_apart, some ten times as long).  Scores are K.Q^T, sums are
 // V^T.P^T (a lane is a row in both), K rows are read with token bits 2 and 3
 // swapped so that a lane's scores are its operand of the second product as they
 // stand.
@@ -531,7 +531,7 @@ __global__ __launch_bounds__(256) void attn_pages_combine_kernel(KvPages c, KvRo
 // in shares of 8 steps, 24 us, 231.
 // ---------------------------------------------------------------------------
 #define PA_SHARES 64
-#define PA_APART 24
+#define PA_APART 24 // scales of blocks that are staged together, log2
 #define PA_LAG 6    // sums are rescaled when a maximum has grown by more than 2^6 ..
 #define PA_Q_LOG2 9 // .. so probabilities are held as 2^9 p, at most 2^15
 
@@ -906,6 +906,8 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
             for (int dt = 0; dt < DT; ++dt) o[dt] *= both;
             m_run = mx;
             o_ref = cur_v;
+            // (products enter the exponent unrounded, their maximum rounded: beyond 2^20 that is too far apart)
+            apart |= (fabsf(mx) > 1048576.f) & (mx > PA_NONE);
         }
         if (cur_odd >> 4) {  // NaN in V: the sums of the rows that see a token of its block
 #pragma unroll

@@ -861,6 +861,7 @@ static int check_attn_pages(const vte_kv_pages* cache, const vte_kv_rows* rows, 
     REQUIRE(n_q >= c->n_kv && n_q <= 65535 && n_q % c->n_kv == 0 && n_q / c->n_kv <= 16,
             "attn_pages: bad head counts %d/%d (groups of at most 16)", n_q, c->n_kv);
     REQUIRE(r->rows >= 1 && r->max_rows >= 1, "attn_pages: no rows");
+    REQUIRE((long long)r->rows * n_q <= (1 << 25), "attn_pages: rows %d x n_q %d above 2^25", r->rows, n_q);
     REQUIRE((long long)r->batch * c->n_kv <= (1 << 20), "attn_pages: batch %d x n_kv %d above 2^20", r->batch, c->n_kv);
     return 0;
 }
