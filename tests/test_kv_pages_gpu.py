@@ -331,6 +331,19 @@ def test_attention_prompts(hip, K, dtype, n_q, n_kv, hd, page):
     check_attention(hip, K, bt, old, new, n_q, dtype, rng, pad=2)
 
 
+@pytest.mark.parametrize("batch", [64, 65, 300, 700])
+@pytest.mark.parametrize("ragged", [False, True])
+def test_attention_of_many_sequences(hip, K, batch, ragged):
+    """More sequences than a wave or a block has lanes, some of which do not run, with few rows and with many."""
+    rng = np.random.default_rng(batch)
+    new = [int(n) for n in (rng.integers(0, 7, batch) if ragged else [1] * batch)]
+    new[batch // 2] = 6 if ragged else 1
+    lens = [int(rng.integers(n, 150)) if n else 0 for n in new]
+    bt = filled(hip, K, rng, lens, 1, 64, 16)
+    pos = [x - n if b % 9 else -1 for b, (x, n) in enumerate(zip(lens, new))]
+    check_attention(hip, K, bt, pos, new, 4, "f16", rng, row_start=ragged)
+
+
 @pytest.mark.parametrize("dtype,hd", [("f16", 128), ("f32", 64)])
 def test_attention_of_some_rows_over_a_long_cache(hip, K, dtype, hd):
     """More rows than one tile has columns, tokens for more shares than are joined at once."""

@@ -149,12 +149,38 @@ __device__ __forceinline__ PaShare pa_share(const KvPages& c, const KvRows& r, i
     __shared__ long long wsum[4];
     __shared__ long long found[5];
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+    auto tiles = [&](const KvSeq& q) { return (long long)c.n_kv * ((pa_tokens(q, cap) + PA_TILE - 1) / PA_TILE); };
+    auto cut = [&](PaShare& s, long long total) {
+        // (a tile for each wave at least; whole rounds of four beyond that left CUs idle: eight documents of 16384 to
+        // 65536 tokens 44.0 -> 41.3 us without, 16 ragged sequences 19.7 -> 18.3 us)
+        s.share = max((total + blocks - 1) / blocks, 4LL);
+        s.t = s.share * block;
+        s.t_end = min(total, s.t + s.share);
+    };
+    if (r.batch <= 64) {  // every wave for itself, a sequence a lane
+        const KvSeq q = kvp_seq(r, min(lane, r.batch - 1));
+        const long long n = lane < r.batch ? tiles(q) : 0, incl = pa_scan(n);
+        auto at = [](long long v, int l) {
+            return (long long)((unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)(v >> 32), l) << 32 |
+                               (unsigned)__builtin_amdgcn_readlane((int)v, l));
+        };
+        PaShare s;
+        cut(s, at(incl, 63));
+        const uint64_t here = __ballot((s.t >= incl - n) & (s.t < incl));
+        const int l = here ? __ffsll((unsigned long long)here) - 1 : 0;  // (none: a block without a share)
+        s.b = l;
+        s.before = at(incl - n, l);
+        s.s.first = __builtin_amdgcn_readlane(q.first, l);
+        s.s.n = __builtin_amdgcn_readlane(q.n, l);
+        s.s.pos = __builtin_amdgcn_readlane(q.pos, l);
+        return s;
+    }
     const int per = (r.batch + 255) / 256;
     long long mine = 0;
     KvSeq mine_last = {0, 0, 0};
     for (int b = tid * per; b < min(r.batch, tid * per + per); ++b) {
         mine_last = kvp_seq(r, b);
-        mine += (long long)c.n_kv * ((pa_tokens(mine_last, cap) + PA_TILE - 1) / PA_TILE);
+        mine += tiles(mine_last);
     }
     long long incl = pa_scan(mine);
     if (lane == 63) wsum[wv] = incl;
@@ -163,11 +189,7 @@ __device__ __forceinline__ PaShare pa_share(const KvPages& c, const KvRows& r, i
     incl += wv > 2 ? w4[0] + w4[1] + w4[2] : wv > 1 ? w4[0] + w4[1] : wv > 0 ? w4[0] : 0;
     const long long total = pa_uniform(w4[0] + w4[1] + w4[2] + w4[3]);
     PaShare s;
-    // (a tile for each wave at least; whole rounds of four beyond that left CUs idle: eight documents of 16384 to 65536
-    // tokens 44.0 -> 41.3 us without, 16 ragged sequences 19.7 -> 18.3 us)
-    s.share = max((total + blocks - 1) / blocks, 4LL);
-    s.t = s.share * block;
-    s.t_end = min(total, s.t + s.share);
+    cut(s, total);
     if (mine > 0 && s.t >= incl - mine && s.t < incl) {
         long long before = incl - mine;
         int b = tid * per;
@@ -175,7 +197,7 @@ __device__ __forceinline__ PaShare pa_share(const KvPages& c, const KvRows& r, i
         if (per > 1)
             for (;; ++b) {
                 q = kvp_seq(r, b);
-                const long long n = (long long)c.n_kv * ((pa_tokens(q, cap) + PA_TILE - 1) / PA_TILE);
+                const long long n = tiles(q);
                 if (s.t < before + n) break;
                 before += n;
             }
