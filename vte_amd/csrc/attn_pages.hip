@@ -779,16 +779,60 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
         find(step + GROUPS);
     };
     find(a + grp);
-    // (q is asked for while the page number is on its way)
+    // q is asked for while the page number is on its way.  The wave's 32 rows by lanes in 128-byte pieces, which change
+    // places in LDS (a row a lane touches a line each: the first tile was there 1.2 us later), in the second buffer, which
+    // nothing is put into before the first barrier; where that is too small, a row a lane.
+    constexpr bool TURN_Q = sizeof(Tile) >= (size_t)WAVES * 4096;
+    constexpr int QP = HD * (int)sizeof(T) / 128;  // pieces of a row
     typedef typename std::conditional<PARTS == 1, half8_t, floatx8_t>::type q8_t;
     q8_t q_raw[KS];
-    {
+    uint4 q_piece[QP][4];
+    if constexpr (TURN_Q) {
+        const uint32_t inv = 0xFFFFFFFFu / (uint32_t)G + 1;  // ri / G = ri inv >> 32 for ri < 2^28, 1 < G <= 16
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int i = min(r0 + 8 * k + (lane >> 3), rows - 1), n = G == 1 ? i : (int)__umulhi((uint32_t)i, inv);
+            const uint8_t* at = reinterpret_cast<const uint8_t*>(q + ((size_t)(s.first + n) * n_q + h * G + i - n * G) * HD) +
+                                (lane & 7) * 16;
+#pragma unroll
+            for (int p = 0; p < QP; ++p) q_piece[p][k] = ldg_g16(at + 128 * p);
+        }
+    } else {
         const T* qp = q + ((size_t)(s.first + qi) * n_q + qh) * HD + 8 * half;
 #pragma unroll
         for (int i = 0; i < KS; ++i) q_raw[i] = *reinterpret_cast<const q8_t*>(qp + 16 * i);
     }
     __builtin_amdgcn_sched_barrier(0);
     load(a + grp);
+    if constexpr (TURN_Q) {
+        uint4* to = reinterpret_cast<uint4*>(&S.tiles[grp][1]) + wv * 256;
+        auto order = [] {  // of the wave's own LDS accesses
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        };
+#pragma unroll
+        for (int p = 0; p < QP; ++p) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int rr = 8 * k + (lane >> 3);
+                to[rr * 8 + ((lane & 7) ^ (rr >> 1 & 7))] = q_piece[p][k];
+            }
+            order();
+#pragma unroll
+            for (int i = 0; i < KS / QP; ++i) {
+                union {
+                    uint4 u[sizeof(q8_t) / 16];
+                    q8_t v;
+                } x;
+#pragma unroll
+                for (int e = 0; e < (int)sizeof(q8_t) / 16; ++e)
+                    x.u[e] = to[row * 8 + (((2 * i + half) * (int)sizeof(q8_t) / 16 + e) ^ (row >> 1 & 7))];
+                q_raw[p * (KS / QP) + i] = x.v;
+            }
+            order();
+        }
+    }
 
     half8_t qb[PARTS][KS];
     float q_unit = 1.f;
