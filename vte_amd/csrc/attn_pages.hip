@@ -604,7 +604,7 @@ struct PaPrompt {
     int nsp;    // shares of a row block
     float* ml;  // [row blocks][n_kv][nsp][128][2]: maximum (log2), sum
     int* ev;    // [row blocks][n_kv][nsp][128]: exponent that the row's sums are relative to
-    float* o;   // [row blocks][n_kv][nsp][128][HD]
+    float* o;   // [row blocks][n_kv][nsp][HD / 8][32-row tile][4 dims of 8][row][4]
 };
 
 // A row's results: dims 32 i + 8 (j / 4) + j % 4 from dst on.
@@ -1088,13 +1088,13 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
         const int d0 = grp * (HD / 2) + 4 * half;  // first dim of mine
         if (pieces > 1) {
             const size_t rec = ((size_t)slot * c.n_kv + h) * pp.nsp + blockIdx.y;
-            float* po = pp.o + (rec * ROWS + wv * 32 + row) * HD + d0;
+            if (r0 + row >= rows) return;
+            floatx4_t* po = reinterpret_cast<floatx4_t*>(pp.o + rec * ROWS * HD) + grp * (HD / 16) * 256 + tid;
 #pragma unroll
             for (int i = 0; i < DT / 2; ++i)
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    *reinterpret_cast<floatx4_t*>(po + 32 * i + 8 * j) =
-                        floatx4_t{mine[i][4 * j], mine[i][4 * j + 1], mine[i][4 * j + 2], mine[i][4 * j + 3]};
+                    po[(4 * i + j) * 256] = floatx4_t{mine[i][4 * j], mine[i][4 * j + 1], mine[i][4 * j + 2], mine[i][4 * j + 3]};
             if (half == 0 && grp == 0) {
                 pp.ml[(rec * ROWS + wv * 32 + row) * 2] = M;
                 pp.ml[(rec * ROWS + wv * 32 + row) * 2 + 1] = L;
@@ -1106,17 +1106,20 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
     }
 }
 
-// Joins the shares of the row blocks: grid (row blocks, n_kv, 128 / rows of a block), HD / 4 threads a row.
+// Joins the shares of the row blocks: grid (row blocks, n_kv, HD / 8).  A block takes 32 rows and 32 dims, a wave 8 of
+// them, as the records have them (1024 bytes on end a load); results change places in LDS: 64 or 128 bytes of a row together.
 template <typename T, int HD>
 __global__ __launch_bounds__(256) void attn_pages_prompt_combine_kernel(KvPages c, KvRows r, PaPrompt pp,
                                                                         T* __restrict__ out, int n_q) {
-    constexpr int TD = HD / 4, ROWS = 128;
+    constexpr int ROWS = 128;
     const int slot = blockIdx.x, h = blockIdx.y, G = n_q / c.n_kv;
     const PaRowBlock R = pa_row_block<ROWS>(r, G, slot);
     if (R.b < 0) return;
-    const int rr = blockIdx.z * (256 / TD) + threadIdx.x / TD, d = threadIdx.x % TD * 4, ri = R.rb * ROWS + rr;
+    const int lane = threadIdx.x & 63, tile = blockIdx.z & 3, part = (blockIdx.z & ~3) + (threadIdx.x >> 6);
+    const int rr = 32 * tile + (lane & 31), rows = R.s.n * G;
+    __shared__ __align__(16) float o_sh[32][32 + 4];
     const int steps = pa_steps<ROWS>(R, G, kvp_capacity(c, r)), share = pa_share_of(steps, pp.nsp);
-    if (steps <= share || ri >= R.s.n * G) return;
+    if (steps <= share || R.rb * ROWS + 32 * tile >= rows) return;
     const int pieces = (steps + share - 1) / share;
     const size_t rec0 = ((size_t)slot * c.n_kv + h) * pp.nsp;
     float M = PA_NONE, L = 0.f;
@@ -1130,7 +1133,7 @@ __global__ __launch_bounds__(256) void attn_pages_prompt_combine_kernel(KvPages 
 #pragma unroll
         for (int i = 0; i < AT_ONCE; ++i) {
             const size_t rec = (rec0 + min(i0 + i, pieces - 1)) * ROWS + rr;
-            o[i] = *reinterpret_cast<const floatx4_t*>(pp.o + rec * HD + d);
+            o[i] = reinterpret_cast<const floatx4_t*>(pp.o + (rec - rr) * HD)[part * 256 + 64 * tile + lane];
             ml[i] = *reinterpret_cast<const float2*>(pp.ml + rec * 2);
             ev[i] = pp.ev[rec];
         }
@@ -1153,9 +1156,16 @@ __global__ __launch_bounds__(256) void attn_pages_prompt_combine_kernel(KvPages 
             O += o[i] * (f * pa_pow2(ev[i] - EV));
         }
     }
-    T* dst = out + ((size_t)(R.s.first + ri / G) * n_q + h * G + ri % G) * HD + d;
+    floatx4_t x;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) st_act<T>(dst + e, L == 0.f ? 0.f : ldexpf(O[e] / L, EV));
+    for (int e = 0; e < 4; ++e) x[e] = L == 0.f ? 0.f : ldexpf(O[e] / L, EV);
+    *reinterpret_cast<floatx4_t*>(&o_sh[lane & 31][8 * (threadIdx.x >> 6) + 4 * (lane >> 5)]) = x;
+    __syncthreads();
+    const int at = threadIdx.x >> 3, d = threadIdx.x % 8 * 4, ri = R.rb * ROWS + 32 * tile + at;
+    if (ri >= rows) return;
+    T* dst = out + ((size_t)(R.s.first + ri / G) * n_q + h * G + ri % G) * HD + (blockIdx.z >> 2) * 32 + d;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) st_act<T>(dst + e, o_sh[at][d + e]);
 }
 
 // ---------------------------------------------------------------------------
@@ -1253,7 +1263,7 @@ static hipError_t attn_hd(const KvPages& c, const KvRows& r, const void* q, void
                        n_q, scale);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || f.p.nsp == 1) return e;
-    hipLaunchKernelGGL((attn_pages_prompt_combine_kernel<T, HD>), dim3((unsigned)f.rbs, c.n_kv, 128 * HD / 1024),
+    hipLaunchKernelGGL((attn_pages_prompt_combine_kernel<T, HD>), dim3((unsigned)f.rbs, c.n_kv, HD / 8),
                        dim3(256), 0, st, c, r, f.p, (T*)out, n_q);
     return hipGetLastError();
 }
