@@ -640,8 +640,12 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_draw_kernel(const float* _
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const SmpScratch sc = smp_scratch(scratch, row, blocks, subs);
     const float T = temperature ? temperature[row] : 1.f;
-    float top = sc.max[0];
-    for (int i = 1; i < blocks; ++i) top = fmaxf(top, sc.max[i]);
+    float part[SMP_SPLIT];  // largest of each part, requested together (past the last one: the last again)
+#pragma unroll
+    for (int i = 0; i < SMP_SPLIT; ++i) part[i] = sc.max[min(i, blocks - 1)];
+    float top = part[0];
+#pragma unroll
+    for (int i = 1; i < SMP_SPLIT; ++i) top = fmaxf(top, part[i]);
     SmpRow r;
     r.x = logits + (size_t)row * vocab;
     r.vocab = vocab;
@@ -682,8 +686,7 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_draw_kernel(const float* _
         int at[SMP_SPLIT];
 #pragma unroll
         for (int i = 0; i < SMP_SPLIT; ++i) {
-            const float part = i < blocks ? sc.max[i] : -INFINITY;
-            at[i] = part > -INFINITY ? tid - smp_apart(r.c, part) : -1;
+            at[i] = i < blocks && part[i] > -INFINITY ? tid - smp_apart(r.c, part[i]) : -1;
             const size_t o = (size_t)(i < blocks ? i : 0) * SMP_BINS + max(at[i], 0);
             mm[i] = sc.mass[o];
             nn[i] = has_k ? sc.count[o] : 0;
@@ -744,9 +747,10 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_draw_kernel(const float* _
         uint64_t w = 0;
         smp_bin(r.c, top, g, w);
         floor_w = fmin(mp, 1.0) * (double)w;  // in units of 2^-44 of bin 0's middle
-        const double y = (log(SMP_ONE) - log(floor_w)) * SMP_PER_UNIT + 0.5;
-        m0 = (int)fmin(fmax(floor(y - 1e-6), 0.0), (double)(SMP_BINS - 1));
-        m1 = (int)fmin(fmax(floor(y + 1e-6), 0.0), (double)(SMP_BINS - 1));
+        // (in 32 bits: within 2e-4 of a bin, as log2 is at most 47 there)
+        const float y = __log2f((float)(floor_w / SMP_ONE)) * (float)(-0.69314718055994530942 * SMP_PER_UNIT) + 0.5f;
+        m0 = (int)fminf(fmaxf(floorf(y - 1e-3f), 0.f), (float)(SMP_BINS - 1));
+        m1 = (int)fminf(fmaxf(floorf(y + 1e-3f), 0.f), (float)(SMP_BINS - 1));
         k_lo = fmin(k_lo, smp_before(S, m0));
         k_hi = fmin(k_hi, (double)S.mass[m1]);
         last = max(last, m1);
