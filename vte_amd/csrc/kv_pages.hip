@@ -356,10 +356,12 @@ __device__ __forceinline__ void kvp_put(T* dst, const uint32_t (&w)[N], float f)
 #pragma unroll
     for (int i = 0; i < 4 * N; ++i) st_act<T>(&r.t[i], (float)((int)(w[i / 4] >> (8 * (i % 4)) & 0xFFu) - KVP_ZERO) * f);
     if constexpr (4 * N * sizeof(T) == 8) {
-        *reinterpret_cast<uint2*>(dst) = r.u2[0];
+        typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+        __builtin_nontemporal_store(u32x2{r.u2[0].x, r.u2[0].y}, reinterpret_cast<u32x2*>(dst));
     } else {
 #pragma unroll
-        for (int i = 0; i < (int)(4 * N * sizeof(T) / 16); ++i) reinterpret_cast<uint4*>(dst)[i] = r.u4[i];
+        for (int i = 0; i < (int)(4 * N * sizeof(T) / 16); ++i)
+            __builtin_nontemporal_store(vte_u32x4{r.u4[i].x, r.u4[i].y, r.u4[i].z, r.u4[i].w}, reinterpret_cast<vte_u32x4*>(dst) + i);
     }
 }
 
