@@ -21,6 +21,7 @@
 #define PA_NONE (-3e38f) // running maximum before anything is seen
 
 typedef _Float16 pa_h2 __attribute__((ext_vector_type(2)));
+typedef float pa_f2 __attribute__((ext_vector_type(2)));
 typedef unsigned pa_u2 __attribute__((ext_vector_type(2)));
 
 // 8 bytes as 8 fp16 whole numbers (byte - 128), or `by` times them (one rounded operation; exact for a power of two
@@ -995,6 +996,8 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
         // Sums: a block's probabilities are formed, and the one's V behind it read, under its products.
         const float shift = (float)PA_Q_LOG2 - m_run;
         const pa_h2 ones = {(_Float16)1.f, (_Float16)1.f};
+        float minus = -1.f;  // (a value that the compiler does not know: p - h as one mixed operation instead of two)
+        asm("" : "+v"(minus));
         union Probs {
             half8_t v;
             pa_h2 h[4];
@@ -1007,10 +1010,11 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
                 const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[kb >> 1][j], kf, shift));
                 const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[kb >> 1][j + 1], kf, shift));
                 Probs(&f)[PARTS] = pf[kb & 1];
-                f[0].h[i] = pa_h2{(_Float16)p0, (_Float16)p1};
+                f[0].h[i] = __builtin_convertvector(pa_f2{p0, p1}, pa_h2);
                 l_run = __builtin_amdgcn_fdot2(f[0].h[i], ones, l_run, false);
                 if constexpr (PARTS == 2) {
-                    f[1].h[i] = pa_h2{(_Float16)(p0 - (float)f[0].h[i][0]), (_Float16)(p1 - (float)f[0].h[i][1])};
+                    const pa_h2 h = f[0].h[i];
+                    f[1].h[i] = __builtin_convertvector(pa_f2{fmaf((float)h[0], minus, p0), fmaf((float)h[1], minus, p1)}, pa_h2);
                     l_run = __builtin_amdgcn_fdot2(f[1].h[i], ones, l_run, false);
                 }
             }
