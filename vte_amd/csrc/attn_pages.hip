@@ -1041,7 +1041,7 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
 #pragma unroll
                 for (int i = 0; i < DT * PARTS; ++i) {
                     __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                    __builtin_amdgcn_sched_group_barrier(0x402, PARTS == 1 ? 24 / DT + 1 : 52 / (2 * DT) + 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x402, PARTS == 1 ? 24 / DT + 1 : 40 / (2 * DT) + 1, 0);
                 }
             }
         }
