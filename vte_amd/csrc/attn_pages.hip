@@ -90,9 +90,8 @@ __device__ __forceinline__ float pa_pow2(int d) { return d < -126 ? 0.f : __uint
 // two records a block are enough.
 //
 // Bound by the cache's bytes where contexts are long: eight documents of 16384 to
-// 65536 tokens, 168 MB, 41 us in all, 4.1 TB/s (a sum over as many bytes reads 4.0,
-// a copy moves 5.0); by latencies where they are short: 2049 tokens 12.2 us, two
-// launches, in the first four loads one after the other (positions, page, bytes, q) and a
+// 65536 tokens, 168 MB, 36 us in all, 4.7 TB/s (a copy moves 5.0); by latencies where
+// they are short: 2049 tokens 11.7 us, two launches, in the first four loads one after the other (positions, page, bytes, q) and a
 // tile's work.  Bytes go from memory to registers, where a lane's 16 are its operand
 // once permuted: no LDS, each is used once, and a wave has the next tile's under way
 // (two blocks of 256 threads a CU is all that those registers leave).
@@ -551,14 +550,14 @@ __global__ __launch_bounds__(256) void attn_pages_combine_kernel(KvPages c, KvRo
 // swapped so that a lane's scores are its operand of the second product as they
 // stand.
 //
-// Bound by issue: a group's step is 32 products a wave (1000 cycles) beside as many
-// cycles of turning bytes and some 800 of softmax, which overlap in part: 2.4 us for
-// two groups' steps.  The runs below fix what stands between two products (left to
+// Bound by issue: a group's step is 32 products a wave (1000 cycles) beside some 500
+// cycles of turning bytes and 900 of softmax, with two waves a SIMD, which overlap in
+// part: 2.4 us for two groups' steps.  The runs below fix what stands between two products (left to
 // itself the compiler read an operand right before each).  Beside that a block starts
-// (4 us: sequence, page, bytes, the first tile) and ends (3 us), which weighs on short
-// ones: four sequences of 2048 new tokens, 32 query and 8 KV heads of 128, 202 us, 680
+// (3 us: sequence, page, bytes, the first tile) and ends (2 us), which weighs on short
+// ones: four sequences of 2048 new tokens, 32 query and 8 KV heads of 128, 195 us, 700
 // TFLOP/s (a large fp16 matrix product: 1100 to 1200); a chunk of 512 after 1536 tokens,
-// in shares of 8 steps, 24 us, 231.
+// in shares of 8 steps, 22 us, 254.
 // ---------------------------------------------------------------------------
 #define PA_SHARES 64
 #define PA_APART 24 // scales of blocks that are staged together, log2
@@ -1211,10 +1210,10 @@ static PaPlan rows_plan(const KvPages& c, const KvRows& r, int hd, int G, void* 
 // The many-rows form: rows of a block, row blocks at most (each sequence may end one early), and shares of each, as many
 // as fill the CUs.
 // Rows of a block: 256 (one group) from 7/4 blocks a CU on, else 128 (two groups).  256 / 128, us, 2048 new tokens a
-// sequence: 1.5 blocks a CU 107.9 / 103.3, 1.75 140 / 156, 2 100.8 / 119.1, 4 202 / 233.
+// sequence: 1.5 blocks a CU 106 / 99, 1.75 134 / 147, 2 97 / 115, 2.25 147 / 143, 4 195 / 222.
 // Shares: of four steps at least, or of two while there are no more than 16; no more than 64.  Three new tokens, 16 query
-// heads, 16 / 32 / 64 / 128 shares, us: after 8192 tokens 22.4 / 20.6 / 23.1 / 23.0, after 32768 51 / 35 / 30 / 35; after
-// 2048 8 / 16 shares 16.5 / 15.6.
+// heads, 16 / 32 / 64 / 128 shares, us: after 8192 tokens 21.3 / 19.4 / 21.9 / 21.8, after 32768 49 / 33 / 29 / 34; after
+// 2048 8 / 16 shares 15.2 / 14.1.
 struct PromptForm {
     int groups;
     long long rbs;
@@ -1241,8 +1240,8 @@ static PromptForm prompt_form(const KvPages& c, const KvRows& r, int hd, int G, 
     f.bytes = n;
     return f;
 }
-// One tile's columns hold them all.  (Few-rows / many-rows form, us: one sequence of 2049 tokens 12.2 / 16.4, 16 ragged ones
-// of up to 8192 18.3 / 32.5, eight of up to 65536 41.2 / 90.5.)
+// One tile's columns hold them all.  (Few-rows / many-rows form, us: one sequence of 2049 tokens 11.7 / 15.4, 16 ragged ones
+// of up to 8192 17.7 / 29.7, eight of up to 65536 36.0 / 88.3.)
 static bool rows_form(const KvRows& r, int G) { return r.max_rows * G <= 16; }
 
 long long attn_pages_scratch_bytes(const KvPages& c, const KvRows& r, int hd, int n_q) {

@@ -23,7 +23,7 @@
 // a launch and four loads in a row (position, page, old exponent and bytes), 3.7 us
 // for one token.  Prompts: bytes, 41 MB of four chunks of 700 to 2048 tokens with
 // their q in 10.7 us, 3.9 TB/s (a large copy reaches 5.0).  With the read-back of the
-// chunks, us: 14.8 WIDE, 44.1 otherwise; one token each of 64 sequences 13.6 / 15.3.
+// chunks, us: 14.7 WIDE, 44.0 otherwise; one token each of 64 sequences 12.6 / 13.9.
 // ---------------------------------------------------------------------------
 struct KvRope {
     const __half *cosc, *sinc;
@@ -342,8 +342,9 @@ __global__ __launch_bounds__(WIDE ? 2 * HD : 128) void kv_pages_append_kernel(Kv
 // HD threads turn one block of one head of K (16 dims of a token each), HD threads
 // the same of V (4 dims of 4 tokens each, whose bytes change places by permutes: a
 // row's stores are then 8 or 16 bytes, as K's; with single values they took twice as
-// long, 48 us for what now takes 23).  Bound by bytes: 102 MB of a ragged batch of 16
-// sequences of up to 8192 tokens, 23 us, 4.4 TB/s (a copy: 5.0).
+// long) and pass the caches by, which 68 MB of rows would fill for nobody: 102 MB read
+// and written for a ragged batch of 16 sequences of up to 8192 tokens in 21.5 us, 4.8
+// TB/s, against 28 (a copy: 5.0).  Loads that pass them by took 32: V's are 4 bytes each.
 // ---------------------------------------------------------------------------
 template <typename T, int N>
 __device__ __forceinline__ void kvp_put(T* dst, const uint32_t (&w)[N], float f) {  // 4 N bytes as values

@@ -24,10 +24,11 @@
 //
 // Bound by the two readings where there are many rows: 256 rows of 151936, 156 MB,
 // bins 41 us (3.8 TB/s; some 25 vector operations and an LDS addition an entry take
-// nearly as long), draw 60 us, of which reading 36 (a broad distribution's ends lie in
+// nearly as long), draw 60, of which reading 36 (a broad distribution's ends lie in
 // bins that nearly all subsets reach into; of a peaked one it reads a few).  Few rows:
-// by latencies, one row 8 + 14 us: merging 4, scans and ends of the filters 7.
-// With unaligned rows (not WIDE) / WIDE, us: one row 24.0 / 22.5, 256 107.2 / 100.6.
+// by latencies, one row 8.5 + 12.5 us: merging 2, scans 2, bins in question 1, their
+// entries 3, the last of the row's blocks 2, ends of the filters 2.
+// With unaligned rows (not WIDE) / WIDE, us: one row 22.1 / 20.7, 256 105.7 / 98.5.
 #include <algorithm>
 #include "vte_common.h"
 
@@ -44,7 +45,7 @@
 #define SMP_SMALL 1024      // entries of a bin that are ordered by counting
 #define SMP_FEW 128         // .. without a split first
 #define SMP_AHEAD 4         // subsets a wave of the draw has in flight (8: one row 16.1 -> 18.6 us, 256 rows the same)
-#define SMP_SPLIT 8         // blocks of a row at most (2: one row 30.6 us, 16 rows 37.8; 8: 22.5, 30.9; 16 as 8)
+#define SMP_SPLIT 8         // blocks of a row at most (2 / 8, us: one row 30.6 / 22.5, 16 rows 37.8 / 30.9; 16 as 8)
 
 // Scratch of a row.
 struct SmpScratch {
