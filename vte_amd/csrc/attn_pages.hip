@@ -489,7 +489,10 @@ __global__ __launch_bounds__(256) void attn_pages_combine_kernel(KvPages c, KvRo
         EV = max(EV, pl.ev[rec * pl.ncol + cc]);
     }
     M = wave_max(M);
-    for (int x = 1; x < 64; x *= 2) EV = max(EV, __shfl_xor(EV, x, 64));
+    EV = max(EV, __builtin_amdgcn_update_dpp(EV, EV, 0xB1, 0xF, 0xF, false));
+    EV = max(EV, __builtin_amdgcn_update_dpp(EV, EV, 0x4E, 0xF, 0xF, false));
+    EV = max(EV, __builtin_amdgcn_update_dpp(EV, EV, 0x141, 0xF, 0xF, false));
+    EV = pa_max4(max(EV, __builtin_amdgcn_update_dpp(EV, EV, 0x140, 0xF, 0xF, false)));
     if (lane == 0) {
         red[0][wv] = M;
         red_ev[wv] = EV;
