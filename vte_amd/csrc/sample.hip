@@ -851,7 +851,7 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_draw_kernel(const float* _
         if (wv == 0) {
             const int token = smp_end_wave(S, r, lane, kb, k, has_p, p, p0, p1, has_m, m0, m1, floor_w, z_lo, z_hi, k_lo, k_hi,
                                            u0, u1, drawn);
-            if (lane == 0) tokens[row] = token;
+            if (lane == 0) tokens[row] = min(token, vocab - 1);
         }
         return;
     }
@@ -884,7 +884,7 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_draw_kernel(const float* _
     int b = u0, same;
     if (u0 != u1) smp_find(S, mine, t, t, b, same);
     const uint64_t place = smp_end<false>(S, r, b, (t - smp_before(S, b)) / smp_middle(b), upto);
-    if (tid == 0) tokens[row] = smp_index(place);
+    if (tid == 0) tokens[row] = min(smp_index(place), vocab - 1);
 }
 
 namespace vte {
