@@ -58,6 +58,24 @@ def test_spreads(hip, K, sigma, top_k, top_p):
     check(hip, K, x, 1.0, top_k, top_p, 0.0, [0.0, 0.25, 0.5, 0.9, 1 - 2.0 ** -53])
 
 
+@pytest.mark.parametrize("n", [1, 2, 63, 64, 65, 128, 129, 512, 513, 1024, 1025, 8191, 8193, 20000])
+@pytest.mark.parametrize("spread", [0.0, 0.02, 0.3])
+def test_entries_in_question(hip, K, n, spread):
+    """The filters and the draw end among n entries of one bin or a few, the rest of the row far below."""
+    rng = np.random.default_rng(n)
+    x = (-25 - rng.random((6, 40000))).astype(np.float32)
+    for row in x:
+        row[rng.permutation(40000)[:n]] = 3 + spread * rng.random(n)
+    check(hip, K, x, top_k=np.array([0, n // 2 + 1, n, 0, 0, n // 3 + 1]), top_p=np.array([0.5, 1.0, 0.9, 0.3, 1.0, 0.7]),
+          min_p=np.array([0, 0, 0, 0.9, 0.8, 0.995]), u=rng.random(6))
+
+
+def test_more_rows_than_compute_units(hip, K):
+    rng = np.random.default_rng(22)
+    check(hip, K, (2 * rng.standard_normal((700, 301))).astype(np.float32), rng.choice([0.0, 0.5, 1.0, 2.0], 700),
+          rng.choice([0, 5, 100], 700), rng.choice([0.5, 0.95, 1.0], 700), rng.choice([0.0, 0.05], 700), rng.random(700))
+
+
 def test_ties_go_to_the_lowest_index(hip, K):
     """Levels of equal logits: the order inside a level is the index's, at top-k and top-p borders too."""
     rng = np.random.default_rng(3)
