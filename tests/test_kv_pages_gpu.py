@@ -172,6 +172,38 @@ def test_append_ragged_prompts(hip, K, page, hd, dtype):
                     assert np.array_equal(now[sl], old[sl]), (n, p, i)
 
 
+@pytest.mark.parametrize("batch", [70, 300])
+def test_append_to_many_sequences(hip, K, batch):
+    """A few rows of each of many sequences, some of none, with rows of nobody before the first one's."""
+    rng = np.random.default_rng(batch)
+    new = [int(n) for n in rng.integers(0, 4, batch)]
+    pos = [int(p) if b % 7 else -1 for b, p in enumerate(rng.integers(0, 40, batch))]
+    lens = [max(p, 0) + n for p, n in zip(pos, new)]
+    bt = Batch(hip, K, rng, lens, 1, 64, 16, width=3)
+    for b, p in enumerate(pos):
+        if p > 0:
+            append_ref(bt, b, 0, *[normal(rng, (p, 1, 64), "f16", 0.3) for _ in "kv"])
+    bt.upload()
+    r = bt.rows(pos, new, pad=2)
+    start = (2 + np.concatenate([[0], np.cumsum(new)])).astype(np.int32)
+    bt.d["start"] = up(hip, start)
+    r.row_start = bt.d["start"].ptr
+    R = int(start[-1])
+    q, k, v = normal(rng, (R, 2, 64), "f16"), normal(rng, (R, 1, 64), "f16"), normal(rng, (R, 1, 64), "f16")
+    cos, sin = build_rope_cache(64, 64, 1e4)
+    out = np.full(q.shape, 9, np.float16)
+    do = up(hip, out)
+    K.kv_pages_append(bt.pages, r, up(hip, k), up(hip, v), q=up(hip, q), q_out=do, n_q=2, rope_cos=up(hip, cos),
+                      rope_sin=up(hip, sin), rope_rows=64, stream=hip.stream)
+    for b, n in enumerate(new):
+        if pos[b] >= 0 and n:
+            at, rows = pos[b] + np.arange(n), slice(start[b], start[b + 1])
+            append_ref(bt, b, pos[b], okv.rotate(k[rows], at, cos, sin), v[rows].astype(np.float32))
+            out[rows] = okv.rotate(q[rows], at, cos, sin).astype(np.float16)
+    assert np.array_equal(down(do), out)
+    bt.check([n if p >= 0 else 0 for n, p in zip(lens, pos)])
+
+
 def test_append_not_finite(hip, K):
     """A block that receives an Inf or a NaN reads as NaN, and later ones of other heads and blocks do not."""
     rng = np.random.default_rng(5)
