@@ -427,9 +427,8 @@ long long vte_attn_pages_scratch_bytes(const vte_kv_pages* cache, const vte_kv_r
  * [rows][n_q][head_dim] (dtype fp16 or fp32; out may be q), n_q / n_kv <= 16,
  * rows * n_q <= 2^25, batch * n_kv <= 2^20.  A row that sees
  * nothing (a sequence that does not run, no pages) gives 0; rows that belong to
- * nobody are left as they were.  Sums and softmax statistics are fp32; with fp16
- * the probabilities enter the products as fp16, with fp32 q and the probabilities
- * enter as two fp16 parts each.  scratch: 16-byte aligned, need not be cleared;
+ * nobody are left as they were.  Sums and softmax statistics are fp32; the
+ * probabilities, and fp32 q, enter the products as two fp16 parts each.  scratch: 16-byte aligned, need not be cleared;
  * calls that may overlap (two streams, two graphs) need one each.  Capturable.
  * Replaces: SplitKVAttentionDispatcher launches (vte/core/split_kv_attention.py:187-217)
  *           for a cache in this form. */

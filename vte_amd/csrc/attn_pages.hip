@@ -18,6 +18,8 @@
 
 #define PA_TILE 64       // tokens of a wave's step: a lane group of 16 holds one block of 16
 #define PA_P_LOG2 14     // probabilities are held as 2^14 p
+#define PA_P_PARTS 2     // fp16 parts of a probability, a rounded one and a rounded rest: with one, fp16 results were off by up
+                         // to 2.8e-4 of them, with two by the 2.1e-4 of their own rounding
 #define PA_NONE (-3e38f) // running maximum before anything is seen
 
 typedef _Float16 pa_h2 __attribute__((ext_vector_type(2)));
@@ -235,7 +237,7 @@ template <typename T, int HD>
 __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(KvPages c, KvRows r, PaPlan pl,
                                                                  const T* q, T* out, int n_q,
                                                                  float scale) {
-    constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;  // fp16 parts of q and of the probabilities
+    constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;  // fp16 parts of q
     constexpr int KC = HD / 64;                    // 16-byte pieces of a K row that a lane holds
     constexpr int DT = HD / 16;
     __shared__ float m_sh[4][16], l_sh[4][16];
@@ -374,7 +376,7 @@ __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(KvPages c, KvRo
             }
             // (a NaN block's tokens are NaN to the columns that see them and nothing to the others)
             const float vf = x.ev == KVP_E_NAN ? NAN : pa_pow2(min(x.ev - evm, 0)) * (float)(1 << PA_P_LOG2);
-            half8_t pa[PARTS][2];
+            half8_t pa[PA_P_PARTS][2];
 #pragma unroll
             for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
@@ -384,13 +386,13 @@ __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(KvPages c, KvRo
                     const float w = 4 * tt + i < live ? p * vf : 0.f;
                     const int u = tt >> 1, j = 4 * (tt & 1) + i;
                     pa[0][u][j] = (_Float16)w;
-                    if constexpr (PARTS == 2) pa[1][u][j] = (_Float16)(w - (float)pa[0][u][j]);
+                    pa[1][u][j] = (_Float16)(w - (float)pa[0][u][j]);
                 }
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
                 const half8_t v0 = pa_half8(x.v[dt].x, x.v[dt].y), v1 = pa_half8(x.v[dt].z, x.v[dt].w);
 #pragma unroll
-                for (int p = 0; p < PARTS; ++p) {
+                for (int p = 0; p < PA_P_PARTS; ++p) {
                     o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pa[p][0], o[dt], 0, 0, 0);
                     o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pa[p][1], o[dt], 0, 0, 0);
                 }
@@ -718,7 +720,7 @@ template <typename T, int HD, int GROUPS>
 __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, KvRows r, PaPrompt pp,
                                                                    const T* q, T* out,
                                                                    int n_q, float scale) {
-    constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;
+    constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;  // fp16 parts of q
     constexpr int WAVES = 8 / GROUPS, ROWS = 32 * WAVES;  // of a group
     constexpr int KS = HD / 16, DT = HD / 32;              // 16-dim steps of a score, 32-dim tiles
     constexpr int NP = 8 * HD / (64 * WAVES);              // 16-byte pieces of K and V a thread stages (1: waves 0..3 K, 4..7 V)
@@ -1003,7 +1005,7 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
         union Probs {
             half8_t v;
             pa_h2 h[4];
-        } pf[2][PARTS];
+        } pf[2][PA_P_PARTS];
         half8_t vb[2][DT];
         auto probs = [&](int kb) {
 #pragma unroll
@@ -1011,14 +1013,12 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
                 const int j = 8 * (kb & 1) + 2 * i;
                 const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[kb >> 1][j], kf, shift));
                 const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[kb >> 1][j + 1], kf, shift));
-                Probs(&f)[PARTS] = pf[kb & 1];
+                Probs(&f)[PA_P_PARTS] = pf[kb & 1];
                 f[0].h[i] = __builtin_convertvector(pa_f2{p0, p1}, pa_h2);
                 l_run = __builtin_amdgcn_fdot2(f[0].h[i], ones, l_run, false);
-                if constexpr (PARTS == 2) {
-                    const pa_h2 h = f[0].h[i];
-                    f[1].h[i] = __builtin_convertvector(pa_f2{fmaf((float)h[0], minus, p0), fmaf((float)h[1], minus, p1)}, pa_h2);
-                    l_run = __builtin_amdgcn_fdot2(f[1].h[i], ones, l_run, false);
-                }
+                const pa_h2 h = f[0].h[i];
+                f[1].h[i] = __builtin_convertvector(pa_f2{fmaf((float)h[0], minus, p0), fmaf((float)h[1], minus, p1)}, pa_h2);
+                l_run = __builtin_amdgcn_fdot2(f[1].h[i], ones, l_run, false);
             }
         };
         auto read_v = [&](int kb) {
@@ -1035,15 +1035,15 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-                for (int p = 0; p < PARTS; ++p)
+                for (int p = 0; p < PA_P_PARTS; ++p)
                     o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vb[kb & 1][dt], pf[kb & 1][p].v, o[dt], 0, 0, 0);
             if (kb < 3) {
                 probs(kb + 1);
                 __builtin_amdgcn_sched_group_barrier(0x100, DT, 0);
 #pragma unroll
-                for (int i = 0; i < DT * PARTS; ++i) {
+                for (int i = 0; i < DT * PA_P_PARTS; ++i) {
                     __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                    __builtin_amdgcn_sched_group_barrier(0x402, PARTS == 1 ? 24 / DT + 1 : 40 / (2 * DT) + 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x402, 40 / (DT * PA_P_PARTS) + 1, 0);
                 }
             }
         }
