@@ -435,7 +435,8 @@ long long vte_attn_pages_scratch_bytes(const vte_kv_pages* cache, const vte_kv_r
 int vte_attn_pages(const vte_kv_pages* cache, const vte_kv_rows* rows, int dtype, const void* q, void* out, int n_q,
                    float scale, void* scratch, long long scratch_bytes, void* stream);
 
-/* Scratch bytes of vte_sample for `rows` rows. */
+/* Scratch bytes of vte_sample for calls of at most `rows` rows (never less for
+ * more rows: memory sized for the largest batch serves the smaller ones). */
 long long vte_sample_scratch_bytes(int rows);
 
 /* The next token of every row of fp32 logits [rows][vocab] (vocab <= 262144).

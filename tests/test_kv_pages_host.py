@@ -168,3 +168,17 @@ def test_sampling_oracle_closed_form(u, token):
     assert osm.sample(x, u=u)[0] == token
     assert osm.sample(x, top_k=1, u=u)[0] == 1 and osm.sample(x, temperature=0, u=u)[0] == 1
     assert osm.sample(x, min_p=0.4, u=u)[0] in (0, 1) and osm.sample(x, top_p=0.4, u=u)[0] == 1
+
+
+def test_sample_scratch_of_more_rows_serves_fewer():
+    """Memory sized for the largest batch is enough as sequences end: the size never falls with the rows, at the borders
+    of 8 parts a row and fewer (32, 36, 42, 51, 64, 85 and 128 rows on 256 compute units) and elsewhere."""
+    K = kernels()
+    size = [K.sample_scratch_bytes(r) for r in range(1, 3000)] + [K.sample_scratch_bytes(65535)]
+    assert size[0] > 0 and all(a <= b for a, b in zip(size, size[1:]))
+
+
+def test_sample_scratch_of_fewer_bytes_is_refused():
+    K = kernels()
+    with pytest.raises(HIPSafetyError, match="scratch"):
+        K.sample(P, 33, 100, P, P, u=P, scratch_bytes=K.sample_scratch_bytes(33) - 1)

@@ -152,6 +152,24 @@ def test_long_parts_of_many_rows(hip, K, vocab):
           rng.choice([0.0, 0.0, 0.05], 172), rng.random(172))
 
 
+@pytest.mark.parametrize("most,rows", [(33, 32), (52, 51), (129, 128), (86, 85), (256, 1)])
+def test_scratch_of_a_larger_batch(hip, K, most, rows):
+    """Draws of fewer rows in memory sized for more: what lies behind it stays as it was.  (The rows' scratch is what the
+    largest vocabulary takes; guards are 2 MiB.)"""
+    rng = np.random.default_rng(most)
+    V, need, guard = 262144, K.sample_scratch_bytes(most), 2 << 20
+    scratch = up(hip, np.full(need + guard, 0xA5, np.uint8))
+    x = (2 * rng.standard_normal((rows, V))).astype(np.float32)
+    tok, u = empty(hip, rows, np.int32), rng.random(rows)
+    K.sample(up(hip, x), rows, V, tok, scratch, top_k=up(hip, np.full(rows, 40, np.int32)), u=up(hip, u), stream=hip.stream,
+             scratch_bytes=need)
+    got = down(tok)
+    assert (down(scratch)[need:] == 0xA5).all()
+    for r in range(0, rows, 9):
+        want, near = osm.sample(x[r], 1.0, 40, u=u[r])
+        assert got[r] == want or near < V * 2.0 ** -44
+
+
 # ---------------------------------------------------------------------------- in the decode step
 @pytest.fixture(scope="module")
 def tiny():

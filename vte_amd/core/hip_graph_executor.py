@@ -697,7 +697,8 @@ class HIPGraphExecutor:
         try:
             self.enqueue_step()
             K.sample(self.logits, B, self.cfg.vocab, sm["tokens"], sm["scratch"], temperature=sm["temperature"],
-                     top_k=sm["top_k"], top_p=sm["top_p"], min_p=sm["min_p"], u=sm["u"], stream=self.hip.stream)
+                     top_k=sm["top_k"], top_p=sm["top_p"], min_p=sm["min_p"], u=sm["u"], stream=self.hip.stream,
+                     scratch_bytes=sm["scratch"].nbytes)
             K.greedy_advance(sm["tokens"], 1, B, self.staging_input, self.staging_kv_offset, self.max_seq - 1,
                              sm["history"], cap, sm["step"], stream=self.hip.stream)
         finally:

@@ -895,8 +895,15 @@ static int sample_blocks(int rows) { return std::max(1, std::min(SMP_SPLIT, devi
 // row, of which little is read, 21.8 / 22.5.
 static int draw_blocks(int rows) { return std::max(1, std::min(16, device_cus() / rows)); }
 
+// What a call of any number of rows up to `rows` takes: fewer rows have more parts, so each number of parts at the most rows
+// that have it (33 rows of 7 parts are less than 32 of 8).
 long long sample_scratch_bytes(int rows) {
-    return (long long)rows * (long long)smp_row_bytes(sample_blocks(rows), (1 << SMP_IDX_BITS) / SMP_SUB);
+    long long most = 0;
+    for (int b = 1; b <= SMP_SPLIT; ++b) {
+        const int r = std::max(1, std::min(rows, device_cus() / b));
+        most = std::max(most, (long long)r * (long long)smp_row_bytes(sample_blocks(r), (1 << SMP_IDX_BITS) / SMP_SUB));
+    }
+    return std::max(most, (long long)rows * (long long)smp_row_bytes(sample_blocks(rows), (1 << SMP_IDX_BITS) / SMP_SUB));
 }
 hipError_t sample(const float* logits, int rows, int vocab, const float* temperature, const int* top_k,
                   const float* top_p, const float* min_p, const double* u, int* tokens, void* scratch,

@@ -338,11 +338,15 @@ class VTEKernels:
                                             scale, _p(scratch), scratch_bytes, self._st(stream)), "vte_attn_pages")
 
     def sample_scratch_bytes(self, rows: int) -> int:
+        """For calls of at most ``rows`` rows."""
         return int(self.lib.vte_sample_scratch_bytes(rows))
 
     def sample(self, logits, rows: int, vocab: int, tokens, scratch, temperature=None, top_k=None, top_p=None,
-               min_p=None, u=None, stream=None) -> None:
-        """tokens[r] drawn from row r of fp32 logits under the rows' settings and uniforms ``u`` (device arrays)."""
+               min_p=None, u=None, stream=None, scratch_bytes=None) -> None:
+        """tokens[r] drawn from row r of fp32 logits under the rows' settings and uniforms ``u`` (device arrays).
+        ``scratch_bytes``: the size of ``scratch``, checked where it is given."""
+        if scratch_bytes is not None and scratch_bytes < self.sample_scratch_bytes(rows):
+            raise HIPSafetyError(f"sample: scratch of {scratch_bytes} bytes, {self.sample_scratch_bytes(rows)} needed")
         self._check(self.lib.vte_sample(_p(logits), rows, vocab, _p(temperature), _p(top_k), _p(top_p), _p(min_p),
                                         _p(u), _p(tokens), _p(scratch), self._st(stream)), "vte_sample")
 
