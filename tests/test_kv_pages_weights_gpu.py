@@ -7,7 +7,7 @@ import pytest
 
 from oracle import kv_pages as okv
 from tests._dev import down, empty, up
-from tests.test_kv_pages_gpu import NP, Batch, filled, normal
+from tests.test_kv_pages_gpu import NP, Batch, append_ref, filled, normal
 
 pytestmark = pytest.mark.gpu
 
@@ -76,6 +76,28 @@ def test_fp16_results_are_off_by_their_own_rounding(hip, K, new, n_q, n_kv, hd):
         # sums: 16 tokens an instruction, two parts of each, 32 for exponentials and rescaling
         check(hip, K, bt, b, pos, [new, new], n_q, "f16", q, chain=2 * 700 // 16 + 32,
               small=2.0 ** -38 if new * n_q // n_kv <= 16 else 2.0 ** -33)
+
+
+def sized(hip, K, rng, n, n_kv, hd, v_size, batch=1, **kw):
+    """Sequence 0 of n tokens whose V are v_size [n] times normal ones (``batch`` - 1 empty ones behind it)."""
+    bt = Batch(hip, K, rng, [n] + [0] * (batch - 1), n_kv, hd, 64, **kw)
+    k, v = rng.standard_normal((2, n, n_kv, hd)).astype(np.float32)
+    append_ref(bt, 0, 0, k, v * np.asarray(v_size, np.float32)[:, None, None])
+    bt.upload()
+    return bt
+
+
+@pytest.mark.parametrize("new,n_q,n_kv,hd,batch", [(128, 1, 1, 128, 1), (70, 2, 1, 64, 1), (600, 16, 1, 128, 1),
+                                                   (130, 16, 4, 64, 140), (4, 4, 1, 128, 1)])
+@pytest.mark.parametrize("at", [448, 704, 720])
+def test_values_of_2_to_130_times_behind_a_row(hip, K, new, n_q, n_kv, hd, batch, at):
+    """V of tokens that a row does not see are 2^130 times those that it sees, from a border of a step on and inside one:
+    groups and shares of which a row sees nothing leave its result alone."""
+    rng = np.random.default_rng(new + at)
+    n = min(800, at + new // 2)
+    bt = sized(hip, K, rng, n, n_kv, hd, np.where(np.arange(n) < at, 2.0 ** -10, 2.0 ** 120), batch)
+    q = normal(rng, (new, n_q, hd), "f32")
+    check(hip, K, bt, 0, [n - new] + [-1] * (batch - 1), [new] + [0] * (batch - 1), n_q, "f32", q, before=at)
 
 
 def test_equal_bits_in_other_pages(hip, K):

@@ -78,6 +78,13 @@ __device__ __forceinline__ float pa_sum4(float v) {
     a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float(a[0]) + __uint_as_float(a[1]);
 }
+// Sums O = sum 2^(s_t - m) 2^(ev_t - e) V_t of two or more parts of a row's tokens, each relative to its own maximum m and
+// exponent e, are joined by what they contribute: with M the largest m, relative to E, the smallest whole number from every
+// (m - M) + e on, so the factor 2^((m - M) + (e - E)) is 1 at most and what vanishes is below 2^-126 of the heaviest part.  (By
+// the largest e alone a part of great V and no weight, or of no token that the row sees, took the others' sums with it.)
+#define PA_E_NONE (-300) // e of a part of no tokens, below all others
+__device__ __forceinline__ float pa_weight(float m, int e, float M) { return ceilf((m - M) + (float)e); }  // its lower bound for E
+__device__ __forceinline__ float pa_joined(float m, int e, float M, int E) { return __builtin_amdgcn_exp2f((m - M) + (float)(e - E)); }
 // 2^d for d <= 0 (0 below the smallest normal).
 __device__ __forceinline__ float pa_pow2(int d) { return d < -126 ? 0.f : __uint_as_float((uint32_t)(d + 127) << 23); }
 
@@ -615,7 +622,7 @@ __device__ __forceinline__ int pa_share_of(int steps, int nsp) {
 struct PaPrompt {
     int nsp;    // shares of a row block
     float* ml;  // [row blocks][n_kv][nsp][128][2]: maximum (log2), sum
-    int* ev;    // [row blocks][n_kv][nsp][128]: exponent that the row's sums are relative to
+    int* ev;    // [row blocks][n_kv][nsp][128]: exponent that the row's sums are relative to (PA_E_NONE: it sees nothing)
     float* o;   // [row blocks][n_kv][nsp][HD / 8][32-row tile][4 dims of 8][row][4]
 };
 
@@ -1072,6 +1079,7 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
         const pa_u2 w = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_run), __float_as_uint(l_run), false, false);
         l_run = __uint_as_float(w[0]) + __uint_as_float(w[1]);
     }
+    if (l_run == 0.f) ev_row = PA_E_NONE;  // (o_ref is of all tokens of its steps, whether the row sees one or not)
     if constexpr (GROUPS == 1) {
         if (r0 + row < rows) pa_store<T, DT>(dst + 4 * half, o, l_run, ev_row);
     } else {  // each group leaves half of the dims to the other
@@ -1090,10 +1098,11 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
         }
         __syncthreads();
         const float m2 = m_sh[grp ^ 1][wv * 32 + row], M = fmaxf(m_run, m2);
-        const int e2 = ev_sh[grp ^ 1][wv * 32 + row], EV = max(ev_row, e2);
+        const int e2 = ev_sh[grp ^ 1][wv * 32 + row];
+        const int EV = (int)fmaxf(fmaxf(pa_weight(m_run, ev_row, M), pa_weight(m2, e2, M)), (float)PA_E_NONE);
         const float f1 = __builtin_amdgcn_exp2f(m_run - M), f2 = __builtin_amdgcn_exp2f(m2 - M);
         const float L = l_run * f1 + l_sh[grp ^ 1][wv * 32 + row] * f2;
-        const float g1 = f1 * pa_pow2(ev_row - EV), g2 = f2 * pa_pow2(e2 - EV);
+        const float g1 = pa_joined(m_run, ev_row, M, EV), g2 = pa_joined(m2, e2, M, EV);
 #pragma unroll
         for (int i = 0; i < DT / 2; ++i)
 #pragma unroll
@@ -1136,7 +1145,7 @@ __global__ __launch_bounds__(256) void attn_pages_prompt_combine_kernel(KvPages 
     const int pieces = (steps + share - 1) / share;
     const size_t rec0 = ((size_t)slot * c.n_kv + h) * pp.nsp;
     float M = PA_NONE, L = 0.f;
-    int EV = KVP_E_MIN;
+    int EV = PA_E_NONE;
     floatx4_t O = {0.f, 0.f, 0.f, 0.f};
     constexpr int AT_ONCE = 8;
     for (int i0 = 0; i0 < pieces; i0 += AT_ONCE) {  // requested together (past the last one: the last again)
@@ -1151,22 +1160,20 @@ __global__ __launch_bounds__(256) void attn_pages_prompt_combine_kernel(KvPages 
             ev[i] = pp.ev[rec];
         }
         float m = M;
-        int x = EV;
 #pragma unroll
-        for (int i = 0; i < AT_ONCE; ++i) {
-            m = fmaxf(m, ml[i].x);
-            x = max(x, ev[i]);
-        }
-        const float old = __builtin_amdgcn_exp2f(M - m);
-        L *= old;
-        O *= old * pa_pow2(EV - x);
+        for (int i = 0; i < AT_ONCE; ++i) m = fmaxf(m, ml[i].x);
+        float x = fmaxf(pa_weight(M, EV, m), (float)PA_E_NONE);
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) x = fmaxf(x, pa_weight(ml[i].x, ev[i], m));
+        L *= __builtin_amdgcn_exp2f(M - m);
+        O *= pa_joined(M, EV, m, (int)x);
         M = m;
-        EV = x;
+        EV = (int)x;
 #pragma unroll
         for (int i = 0; i < AT_ONCE; ++i) {
-            const float f = i0 + i < pieces ? __builtin_amdgcn_exp2f(ml[i].x - M) : 0.f;
-            L = fmaf(ml[i].y, f, L);
-            O += o[i] * (f * pa_pow2(ev[i] - EV));
+            const bool in = i0 + i < pieces;
+            L = fmaf(ml[i].y, in ? __builtin_amdgcn_exp2f(ml[i].x - M) : 0.f, L);
+            O += o[i] * (in ? pa_joined(ml[i].x, ev[i], M, EV) : 0.f);
         }
     }
     floatx4_t x;
