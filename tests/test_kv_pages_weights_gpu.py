@@ -100,6 +100,42 @@ def test_values_of_2_to_130_times_behind_a_row(hip, K, new, n_q, n_kv, hd, batch
     check(hip, K, bt, 0, [n - new] + [-1] * (batch - 1), [new] + [0] * (batch - 1), n_q, "f32", q, before=at)
 
 
+@pytest.mark.parametrize("n_kv,batch", [(4, 140), (1, 1)])
+def test_values_that_grow_twice_behind_a_row(hip, K, n_kv, batch):
+    """V grow by 2^80 and, a step later, by 2^80 again, each less than fp32 holds, together more: rows before the first
+    growth, and those between the two.  (Of 140 sequences the row blocks are 256 rows, which span both.)"""
+    rng = np.random.default_rng(n_kv)
+    n, new = 900, 300
+    bt = sized(hip, K, rng, n, n_kv, 64, 2.0 ** np.repeat([-80.0, 0.0, 80.0], [704, 64, 132]), batch)
+    q = normal(rng, (new, n_kv, 64), "f32")
+    pos, rows = [n - new] + [-1] * (batch - 1), [new] + [0] * (batch - 1)
+    check(hip, K, bt, 0, pos, rows, n_kv, "f32", q, before=704)
+    check(hip, K, bt, 0, pos, rows, n_kv, "f32", q, before=768)
+
+
+@pytest.mark.parametrize("new,n_q", [(70, 2), (150, 16)])
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("at", [0, 64, 96, 128])
+def test_a_huge_value_of_vanishing_weight(hip, K, dtype, new, n_q, at):
+    """A block's V is 2^power times the others', its tokens' probability 2^-drop of theirs: what the others contribute
+    stays, whichever is heavier, wherever the block lies."""
+    hd, n = 128, 300
+    for power, drop in ((40, 100), (120, 160), (60, 60), (20, 26), (20, 33), (14, 30), (30, 45), (12, 40), (110, 100)):
+        rng = np.random.default_rng(power + drop)
+        bt = Batch(hip, K, rng, [n], 1, hd, 64)
+        k, v = rng.standard_normal((2, n, 1, hd)).astype(np.float32)
+        k[:, :, 0] = 0
+        k[at:at + 16, :, 0] = -drop * math.log(2) * math.sqrt(hd) / 16
+        v[at:at + 16] *= 2.0 ** power
+        append_ref(bt, 0, 0, k, v)
+        bt.upload()
+        q = normal(rng, (new, n_q, hd), dtype)
+        q[:, :, 0] = 16
+        few = n_q * new <= 16
+        check(hip, K, bt, 0, [n - new], [new], n_q, dtype, q, chain=2 * n // 16 + 32 if few else None,
+              small=2.0 ** -38 if power > 12 or few else 2.0 ** -22, what=(power, drop))
+
+
 def test_equal_bits_in_other_pages(hip, K):
     """The same batch in other pages: its sums are cut at the same places, so its bits are equal.  (In another batch they
     are cut elsewhere, and equal within the bounds only.)"""

@@ -555,9 +555,12 @@ __global__ __launch_bounds__(256) void attn_pages_combine_kernel(KvPages c, KvRo
 // of a step become fp16 once per group on their way into LDS, times 2^(e - ref)
 // with ref the largest exponent of the step (K) or so far (V), so a step's scores
 // and sums have one scale.  That is exact while no block lies below 2^-24 of ref
-// (PA_APART); a row's result must not depend on how large tokens are that it does
-// not see, so a wave that met such a block, or a score beyond 2^20, does its rows over,
-// block by block (pa_apart, some ten times as long).  Scores are K.Q^T, sums are
+// (PA_APART).  A probability is off by up to 2^-34 of its row's largest (half the
+// smallest fp16 of 2^9 p), times its V: V scales further apart than 2^12 in a group's
+// steps (PA_APART_V; 2^-22 a token) would let that reach a result of smaller tokens.
+// And a row's result must not depend on how large tokens are that it does not see.
+// So a wave that met such blocks, or a score beyond 2^20, does its rows over, block by
+// block (pa_apart, some ten times as long).  Scores are K.Q^T, sums are
 // V^T.P^T (a lane is a row in both), K rows are read with token bits 2 and 3
 // swapped so that a lane's scores are its operand of the second product as they
 // stand.
@@ -572,7 +575,8 @@ __global__ __launch_bounds__(256) void attn_pages_combine_kernel(KvPages c, KvRo
 // in shares of 8 steps, 22 us, 254.
 // ---------------------------------------------------------------------------
 #define PA_SHARES 64
-#define PA_APART 24 // scales of blocks that are staged together, log2
+#define PA_APART 24 // scales of K blocks that are staged together, log2
+#define PA_APART_V 12 // of V blocks whose sums are held together (below)
 #define PA_LAG 6    // sums are rescaled when a maximum has grown by more than 2^6 ..
 #define PA_Q_LOG2 9 // .. so probabilities are held as 2^9 p, at most 2^15
 
@@ -647,7 +651,8 @@ __device__ __forceinline__ void pa_store(T* dst, const floatx16_t (&o)[N], float
 }
 
 // The sums of a wave's rows over steps first, first + GROUPS, .. below z with one scale per block and row: K and V as
-// whole numbers, scores in fp32 by two-element products, each row's sums relative to the largest exponent it sees.
+// whole numbers, scores in fp32 by two-element products, each row's sums relative to its heaviest block's 2^(s - m + ev)
+// (ev_row, as pa_weight has it), weights in fp32.
 // Blocks of the least exponent hold zeros, or values below 2^-119 that count as zeros beside larger ones: they alone do
 // not lead here.
 template <typename T, int HD, int GROUPS, int PARTS, int KS, int DT>
@@ -657,7 +662,7 @@ __device__ __forceinline__ void pa_apart(const KvPages& c, const int* table, int
     const int bl = c.page_log2 - 4;
     m_run = PA_NONE;
     l_run = 0.f;
-    ev_row = KVP_E_MIN;
+    ev_row = PA_E_NONE;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -670,7 +675,7 @@ __device__ __forceinline__ void pa_apart(const KvPages& c, const int* table, int
         const int ek = c.k_exp[at], ev = c.v_exp[at], n = end - blk * KVP_BLOCK;  // places that the row sees
         const uint8_t* kr = c.k + at * (KVP_BLOCK * HD) + 8 * half;
         const uint8_t* vr = c.v + at * (KVP_BLOCK * HD) + 4 * half * KVP_BLOCK;
-        float w[KVP_BLOCK], mx = m_run;
+        float w[KVP_BLOCK], top = -INFINITY;  // of the block
         const float kf = kvp_scale(ek) * c2;
 #pragma unroll
         for (int t = 0; t < KVP_BLOCK; ++t) {
@@ -692,17 +697,17 @@ __device__ __forceinline__ void pa_apart(const KvPages& c, const int* table, int
             }
             const pa_u2 u = __builtin_amdgcn_permlane32_swap(__float_as_uint(s), __float_as_uint(s), false, false);
             w[t] = t < n ? (__uint_as_float(u[0]) + __uint_as_float(u[1])) * kf : -INFINITY;
-            mx = fmaxf(mx, w[t]);
+            top = fmaxf(top, w[t]);
         }
-        const int evm = n > 0 ? max(ev_row, ev) : ev_row;
-        const float corr = __builtin_amdgcn_exp2f(m_run - mx), both = corr * pa_pow2(ev_row - evm);
-        const float vf = ev == KVP_E_NAN ? NAN : pa_pow2(min(ev - evm, 0));
-        l_run *= corr;
+        const float mx = fmaxf(m_run, top);
+        const int evm = (int)fmaxf(fmaxf(pa_weight(m_run, ev_row, mx), pa_weight(top, ev, mx)), (float)PA_E_NONE);
+        const float both = pa_joined(m_run, ev_row, mx, evm), d = ev == KVP_E_NAN ? NAN : (float)(ev - evm + PA_Q_LOG2);
+        l_run *= __builtin_amdgcn_exp2f(m_run - mx);
 #pragma unroll
         for (int t = 0; t < KVP_BLOCK; ++t) {
-            const float p = __builtin_amdgcn_exp2f(w[t] - mx + (float)PA_Q_LOG2);
-            l_run += p;
-            w[t] = t < n ? p * vf : 0.f;
+            const float x = w[t] - mx;
+            l_run += __builtin_amdgcn_exp2f(x + (float)PA_Q_LOG2);
+            w[t] = t < n ? __builtin_amdgcn_exp2f(x + d) : 0.f;
         }
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
@@ -889,6 +894,7 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
     int k_ref = KVP_E_MIN, v_ref = KVP_E_MIN;           // of the step staged last: its largest, the largest so far
     int next_odd = 0;                                   // its blocks without a page, and with NaN in V
     int apart = 0;                                      // some blocks' scales lie too far apart for all this
+    int v_low = 1000;                                   // lane j & 3: the least V exponent of its blocks so far, zeros aside
     int by_k = 0, by_v = 0;                             // lane j & 3: block j's factors, fp16
     auto scales = [&] {
         const int my_k = got ? ek : -1000, my_v = got ? ev : -1000;  // -1000: times 0
@@ -896,13 +902,11 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
             x = max(x, __builtin_amdgcn_update_dpp(0, x, 0xB1, 0xF, 0xF, false));
             return __builtin_amdgcn_readfirstlane(max(x, __builtin_amdgcn_update_dpp(0, x, 0x4E, 0xF, 0xF, false)));
         };
-        const int v_old = v_ref;
         k_ref = max(max4(my_k), KVP_E_MIN);
-        v_ref = max(max4(my_v), v_old);
+        v_ref = max(max4(my_v), v_ref);
+        v_low = my_v > KVP_E_MIN ? min(v_low, my_v) : v_low;
         next_odd = (int)(__ballot(!got) & 15) | (int)(__ballot(my_v == KVP_E_NAN) & 15) << 4;
-        // (the last one: sums that vanish in fp32 beside larger ones)
-        apart |= ((my_k > KVP_E_MIN) & (my_k < k_ref - PA_APART)) | ((my_v > KVP_E_MIN) & (my_v < v_ref - PA_APART)) |
-                 ((v_old > KVP_E_MIN) & (v_ref - v_old > 96));
+        apart |= ((my_k > KVP_E_MIN) & (my_k < k_ref - PA_APART)) | (v_low < v_ref - PA_APART_V);
         // (NaN in V is dealt with where its rows are: 0 times it would reach rows that do not see it)
         by_k = my_k == KVP_E_NAN ? 0x7E00 : (int)__builtin_bit_cast(unsigned short, (_Float16)pa_pow2(my_k - k_ref));
         by_v = my_v == KVP_E_NAN ? 0 : (int)__builtin_bit_cast(unsigned short, (_Float16)pa_pow2(my_v - v_ref));
