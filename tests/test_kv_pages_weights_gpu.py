@@ -17,24 +17,20 @@ def weighted(q, k, v, unit, pos, scale, dtype, chain, small):
     scales ``unit`` [tokens], row i at pos[i]; 64 bits.
 
     The result's rounding: 2^-11 of it (fp16; 2^-25 below 2^-14), 2^-24 (fp32).  A weight: two fp16 parts, a rounded
-    one and a rounded rest of at most 2^-11 of it (2^-22), where that is below the normal numbers ``small`` times the
-    heaviest token's 2^(scale) for each of its n tokens of at most 127 steps; 2^-20 with the exponential's own rounding.
+    one and a rounded rest of at most 2^-11 of it (2^-22), 2^-20 with the exponential's own rounding; where the rest is
+    below the normal fp16 numbers, ``small`` of the largest weight times scale, for each of n tokens of 127 steps at most.
     A score: sums of hd + 3 roundings of 2^-24 of the sum of |q k| (fp32 q as two fp16 parts: 2^-21 more), which
     reach the result by the token's weight, in both sums.  Sums: ``chain`` roundings of 2^-24 one after the other."""
     s = q @ k.T * scale
     s[np.arange(len(k))[None] > np.asarray(pos)[:, None]] = -np.inf
     p = np.exp(s - s.max(1, keepdims=True))
     p /= p.sum(1, keepdims=True)
-    err = p * (np.abs(q) @ np.abs(k).T * scale * ((hd_of(q) + 3) * 2.0 ** -24 + (2.0 ** -21 if dtype == "f32" else 0)))
+    err = p * (np.abs(q) @ np.abs(k).T * scale * ((q.shape[1] + 3) * 2.0 ** -24 + (2.0 ** -21 if dtype == "f32" else 0)))
     out, mag = p @ v, p @ np.abs(v)
     n = np.minimum(np.asarray(pos) + 1, len(k))
     tol = (2.0 ** -20 + chain * 2.0 ** -24) * mag + err @ np.abs(v) + err.sum(1)[:, None] * np.abs(out)
     tol += (n * 127 * small * (p * unit).max(1))[:, None]
     return out, tol + (2.0 ** -11 * np.abs(out) + 2.0 ** -25 if dtype == "f16" else 2.0 ** -24 * np.abs(out))
-
-
-def hd_of(q):
-    return q.shape[1]
 
 
 def run(hip, K, bt, pos, new, n_q, dtype, q, scale):
@@ -113,7 +109,7 @@ def test_values_that_grow_twice_behind_a_row(hip, K, n_kv, batch):
     check(hip, K, bt, 0, pos, rows, n_kv, "f32", q, before=768)
 
 
-@pytest.mark.parametrize("new,n_q", [(70, 2), (150, 16)])
+@pytest.mark.parametrize("new,n_q", [(1, 4), (4, 4), (70, 2), (150, 16)])
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
 @pytest.mark.parametrize("at", [0, 64, 96, 128])
 def test_a_huge_value_of_vanishing_weight(hip, K, dtype, new, n_q, at):

@@ -7,10 +7,12 @@
 //   s_t = scale 2^ek(t) q.K_t,  out = sum_t p_t 2^ev(t) V_t / sum_t p_t,  p_t = exp(s_t - max)
 // over whole-number K and V.  Bytes become fp16 exactly (0x6400 | byte is 1024 +
 // byte; minus 1152), so both products run on 16x16x32 or 32x32x16 fp16 MFMAs with
-// no rounding of K or V.  The V scale is folded into the probability, relative to
-// the largest exponent seen (2^14 p 2^(ev - ref), at most 2^14), which is why
-// byte 0..255 of a masked token times probability 0 is the only thing a place that
-// nobody sees can add: its exponent, which may be anything, is never used.
+// no rounding of K or V.  With few rows the V scale is folded into the probability, as
+// 2^14 2^(s_t - max + ev(t) - e): e is a whole number, at most 1 above the largest of
+// what stands before it, so that the heaviest token's is 2^13 to 2^14, half the smallest
+// fp16 is 2^-38 of it, and V of vanishing weight costs the others nothing.  A token that
+// nobody sees adds its byte, 0..255, times probability 0: its exponent, which may be
+// anything, is never used.
 #include <algorithm>
 #include <type_traits>
 #include "attn_tile.h"
@@ -66,12 +68,6 @@ __device__ __forceinline__ float pa_max4(float v) {
     a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
 }
-__device__ __forceinline__ int pa_max4(int v) {
-    pa_u2 a = __builtin_amdgcn_permlane16_swap((unsigned)v, (unsigned)v, false, false);
-    v = max((int)a[0], (int)a[1]);
-    a = __builtin_amdgcn_permlane32_swap((unsigned)v, (unsigned)v, false, false);
-    return max((int)a[0], (int)a[1]);
-}
 __device__ __forceinline__ float pa_sum4(float v) {
     pa_u2 a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
@@ -109,7 +105,7 @@ struct PaPlan {
     int blocks;  // grid of the main launch
     int ncol;    // columns (rows of the second form) of a record
     float* ml;   // [2 blocks][ncol][2]: maximum (log2), sum
-    int* ev;     // [2 blocks][ncol]: exponent that the sums are relative to
+    int* ev;     // [2 blocks][ncol]: exponent that the sums are relative to (PA_E_NONE: nothing seen)
     float* o;    // [2 blocks][ncol][HD]
     int2* seg;   // [segments]: first block, pieces
 };
@@ -339,7 +335,7 @@ __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(KvPages c, KvRo
         const float c2 = scale * 1.44269504088896340736f * q_unit;  // exp(scale s) = 2^(c2 s)
 
         float m_run = PA_NONE, l_run = 0.f;
-        int ev_ref = KVP_E_MIN;  // largest V exponent that the column has seen
+        int ev_ref = PA_E_NONE;  // exponent that o is relative to
         floatx4_t o[DT];  // lane: column col, dims 16 dt + 4 grp + i
 #pragma unroll
         for (int i = 0; i < DT; ++i) o[i] = floatx4_t{0.f, 0.f, 0.f, 0.f};
@@ -362,35 +358,34 @@ __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(KvPages c, KvRo
             }
             const float kf = kvp_scale(x.ek) * c2;
             const int live = x.has ? end - p0 : 0;  // places of the block that this column sees
-            float mx = m_run;
+            float top = -INFINITY;  // of this lane group's block
 #pragma unroll
             for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     sc[tt][i] = 4 * tt + i < live ? sc[tt][i] * kf : -INFINITY;
-                    mx = fmaxf(mx, sc[tt][i]);
+                    top = fmaxf(top, sc[tt][i]);
                 }
-            mx = pa_max4(mx);
-            const int evm = max(ev_ref, pa_max4(live > 0 ? x.ev : KVP_E_MIN));
+            const float mx = fmaxf(m_run, pa_max4(top));
+            const int evm = (int)fmaxf(fmaxf(pa_max4(pa_weight(top, x.ev, mx)), pa_weight(m_run, ev_ref, mx)), (float)PA_E_NONE);
             if (__any((mx > m_run) | (evm > ev_ref))) {
-                const float corr = __builtin_amdgcn_exp2f(m_run - mx);
-                l_run *= corr;
-                const float both = corr * pa_pow2(ev_ref - evm);
+                l_run *= __builtin_amdgcn_exp2f(m_run - mx);
+                const float both = pa_joined(m_run, ev_ref, mx, evm);
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) o[dt] *= both;
                 m_run = mx;
                 ev_ref = evm;
             }
             // (a NaN block's tokens are NaN to the columns that see them and nothing to the others)
-            const float vf = x.ev == KVP_E_NAN ? NAN : pa_pow2(min(x.ev - evm, 0)) * (float)(1 << PA_P_LOG2);
+            const float d = x.ev == KVP_E_NAN ? NAN : (float)(x.ev - evm + PA_P_LOG2);
             half8_t pa[PA_P_PARTS][2];
 #pragma unroll
             for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float p = __builtin_amdgcn_exp2f(sc[tt][i] - mx);
-                    l_run += p;
-                    const float w = 4 * tt + i < live ? p * vf : 0.f;
+                    const float y = sc[tt][i] - mx;
+                    l_run += __builtin_amdgcn_exp2f(y);
+                    const float w = 4 * tt + i < live ? __builtin_amdgcn_exp2f(y + d) : 0.f;
                     const int u = tt >> 1, j = 4 * (tt & 1) + i;
                     pa[0][u][j] = (_Float16)w;
                     pa[1][u][j] = (_Float16)(w - (float)pa[0][u][j]);
@@ -433,14 +428,16 @@ __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(KvPages c, KvRo
         for (int i = tid; i < ncol * (HD / 4); i += 256) {
             const int cc = i / (HD / 4), d = i % (HD / 4) * 4;
             const float M = fmaxf(fmaxf(m_sh[0][cc], m_sh[1][cc]), fmaxf(m_sh[2][cc], m_sh[3][cc]));
-            const int EV = max(max(ev_sh[0][cc], ev_sh[1][cc]), max(ev_sh[2][cc], ev_sh[3][cc]));
+            float top = (float)PA_E_NONE;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) top = fmaxf(top, pa_weight(m_sh[w][cc], ev_sh[w][cc], M));
+            const int EV = (int)top;
             float L = 0.f;
             floatx4_t O = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-                const float f = __builtin_amdgcn_exp2f(m_sh[w][cc] - M);
-                L = fmaf(l_sh[w][cc], f, L);
-                O += *reinterpret_cast<const floatx4_t*>(&o_sh[w][cc][d]) * (f * pa_pow2(ev_sh[w][cc] - EV));
+                L = fmaf(l_sh[w][cc], __builtin_amdgcn_exp2f(m_sh[w][cc] - M), L);
+                O += *reinterpret_cast<const floatx4_t*>(&o_sh[w][cc][d]) * pa_joined(m_sh[w][cc], ev_sh[w][cc], M, EV);
             }
             if (pieces == 1) {
                 const int i_row = cc / G;
@@ -470,8 +467,7 @@ __global__ __launch_bounds__(256) void attn_pages_combine_kernel(KvPages c, KvRo
     constexpr int TD = HD / 4, GR = 256 / TD;  // threads of a row, groups of pieces
     __shared__ float w_sh[256];
     __shared__ __align__(16) float o_sh[GR][HD + 4];
-    __shared__ float red[2][4];
-    __shared__ int red_ev[4];
+    __shared__ float red[4];
     const int seg = blockIdx.x, cc = blockIdx.y, b = seg / c.n_kv, h = seg - b * c.n_kv, tid = threadIdx.x;
     const int lane = tid & 63, wv = tid >> 6, g = tid / TD, d = tid % TD * 4;
     const int G = n_q / c.n_kv, cap = kvp_capacity(c, r);
@@ -490,34 +486,26 @@ __global__ __launch_bounds__(256) void attn_pages_combine_kernel(KvPages c, KvRo
     floatx4_t early[2];  // the group's first pieces, under the way to their weights
 #pragma unroll
     for (int u = 0; u < 2; ++u) early[u] = sums(min(g + u * GR, sg.y - 1));
-    float M = PA_NONE;
-    int EV = KVP_E_MIN;
-    for (int i = tid; i < sg.y; i += 256) {
-        const size_t rec = pa_rec(sg.x, i);
-        M = fmaxf(M, pl.ml[(rec * pl.ncol + cc) * 2]);
-        EV = max(EV, pl.ev[rec * pl.ncol + cc]);
-    }
+    // every wave for itself, its first 64 pieces requested together
+    auto max_of = [&](int i) { return pl.ml[(pa_rec(sg.x, i) * pl.ncol + cc) * 2]; };
+    auto exp_of = [&](int i) { return pl.ev[pa_rec(sg.x, i) * pl.ncol + cc]; };
+    const float m0 = max_of(min(lane, sg.y - 1));
+    const int e0 = exp_of(min(lane, sg.y - 1));
+    float M = m0;
+    for (int i = 64 + lane; i < sg.y; i += 64) M = fmaxf(M, max_of(i));
     M = wave_max(M);
-    EV = max(EV, __builtin_amdgcn_update_dpp(EV, EV, 0xB1, 0xF, 0xF, false));
-    EV = max(EV, __builtin_amdgcn_update_dpp(EV, EV, 0x4E, 0xF, 0xF, false));
-    EV = max(EV, __builtin_amdgcn_update_dpp(EV, EV, 0x141, 0xF, 0xF, false));
-    EV = pa_max4(max(EV, __builtin_amdgcn_update_dpp(EV, EV, 0x140, 0xF, 0xF, false)));
-    if (lane == 0) {
-        red[0][wv] = M;
-        red_ev[wv] = EV;
-    }
-    __syncthreads();
-    M = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-    EV = max(max(red_ev[0], red_ev[1]), max(red_ev[2], red_ev[3]));
+    float top = fmaxf(pa_weight(m0, e0, M), (float)PA_E_NONE);
+    for (int i = 64 + lane; i < sg.y; i += 64) top = fmaxf(top, pa_weight(max_of(i), exp_of(i), M));
+    const int EV = (int)wave_max(top);
     float l = 0.f;
     floatx4_t O = {0.f, 0.f, 0.f, 0.f};
     for (int i0 = 0; i0 < sg.y; i0 += 256) {  // 256 pieces at a time
         const int n = min(256, sg.y - i0);
         if (tid < n) {
             const size_t rec = pa_rec(sg.x, i0 + tid);
-            const float f = __builtin_amdgcn_exp2f(pl.ml[(rec * pl.ncol + cc) * 2] - M);
-            l = fmaf(pl.ml[(rec * pl.ncol + cc) * 2 + 1], f, l);
-            w_sh[tid] = f * pa_pow2(pl.ev[rec * pl.ncol + cc] - EV);
+            const float m = pl.ml[(rec * pl.ncol + cc) * 2];
+            l = fmaf(pl.ml[(rec * pl.ncol + cc) * 2 + 1], __builtin_amdgcn_exp2f(m - M), l);
+            w_sh[tid] = pa_joined(m, pl.ev[rec * pl.ncol + cc], M, EV);
         }
         __syncthreads();
         if (i0 == 0) {
@@ -530,10 +518,10 @@ __global__ __launch_bounds__(256) void attn_pages_combine_kernel(KvPages c, KvRo
         __syncthreads();
     }
     l = wave_sum(l);
-    if (lane == 0) red[1][wv] = l;
+    if (lane == 0) red[wv] = l;
     *reinterpret_cast<floatx4_t*>(&o_sh[g][d]) = O;
     __syncthreads();
-    const float L = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+    const float L = (red[0] + red[1]) + (red[2] + red[3]);
     if (tid < HD) {
         float x = 0.f;
 #pragma unroll
