@@ -119,6 +119,35 @@ def test_extreme_temperatures(hip, K, temperature):
     check(hip, K, x, temperature, [0, 0, 3, 40, 0, 0, 5, 0], [1, 0.5, 1, 0.9, 0.99, 1, 0.5, 1], 0.0, rng.random(8))
 
 
+def halfway(T, count):
+    """Values x > 0 whose 32 x / T (the factor rounded to fp64) rounds to N + 1/2 in fp64, N even, and lies above it."""
+    from fractions import Fraction
+    T = np.float32(T)
+    s = np.float64(32.0) / np.float64(T)
+    x = np.random.default_rng(0).uniform(1, 40, 400000).astype(np.float32)
+    y = x.astype(np.float64) * s
+    tie = x[(y - np.floor(y) == 0.5) & (np.floor(y) % 2 == 0)]
+    return [v for v in tie if Fraction(float(v)) * Fraction(float(s)) > Fraction(float(np.float64(v) * s))][:count]
+
+
+@pytest.mark.parametrize("T", [1e-8, 1e-9, 3e-10])
+@pytest.mark.parametrize("rows,vocab", [(8, 300), (172, 20000), (172, 100003)])
+def test_largest_entry_halfway_between_two_bins(hip, K, T, rows, vocab):
+    """The largest entry is in the first bin of its scale however its place there is rounded: it alone has weight, or
+    shares it with its equals, early and late in the row."""
+    values = halfway(T, 8)
+    assert values
+    rng = np.random.default_rng(int(1 / T))
+    x = rng.uniform(-5, 0.9, (rows, vocab)).astype(np.float32)
+    at = rng.integers(0, vocab, (rows, 2))
+    for r in range(rows):
+        x[r, at[r]] = values[r % len(values)]
+    u = rng.random(rows)
+    got = draw(hip, K, x, np.float32(T), top_p=0.9, min_p=np.where(np.arange(rows) % 2, 0.5, 0.0), u=u)
+    # (top-p keeps both: the mass before the second, 1/2, is below 0.9)
+    assert list(got) == [int(np.sort(at[r])[int(u[r] * 2)]) for r in range(rows)]
+
+
 def test_no_settings_is_the_plain_draw(hip, K):
     rng = np.random.default_rng(12)
     x = rng.standard_normal((4, 999)).astype(np.float32)

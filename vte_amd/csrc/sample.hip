@@ -106,7 +106,9 @@ __device__ __forceinline__ SmpScale smp_scale(float max, float T) {
     const double y = (double)max * c.s;
     c.whole = fabs(y) < 35184372088832.0 && c.s > 0.0;  // 2^45: from 2^40 on neighbours are 2^16 bins apart
     c.flat = !c.whole && !(c.s > 0.0) && max < INFINITY;
-    c.top = c.whole ? __double2loint(y + SMP_ROUND) : 0;
+    // (As smp_bin rounds the largest entry itself.  The product rounded first comes to lie on a half for 1 of 30000 values at
+    // T = 1e-9, and the largest entry then lay above the first bin, out of every one.)
+    c.top = c.whole ? __double2loint(fma((double)max, c.s, SMP_ROUND)) : 0;
     const double low = c.whole ? (y - 1.5 * SMP_BINS) / c.s : 0.0;
     c.low = fmaxf(low < -3.4e38 ? -3.4e38f : (float)(low - 1.2e-7 * fabs(low) - 1e-45), -3.4028234664e38f);
     return c;
@@ -152,7 +154,7 @@ __device__ __forceinline__ int smp_inside(const SmpScale& c, float x) {
 }
 // Bins from the scale's largest value up to a larger one; SMP_ROOM + 1 where that is more than SMP_ROOM.
 __device__ __forceinline__ int smp_above(const SmpScale& c, float top) {
-    const double d = rint((double)top * c.s) - rint((double)c.max * c.s);
+    const double d = fma((double)top, c.s, SMP_ROUND) - fma((double)c.max, c.s, SMP_ROUND);  // (differences of bins as smp_bin has them)
     return d <= (double)SMP_BINS ? (int)d : SMP_BINS + 1;
 }
 // Bins between the largest values of a part and of the row; SMP_BINS or more: none of the part's matter.
@@ -762,7 +764,7 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_draw_kernel(const float* _
     smp_find(S, mine, drawn(k_lo), drawn(k_hi), u0, u1);
     last = max(last, u1);
     // as ranges of values in fp32, wider than the bins by more than its roundings: what else they hold goes by bin later
-    const double y_top = rint((double)top * r.c.s), unit = (double)T / SMP_PER_UNIT;
+    const double y_top = fma((double)top, r.c.s, SMP_ROUND) - SMP_ROUND, unit = (double)T / SMP_PER_UNIT;
     struct Range {
         float low, high;
     };
