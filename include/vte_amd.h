@@ -448,7 +448,8 @@ long long vte_sample_scratch_bytes(int rows);
  * (mass of the top-k) before them, min-p those of weight >= min_p; the token is
  * the first kept one whose mass up to and with it exceeds u * (kept mass).
  * Greedy: the largest logit, the lowest index among equal ones.  A NaN logit has
- * no weight; a row of nothing but -Inf and NaN gives -1; +Inf entries share the
+ * no weight; a row of nothing but -Inf and NaN gives -1, as does one whose logits
+ * change under the call if no entry fits its sums any more; +Inf entries share the
  * draw.  Sums are exact (64-bit whole numbers; an entry below 2^-45 of the
  * largest has no weight), so a token depends on its row and settings alone.
  * scratch: 16-byte aligned, need not be cleared; calls that may overlap need one

@@ -87,6 +87,11 @@ __device__ __forceinline__ float smp_value(uint64_t place) {
 __device__ __forceinline__ int smp_index(uint64_t place) {
     return ((1 << SMP_IDX_BITS) - 1) - (int)(place & ((1 << SMP_IDX_BITS) - 1));
 }
+// A drawn entry's token; -1 where none was found, which takes logits that change under the call.
+__device__ __forceinline__ int smp_token(uint64_t place, int vocab) {
+    const int i = smp_index(place);
+    return place != 0 && i < vocab ? i : -1;
+}
 
 // Where a row's bins lie: the largest value (of the row or of a part), 32 / T, and the low word of round(32 max / T).
 // Rounding adds 1.5 2^52, whose low word then holds the whole number: differences of up to 2^31 bins are right, and
@@ -487,7 +492,10 @@ __device__ uint64_t smp_end(SmpShared& S, const SmpRow& r, int b, double t, uint
     t = fmax(t, COUNT ? 1.0 : 0.0);
     auto collect = [&](int step) {  // the bin's entries (of one step) into place and m, SMP_SMALL at most
         __syncthreads();
-        if (tid == 0) S.n_match = 0;
+        if (tid == 0) {
+            S.n_match = 0;
+            S.found = 0;  // (no entry's place; what a split found has been read)
+        }
         __syncthreads();
         smp_each(S, r, [&](uint64_t c, int g, uint64_t m) {
             if (g != b || (step >= 0 && smp_inside(r.c, smp_value(c)) != step)) return;
@@ -588,9 +596,9 @@ __device__ __forceinline__ int smp_end_wave(const SmpShared& S, const SmpRow& r,
         const bool passes = count ? (double)rank >= t : (double)sum > t;
         const bool passed = count ? (double)(rank - 1) >= t : (double)(sum - m) > t;
         const uint64_t here = __ballot(g == b && ((passes && !passed) || (!passes && rank == __popcll(in))));
-        const int l = __ffsll((unsigned long long)here) - 1;
-        upto = smp_lane(sum, l);
-        return smp_lane(c, l);
+        const int l = here ? __ffsll((unsigned long long)here) - 1 : 0;
+        upto = here ? smp_lane(sum, l) : 0;
+        return here ? smp_lane(c, l) : 0;
     };
     auto find = [&](double t) {  // as smp_find: bins whose running weight does not exceed t (is below all) come before
         const double all = (double)S.mass[SMP_BINS - 1];
@@ -627,7 +635,7 @@ __device__ __forceinline__ int smp_end_wave(const SmpShared& S, const SmpRow& r,
     }
     const double t = drawn(fmin(fmax(kept, k_lo), k_hi));
     const int b = u0 != u1 ? find(t) : u0;
-    return smp_index(end(b, (t - smp_before(S, b)) / smp_middle(b), false, upto));
+    return smp_token(end(b, (t - smp_before(S, b)) / smp_middle(b), false, upto), r.vocab);
 }
 
 template <bool WIDE>
@@ -670,7 +678,7 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_draw_kernel(const float* _
 #pragma unroll
             for (int e = 3; e >= 0; --e) at = f.x[e] == top ? min(at, smp_at<WIDE>(S.n, lane, e)) : at;
             for (int d = 1; d < 64; d *= 2) at = min(at, __shfl_xor(at, d, 64));
-            if (lane == 0) tokens[row] = at;
+            if (lane == 0) tokens[row] = at < vocab ? at : -1;
         }
         return;
     }
@@ -853,7 +861,7 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_draw_kernel(const float* _
         if (wv == 0) {
             const int token = smp_end_wave(S, r, lane, kb, k, has_p, p, p0, p1, has_m, m0, m1, floor_w, z_lo, z_hi, k_lo, k_hi,
                                            u0, u1, drawn);
-            if (lane == 0) tokens[row] = min(token, vocab - 1);
+            if (lane == 0) tokens[row] = token;
         }
         return;
     }
@@ -886,7 +894,7 @@ __global__ __launch_bounds__(SMP_THREADS) void sample_draw_kernel(const float* _
     int b = u0, same;
     if (u0 != u1) smp_find(S, mine, t, t, b, same);
     const uint64_t place = smp_end<false>(S, r, b, (t - smp_before(S, b)) / smp_middle(b), upto);
-    if (tid == 0) tokens[row] = min(smp_index(place), vocab - 1);
+    if (tid == 0) tokens[row] = smp_token(place, vocab);
 }
 
 namespace vte {
