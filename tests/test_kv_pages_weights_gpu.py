@@ -84,7 +84,7 @@ def sized(hip, K, rng, n, n_kv, hd, v_size, batch=1, **kw):
 
 
 @pytest.mark.parametrize("new,n_q,n_kv,hd,batch", [(128, 1, 1, 128, 1), (70, 2, 1, 64, 1), (600, 16, 1, 128, 1),
-                                                   (130, 16, 4, 64, 140), (4, 4, 1, 128, 1)])
+                                                   (130, 16, 4, 64, 160), (4, 4, 1, 128, 1)])
 @pytest.mark.parametrize("at", [448, 704, 720])
 def test_values_of_2_to_130_times_behind_a_row(hip, K, new, n_q, n_kv, hd, batch, at):
     """V of tokens that a row does not see are 2^130 times those that it sees, from a border of a step on and inside one:
@@ -96,10 +96,10 @@ def test_values_of_2_to_130_times_behind_a_row(hip, K, new, n_q, n_kv, hd, batch
     check(hip, K, bt, 0, [n - new] + [-1] * (batch - 1), [new] + [0] * (batch - 1), n_q, "f32", q, before=at)
 
 
-@pytest.mark.parametrize("n_kv,batch", [(4, 140), (1, 1)])
+@pytest.mark.parametrize("n_kv,batch", [(4, 160), (1, 1)])
 def test_values_that_grow_twice_behind_a_row(hip, K, n_kv, batch):
     """V grow by 2^80 and, a step later, by 2^80 again, each less than fp32 holds, together more: rows before the first
-    growth, and those between the two.  (Of 140 sequences the row blocks are 256 rows, which span both.)"""
+    growth, and those between the two.  (Of 160 sequences the row blocks are 256 rows, which span both.)"""
     rng = np.random.default_rng(n_kv)
     n, new = 900, 300
     bt = sized(hip, K, rng, n, n_kv, 64, 2.0 ** np.repeat([-80.0, 0.0, 80.0], [704, 64, 132]), batch)

@@ -1211,11 +1211,13 @@ static PaPlan rows_plan(const KvPages& c, const KvRows& r, int hd, int G, void* 
 }
 // The many-rows form: rows of a block, row blocks at most (each sequence may end one early), and shares of each, as many
 // as fill the CUs.
-// Rows of a block: 256 (one group) from 7/4 blocks a CU on, else 128 (two groups).  256 / 128, us, 2048 new tokens a
-// sequence: 1.5 blocks a CU 106 / 99, 1.75 134 / 147, 2 97 / 115, 2.25 147 / 143, 4 195 / 222.
+// Rows of a block: 256 (one group) from 9/4 blocks a CU on, else 128 (two groups).  256 / 128, us, fp16, four sequences of
+// 2048 new tokens, heads of 128: 1.5 blocks a CU 120 / 103, 1.77 134 / 122, 2 151 / 128, 2.27 146 / 146, 2.5 156 / 161, 3
+// 175 / 195, 4 222 / 248; fp32 1.77 153 / 141, 2.27 175 / 178, 3 215 / 240; ragged prompts of 100 to 900 tokens 1.75 75 / 79,
+// 2.45 95 / 103.
 // Shares: of four steps at least, or of two while there are no more than 16; no more than 64.  Three new tokens, 16 query
-// heads, 16 / 32 / 64 / 128 shares, us: after 8192 tokens 21.3 / 19.4 / 21.9 / 21.8, after 32768 49 / 33 / 29 / 34; after
-// 2048 8 / 16 shares 15.2 / 14.1.
+// heads, 16 / 32 / 64 / 128 shares, us: after 8192 tokens 23.0 / 19.8 / 21.8 / 22.0, after 32768 57 / 37 / 30 / 34; after
+// 2048 8 / 16 shares 16.0 / 14.4.
 struct PromptForm {
     int groups;
     long long rbs;
@@ -1225,7 +1227,7 @@ struct PromptForm {
 static PromptForm prompt_form(const KvPages& c, const KvRows& r, int hd, int G, void* scratch) {
     PromptForm f;
     auto blocks = [&](int rows) { return ((long long)r.rows * G + rows - 1) / rows + r.batch - 1; };
-    f.groups = blocks(256) * c.n_kv * 4 >= 7 * device_cus() ? 1 : 2;
+    f.groups = blocks(256) * c.n_kv * 4 >= 9 * device_cus() ? 1 : 2;
     f.rbs = blocks(f.groups == 1 ? 256 : 128);
     const long long steps = (((long long)r.max_pages << c.page_log2) + PA_TILE - 1) / PA_TILE;
     const long long most = std::max(std::min(16LL, steps / 2), std::min<long long>(PA_SHARES, steps / 4));
@@ -1242,8 +1244,8 @@ static PromptForm prompt_form(const KvPages& c, const KvRows& r, int hd, int G, 
     f.bytes = n;
     return f;
 }
-// One tile's columns hold them all.  (Few-rows / many-rows form, us: one sequence of 2049 tokens 11.7 / 15.4, 16 ragged ones
-// of up to 8192 17.7 / 29.7, eight of up to 65536 36.0 / 88.3.)
+// One tile's columns hold them all.  (Few-rows / many-rows form, us: one sequence of 2049 tokens 11.8 / 16.9, 16 ragged ones
+// of up to 8192 18.1 / 34.5, eight of up to 65536 37.0 / 105.)
 static bool rows_form(const KvRows& r, int G) { return r.max_rows * G <= 16; }
 
 long long attn_pages_scratch_bytes(const KvPages& c, const KvRows& r, int hd, int n_q) {
