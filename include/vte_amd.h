@@ -385,7 +385,8 @@ typedef struct vte_kv_pages {
  * page_table: device int [batch][max_pages]; entry j holds the page of positions
  * j * page_tokens ..; an entry outside [0, n_pages) is no page: rows for it are
  * dropped, its tokens are not seen.  Positions past max_pages * page_tokens are
- * dropped likewise.  A page that a call writes must belong to one sequence. */
+ * dropped likewise.  A page that a call writes must belong to one sequence and
+ * stand in its table once. */
 typedef struct vte_kv_rows {
     int batch, rows, max_rows, max_pages;
     const int *row_start, *kv_offset, *page_table;
@@ -419,7 +420,8 @@ int vte_kv_pages_append(const vte_kv_pages* cache, const vte_kv_rows* rows, int 
 int vte_kv_pages_read(const vte_kv_pages* cache, const vte_kv_rows* rows, int dtype, void* k_out, void* v_out,
                       int out_rows, void* stream);
 
-/* Scratch bytes of vte_attn_pages (-1: rejected arguments). */
+/* Scratch bytes of vte_attn_pages for these rows and pages per table (-1: rejected
+ * arguments).  Fewer rows can need more: ask for each shape. */
 long long vte_attn_pages_scratch_bytes(const vte_kv_pages* cache, const vte_kv_rows* rows, int n_q);
 
 /* Attention of the new rows over the paged cache (which holds them already):
@@ -428,8 +430,13 @@ long long vte_attn_pages_scratch_bytes(const vte_kv_pages* cache, const vte_kv_r
  * rows * n_q <= 2^25, batch * n_kv <= 2^20.  A row that sees
  * nothing (a sequence that does not run, no pages) gives 0; rows that belong to
  * nobody are left as they were.  Sums and softmax statistics are fp32; the
- * probabilities, and fp32 q, enter the products as two fp16 parts each.  scratch: 16-byte aligned, need not be cleared;
- * calls that may overlap (two streams, two graphs) need one each.  Capturable.
+ * probabilities, and fp32 q, enter the products as two fp16 parts each.  A
+ * result's error goes by what the tokens it sees contribute (weight times |V|): V of
+ * a vanishing weight, or of tokens that the row does not see (in blocks of their
+ * own), costs it nothing however large.  Many rows over V scales more than 2^12
+ * apart, or scores beyond 2^20, take some ten times as long.  scratch: 16-byte
+ * aligned, need not be cleared; calls that may overlap (two streams, two graphs)
+ * need one each.  Capturable.
  * Replaces: SplitKVAttentionDispatcher launches (vte/core/split_kv_attention.py:187-217)
  *           for a cache in this form. */
 int vte_attn_pages(const vte_kv_pages* cache, const vte_kv_rows* rows, int dtype, const void* q, void* out, int n_q,
@@ -450,8 +457,11 @@ long long vte_sample_scratch_bytes(int rows);
  * Greedy: the largest logit, the lowest index among equal ones.  A NaN logit has
  * no weight; a row of nothing but -Inf and NaN gives -1, as does one whose logits
  * change under the call if no entry fits its sums any more; +Inf entries share the
- * draw.  Sums are exact (64-bit whole numbers; an entry below 2^-45 of the
- * largest has no weight), so a token depends on its row and settings alone.
+ * draw.  Sums are 64-bit whole numbers, the same in any order, so a token depends
+ * on its row and settings alone.  Weights below e^-32 of the largest are none, nor
+ * are those of one step of e^(1/32) that are below 2^-45 of it together; masses are
+ * off by vocab * 2^-44 of the largest weight at most (a border or u nearer than
+ * that to another token's end may fall to either, always to the same one).
  * scratch: 16-byte aligned, need not be cleared; calls that may overlap need one
  * each.  Capturable.
  * Replaces: Sampler.sample (vte/core/sampler.py:54-129) after the repetition

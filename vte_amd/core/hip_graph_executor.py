@@ -643,8 +643,10 @@ class HIPGraphExecutor:
         back to back.  ``uniforms`` [n_steps, B]: the draws' random numbers in
         [0, 1).  Settings are one value or one per sequence (temperature <= 0:
         greedy; no repetition penalty).  Returns the tokens, [n_steps, B]; each
-        is what ``vte_sample`` draws from the step's logits (the host sampler's
-        draw, vte/core/sampler.py:54-129, for the same random number)."""
+        is what ``vte_sample`` draws from the step's logits: with 0 < top_p < 1
+        the host sampler's draw (vte/core/sampler.py:54-129) for the same random
+        number, with top_p off (the default) the same distribution, drawn by
+        value instead of in the host's order of candidates."""
         if self.prefill_of is not None:
             raise HIPSafetyError("a prefill executor's columns are one sequence's tokens; decode through the owner")
         if n_steps < 1 or max(kv_offsets) + n_steps > self.max_seq:

@@ -95,9 +95,9 @@ __device__ __forceinline__ float pa_pow2(int d) { return d < -126 ? 0.f : __uint
 // two records a block are enough.
 //
 // Bound by the cache's bytes where contexts are long: eight documents of 16384 to
-// 65536 tokens, 168 MB, 36 us in all, 4.7 TB/s (a copy moves 5.0); by latencies where
-// they are short: 2049 tokens 11.7 us, two launches, in the first four loads one after the other (positions, page, bytes, q) and a
-// tile's work.  Bytes go from memory to registers, where a lane's 16 are its operand
+// 65536 tokens, 168 MB, 37.2 us in all, 4.5 TB/s (a copy moves 5.0; fp32 q 37.7); by
+// latencies where they are short: 2049 tokens 11.9 us (fp32 q 13.9), two launches, in the
+// first four loads one after the other (positions, page, bytes, q) and a tile's work.  Bytes go from memory to registers, where a lane's 16 are its operand
 // once permuted: no LDS, each is used once, and a wave has the next tile's under way
 // (two blocks of 256 threads a CU is all that those registers leave).
 // ---------------------------------------------------------------------------
@@ -553,14 +553,16 @@ __global__ __launch_bounds__(256) void attn_pages_combine_kernel(KvPages c, KvRo
 // swapped so that a lane's scores are its operand of the second product as they
 // stand.
 //
-// Bound by issue: a group's step is 32 products a wave (1000 cycles) beside some 500
-// cycles of turning bytes and 900 of softmax, with two waves a SIMD, which overlap in
-// part: 2.4 us for two groups' steps.  The runs below fix what stands between two products (left to
+// Bound by issue: a group's step is 48 products a wave (1500 cycles; fp32 q 64, heads of
+// 64 half as many) beside some 500 cycles of turning bytes and 1200 of softmax and
+// splitting probabilities, with two waves a SIMD, which overlap in part: 2.8 us for two
+// groups' steps (fp32 q 3.0, heads of 64 2.1 and 2.2).  The runs below fix what stands between two products (left to
 // itself the compiler read an operand right before each).  Beside that a block starts
 // (3 us: sequence, page, bytes, the first tile) and ends (2 us), which weighs on short
-// ones: four sequences of 2048 new tokens, 32 query and 8 KV heads of 128, 195 us, 700
-// TFLOP/s (a large fp16 matrix product: 1100 to 1200); a chunk of 512 after 1536 tokens,
-// in shares of 8 steps, 22 us, 254.
+// ones: four sequences of 2048 new tokens, 32 query and 8 KV heads of 128, 222 to 230 us,
+// 600 to 620 TFLOP/s (a large fp16 matrix product: 1100 to 1200; the second part of the
+// probabilities is not counted, but takes a third of the products); a chunk of 512 after
+// 1536 tokens, in shares of 8 steps, 24.3 us, 232.
 // ---------------------------------------------------------------------------
 #define PA_SHARES 64
 #define PA_APART 24 // scales of K blocks that are staged together, log2
