@@ -442,6 +442,116 @@ long long vte_attn_pages_scratch_bytes(const vte_kv_pages* cache, const vte_kv_r
 int vte_attn_pages(const vte_kv_pages* cache, const vte_kv_rows* rows, int dtype, const void* q, void* out, int n_q,
                    float scale, void* scratch, long long scratch_bytes, void* stream);
 
+/* Scratch bytes of vte_attn_pages_window (-1: rejected arguments); as those of vte_attn_pages. */
+long long vte_attn_pages_window_scratch_bytes(const vte_kv_pages* cache, const vte_kv_rows* rows, int n_q, int window,
+                                              int sinks);
+
+/* As vte_attn_pages, of rows that see a sliding window and the first tokens: row i
+ * of sequence b, at position p = kv_offset[b] + i, sees tokens t <= p with
+ * t > p - window or t < sinks (window >= 1, the row's own token among them; sinks
+ * >= 0).  Pages of which no row of the call sees a token are not read: their entries
+ * may be -1.  Time and scratch go by the window, not by the sequence's length.
+ * No counterpart in the reference. */
+int vte_attn_pages_window(const vte_kv_pages* cache, const vte_kv_rows* rows, int dtype, const void* q, void* out,
+                          int n_q, float scale, int window, int sinks, void* scratch, long long scratch_bytes,
+                          void* stream);
+
+/* ---- norm and rotation of heads ----
+ * How a model's q and k heads are written.  A head x of head_dim values becomes
+ *   y = x * w / sqrt(mean(x^2) + eps)              (w: q_norm or k_norm, fp16 [head_dim]; NULL: y = x)
+ * and of its first rotary_dim dims (even; 0: all) pair i = (a, b) becomes
+ *   amplitude * (a cos t - b sin t, a sin t + b cos t),  t = position * freq[i]
+ * with freq device double [rotary_dim / 2], radians per position (NULL: no rotation),
+ * a and b at dims i and i + rotary_dim / 2, or, interleaved, 2 i and 2 i + 1.  Angles
+ * are formed in 64 bits, all else is fp32 (sums of squares too: |x| from 2^60 on may
+ * overflow them), rounded once at the end.  The struct is read by the host call only.
+ * Scaled rotations for long contexts are frequencies and an amplitude:
+ * vte_amd.core.rope_cache.rope_frequencies makes them. */
+typedef struct vte_head_form {
+    const void *q_norm, *k_norm;
+    const double* freq;
+    float eps, amplitude; /* eps in (0, 1] where there is a norm */
+    int rotary_dim, interleaved;
+} vte_head_form;
+
+/* q_out, k_out = the rows' heads as `form` has them, row i at positions[i] (device int
+ * [rows]; below 0: the row is left as it is in q_out and k_out; NULL without a
+ * rotation).  q [rows][n_q][head_dim], k [rows][n_kv][head_dim] (dtype fp16 or fp32),
+ * rows q_stride / k_stride elements apart (0: contiguous); q_out and k_out contiguous,
+ * or q and k themselves, with their strides.  q or k may be NULL.  head_dim 64, 128 or
+ * 256; rows <= 2^24, rows * (n_q + n_kv) <= 2^27.  Rows and norms that are 16-byte
+ * aligned, with neighbouring pairs or a rotary_dim that is a multiple of 16, take the
+ * fast form.
+ * Replaces: rope_kernel (rope.hip.template:17-137) where heads are normed or positions
+ *           lie behind its tables. */
+int vte_qk_norm_rope(const vte_head_form* form, int dtype, int head_dim, int rows, const int* positions, const void* q,
+                     void* q_out, int n_q, long long q_stride, const void* k, void* k_out, int n_kv, long long k_stride,
+                     void* stream);
+
+/* As vte_kv_pages_append, with k and q as `form` has them (no tables, so no last
+ * position but the page table's end; q may come without a rotation). */
+int vte_kv_pages_append_norm(const vte_kv_pages* cache, const vte_kv_rows* rows, const vte_head_form* form, int dtype,
+                             const void* k, const void* v, long long k_stride, long long v_stride, const void* q,
+                             void* q_out, int n_q, long long q_stride, void* stream);
+
+/* ---- pages as a pool that sequences share ----
+ * page_table int [batch][max_pages] as vte_kv_rows has it (one for all layers), refs
+ * int [n_pages]: the users of each page, 0: free (no entry may name a free page).  The
+ * program zeroes refs once and sets the table to -1; it may count users of its own (a
+ * prompt kept for later).  Both are device memory.  n_pages <= 2^24.
+ * What the calls do goes by their inputs alone: new pages are the lowest free ones, in
+ * the order of the list.  Sequences outside [0, batch) are passed over.  A call on these
+ * arrays must have ended (or stand before on the same stream) when the next one starts.
+ * All are capturable.  No counterpart in the reference. */
+typedef struct vte_kv_tables {
+    int *page_table, *refs;
+    int batch, max_pages, n_pages, page_tokens;
+} vte_kv_tables;
+
+/* Pages src[i] -> dst[i] (device int [n], n <= 2^24) of all layers (host array of
+ * n_layers <= 512 pools of one shape; pages of at most 2^30 bytes), exponents with them.  Pairs
+ * of which one is no page are passed over.  No page may be a dst twice, or a dst and a src. */
+int vte_kv_pages_copy(const vte_kv_pages* layers, int n_layers, const int* src, const int* dst, int n, void* stream);
+
+/* Give pages back: of sequences seqs[i], i < n <= 65535 (NULL: 0 .. n - 1), the entries of
+ * pages that hold only tokens keep .. end[i] - behind - 1 (end device int [n]; NULL: all
+ * from `keep` on; below 0: none) become -1, and their pages have one user less.  A
+ * sequence that ended: keep 0, end NULL.  Behind a window: keep = sinks, end = kv_offset,
+ * behind = window - 1. */
+int vte_kv_pages_free(const vte_kv_tables* tables, int n, const int* seqs, int keep, const int* end, int behind,
+                      void* stream);
+
+/* Room: of sequences seqs[i] (NULL: 0 .. n - 1) every entry of tokens start[i] ..
+ * start[i] + count - 1 (those below stop[i], where stop is given; start below 0: none)
+ * that is no page gets one.  n * (pages of count tokens + 1) <= 2^24.  missing (device
+ * int, may be NULL) = how many entries got none because no page was free. */
+int vte_kv_pages_reserve(const vte_kv_tables* tables, int n, const int* seqs, const int* start, const int* stop,
+                         int count, int* missing, void* stream);
+
+/* Scratch bytes of vte_kv_pages_fork for n children (0: n outside 1..65535). */
+long long vte_kv_pages_fork_scratch_bytes(int n);
+
+/* Sequence children[i] becomes the first lengths[i] tokens of parents[i]: its former
+ * pages are given back, whole pages are shared with the parent (which neither may write
+ * again below lengths[i]), the page in which they end is copied to a new one in every
+ * layer.  Entries that are no page stay so.  Where no page is free the last entry is -1;
+ * missing (device int, may be NULL) counts those.  A child must be in the list once, and
+ * not be a parent in it; a child that is its own parent, or a length below 0, is passed
+ * over. */
+int vte_kv_pages_fork(const vte_kv_pages* layers, int n_layers, const vte_kv_tables* tables, int n, const int* parents,
+                      const int* children, const int* lengths, int* missing, void* scratch, long long scratch_bytes,
+                      void* stream);
+
+/* Scratch bytes of vte_kv_pages_compact (-1: rejected arguments). */
+long long vte_kv_pages_compact_scratch_bytes(const vte_kv_tables* tables);
+
+/* The pool's used pages (refs above 0) become its first ones: with U of them, the k-th
+ * used page from U on moves to the k-th free one below U, in every layer; entries and
+ * refs follow (an entry that names a free page becomes -1).  used (device int) = U;
+ * where (device int [n_pages]) = the place each used page has now, -1 of free ones. */
+int vte_kv_pages_compact(const vte_kv_pages* layers, int n_layers, const vte_kv_tables* tables, int* where, int* used,
+                         void* scratch, long long scratch_bytes, void* stream);
+
 /* Scratch bytes of vte_sample for calls of at most `rows` rows (never less for
  * more rows: memory sized for the largest batch serves the smaller ones). */
 long long vte_sample_scratch_bytes(int rows);

@@ -117,6 +117,32 @@ __device__ __forceinline__ int pa_tokens(const KvSeq& s, int cap) {
     return s.n == 0 ? 0 : (s.n < cap - s.pos ? s.pos + s.n : cap);
 }
 
+// Windows.  A row at position p sees the tokens from p + 1 - window on and the first `sinks` ones, none behind itself.  Tiles
+// that none of the rows at hand sees are left out: those that are walked are numbered through, `head` at the front and from
+// there on those `skip` further.  (WIN false: all of them, and the kernels are those of the attention without windows.)
+struct PaWindow {
+    int window, sinks;
+};
+struct PaSpan {
+    int n, head, skip;
+    template <bool WIN>
+    __device__ __forceinline__ int real(int i) const { return WIN && i >= head ? i + skip : i; }
+};
+// Of rows from position `first` on, which see tokens below `end` (`end` 0: no rows).
+template <bool WIN>
+__device__ __forceinline__ PaSpan pa_span(int first, int end, const PaWindow& w) {
+    const int nt = (end + PA_TILE - 1) / PA_TILE;
+    if constexpr (!WIN) return PaSpan{nt, nt, 0};
+    const int low = min(max(first + 1 - w.window, 0) / PA_TILE, nt);
+    const int head = min((min(w.sinks, end) + PA_TILE - 1) / PA_TILE, low);
+    return PaSpan{nt - (low - head), head, low - head};
+}
+// Which of the 16 tokens from t0 on a row sees, one bit each, where it sees those in [low, end) and below `sinks`.
+__device__ __forceinline__ uint32_t pa_below(int n) { return n >= 16 ? 0xFFFFu : n <= 0 ? 0u : (1u << n) - 1; }
+__device__ __forceinline__ uint32_t pa_seen(int t0, int low, int end, int sinks) {
+    return pa_below(end - t0) & (~pa_below(low - t0) | pa_below(sinks - t0));
+}
+
 // The block's share [t, t_end) of all tiles, and the sequence that t lies in with
 // the number of tiles before it.
 struct PaShare {
@@ -150,11 +176,12 @@ __device__ __forceinline__ V pa_scan(V v) {
     v += pa_from<0x143, 0xC>(v);
     return v;
 }
-__device__ __forceinline__ PaShare pa_share(const KvPages& c, const KvRows& r, int cap, int block, int blocks) {
+template <bool WIN>
+__device__ __forceinline__ PaShare pa_share(const KvPages& c, const KvRows& r, int cap, int block, int blocks, const PaWindow& w) {
     __shared__ long long wsum[4];
     __shared__ long long found[5];
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-    auto tiles = [&](const KvSeq& q) { return (long long)c.n_kv * ((pa_tokens(q, cap) + PA_TILE - 1) / PA_TILE); };
+    auto tiles = [&](const KvSeq& q) { return (long long)c.n_kv * pa_span<WIN>(q.pos, pa_tokens(q, cap), w).n; };
     auto cut = [&](PaShare& s, long long total) {
         // (a tile for each wave at least; whole rounds of four beyond that left CUs idle: eight documents of 16384 to
         // 65536 tokens 44.0 -> 41.3 us without, 16 ragged sequences 19.7 -> 18.3 us)
@@ -236,10 +263,10 @@ struct PaTile {
     bool has;  // the lane's block has a page
 };
 
-template <typename T, int HD>
+template <typename T, int HD, bool WIN>
 __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(KvPages c, KvRows r, PaPlan pl,
                                                                  const T* q, T* out, int n_q,
-                                                                 float scale) {
+                                                                 float scale, PaWindow w) {
     constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;  // fp16 parts of q
     constexpr int KC = HD / 64;                    // 16-byte pieces of a K row that a lane holds
     constexpr int DT = HD / 16;
@@ -250,13 +277,15 @@ __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(KvPages c, KvRo
     const int col = lane & 15, grp = lane >> 4;
     const int G = n_q / c.n_kv, cap = kvp_capacity(c, r);
     const int bl = c.page_log2 - 4;  // log2 of a page's blocks
-    PaShare sh = pa_share(c, r, cap, blockIdx.x, pl.blocks);
+    PaShare sh = pa_share<WIN>(c, r, cap, blockIdx.x, pl.blocks, w);
     int b = sh.b;
     long long t = sh.t, before = sh.before;
     KvSeq s = sh.s;
 
     while (t < sh.t_end) {
-        const int len = pa_tokens(s, cap), nt = (len + PA_TILE - 1) / PA_TILE;
+        const int len = pa_tokens(s, cap);
+        const PaSpan span = pa_span<WIN>(s.pos, len, w);
+        const int nt = span.n;
         if (t - before >= (long long)nt * c.n_kv) {  // the next sequence
             before += (long long)nt * c.n_kv;
             s = kvp_seq(r, ++b);
@@ -274,10 +303,11 @@ __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(KvPages c, KvRo
         const int ncol = s.n * G, ci = min(col, ncol - 1);
         const int qi = ci / G, qh = h * G + ci - qi * G;
         const int end = col < ncol ? kvp_len(s.pos + qi, cap) : 0;
+        const int low = WIN ? max(s.pos + qi + 1 - w.window, 0) : 0;
         // K row of 16-row tile tt: token 16 (col / 4) + 4 tt + col % 4, so that the scores a lane gets from the four
         // tiles are those of block grp in order, which is the order V's 16 bytes hold its tokens in.
         auto load = [&](PaTile<HD>& x, int tile) {
-            const int t0 = tile * PA_TILE;
+            const int t0 = span.template real<WIN>(tile) * PA_TILE;
             const int last = (len - 1) >> 4;  // blocks past the end read the last one (their tokens are masked)
             const int kb = min((t0 >> 4) + (col >> 2), last), vb = min((t0 >> 4) + grp, last);
             const int kp = table[kb >> bl], vp = table[vb >> bl];
@@ -341,7 +371,7 @@ __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(KvPages c, KvRo
         for (int i = 0; i < DT; ++i) o[i] = floatx4_t{0.f, 0.f, 0.f, 0.f};
 
         auto step = [&](const PaTile<HD>& x, int tile) {
-            const int p0 = tile * PA_TILE + 16 * grp;  // this lane group's block
+            const int p0 = span.template real<WIN>(tile) * PA_TILE + 16 * grp;  // this lane group's block
             floatx4_t sc[4];
 #pragma unroll
             for (int tt = 0; tt < 4; ++tt) {
@@ -358,12 +388,15 @@ __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(KvPages c, KvRo
             }
             const float kf = kvp_scale(x.ek) * c2;
             const int live = x.has ? end - p0 : 0;  // places of the block that this column sees
+            uint32_t bits = 0;                      // (with a window)
+            if constexpr (WIN) bits = x.has ? pa_seen(p0, low, end, w.sinks) : 0;
+            auto sees = [&](int i) { return WIN ? (bits >> i & 1) != 0 : i < live; };
             float top = -INFINITY;  // of this lane group's block
 #pragma unroll
             for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    sc[tt][i] = 4 * tt + i < live ? sc[tt][i] * kf : -INFINITY;
+                    sc[tt][i] = sees(4 * tt + i) ? sc[tt][i] * kf : -INFINITY;
                     top = fmaxf(top, sc[tt][i]);
                 }
             const float mx = fmaxf(m_run, pa_max4(top));
@@ -385,10 +418,10 @@ __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(KvPages c, KvRo
                 for (int i = 0; i < 4; ++i) {
                     const float y = sc[tt][i] - mx;
                     l_run += __builtin_amdgcn_exp2f(y);
-                    const float w = 4 * tt + i < live ? __builtin_amdgcn_exp2f(y + d) : 0.f;
+                    const float p = sees(4 * tt + i) ? __builtin_amdgcn_exp2f(y + d) : 0.f;
                     const int u = tt >> 1, j = 4 * (tt & 1) + i;
-                    pa[0][u][j] = (_Float16)w;
-                    pa[1][u][j] = (_Float16)(w - (float)pa[0][u][j]);
+                    pa[0][u][j] = (_Float16)p;
+                    pa[1][u][j] = (_Float16)(p - (float)pa[0][u][j]);
                 }
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
@@ -461,9 +494,9 @@ __global__ __launch_bounds__(256, 2) void attn_pages_rows_kernel(KvPages c, KvRo
 
 // Combine of the segments that were cut, and zeros for the rows that see nothing:
 // grid (segments, ncol), HD / 4 threads per group of pieces.
-template <typename T, int HD>
+template <typename T, int HD, bool WIN>
 __global__ __launch_bounds__(256) void attn_pages_combine_kernel(KvPages c, KvRows r, PaPlan pl, T* __restrict__ out,
-                                                                 int n_q) {
+                                                                 int n_q, PaWindow win) {
     constexpr int TD = HD / 4, GR = 256 / TD;  // threads of a row, groups of pieces
     __shared__ float w_sh[256];
     __shared__ __align__(16) float o_sh[GR][HD + 4];
@@ -474,7 +507,8 @@ __global__ __launch_bounds__(256) void attn_pages_combine_kernel(KvPages c, KvRo
     const KvSeq s = kvp_place(r, b);
     if (cc >= s.n * G) return;
     T* dst = out + ((size_t)(s.first + cc / G) * n_q + h * G + cc % G) * HD;
-    if (s.pos < 0) {
+    // (a window may lie behind the table)
+    if (s.pos < 0 || (WIN && pa_span<WIN>(s.pos, pa_tokens(s, cap), win).n == 0)) {
         if (tid < HD) st_act<T>(dst + tid, 0.f);
         return;
     }
@@ -603,11 +637,11 @@ __device__ __forceinline__ PaRowBlock pa_row_block(const KvRows& r, int G, int s
     return R;
 }
 // Steps of a row block, and the steps of one of its nsp shares (even: both groups get as many).
-template <int ROWS>
-__device__ __forceinline__ int pa_steps(const PaRowBlock& R, int G, int cap) {
-    if (R.s.pos < 0) return 0;
+template <int ROWS, bool WIN>
+__device__ __forceinline__ PaSpan pa_steps(const PaRowBlock& R, int G, int cap, const PaWindow& w) {
+    if (R.s.pos < 0) return PaSpan{0, 0, 0};
     const int last = min((R.rb * ROWS + ROWS - 1) / G, R.s.n - 1);
-    return ((R.s.pos < cap - last ? R.s.pos + last + 1 : cap) + PA_TILE - 1) / PA_TILE;
+    return pa_span<WIN>(R.s.pos + R.rb * ROWS / G, R.s.pos < cap - last ? R.s.pos + last + 1 : cap, w);
 }
 __device__ __forceinline__ int pa_share_of(int steps, int nsp) {
     return nsp == 1 ? steps : ((steps + nsp - 1) / nsp + 1) / 2 * 2;
@@ -645,10 +679,11 @@ __device__ __forceinline__ void pa_store(T* dst, const floatx16_t (&o)[N], float
 // (ev_row, as pa_weight has it), weights in fp32.
 // Blocks of the least exponent hold zeros, or values below 2^-119 that count as zeros beside larger ones: they alone do
 // not lead here.
-template <typename T, int HD, int GROUPS, int PARTS, int KS, int DT>
+template <typename T, int HD, int GROUPS, bool WIN, int PARTS, int KS, int DT>
 __device__ __forceinline__ void pa_apart(const KvPages& c, const int* table, int max_pages, int h, int first, int z,
-                                         int seg_end, int end, int half, const half8_t (&qb)[PARTS][KS], float c2,
-                                         float& m_run, float& l_run, int& ev_row, floatx16_t (&o)[DT]) {
+                                         const PaSpan& span, int seg_end, int low, int end, int sinks, int half,
+                                         const half8_t (&qb)[PARTS][KS], float c2, float& m_run, float& l_run, int& ev_row,
+                                         floatx16_t (&o)[DT]) {
     const int bl = c.page_log2 - 4;
     m_run = PA_NONE;
     l_run = 0.f;
@@ -657,12 +692,15 @@ __device__ __forceinline__ void pa_apart(const KvPages& c, const int* table, int
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
-    for (int blk = 4 * first; blk < 4 * z && blk * KVP_BLOCK < seg_end;
-         blk += blk % 4 == 3 ? 4 * GROUPS - 3 : 1) {
+    for (int at_step = 4 * first; at_step < 4 * z; at_step += at_step % 4 == 3 ? 4 * GROUPS - 3 : 1) {
+        const int blk = 4 * span.template real<WIN>(at_step >> 2) + (at_step & 3);
+        if (blk * KVP_BLOCK >= seg_end) break;
         const int page = table[min(blk >> bl, max_pages - 1)];
         if ((unsigned)page >= (unsigned)c.n_pages) continue;
         const size_t at = (((size_t)page * c.n_kv + h) << bl) + (blk & ((1 << bl) - 1));
         const int ek = c.k_exp[at], ev = c.v_exp[at], n = end - blk * KVP_BLOCK;  // places that the row sees
+        const uint32_t bits = WIN ? pa_seen(blk * KVP_BLOCK, low, end, sinks) : 0;
+        auto sees = [&](int t) { return WIN ? (bits >> t & 1) != 0 : t < n; };
         const uint8_t* kr = c.k + at * (KVP_BLOCK * HD) + 8 * half;
         const uint8_t* vr = c.v + at * (KVP_BLOCK * HD) + 4 * half * KVP_BLOCK;
         float w[KVP_BLOCK], top = -INFINITY;  // of the block
@@ -686,7 +724,7 @@ __device__ __forceinline__ void pa_apart(const KvPages& c, const int* table, int
                 }
             }
             const pa_u2 u = __builtin_amdgcn_permlane32_swap(__float_as_uint(s), __float_as_uint(s), false, false);
-            w[t] = t < n ? (__uint_as_float(u[0]) + __uint_as_float(u[1])) * kf : -INFINITY;
+            w[t] = sees(t) ? (__uint_as_float(u[0]) + __uint_as_float(u[1])) * kf : -INFINITY;
             top = fmaxf(top, w[t]);
         }
         const float mx = fmaxf(m_run, top);
@@ -697,7 +735,7 @@ __device__ __forceinline__ void pa_apart(const KvPages& c, const int* table, int
         for (int t = 0; t < KVP_BLOCK; ++t) {
             const float x = w[t] - mx;
             l_run += __builtin_amdgcn_exp2f(x + (float)PA_Q_LOG2);
-            w[t] = t < n ? __builtin_amdgcn_exp2f(x + d) : 0.f;
+            w[t] = sees(t) ? __builtin_amdgcn_exp2f(x + d) : 0.f;
         }
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
@@ -718,10 +756,10 @@ __device__ __forceinline__ void pa_apart(const KvPages& c, const int* table, int
 
 // grid (row blocks * n_kv, nsp), the last row blocks (which see most) first, whatever their head: with the heads one after
 // the other some started long ones late (four ragged fp32 prompts 65 -> 53 us).  nsp > 1 with two groups only.
-template <typename T, int HD, int GROUPS>
+template <typename T, int HD, int GROUPS, bool WIN>
 __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, KvRows r, PaPrompt pp,
                                                                    const T* q, T* out,
-                                                                   int n_q, float scale) {
+                                                                   int n_q, float scale, PaWindow win) {
     constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;  // fp16 parts of q
     constexpr int WAVES = 8 / GROUPS, ROWS = 32 * WAVES;  // of a group
     constexpr int KS = HD / 16, DT = HD / 32;              // 16-dim steps of a score, 32-dim tiles
@@ -749,7 +787,8 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
     const PaRowBlock R = pa_row_block<ROWS>(r, G, slot);
     if (R.b < 0) return;
     const KvSeq s = R.s;
-    const int steps = pa_steps<ROWS>(R, G, cap), share = pa_share_of(steps, pp.nsp);
+    const PaSpan span = pa_steps<ROWS, WIN>(R, G, cap, win);
+    const int steps = span.n, share = pa_share_of(steps, pp.nsp);
     const int a = blockIdx.y * share, z = min(steps, a + share), pieces = steps ? (steps + share - 1) / share : 1;
     if (a >= z && !(steps == 0 && blockIdx.y == 0)) return;
     const int* table = r.page_table + (size_t)R.b * r.max_pages;
@@ -766,6 +805,8 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
     const int end = r0 + row < rows ? kvp_len(s.pos + qi, cap) : 0;
     const int seg_end = kvp_len(s.pos + min((R.rb * ROWS + ROWS - 1) / G, s.n - 1), cap);  // of the row block
     const int shortest = r0 + 31 < rows ? kvp_len(s.pos + r0 / G, cap) : 0;  // of the wave
+    const int low = WIN ? max(s.pos + qi + 1 - win.window, 0) : 0;
+    const int lowest = WIN ? max(s.pos + min(r0 + 31, rows - 1) / G + 1 - win.window, 0) : 0;  // of the wave's last row
 
     // Staging: registers, then LDS.  Lane j & 3 knows block j's page and exponents; a wave's pieces lie in one block.
     uint4 stage[NP];
@@ -776,10 +817,14 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
     // the step after the one in which it is asked for.)
     int ek, ev, page;
     bool got;  // block j of the step in the registers is of use
-    auto find = [&](int step) { page = table[min((4 * step + (lane & 3)) >> bl, r.max_pages - 1)]; };
-    auto load = [&](int step) {
+    auto find = [&](int i) {
+        const int step = span.template real<WIN>(i);
+        page = table[min((4 * step + (lane & 3)) >> bl, r.max_pages - 1)];
+    };
+    auto load = [&](int i0) {
+        const int step = span.template real<WIN>(i0);
         const int blk = 4 * step + (lane & 3);
-        const bool used = (step < z) & (blk * KVP_BLOCK < seg_end) & ((unsigned)page < (unsigned)c.n_pages);
+        const bool used = (i0 < z) & (blk * KVP_BLOCK < seg_end) & ((unsigned)page < (unsigned)c.n_pages);
         const size_t i = (((size_t)(used ? page : 0) * c.n_kv + h) << bl) + (blk & ((1 << bl) - 1));
         ek = c.k_exp[i];
         ev = c.v_exp[i];
@@ -790,7 +835,7 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
             stage[u] = ldg_g16((is_v(u) ? c.v : c.k) + at * (KVP_BLOCK * HD) + (first(u) % HD + lane) * 16);
         }
         got = used;
-        find(step + GROUPS);
+        find(i0 + GROUPS);
     };
     find(a + grp);
     // q is asked for while the page number is on its way.  The wave's 32 rows by lanes in 128-byte pieces, which change
@@ -915,7 +960,7 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
     // K row of 32-token tile tt: token with bits 2 and 3 of the lane's row swapped
     const int kt = (row & 0x13) | (row & 4) << 1 | (row & 8) >> 1;
     // `ends`: some of the wave's rows do not see all of the step, or a block of it has no page or NaN in V
-    auto work = [&](const Tile& D, Tile& next, int step, bool ends) {
+    auto work = [&](const Tile& D, Tile& next, int i0, int step, bool ends) {
         const int cur_k = k_ref, cur_v = v_ref, cur_odd = next_odd;
         // Scores: under every four products the next four operands are read and a part of the next step's bytes is turned.
         constexpr int RUN = 4, RUNS = 2 * KS / RUN;
@@ -952,17 +997,19 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
             }
         }
         __builtin_amdgcn_sched_barrier(0);
-        load(step + 2 * GROUPS);
+        load(i0 + 2 * GROUPS);
         // lane: its row's scores of tokens 32 tt + 16 (j / 8) + 8 half + j % 8
         const int live = end - step * PA_TILE - 8 * half;
         if (ends) {
 #pragma unroll
             for (int kb = 0; kb < 4; ++kb) {
                 const int n = cur_odd >> kb & 1 ? 0 : live - 16 * kb;
+                uint32_t bits = 0;
+                if constexpr (WIN) bits = cur_odd >> kb & 1 ? 0 : pa_seen(step * PA_TILE + 16 * kb + 8 * half, low, end, win.sinks);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const int i = 8 * (kb & 1) + j;
-                    sc[kb >> 1][i] = j < n ? sc[kb >> 1][i] : -INFINITY;
+                    sc[kb >> 1][i] = (WIN ? (bits >> j & 1) != 0 : j < n) ? sc[kb >> 1][i] : -INFINITY;
                 }
             }
         }
@@ -991,7 +1038,8 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
         if (cur_odd >> 4) {  // NaN in V: the sums of the rows that see a token of its block
 #pragma unroll
             for (int kb = 0; kb < 4; ++kb)
-                if ((cur_odd >> (4 + kb) & 1) && end - step * PA_TILE > 16 * kb) {
+                if ((cur_odd >> (4 + kb) & 1) && (WIN ? pa_seen(step * PA_TILE + 16 * kb, low, end, win.sinks) != 0
+                                                      : end - step * PA_TILE > 16 * kb)) {
 #pragma unroll
                     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -1059,14 +1107,17 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
     int buf = 0;
     // (A group without a last step, and a wave whose rows end before the block's, go along with everything masked.)
     for (int step = a + grp; step < z + grp; step += GROUPS) {
-        work(S.tiles[grp][buf], S.tiles[grp][buf ^ 1], step, step * PA_TILE + PA_TILE > shortest || next_odd != 0);
+        const int at = span.template real<WIN>(step) * PA_TILE;
+        const bool ends = at + PA_TILE > shortest || (WIN && at < lowest && at + PA_TILE > win.sinks);
+        work(S.tiles[grp][buf], S.tiles[grp][buf ^ 1], step, at / PA_TILE, ends || next_odd != 0);
         __syncthreads();
         buf ^= 1;
     }
 
     int ev_row = o_ref;  // of this lane's row
     if (__any(apart))
-        pa_apart<T, HD, GROUPS>(c, table, r.max_pages, h, a + grp, z, seg_end, end, half, qb, c2, m_run, l_run, ev_row, o);
+        pa_apart<T, HD, GROUPS, WIN>(c, table, r.max_pages, h, a + grp, z, span, seg_end, low, end, win.sinks, half, qb, c2, m_run,
+                                     l_run, ev_row, o);
 
     // ---- results ----
     {
@@ -1124,9 +1175,9 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
 
 // Joins the shares of the row blocks: grid (row blocks, n_kv, HD / 8).  A block takes 32 rows and 32 dims, a wave 8 of
 // them, as the records have them (1024 bytes on end a load); results change places in LDS: 64 or 128 bytes of a row together.
-template <typename T, int HD>
+template <typename T, int HD, bool WIN>
 __global__ __launch_bounds__(256) void attn_pages_prompt_combine_kernel(KvPages c, KvRows r, PaPrompt pp,
-                                                                        T* __restrict__ out, int n_q) {
+                                                                        T* __restrict__ out, int n_q, PaWindow win) {
     constexpr int ROWS = 128;
     const int slot = blockIdx.x, h = blockIdx.y, G = n_q / c.n_kv;
     const PaRowBlock R = pa_row_block<ROWS>(r, G, slot);
@@ -1134,7 +1185,7 @@ __global__ __launch_bounds__(256) void attn_pages_prompt_combine_kernel(KvPages 
     const int lane = threadIdx.x & 63, tile = blockIdx.z & 3, part = (blockIdx.z & ~3) + (threadIdx.x >> 6);
     const int rr = 32 * tile + (lane & 31), rows = R.s.n * G;
     __shared__ __align__(16) float o_sh[32][32 + 4];
-    const int steps = pa_steps<ROWS>(R, G, kvp_capacity(c, r)), share = pa_share_of(steps, pp.nsp);
+    const int steps = pa_steps<ROWS, WIN>(R, G, kvp_capacity(c, r), win).n, share = pa_share_of(steps, pp.nsp);
     if (steps <= share || R.rb * ROWS + 32 * tile >= rows) return;
     const int pieces = (steps + share - 1) / share;
     const size_t rec0 = ((size_t)slot * c.n_kv + h) * pp.nsp;
@@ -1189,11 +1240,17 @@ namespace vte {
 
 static long long pa_up(long long x) { return (x + 15) / 16 * 16; }
 
+// Tiles that `rows` rows of one sequence, one after the other, see at most, with the window of `w` (window 0: none).
+static long long most_tiles(const KvPages& c, const KvRows& r, long long rows, const PaWindow& w) {
+    const long long all = (((long long)r.max_pages << c.page_log2) + PA_TILE - 1) / PA_TILE;
+    if (w.window == 0) return all;
+    return std::min(all, (w.window + rows + PA_TILE - 2) / PA_TILE + 1 + ((long long)w.sinks + PA_TILE - 1) / PA_TILE);
+}
 // Blocks of the few-rows form: two per CU (their registers allow no more), and
-// no more than the table's capacity has shares of four tiles.
-static PaPlan rows_plan(const KvPages& c, const KvRows& r, int hd, int G, void* scratch, long long* bytes) {
+// no more than the table's capacity, or the window, has shares of four tiles.
+static PaPlan rows_plan(const KvPages& c, const KvRows& r, int hd, int G, const PaWindow& w, void* scratch, long long* bytes) {
     const long long segments = (long long)r.batch * c.n_kv;
-    const long long tiles = segments * ((((long long)r.max_pages << c.page_log2) + PA_TILE - 1) / PA_TILE);
+    const long long tiles = segments * most_tiles(c, r, r.max_rows, w);
     PaPlan p;
     p.blocks = (int)std::min<long long>(2 * device_cus(), (tiles + 3) / 4);
     p.ncol = r.max_rows * G;
@@ -1226,12 +1283,12 @@ struct PromptForm {
     PaPrompt p;
     long long bytes;
 };
-static PromptForm prompt_form(const KvPages& c, const KvRows& r, int hd, int G, void* scratch) {
+static PromptForm prompt_form(const KvPages& c, const KvRows& r, int hd, int G, const PaWindow& w, void* scratch) {
     PromptForm f;
     auto blocks = [&](int rows) { return ((long long)r.rows * G + rows - 1) / rows + r.batch - 1; };
     f.groups = blocks(256) * c.n_kv * 4 >= 9 * device_cus() ? 1 : 2;
     f.rbs = blocks(f.groups == 1 ? 256 : 128);
-    const long long steps = (((long long)r.max_pages << c.page_log2) + PA_TILE - 1) / PA_TILE;
+    const long long steps = most_tiles(c, r, std::min(r.max_rows, 128 / G + 2), w);
     const long long most = std::max(std::min(16LL, steps / 2), std::min<long long>(PA_SHARES, steps / 4));
     f.p.nsp = (int)std::max(1LL, std::min(most, device_cus() / (f.rbs * c.n_kv)));
     const long long recs = f.p.nsp == 1 ? 0 : f.rbs * c.n_kv * f.p.nsp;
@@ -1250,45 +1307,60 @@ static PromptForm prompt_form(const KvPages& c, const KvRows& r, int hd, int G, 
 // of up to 8192 18.1 / 34.5, eight of up to 65536 37.0 / 105.)
 static bool rows_form(const KvRows& r, int G) { return r.max_rows * G <= 16; }
 
-long long attn_pages_scratch_bytes(const KvPages& c, const KvRows& r, int hd, int n_q) {
+static long long scratch_bytes(const KvPages& c, const KvRows& r, int hd, int n_q, const PaWindow& w) {
     const int G = n_q / c.n_kv;
-    if (!rows_form(r, G)) return prompt_form(c, r, hd, G, nullptr).bytes;
+    if (!rows_form(r, G)) return prompt_form(c, r, hd, G, w, nullptr).bytes;
     long long n;
-    rows_plan(c, r, hd, G, nullptr, &n);
+    rows_plan(c, r, hd, G, w, nullptr, &n);
     return n;
 }
+long long attn_pages_scratch_bytes(const KvPages& c, const KvRows& r, int hd, int n_q) {
+    return scratch_bytes(c, r, hd, n_q, PaWindow{0, 0});
+}
+long long attn_pages_window_scratch_bytes(const KvPages& c, const KvRows& r, int hd, int n_q, int window, int sinks) {
+    return scratch_bytes(c, r, hd, n_q, PaWindow{window, sinks});
+}
 
-template <typename T, int HD>
+template <typename T, int HD, bool WIN>
 static hipError_t attn_hd(const KvPages& c, const KvRows& r, const void* q, void* out, int n_q, float scale,
-                          void* scratch, hipStream_t st) {
+                          const PaWindow& w, void* scratch, hipStream_t st) {
     const int G = n_q / c.n_kv;
     long long bytes;
     if (rows_form(r, G)) {
-        const PaPlan p = rows_plan(c, r, HD, G, scratch, &bytes);
-        hipLaunchKernelGGL((attn_pages_rows_kernel<T, HD>), dim3(p.blocks), dim3(256), 0, st, c, r, p, (const T*)q,
-                           (T*)out, n_q, scale);
+        const PaPlan p = rows_plan(c, r, HD, G, w, scratch, &bytes);
+        hipLaunchKernelGGL((attn_pages_rows_kernel<T, HD, WIN>), dim3(p.blocks), dim3(256), 0, st, c, r, p, (const T*)q,
+                           (T*)out, n_q, scale, w);
         hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
-        hipLaunchKernelGGL((attn_pages_combine_kernel<T, HD>), dim3(r.batch * c.n_kv, p.ncol), dim3(256), 0, st, c, r,
-                           p, (T*)out, n_q);
+        hipLaunchKernelGGL((attn_pages_combine_kernel<T, HD, WIN>), dim3(r.batch * c.n_kv, p.ncol), dim3(256), 0, st, c, r,
+                           p, (T*)out, n_q, w);
         return hipGetLastError();
     }
-    const PromptForm f = prompt_form(c, r, HD, G, scratch);
-    auto kernel = f.groups == 1 ? attn_pages_prompt_kernel<T, HD, 1> : attn_pages_prompt_kernel<T, HD, 2>;
+    const PromptForm f = prompt_form(c, r, HD, G, w, scratch);
+    auto kernel = f.groups == 1 ? attn_pages_prompt_kernel<T, HD, 1, WIN> : attn_pages_prompt_kernel<T, HD, 2, WIN>;
     hipLaunchKernelGGL(kernel, dim3((unsigned)(f.rbs * c.n_kv), f.p.nsp), dim3(512), 0, st, c, r, f.p, (const T*)q, (T*)out,
-                       n_q, scale);
+                       n_q, scale, w);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || f.p.nsp == 1) return e;
-    hipLaunchKernelGGL((attn_pages_prompt_combine_kernel<T, HD>), dim3((unsigned)f.rbs, c.n_kv, HD / 8),
-                       dim3(256), 0, st, c, r, f.p, (T*)out, n_q);
+    hipLaunchKernelGGL((attn_pages_prompt_combine_kernel<T, HD, WIN>), dim3((unsigned)f.rbs, c.n_kv, HD / 8),
+                       dim3(256), 0, st, c, r, f.p, (T*)out, n_q, w);
     return hipGetLastError();
 }
-hipError_t attn_pages(const KvPages& c, const KvRows& r, int hd, bool f16, const void* q, void* out, int n_q,
-                      float scale, void* scratch, hipStream_t st) {
-#define PA_ATTN(T, HD) attn_hd<T, HD>(c, r, q, out, n_q, scale, scratch, st)
+template <bool WIN>
+static hipError_t attn_any(const KvPages& c, const KvRows& r, int hd, bool f16, const void* q, void* out, int n_q, float scale,
+                           const PaWindow& w, void* scratch, hipStream_t st) {
+#define PA_ATTN(T, HD) attn_hd<T, HD, WIN>(c, r, q, out, n_q, scale, w, scratch, st)
     if (hd == 128) return f16 ? PA_ATTN(__half, 128) : PA_ATTN(float, 128);
     return f16 ? PA_ATTN(__half, 64) : PA_ATTN(float, 64);
 #undef PA_ATTN
+}
+hipError_t attn_pages(const KvPages& c, const KvRows& r, int hd, bool f16, const void* q, void* out, int n_q,
+                      float scale, void* scratch, hipStream_t st) {
+    return attn_any<false>(c, r, hd, f16, q, out, n_q, scale, PaWindow{0, 0}, scratch, st);
+}
+hipError_t attn_pages_window(const KvPages& c, const KvRows& r, int hd, bool f16, const void* q, void* out, int n_q,
+                             float scale, int window, int sinks, void* scratch, hipStream_t st) {
+    return attn_any<true>(c, r, hd, f16, q, out, n_q, scale, PaWindow{window, sinks}, scratch, st);
 }
 
 }  // namespace vte

@@ -13,6 +13,7 @@
 #include "vte_common.h"
 #include "fused_kernels.h"
 #include "decode_persistent.h"
+#include "head_turn.h"
 #include "kv_pages.h"
 #include <algorithm>
 #include <cmath>
@@ -79,6 +80,28 @@ hipError_t kv_pages_read(const KvPages& c, const KvRows& r, int hd, bool f16, vo
 long long attn_pages_scratch_bytes(const KvPages& c, const KvRows& r, int hd, int n_q);
 hipError_t attn_pages(const KvPages& c, const KvRows& r, int hd, bool f16, const void* q, void* out, int n_q,
                       float scale, void* scratch, hipStream_t st);
+long long attn_pages_window_scratch_bytes(const KvPages& c, const KvRows& r, int hd, int n_q, int window, int sinks);
+hipError_t attn_pages_window(const KvPages& c, const KvRows& r, int hd, bool f16, const void* q, void* out, int n_q,
+                             float scale, int window, int sinks, void* scratch, hipStream_t st);
+hipError_t qk_norm_rope(const HeadForm& f, int hd, bool f16, const void* q, void* q_out, int n_q, long long qs,
+                        const void* k, void* k_out, int n_kv, long long ks, int rows, const int* positions,
+                        hipStream_t st);
+hipError_t kv_pages_append_norm(const KvPages& c, const KvRows& r, int hd, bool f16, const HeadForm& f, const void* k,
+                                const void* v, const void* q, void* q_out, int n_q, long long ks, long long vs,
+                                long long qs, hipStream_t st);
+hipError_t kv_pages_copy(const KvPages* layers, int n_layers, int hd, const int* src, const int* dst, int n,
+                         hipStream_t st);
+hipError_t kv_pages_free(const KvTables& t, int n, const int* seqs, int keep, const int* end, int behind,
+                         hipStream_t st);
+int kv_pages_reserve_slots(const KvTables& t, int count);
+hipError_t kv_pages_reserve(const KvTables& t, int n, const int* seqs, const int* start, const int* stop, int count,
+                            int* missing, hipStream_t st);
+long long kv_pages_fork_scratch_bytes(int n);
+hipError_t kv_pages_fork(const KvPages* layers, int n_layers, int hd, const KvTables& t, int n, const int* parents,
+                         const int* children, const int* lengths, int* missing, void* scratch, hipStream_t st);
+long long kv_pages_compact_scratch_bytes(const KvTables& t);
+hipError_t kv_pages_compact(const KvPages* layers, int n_layers, int hd, const KvTables& t, int* where, int* used,
+                            void* scratch, hipStream_t st);
 long long sample_scratch_bytes(int rows);
 hipError_t sample(const float* logits, int rows, int vocab, const float* temperature, const int* top_k,
                   const float* top_p, const float* min_p, const double* u, int* tokens, void* scratch,
@@ -768,6 +791,15 @@ int vte_decode_batch_step(const vte_decode_model* m, void* ws, int batch, long l
 
 // ------------------------------------------------------------------ 8-bit paged KV cache, sampling
 
+static int log2_of(int page_tokens) {
+    int log2 = 4;
+    while ((1 << log2) < page_tokens) ++log2;
+    return log2;
+}
+static KvPages pages_of(const vte_kv_pages* c) {
+    return KvPages{(uint8_t*)c->k, (uint8_t*)c->v, (int8_t*)c->k_exp, (int8_t*)c->v_exp, c->n_pages,
+                   log2_of(c->page_tokens), c->n_kv};
+}
 static int check_pages(const char* who, const vte_kv_pages* c, const vte_kv_rows* r, KvPages* kc, KvRows* kr) {
     REQUIRE(c && r, "%s: null cache or rows", who);
     REQUIRE(c->head_dim == 64 || c->head_dim == 128, "%s: head_dim %d (64 or 128)", who, c->head_dim);
@@ -783,9 +815,7 @@ static int check_pages(const char* who, const vte_kv_pages* c, const vte_kv_rows
             "%s: max_pages %d: a table holds at least 1 page and at most 2^30 tokens", who, r->max_pages);
     REQUIRE(r->row_start || (r->rows == r->batch && r->max_rows == 1) || (r->rows == 0 && r->max_rows == 0),
             "%s: without row_start rows is the batch and max_rows 1 (or both 0)", who);
-    int log2 = 4;
-    while ((1 << log2) < c->page_tokens) ++log2;
-    *kc = KvPages{(uint8_t*)c->k, (uint8_t*)c->v, (int8_t*)c->k_exp, (int8_t*)c->v_exp, c->n_pages, log2, c->n_kv};
+    *kc = pages_of(c);
     *kr = KvRows{r->row_start, r->kv_offset, r->page_table, r->batch, r->rows, r->max_rows, r->max_pages};
     return 0;
 }
@@ -795,6 +825,31 @@ static int check_pages_memory(const char* who, const vte_kv_pages* c, const vte_
     REQUIRE(aligned(r->row_start, 4) && aligned(r->kv_offset, 4) && aligned(r->page_table, 4),
             "%s: 4-byte alignment of the row description", who);
     REQUIRE(dtype == VTE_F32 || dtype == VTE_F16, "%s: dtype must be 0 (f32) or 1 (f16)", who);
+    return 0;
+}
+
+// The rows of an append; the strides they have.
+static int check_append(const char* who, const KvPages& c, const KvRows& r, int hd, int dtype, const void* k, const void* v,
+                        long long k_stride, long long v_stride, const void* q, const void* q_out, int n_q,
+                        long long q_stride, long long* ks, long long* vs, long long* qs) {
+    const size_t size = dtype == VTE_F16 ? 2 : 4;
+    const long long row = (long long)c.n_kv * hd;
+    REQUIRE(r.rows >= 1 && r.max_rows >= 1, "%s: no rows", who);
+    REQUIRE(k && v, "%s: null k or v", who);
+    REQUIRE(aligned(k, size) && aligned(v, size) && aligned(q, size) && aligned(q_out, size),
+            "%s: k, v and q must be aligned to their type", who);
+    *ks = k_stride ? k_stride : row;
+    *vs = v_stride ? v_stride : row;
+    REQUIRE(*ks >= row && *vs >= row && *ks < (1LL << 31) && *vs < (1LL << 31),
+            "%s: k_stride %lld / v_stride %lld below a row of %d x %d", who, k_stride, v_stride, c.n_kv, hd);
+    REQUIRE((q == nullptr) == (q_out == nullptr), "%s: q and q_out go together", who);
+    *qs = q && !q_stride ? (long long)n_q * hd : q_stride;
+    if (q) {
+        REQUIRE(n_q >= 1 && n_q <= 65535 && *qs >= (long long)n_q * hd && *qs < (1LL << 31), "%s: n_q %d, q_stride %lld",
+                who, n_q, q_stride);
+        REQUIRE(q != q_out || *qs == (long long)n_q * hd, "%s: in place q must be contiguous", who);
+        REQUIRE((long long)r.rows * n_q <= (1 << 25), "%s: rows %d x n_q %d above 2^25", who, r.rows, n_q);
+    }
     return 0;
 }
 
@@ -808,24 +863,11 @@ int vte_kv_pages_append(const vte_kv_pages* cache, const vte_kv_rows* rows, int 
     if (!rc) rc = check_pages_memory("kv_pages_append", cache, rows, dtype);
     if (rc) return rc;
     const int hd = cache->head_dim;
-    const size_t size = dtype == VTE_F16 ? 2 : 4;
-    REQUIRE(r.rows >= 1 && r.max_rows >= 1, "kv_pages_append: no rows");
-    REQUIRE(k && v, "kv_pages_append: null k or v");
-    REQUIRE(aligned(k, size) && aligned(v, size) && aligned(q, size) && aligned(q_out, size),
-            "kv_pages_append: k, v and q must be aligned to their type");
-    const long long ks = k_stride ? k_stride : (long long)c.n_kv * hd, vs = v_stride ? v_stride : (long long)c.n_kv * hd;
-    REQUIRE(ks >= (long long)c.n_kv * hd && vs >= (long long)c.n_kv * hd && ks < (1LL << 31) && vs < (1LL << 31),
-            "kv_pages_append: k_stride %lld / v_stride %lld below a row of %d x %d", k_stride, v_stride, c.n_kv, hd);
+    long long ks, vs, qs;
+    rc = check_append("kv_pages_append", c, r, hd, dtype, k, v, k_stride, v_stride, q, q_out, n_q, q_stride, &ks, &vs, &qs);
+    if (rc) return rc;
     REQUIRE((rope_cos == nullptr) == (rope_sin == nullptr), "kv_pages_append: one rotation table of two");
-    REQUIRE((q == nullptr) == (q_out == nullptr), "kv_pages_append: q and q_out go together");
     REQUIRE(!q || rope_cos, "kv_pages_append: q without rotation tables");
-    const long long qs = q && !q_stride ? (long long)n_q * hd : q_stride;
-    if (q) {
-        REQUIRE(n_q >= 1 && n_q <= 65535 && qs >= (long long)n_q * hd && qs < (1LL << 31),
-                "kv_pages_append: n_q %d, q_stride %lld", n_q, q_stride);
-        REQUIRE(q != q_out || qs == (long long)n_q * hd, "kv_pages_append: in place q must be contiguous");
-        REQUIRE((long long)r.rows * n_q <= (1 << 25), "kv_pages_append: rows %d x n_q %d above 2^25", r.rows, n_q);
-    }
     if (rope_cos) {
         REQUIRE(rope_rows >= 1, "kv_pages_append: rope_rows %d", rope_rows);
         REQUIRE(rope_type >= 0 && rope_type <= 2, "kv_pages_append: rope_type %d unknown", rope_type);
@@ -855,21 +897,21 @@ int vte_kv_pages_read(const vte_kv_pages* cache, const vte_kv_rows* rows, int dt
                       "vte_kv_pages_read launch");
 }
 
-static int check_attn_pages(const vte_kv_pages* cache, const vte_kv_rows* rows, int n_q, KvPages* c, KvRows* r) {
-    int rc = check_pages("attn_pages", cache, rows, c, r);
+static int check_attn_pages(const char* who, const vte_kv_pages* cache, const vte_kv_rows* rows, int n_q, KvPages* c, KvRows* r) {
+    int rc = check_pages(who, cache, rows, c, r);
     if (rc) return rc;
     REQUIRE(n_q >= c->n_kv && n_q <= 65535 && n_q % c->n_kv == 0 && n_q / c->n_kv <= 16,
-            "attn_pages: bad head counts %d/%d (groups of at most 16)", n_q, c->n_kv);
-    REQUIRE(r->rows >= 1 && r->max_rows >= 1, "attn_pages: no rows");
-    REQUIRE((long long)r->rows * n_q <= (1 << 25), "attn_pages: rows %d x n_q %d above 2^25", r->rows, n_q);
-    REQUIRE((long long)r->batch * c->n_kv <= (1 << 20), "attn_pages: batch %d x n_kv %d above 2^20", r->batch, c->n_kv);
+            "%s: bad head counts %d/%d (groups of at most 16)", who, n_q, c->n_kv);
+    REQUIRE(r->rows >= 1 && r->max_rows >= 1, "%s: no rows", who);
+    REQUIRE((long long)r->rows * n_q <= (1 << 25), "%s: rows %d x n_q %d above 2^25", who, r->rows, n_q);
+    REQUIRE((long long)r->batch * c->n_kv <= (1 << 20), "%s: batch %d x n_kv %d above 2^20", who, r->batch, c->n_kv);
     return 0;
 }
 
 long long vte_attn_pages_scratch_bytes(const vte_kv_pages* cache, const vte_kv_rows* rows, int n_q) {
     KvPages c;
     KvRows r;
-    if (check_attn_pages(cache, rows, n_q, &c, &r)) return -1;
+    if (check_attn_pages("attn_pages", cache, rows, n_q, &c, &r)) return -1;
     return vte::attn_pages_scratch_bytes(c, r, cache->head_dim, n_q);
 }
 
@@ -877,7 +919,7 @@ int vte_attn_pages(const vte_kv_pages* cache, const vte_kv_rows* rows, int dtype
                    float scale, void* scratch, long long scratch_bytes, void* stream) {
     KvPages c;
     KvRows r;
-    int rc = check_attn_pages(cache, rows, n_q, &c, &r);
+    int rc = check_attn_pages("attn_pages", cache, rows, n_q, &c, &r);
     if (!rc) rc = check_pages_memory("attn_pages", cache, rows, dtype);
     if (rc) return rc;
     REQUIRE(q && out && scratch, "attn_pages: null pointer");
@@ -888,6 +930,220 @@ int vte_attn_pages(const vte_kv_pages* cache, const vte_kv_rows* rows, int dtype
     return hip_status(vte::attn_pages(c, r, cache->head_dim, dtype == VTE_F16, q, out, n_q, scale, scratch,
                                       (hipStream_t)stream),
                       "vte_attn_pages launch");
+}
+
+static int check_window(int window, int sinks) {
+    REQUIRE(window >= 1 && sinks >= 0, "attn_pages_window: window %d below 1 or sinks %d below 0", window, sinks);
+    return 0;
+}
+
+long long vte_attn_pages_window_scratch_bytes(const vte_kv_pages* cache, const vte_kv_rows* rows, int n_q, int window,
+                                              int sinks) {
+    KvPages c;
+    KvRows r;
+    if (check_attn_pages("attn_pages_window", cache, rows, n_q, &c, &r) || check_window(window, sinks)) return -1;
+    return vte::attn_pages_window_scratch_bytes(c, r, cache->head_dim, n_q, window, sinks);
+}
+
+int vte_attn_pages_window(const vte_kv_pages* cache, const vte_kv_rows* rows, int dtype, const void* q, void* out,
+                          int n_q, float scale, int window, int sinks, void* scratch, long long scratch_bytes,
+                          void* stream) {
+    KvPages c;
+    KvRows r;
+    int rc = check_attn_pages("attn_pages_window", cache, rows, n_q, &c, &r);
+    if (!rc) rc = check_pages_memory("attn_pages_window", cache, rows, dtype);
+    if (!rc) rc = check_window(window, sinks);
+    if (rc) return rc;
+    REQUIRE(q && out && scratch, "attn_pages_window: null pointer");
+    REQUIRE(aligned(q, 16) && aligned(out, 16) && aligned(scratch, 16), "attn_pages_window: 16-byte alignment");
+    REQUIRE(scale > 0.f && scale <= 1e6f, "attn_pages_window: scale outside (0, 1e6]");
+    const long long need = vte::attn_pages_window_scratch_bytes(c, r, cache->head_dim, n_q, window, sinks);
+    REQUIRE(scratch_bytes >= need, "attn_pages_window: scratch of %lld bytes, %lld needed", scratch_bytes, need);
+    return hip_status(vte::attn_pages_window(c, r, cache->head_dim, dtype == VTE_F16, q, out, n_q, scale, window, sinks,
+                                             scratch, (hipStream_t)stream),
+                      "vte_attn_pages_window launch");
+}
+
+// ------------------------------------------------------------------ norm and rotation of heads
+
+static int check_form(const char* who, const vte_head_form* f, int hd, HeadForm* out) {
+    REQUIRE(f, "%s: null form", who);
+    REQUIRE(aligned(f->q_norm, 2) && aligned(f->k_norm, 2) && aligned(f->freq, 8),
+            "%s: norms must be 2-byte and frequencies 8-byte aligned", who);
+    REQUIRE(!(f->q_norm || f->k_norm) || (f->eps > 0.f && f->eps <= 1.f), "%s: eps outside (0, 1]", who);
+    const int rot = f->rotary_dim ? f->rotary_dim : hd;
+    if (f->freq) {
+        REQUIRE(rot >= 2 && rot <= hd && rot % 2 == 0, "%s: bad rotary_dim %d", who, f->rotary_dim);
+        REQUIRE(std::isfinite(f->amplitude), "%s: amplitude is not finite", who);
+    }
+    *out = HeadForm{(const __half*)f->q_norm, (const __half*)f->k_norm, f->freq, f->eps, f->amplitude,
+                    f->freq ? rot : 0, f->interleaved != 0};
+    return 0;
+}
+
+int vte_qk_norm_rope(const vte_head_form* form, int dtype, int head_dim, int rows, const int* positions, const void* q,
+                     void* q_out, int n_q, long long q_stride, const void* k, void* k_out, int n_kv, long long k_stride,
+                     void* stream) {
+    REQUIRE(dtype == VTE_F32 || dtype == VTE_F16, "qk_norm_rope: dtype must be 0 (f32) or 1 (f16)");
+    REQUIRE(head_dim == 64 || head_dim == 128 || head_dim == 256, "qk_norm_rope: head_dim %d (64, 128 or 256)", head_dim);
+    HeadForm f;
+    if (int rc = check_form("qk_norm_rope", form, head_dim, &f)) return rc;
+    REQUIRE(rows >= 1 && rows <= (1 << 24), "qk_norm_rope: rows %d outside 1..2^24", rows);
+    REQUIRE((q == nullptr) == (q_out == nullptr) && (k == nullptr) == (k_out == nullptr),
+            "qk_norm_rope: q and q_out, k and k_out go together");
+    REQUIRE(q || k, "qk_norm_rope: neither q nor k");
+    REQUIRE(positions || !f.freq, "qk_norm_rope: a rotation without positions");
+    const size_t size = dtype == VTE_F16 ? 2 : 4;
+    REQUIRE(aligned(q, size) && aligned(q_out, size) && aligned(k, size) && aligned(k_out, size) && aligned(positions, 4),
+            "qk_norm_rope: q, k and positions must be aligned to their type");
+    if (!q) n_q = 0;
+    if (!k) n_kv = 0;
+    const long long qs = q && q_stride ? q_stride : (long long)n_q * head_dim;
+    const long long ks = k && k_stride ? k_stride : (long long)n_kv * head_dim;
+    REQUIRE(!q || (n_q >= 1 && n_q <= 65535 && qs >= (long long)n_q * head_dim && qs < (1LL << 31)),
+            "qk_norm_rope: n_q %d, q_stride %lld", n_q, q_stride);
+    REQUIRE(!k || (n_kv >= 1 && n_kv <= 65535 && ks >= (long long)n_kv * head_dim && ks < (1LL << 31)),
+            "qk_norm_rope: n_kv %d, k_stride %lld", n_kv, k_stride);
+    REQUIRE((long long)rows * (n_q + n_kv) <= (1 << 27), "qk_norm_rope: rows %d x heads %d above 2^27", rows, n_q + n_kv);
+    return hip_status(vte::qk_norm_rope(f, head_dim, dtype == VTE_F16, q, q_out, n_q, qs, k, k_out, n_kv, ks, rows,
+                                        positions, (hipStream_t)stream),
+                      "vte_qk_norm_rope launch");
+}
+
+int vte_kv_pages_append_norm(const vte_kv_pages* cache, const vte_kv_rows* rows, const vte_head_form* form, int dtype,
+                             const void* k, const void* v, long long k_stride, long long v_stride, const void* q,
+                             void* q_out, int n_q, long long q_stride, void* stream) {
+    KvPages c;
+    KvRows r;
+    HeadForm f;
+    long long ks, vs, qs;
+    int rc = check_pages("kv_pages_append_norm", cache, rows, &c, &r);
+    if (!rc) rc = check_pages_memory("kv_pages_append_norm", cache, rows, dtype);
+    if (!rc) rc = check_form("kv_pages_append_norm", form, cache->head_dim, &f);
+    if (!rc)
+        rc = check_append("kv_pages_append_norm", c, r, cache->head_dim, dtype, k, v, k_stride, v_stride, q, q_out, n_q,
+                          q_stride, &ks, &vs, &qs);
+    if (rc) return rc;
+    return hip_status(vte::kv_pages_append_norm(c, r, cache->head_dim, dtype == VTE_F16, f, k, v, q, q_out, n_q, ks, vs,
+                                                qs, (hipStream_t)stream),
+                      "vte_kv_pages_append_norm launch");
+}
+
+// ------------------------------------------------------------------ pages as a pool
+
+static int check_tables(const char* who, const vte_kv_tables* t, int n, KvTables* kt) {
+    REQUIRE(t, "%s: null tables", who);
+    REQUIRE(t->page_table && t->refs && aligned(t->page_table, 4) && aligned(t->refs, 4),
+            "%s: page_table and refs must be there, 4-byte aligned", who);
+    REQUIRE(t->batch >= 1 && t->batch <= 65535, "%s: batch %d outside 1..65535", who, t->batch);
+    REQUIRE(t->n_pages >= 1 && t->n_pages <= (1 << 24), "%s: n_pages %d outside 1..2^24", who, t->n_pages);
+    REQUIRE(t->page_tokens >= 16 && t->page_tokens <= 4096 && (t->page_tokens & (t->page_tokens - 1)) == 0,
+            "%s: page_tokens %d is no power of two in 16..4096", who, t->page_tokens);
+    REQUIRE(t->max_pages >= 1 && (long long)t->max_pages * t->page_tokens <= (1 << 30),
+            "%s: max_pages %d: a table holds at least 1 page and at most 2^30 tokens", who, t->max_pages);
+    REQUIRE(n >= 1 && n <= 65535, "%s: n %d outside 1..65535", who, n);
+    *kt = KvTables{t->page_table, t->refs, t->batch, t->max_pages, t->n_pages, log2_of(t->page_tokens)};
+    return 0;
+}
+// Every layer's pool, of one shape (tables: and of theirs).
+static const int MAX_LAYERS = 512;
+struct Layers {
+    KvPages at[MAX_LAYERS];
+};
+static int check_layers(const char* who, const vte_kv_pages* layers, int n_layers, const vte_kv_tables* t, Layers* out) {
+    REQUIRE(layers && n_layers >= 1 && n_layers <= MAX_LAYERS, "%s: %d layers (1..%d)", who, n_layers, MAX_LAYERS);
+    const vte_kv_pages& a = layers[0];
+    REQUIRE(a.head_dim == 64 || a.head_dim == 128, "%s: head_dim %d (64 or 128)", who, a.head_dim);
+    REQUIRE(a.n_kv >= 1 && a.n_kv <= 65535, "%s: n_kv %d", who, a.n_kv);
+    REQUIRE(a.n_pages >= 1, "%s: n_pages %d", who, a.n_pages);
+    REQUIRE(a.page_tokens >= 16 && a.page_tokens <= 4096 && (a.page_tokens & (a.page_tokens - 1)) == 0,
+            "%s: page_tokens %d is no power of two in 16..4096", who, a.page_tokens);
+    REQUIRE((long long)a.n_kv * a.page_tokens * a.head_dim <= (1 << 30), "%s: pages of more than 2^30 bytes", who);
+    REQUIRE(!t || (t->n_pages == a.n_pages && t->page_tokens == a.page_tokens), "%s: layers and tables differ in their pages", who);
+    for (int i = 0; i < n_layers; ++i) {
+        const vte_kv_pages& c = layers[i];
+        REQUIRE(c.n_pages == a.n_pages && c.page_tokens == a.page_tokens && c.n_kv == a.n_kv && c.head_dim == a.head_dim,
+                "%s: layer %d differs from layer 0", who, i);
+        REQUIRE(c.k && c.v && c.k_exp && c.v_exp && aligned(c.k, 16) && aligned(c.v, 16),
+                "%s: the pages of layer %d must be there, 16-byte aligned", who, i);
+        out->at[i] = pages_of(&c);
+    }
+    return 0;
+}
+
+int vte_kv_pages_copy(const vte_kv_pages* layers, int n_layers, const int* src, const int* dst, int n, void* stream) {
+    Layers L;
+    if (int rc = check_layers("kv_pages_copy", layers, n_layers, nullptr, &L)) return rc;
+    REQUIRE(src && dst && aligned(src, 4) && aligned(dst, 4), "kv_pages_copy: src and dst must be there, 4-byte aligned");
+    REQUIRE(n >= 1 && n <= (1 << 24), "kv_pages_copy: n %d outside 1..2^24", n);
+    return hip_status(vte::kv_pages_copy(L.at, n_layers, layers->head_dim, src, dst, n, (hipStream_t)stream),
+                      "vte_kv_pages_copy launch");
+}
+
+int vte_kv_pages_free(const vte_kv_tables* tables, int n, const int* seqs, int keep, const int* end, int behind,
+                      void* stream) {
+    KvTables t;
+    if (int rc = check_tables("kv_pages_free", tables, n, &t)) return rc;
+    REQUIRE(keep >= 0 && behind >= 0, "kv_pages_free: keep %d, behind %d", keep, behind);
+    REQUIRE(aligned(seqs, 4) && aligned(end, 4), "kv_pages_free: 4-byte alignment");
+    REQUIRE(seqs || n <= t.batch, "kv_pages_free: %d sequences of %d", n, t.batch);
+    return hip_status(vte::kv_pages_free(t, n, seqs, keep, end, behind, (hipStream_t)stream), "vte_kv_pages_free launch");
+}
+
+int vte_kv_pages_reserve(const vte_kv_tables* tables, int n, const int* seqs, const int* start, const int* stop,
+                         int count, int* missing, void* stream) {
+    KvTables t;
+    if (int rc = check_tables("kv_pages_reserve", tables, n, &t)) return rc;
+    REQUIRE(start && aligned(start, 4) && aligned(seqs, 4) && aligned(stop, 4) && aligned(missing, 4),
+            "kv_pages_reserve: start must be there, all 4-byte aligned");
+    REQUIRE(seqs || n <= t.batch, "kv_pages_reserve: %d sequences of %d", n, t.batch);
+    REQUIRE(count >= 1, "kv_pages_reserve: count %d", count);
+    REQUIRE((long long)n * vte::kv_pages_reserve_slots(t, count) <= (1 << 24),
+            "kv_pages_reserve: %d sequences x pages of %d tokens above 2^24", n, count);
+    return hip_status(vte::kv_pages_reserve(t, n, seqs, start, stop, count, missing, (hipStream_t)stream),
+                      "vte_kv_pages_reserve launch");
+}
+
+long long vte_kv_pages_fork_scratch_bytes(int n) { return n >= 1 && n <= 65535 ? vte::kv_pages_fork_scratch_bytes(n) : 0; }
+
+int vte_kv_pages_fork(const vte_kv_pages* layers, int n_layers, const vte_kv_tables* tables, int n, const int* parents,
+                      const int* children, const int* lengths, int* missing, void* scratch, long long scratch_bytes,
+                      void* stream) {
+    KvTables t;
+    Layers L;
+    int rc = check_tables("kv_pages_fork", tables, n, &t);
+    if (!rc) rc = check_layers("kv_pages_fork", layers, n_layers, tables, &L);
+    if (rc) return rc;
+    REQUIRE(parents && children && lengths && aligned(parents, 4) && aligned(children, 4) && aligned(lengths, 4) &&
+                aligned(missing, 4), "kv_pages_fork: parents, children and lengths must be there, 4-byte aligned");
+    REQUIRE(scratch && aligned(scratch, 16) && scratch_bytes >= vte::kv_pages_fork_scratch_bytes(n),
+            "kv_pages_fork: scratch of %lld bytes, %lld needed, 16-byte aligned", scratch_bytes,
+            vte::kv_pages_fork_scratch_bytes(n));
+    return hip_status(vte::kv_pages_fork(L.at, n_layers, layers->head_dim, t, n, parents, children, lengths, missing,
+                                         scratch, (hipStream_t)stream),
+                      "vte_kv_pages_fork launch");
+}
+
+long long vte_kv_pages_compact_scratch_bytes(const vte_kv_tables* tables) {
+    KvTables t;
+    if (check_tables("kv_pages_compact", tables, 1, &t)) return -1;
+    return vte::kv_pages_compact_scratch_bytes(t);
+}
+
+int vte_kv_pages_compact(const vte_kv_pages* layers, int n_layers, const vte_kv_tables* tables, int* where, int* used,
+                         void* scratch, long long scratch_bytes, void* stream) {
+    KvTables t;
+    Layers L;
+    int rc = check_tables("kv_pages_compact", tables, 1, &t);
+    if (!rc) rc = check_layers("kv_pages_compact", layers, n_layers, tables, &L);
+    if (rc) return rc;
+    REQUIRE(where && used && aligned(where, 4) && aligned(used, 4), "kv_pages_compact: where and used must be there, 4-byte aligned");
+    REQUIRE(scratch && aligned(scratch, 16) && scratch_bytes >= vte::kv_pages_compact_scratch_bytes(t),
+            "kv_pages_compact: scratch of %lld bytes, %lld needed, 16-byte aligned", scratch_bytes,
+            vte::kv_pages_compact_scratch_bytes(t));
+    return hip_status(vte::kv_pages_compact(L.at, n_layers, layers->head_dim, t, where, used, scratch,
+                                            (hipStream_t)stream),
+                      "vte_kv_pages_compact launch");
 }
 
 long long vte_sample_scratch_bytes(int rows) { return rows >= 1 ? vte::sample_scratch_bytes(rows) : 0; }

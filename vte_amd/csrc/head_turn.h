@@ -1,0 +1,151 @@
+// Norm of a head and its rotation by position, shared by the kernels that write q
+// and k (qk_norm.hip, the append of kv_pages.hip), gfx950.
+//
+//   y = x w / sqrt(mean(x^2) + eps), then of the first `rot` dims pair i = (a, b)
+//   becomes A (a cos t - b sin t, a sin t + b cos t), t = position * freq[i].
+//
+// No tables: far positions would need long ones, and fp16 ones hold a cosine to
+// 2^-12 only.  The angle is formed in 64 bits (a position of 2^20 times a frequency
+// near 1 leaves 2^-32 of a turn of error; in 32 bits it would be 2^-5), reduced to
+// within half a quarter turn there, and the rest is two short polynomials in fp32.
+#pragma once
+#include "vte_common.h"
+
+struct HeadForm {
+    const __half *q_norm, *k_norm;  // null: not normed
+    const double* freq;             // radians a position; null: no rotation
+    float eps, amplitude;
+    int rot, inter;                 // dims that rotate; whether pairs are neighbours (else half of `rot` apart)
+};
+
+// Eight consecutive elements.
+template <typename T>
+__device__ __forceinline__ void kvp_ld8(const T* p, float (&v)[8]) {
+    if constexpr (sizeof(T) == 2) {
+        const uint4 t = *reinterpret_cast<const uint4*>(p);
+        const uint32_t w[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = h2f_bits(w[i]);
+            v[2 * i + 1] = h2f_bits(w[i] >> 16);
+        }
+    } else {
+        const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    }
+}
+template <typename T>
+__device__ __forceinline__ void kvp_st8(T* p, const float (&v)[8]) {
+    if constexpr (sizeof(T) == 2) {
+        union {
+            __half h[8];
+            uint4 u;
+        } r;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r.h[i] = __float2half(v[i]);
+        *reinterpret_cast<uint4*>(p) = r.u;
+    } else {
+        reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+        reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    }
+}
+
+// amplitude * (cos, sin) of position * freq.  The angle in quarter turns is n + r, |r| <= 1/2; Taylor series of
+// sin(pi/2 r) and cos(pi/2 r) to r^9 and r^10 (what is left out is below 2^-28 of either).
+__device__ __forceinline__ void ht_angle(double position, double freq, float amplitude, float& c, float& s) {
+    double t = position * (freq * 0.15915494309189533577);  // turns
+    t = 4.0 * (t - rint(t));
+    const double n = rint(t);
+    const float r = (float)(t - n), x = r * r;
+    const float sn = r * fmaf(fmaf(fmaf(fmaf(1.60441185e-4f, x, -4.68175414e-3f), x, 7.96926262e-2f), x, -6.45964098e-1f), x,
+                              1.57079633f);
+    const float cs = fmaf(fmaf(fmaf(fmaf(fmaf(-2.52020424e-5f, x, 9.19260274e-4f), x, -2.08634807e-2f), x, 2.53669508e-1f), x,
+                               -1.23370055f), x, 1.f);
+    const int q = (int)n;  // -2 .. 2
+    c = (q & 1 ? sn : cs) * ((q + 1) & 2 ? -amplitude : amplitude);
+    s = (q & 1 ? cs : sn) * (q & 2 ? -amplitude : amplitude);
+}
+__device__ __forceinline__ void ht_turn(float& a, float& b, float c, float s) {
+    const float x = a, y = b;
+    a = fmaf(x, c, -(y * s));
+    b = fmaf(x, s, y * c);
+}
+
+// ---- 16 dims a thread: HD / 16 neighbouring lanes hold a head.  Needs rot % 16 = 0 or neighbouring pairs.
+// The two runs of 8 dims that thread u holds.
+__device__ __forceinline__ void ht_runs(const HeadForm& f, int u, int& d0, int& d1) {
+    if (f.freq != nullptr && !f.inter && 16 * u < f.rot) {
+        d0 = 8 * u;
+        d1 = d0 + f.rot / 2;
+    } else {  // (behind the rotated dims the rest in order)
+        d0 = 16 * u;
+        d1 = d0 + 8;
+    }
+}
+// Sum over N neighbouring lanes (4, 8 or 16).
+template <int N>
+__device__ __forceinline__ float ht_sum(float v) {
+    v += VTE_DPP_F(v, 0xB1);
+    v += VTE_DPP_F(v, 0x4E);
+    if constexpr (N >= 8) v += VTE_DPP_F(v, 0x141);
+    if constexpr (N >= 16) v += VTE_DPP_F(v, 0x140);
+    return v;
+}
+template <int HD>
+__device__ __forceinline__ void ht_norm16(const __half* w, float eps, int d0, int d1, float (&x)[8], float (&y)[8]) {
+    float a[8], b[8], sum = 0.f;
+    kvp_ld8(w + d0, a);
+    kvp_ld8(w + d1, b);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum = fmaf(x[e], x[e], fmaf(y[e], y[e], sum));
+    const float inv = rsqrtf(ht_sum<HD / 16>(sum) * (1.f / HD) + eps);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        x[e] *= inv * a[e];
+        y[e] *= inv * b[e];
+    }
+}
+// cos and sin of the thread's eight pairs (those that do not rotate: 1 and 0).
+__device__ __forceinline__ void ht_angles16(const HeadForm& f, int u, int position, float (&c)[8], float (&s)[8]) {
+    const double p = (double)position;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        c[e] = 1.f;
+        s[e] = 0.f;
+        if (8 * u + e < f.rot / 2) ht_angle(p, f.freq[8 * u + e], f.amplitude, c[e], s[e]);
+    }
+}
+// (Pairs that do not rotate are left alone: times 0 an infinite neighbour would make NaN of them.)
+__device__ __forceinline__ void ht_turn16(const HeadForm& f, int u, const float (&c)[8], const float (&s)[8], float (&x)[8],
+                                          float (&y)[8]) {
+    const int n = f.rot / 2 - 8 * u;  // pairs from here on rotate
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        if (e >= n) continue;
+        if (!f.inter) ht_turn(x[e], y[e], c[e], s[e]);
+        else if (e < 4) ht_turn(x[2 * e], x[2 * e + 1], c[e], s[e]);  // pairs lie side by side
+        else ht_turn(y[2 * e - 8], y[2 * e - 7], c[e], s[e]);
+    }
+}
+
+// ---- one pair a thread: any rotation.
+// Dims of pair i of a head, and whether it rotates.
+__device__ __forceinline__ bool ht_pair(const HeadForm& f, int i, int& d0, int& d1) {
+    const bool turns = f.freq != nullptr && i < f.rot / 2;
+    if (turns && !f.inter) {
+        d0 = i;
+        d1 = i + f.rot / 2;
+    } else {
+        d0 = 2 * i;
+        d1 = 2 * i + 1;
+    }
+    return turns;
+}
+// Sum over N neighbouring lanes (32 or 64).
+template <int N>
+__device__ __forceinline__ float ht_sum_lanes(float v) {
+#pragma unroll
+    for (int d = 1; d < N; d <<= 1) v += __shfl_xor(v, d, 64);
+    return v;
+}

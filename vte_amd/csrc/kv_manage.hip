@@ -1,0 +1,424 @@
+// The pages of a paged KV cache as a pool that sequences share: copies, pages given back, room for new tokens, forks
+// and compaction, gfx950.  No counterpart in the reference, whose sequences own a fixed range each
+// (vte/compiler/qwen_mapper.py:300-351).
+//
+// refs[p] is the number of users of page p (table entries, and whatever else the program counts); 0: free.  One table and
+// one refs array serve the pools of all layers: only copies touch bytes.  New pages are always the lowest free ones, in
+// the order of the call's list, so what a call does depends on its inputs alone and not on which block came first; users
+// are counted by integer atomics, whose order does not matter.  Entries are exchanged, not written, and what stood there
+// loses a user: a sequence listed twice costs no page.
+#include <algorithm>
+#include "kv_pages.h"
+
+#define KVM_LAYERS 64    // of a copy launch: 2 KB of arguments
+#define KVM_CHUNK 1024   // pages a block counts
+#define KVM_PIECE 1024   // 16-byte words that a block copies
+
+struct KvLayers {
+    uint8_t *k[KVM_LAYERS], *v[KVM_LAYERS];
+    int8_t *k_exp[KVM_LAYERS], *v_exp[KVM_LAYERS];
+};
+
+__device__ __forceinline__ bool kvm_is_page(const KvTables& t, int p) { return (unsigned)p < (unsigned)t.n_pages; }
+// One user less (not below none, whatever the count was).
+__device__ __forceinline__ void kvm_release(const KvTables& t, int p) {
+    if (!kvm_is_page(t, p)) return;
+    if (atomicSub(&t.refs[p], 1) <= 0) atomicAdd(&t.refs[p], 1);
+}
+// Entry j of a row becomes p, whose user it already counts as.
+__device__ __forceinline__ void kvm_set(const KvTables& t, int row, int j, int p) {
+    kvm_release(t, atomicExch(&t.table[(size_t)row * t.max_pages + j], p));
+}
+
+// ---------------------------------------------------------------------------
+// Copies: pages src[i] -> dst[i] of every layer, i < n (n_dev: read on the device); pairs of which one is no page are
+// skipped.  An item is KVM_PIECE words of K then V of one pair and layer, its first one takes the exponents along.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ void kvm_copy(const KvLayers& L, int n_layers, int layer_words, int exps, int n_pages,
+                                         const int* src, const int* dst, int n) {
+    const int words = 2 * layer_words;  // 16-byte words of a page, K and V
+    const int pieces = (words + KVM_PIECE - 1) / KVM_PIECE;
+    const long long items = (long long)n * n_layers * pieces;
+    for (long long it = blockIdx.x; it < items; it += gridDim.x) {
+        const int piece = (int)(it % pieces), i = (int)(it / pieces / n_layers), l = (int)(it / pieces % n_layers);
+        const int a = src[i], b = dst[i];
+        if ((unsigned)a >= (unsigned)n_pages || (unsigned)b >= (unsigned)n_pages) continue;
+        uint4 x[KVM_PIECE / 256];
+#pragma unroll
+        for (int u = 0; u < KVM_PIECE / 256; ++u) {
+            const int w = piece * KVM_PIECE + u * 256 + threadIdx.x;
+            if (w < words) x[u] = ldg_g16(w < layer_words ? L.k[l] + ((size_t)a * layer_words + w) * 16
+                                                          : L.v[l] + ((size_t)a * layer_words + w - layer_words) * 16);
+        }
+#pragma unroll
+        for (int u = 0; u < KVM_PIECE / 256; ++u) {
+            const int w = piece * KVM_PIECE + u * 256 + threadIdx.x;
+            if (w < words) *reinterpret_cast<uint4*>(w < layer_words ? L.k[l] + ((size_t)b * layer_words + w) * 16
+                                                                     : L.v[l] + ((size_t)b * layer_words + w - layer_words) * 16) = x[u];
+        }
+        if (piece == 0)
+            for (int e = threadIdx.x; e < exps; e += 256) {
+                L.k_exp[l][(size_t)b * exps + e] = L.k_exp[l][(size_t)a * exps + e];
+                L.v_exp[l][(size_t)b * exps + e] = L.v_exp[l][(size_t)a * exps + e];
+            }
+    }
+}
+__global__ __launch_bounds__(256) void kv_copy_kernel(KvLayers L, int n_layers, int layer_words, int exps, int n_pages,
+                                                      const int* __restrict__ src, const int* __restrict__ dst, int n) {
+    kvm_copy(L, n_layers, layer_words, exps, n_pages, src, dst, n);
+}
+
+// ---------------------------------------------------------------------------
+// Pages given back: entries of whole pages of tokens keep .. end[i] - behind - 1.  grid (entries, sequences).
+// ---------------------------------------------------------------------------
+__global__ __launch_bounds__(256) void kv_free_kernel(KvTables t, const int* __restrict__ seqs, int keep,
+                                                      const int* __restrict__ end, int behind) {
+    const int row = seqs != nullptr ? seqs[blockIdx.y] : (int)blockIdx.y;
+    if ((unsigned)row >= (unsigned)t.batch) return;
+    const int j = blockIdx.x * 256 + threadIdx.x;
+    const int low = (int)(((long long)keep + (1 << t.page_log2) - 1) >> t.page_log2);
+    int high = t.max_pages;
+    if (end != nullptr) high = min(high, end[blockIdx.y] < 0 ? 0 : max(end[blockIdx.y] - behind, 0) >> t.page_log2);
+    if (j < low || j >= high) return;
+    if (t.table[(size_t)row * t.max_pages + j] != -1) kvm_set(t, row, j, -1);
+}
+
+// ---------------------------------------------------------------------------
+// New pages, by one block of 1024 threads.  `want(slot)` says whether a slot of 0 .. slots - 1 needs one, `give(slot, rank,
+// page)` takes it (page -1: there are no more).  The result: slots that got none.
+// Free pages are found 4096 at a time into a ring in LDS, only when a slot needs them.
+// ---------------------------------------------------------------------------
+#define KVM_RING 8192
+template <class Want, class Give>
+__device__ __forceinline__ int kvm_new_pages(const KvTables& t, int slots, Want want, Give give) {
+    __shared__ int ring[KVM_RING];
+    __shared__ int sums[16];
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+    auto scan = [&](int v, int& total) {  // the sum before this thread's, and of all
+        int incl = v;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int o = __shfl_up(incl, d, 64);
+            incl += lane >= d ? o : 0;
+        }
+        __syncthreads();
+        if (lane == 63) sums[wv] = incl;
+        __syncthreads();
+        int before = 0;
+        total = 0;
+#pragma unroll
+        for (int w = 0; w < 16; ++w) {
+            before += w < wv ? sums[w] : 0;
+            total += sums[w];
+        }
+        return before + incl - v;
+    };
+    int head = 0, have = 0, next = 0, missing = 0, done = 0;  // of the ring; the first page not looked at; slots served
+    for (int s0 = 0; s0 < slots; s0 += 1024) {
+        const bool w = s0 + tid < slots && want(s0 + tid);
+        int n;
+        const int rank = scan(w, n);
+        while (have < n && next < t.n_pages) {
+            int r[4], count = 0;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int p = next + 4 * tid + u;
+                r[u] = p < t.n_pages && t.refs[p] <= 0;
+                count += r[u];
+            }
+            int found;
+            int at = head + have + scan(count, found);
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (r[u]) ring[at++ & (KVM_RING - 1)] = next + 4 * tid + u;
+            have += found;
+            next += 4096;
+        }
+        __syncthreads();
+        if (w) {
+            const int page = rank < have ? ring[(head + rank) & (KVM_RING - 1)] : -1;
+            if (page >= 0) {
+                atomicExch(&t.refs[page], 1);
+                __threadfence_block();  // (before the entry that shows it to others, which may release it)
+            }
+            give(s0 + tid, done + rank, page);
+        }
+        const int got = min(n, have);
+        head += got;
+        have -= got;
+        missing += n - got;
+        done += n;
+        __syncthreads();
+    }
+    return missing;
+}
+
+// Entries of tokens start[i] .. start[i] + count - 1 (below stop[i]) of each sequence; `per` slots a sequence.
+__global__ __launch_bounds__(1024) void kv_reserve_kernel(KvTables t, int n, const int* __restrict__ seqs,
+                                                          const int* __restrict__ start, const int* __restrict__ stop,
+                                                          int count, int per, int* missing) {
+    auto entry = [&](int slot, int& row, int& j) {
+        const int i = slot / per;
+        row = seqs != nullptr ? seqs[i] : i;
+        if ((unsigned)row >= (unsigned)t.batch || start[i] < 0) return false;
+        long long end = min((long long)start[i] + count, (long long)t.max_pages << t.page_log2);
+        if (stop != nullptr) end = min(end, (long long)stop[i]);
+        const long long at = (start[i] >> t.page_log2) + (long long)(slot - i * per);
+        j = (int)at;
+        return at << t.page_log2 < end && end > start[i];
+    };
+    const int short_of = kvm_new_pages(
+        t, n * per,
+        [&](int slot) {
+            int row, j;
+            return entry(slot, row, j) && !kvm_is_page(t, t.table[(size_t)row * t.max_pages + j]);
+        },
+        [&](int slot, int, int page) {
+            int row, j;
+            if (page >= 0 && entry(slot, row, j)) kvm_set(t, row, j, page);
+        });
+    if (missing != nullptr && threadIdx.x == 0) *missing = short_of;
+}
+
+// ---------------------------------------------------------------------------
+// Forks.  First the whole pages of a parent's first tokens are shared with the child, whose own go (grid (entries,
+// children)); then one block finds a page for each child whose last page is begun, and lists what is to be copied.
+// A child that is its own parent stays as it is.
+// ---------------------------------------------------------------------------
+struct KvFork {
+    const int *parents, *children, *lengths;
+    int n;
+};
+__device__ __forceinline__ bool kvm_fork(const KvTables& t, const KvFork& f, int i, int& parent, int& child, int& length) {
+    parent = f.parents[i];
+    child = f.children[i];
+    length = f.lengths[i];
+    return (unsigned)parent < (unsigned)t.batch && (unsigned)child < (unsigned)t.batch && parent != child && length >= 0;
+}
+__global__ __launch_bounds__(256) void kv_fork_kernel(KvTables t, KvFork f) {
+    const int j = blockIdx.x * 256 + threadIdx.x;
+    int parent, child, length;
+    if (!kvm_fork(t, f, blockIdx.y, parent, child, length) || j >= t.max_pages) return;
+    int p = -1;
+    if (j < length >> t.page_log2) {
+        p = t.table[(size_t)parent * t.max_pages + j];
+        if (kvm_is_page(t, p)) atomicAdd(&t.refs[p], 1);
+        else p = -1;
+    }
+    kvm_set(t, child, j, p);
+}
+__global__ __launch_bounds__(1024) void kv_fork_last_kernel(KvTables t, KvFork f, int* src, int* dst, int* missing) {
+    auto begun = [&](int i, int& child, int& j, int& page) {
+        int parent, length;
+        if (!kvm_fork(t, f, i, parent, child, length)) return false;
+        j = length >> t.page_log2;
+        if ((length & ((1 << t.page_log2) - 1)) == 0 || j >= t.max_pages) return false;
+        page = t.table[(size_t)parent * t.max_pages + j];
+        return kvm_is_page(t, page);
+    };
+    for (int i = threadIdx.x; i < f.n; i += 1024) src[i] = dst[i] = -1;
+    __syncthreads();
+    const int short_of = kvm_new_pages(
+        t, f.n,
+        [&](int i) {
+            int child, j, page;
+            return begun(i, child, j, page);
+        },
+        [&](int i, int rank, int to) {
+            int child, j, page;
+            if (to < 0) return;
+            if (!begun(i, child, j, page)) {  // (a parent that is a child as well and lost it just now)
+                kvm_release(t, to);
+                return;
+            }
+            src[i] = page;
+            dst[i] = to;
+            kvm_set(t, child, j, to);
+        });
+    if (missing != nullptr && threadIdx.x == 0) *missing = short_of;
+}
+
+// ---------------------------------------------------------------------------
+// Compaction: with U used pages, the k-th used page from U on moves to the k-th free one below U.  Counts per chunk; then
+// every block knows U and what lies before its chunk, lists its pages' places and writes where each page goes, those
+// that move as -2 - k until the copies' launch, which knows the lists.
+// ---------------------------------------------------------------------------
+struct KvMoves {
+    int *counts, *src, *dst, *moves;  // used pages of each chunk; pairs; how many
+};
+__global__ __launch_bounds__(256) void kv_count_kernel(KvTables t, int* __restrict__ counts) {
+    __shared__ int sums[4];
+    int n = 0;
+    for (int u = 0; u < KVM_CHUNK / 256; ++u) {
+        const int p = blockIdx.x * KVM_CHUNK + u * 256 + threadIdx.x;
+        n += __popcll(__ballot(p < t.n_pages && t.refs[p] > 0));
+    }
+    if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = n;
+    __syncthreads();
+    if (threadIdx.x == 0) counts[blockIdx.x] = sums[0] + sums[1] + sums[2] + sums[3];
+}
+__global__ __launch_bounds__(256) void kv_place_kernel(KvTables t, KvMoves m, int chunks, int* __restrict__ where,
+                                                       int* __restrict__ used) {
+    __shared__ int sums[3][4];
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+    auto all = [&](int row, int v) {  // the block's sum
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d, 64);
+        if (lane == 0) sums[row][wv] = v;
+        __syncthreads();
+        return sums[row][0] + sums[row][1] + sums[row][2] + sums[row][3];
+    };
+    int v = 0;
+    for (int c = tid; c < chunks; c += 256) v += m.counts[c];
+    const int U = all(0, v), cut = U / KVM_CHUNK;  // (U is in chunk `cut`, which may be one behind the last)
+    v = 0;
+    for (int c = tid; c < chunks; c += 256) v += c < cut ? m.counts[c] : 0;
+    for (int p = cut * KVM_CHUNK + tid; p < U; p += 256) v += t.refs[p] > 0;
+    const int below = all(1, v);  // used pages below U
+    v = 0;
+    for (int c = tid; c < (int)blockIdx.x; c += 256) v += m.counts[c];
+    int before = all(2, v);       // used pages before the chunk
+    if (blockIdx.x == 0 && tid == 0) {
+        *used = U;
+        *m.moves = U - below;
+    }
+    __shared__ int row_sums[4][4];
+    uint64_t bits[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        const int p = blockIdx.x * KVM_CHUNK + u * 256 + tid;
+        bits[u] = __ballot(p < t.n_pages && t.refs[p] > 0);
+        if (lane == 0) row_sums[u][wv] = __popcll(bits[u]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        const int p = blockIdx.x * KVM_CHUNK + u * 256 + tid;
+        int n = before + __popcll(bits[u] & ((1ull << lane) - 1));  // used pages before p
+        for (int w = 0; w < 4; ++w) {
+            n += w < wv ? row_sums[u][w] : 0;
+            before += row_sums[u][w];
+        }
+        if (p >= t.n_pages) continue;
+        const bool mine = bits[u] >> lane & 1;
+        if (mine && p >= U) {
+            m.src[n - below] = p;
+            where[p] = -2 - (n - below);
+        } else {
+            if (!mine && p < U) m.dst[p - n] = p;
+            where[p] = mine ? p : -1;
+        }
+    }
+}
+// (first: the launch that also rewrites tables, counts and `where`)
+__global__ __launch_bounds__(256) void kv_move_kernel(KvLayers L, int n_layers, int layer_words, int exps, KvTables t, KvMoves m,
+                                                      int* where, bool first) {
+    const int n = *m.moves;
+    if (first) {
+        const long long step = (long long)gridDim.x * 256, at = (long long)blockIdx.x * 256 + threadIdx.x;
+        for (long long e = at; e < (long long)t.batch * t.max_pages; e += step) {
+            const int p = t.table[e];
+            if (!kvm_is_page(t, p)) continue;
+            const int w = where[p];  // (-2 - k, or already the place that stands for)
+            t.table[e] = w <= -2 ? m.dst[-2 - w] : w;
+        }
+        for (long long k = at; k < n; k += step) {
+            const int a = m.src[k], b = m.dst[k];
+            where[a] = b;
+            t.refs[b] = t.refs[a];
+            t.refs[a] = 0;
+        }
+    }
+    kvm_copy(L, n_layers, layer_words, exps, t.n_pages, m.src, m.dst, n);
+}
+
+// ---------------------------------------------------------------------------
+// Host launchers
+// ---------------------------------------------------------------------------
+namespace vte {
+
+static KvLayers layers_of(const KvPages* layers, int n) {
+    KvLayers L = {};
+    for (int i = 0; i < n; ++i) {
+        L.k[i] = layers[i].k;
+        L.v[i] = layers[i].v;
+        L.k_exp[i] = layers[i].k_exp;
+        L.v_exp[i] = layers[i].v_exp;
+    }
+    return L;
+}
+struct CopyShape {
+    int words, exps, pieces;
+};
+static CopyShape copy_shape(const KvPages& c, int hd) {
+    CopyShape s;
+    s.words = (int)((((long long)c.n_kv << c.page_log2) * hd) / 16);
+    s.exps = c.n_kv << (c.page_log2 - 4);
+    s.pieces = (2 * s.words + KVM_PIECE - 1) / KVM_PIECE;
+    return s;
+}
+static unsigned copy_blocks(long long items) { return (unsigned)std::max(1LL, std::min<long long>(items, 16 * device_cus())); }
+
+hipError_t kv_pages_copy(const KvPages* layers, int n_layers, int hd, const int* src, const int* dst, int n, hipStream_t st) {
+    const CopyShape s = copy_shape(layers[0], hd);
+    for (int l = 0; l < n_layers; l += KVM_LAYERS) {
+        const int m = std::min(KVM_LAYERS, n_layers - l);
+        hipLaunchKernelGGL(kv_copy_kernel, dim3(copy_blocks((long long)n * m * s.pieces)), dim3(256), 0, st,
+                           layers_of(layers + l, m), m, s.words, s.exps, layers[0].n_pages, src, dst, n);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+hipError_t kv_pages_free(const KvTables& t, int n, const int* seqs, int keep, const int* end, int behind, hipStream_t st) {
+    hipLaunchKernelGGL(kv_free_kernel, dim3((t.max_pages + 255) / 256, n), dim3(256), 0, st, t, seqs, keep, end, behind);
+    return hipGetLastError();
+}
+// Slots of a sequence: pages that `count` tokens touch at most.
+int kv_pages_reserve_slots(const KvTables& t, int count) {
+    return (int)std::min<long long>(t.max_pages, ((long long)count - 1 >> t.page_log2) + 2);
+}
+hipError_t kv_pages_reserve(const KvTables& t, int n, const int* seqs, const int* start, const int* stop, int count,
+                            int* missing, hipStream_t st) {
+    hipLaunchKernelGGL(kv_reserve_kernel, dim3(1), dim3(1024), 0, st, t, n, seqs, start, stop, count,
+                       kv_pages_reserve_slots(t, count), missing);
+    return hipGetLastError();
+}
+long long kv_pages_fork_scratch_bytes(int n) { return 8LL * n; }
+hipError_t kv_pages_fork(const KvPages* layers, int n_layers, int hd, const KvTables& t, int n, const int* parents,
+                         const int* children, const int* lengths, int* missing, void* scratch, hipStream_t st) {
+    const KvFork f{parents, children, lengths, n};
+    int* src = static_cast<int*>(scratch);
+    hipLaunchKernelGGL(kv_fork_kernel, dim3((t.max_pages + 255) / 256, n), dim3(256), 0, st, t, f);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(kv_fork_last_kernel, dim3(1), dim3(1024), 0, st, t, f, src, src + n, missing);
+    e = hipGetLastError();
+    return e != hipSuccess ? e : kv_pages_copy(layers, n_layers, hd, src, src + n, n, st);
+}
+static int chunks_of(const KvTables& t) { return (t.n_pages + KVM_CHUNK - 1) / KVM_CHUNK; }
+long long kv_pages_compact_scratch_bytes(const KvTables& t) { return 4LL * (4 + chunks_of(t) + 2LL * t.n_pages); }
+hipError_t kv_pages_compact(const KvPages* layers, int n_layers, int hd, const KvTables& t, int* where, int* used, void* scratch,
+                            hipStream_t st) {
+    KvMoves m;
+    m.moves = static_cast<int*>(scratch);
+    m.counts = m.moves + 4;
+    m.src = m.counts + chunks_of(t);
+    m.dst = m.src + t.n_pages;
+    hipLaunchKernelGGL(kv_count_kernel, dim3(chunks_of(t)), dim3(256), 0, st, t, m.counts);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(kv_place_kernel, dim3(chunks_of(t)), dim3(256), 0, st, t, m, chunks_of(t), where, used);
+    e = hipGetLastError();
+    const CopyShape s = copy_shape(layers[0], hd);
+    for (int l = 0; l < n_layers && e == hipSuccess; l += KVM_LAYERS) {
+        const int n = std::min(KVM_LAYERS, n_layers - l);
+        const long long items = std::max((long long)(t.n_pages / 2) * n * s.pieces, (long long)t.batch * t.max_pages / 256 + 1);
+        hipLaunchKernelGGL(kv_move_kernel, dim3(copy_blocks(items)), dim3(256), 0, st, layers_of(layers + l, n), n, s.words,
+                           s.exps, t, m, where, l == 0);
+        e = hipGetLastError();
+    }
+    return e;
+}
+
+}  // namespace vte

@@ -26,6 +26,11 @@ struct KvPages {
     int8_t *k_exp, *v_exp;
     int n_pages, page_log2, n_kv;
 };
+// Page tables of all sequences, and the number of users of each page (0: free).
+struct KvTables {
+    int *table, *refs;
+    int batch, max_pages, n_pages, page_log2;
+};
 struct KvRows {
     const int *row_start, *kv_offset, *page_table;
     int batch, rows, max_rows, max_pages;

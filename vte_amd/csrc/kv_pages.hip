@@ -2,6 +2,8 @@
 // No counterpart in the reference, whose cache is one fp16 range per sequence
 // (vte/compiler/templates/rdna/kv_cache_append.hip.template:13-39).
 #include <algorithm>
+#include <type_traits>
+#include "head_turn.h"
 #include "kv_pages.h"
 
 // ---------------------------------------------------------------------------
@@ -57,39 +59,6 @@ __device__ __forceinline__ void kvp_rotate(float& a, float& b, float c, float s)
     b = xs + yc;
 }
 
-// Eight consecutive elements.
-template <typename T>
-__device__ __forceinline__ void kvp_ld8(const T* p, float (&v)[8]) {
-    if constexpr (sizeof(T) == 2) {
-        const uint4 t = *reinterpret_cast<const uint4*>(p);
-        const uint32_t w[4] = {t.x, t.y, t.z, t.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[2 * i] = h2f_bits(w[i]);
-            v[2 * i + 1] = h2f_bits(w[i] >> 16);
-        }
-    } else {
-        const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    }
-}
-template <typename T>
-__device__ __forceinline__ void kvp_st8(T* p, const float (&v)[8]) {
-    if constexpr (sizeof(T) == 2) {
-        union {
-            __half h[8];
-            uint4 u;
-        } r;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) r.h[i] = __float2half(v[i]);
-        *reinterpret_cast<uint4*>(p) = r.u;
-    } else {
-        reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-        reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-    }
-}
-
 // Eight bytes to the left of a grown scale: rounded shifts of the whole numbers.
 __device__ __forceinline__ uint32_t kvp_shift4(uint32_t w, float f) {
     uint32_t r = 0;
@@ -107,17 +76,22 @@ __device__ __forceinline__ uint2 kvp_code8(const float (&v)[8], float inv) {
     return r;
 }
 
-template <typename T, int HD, bool WIDE>
-__global__ __launch_bounds__(WIDE ? 2 * HD : 128) void kv_pages_append_kernel(KvPages c, KvRows r, KvRope rp, const T* __restrict__ k,
+template <typename T, int HD, bool WIDE, class R>
+__global__ __launch_bounds__(WIDE ? 2 * HD : 128) void kv_pages_append_kernel(KvPages c, KvRows r, R rp, const T* __restrict__ k,
                                                               const T* __restrict__ v, const T* q, T* q_out, int n_q,
                                                               long long k_stride, long long v_stride,
                                                               long long q_stride, int seq_blocks) {
+    constexpr bool NORM = std::is_same<R, HeadForm>::value;  // heads normed, rotated by frequencies; else by tables
     constexpr int NP = HD / 2;           // pairs of a head
     constexpr int TOK = KVP_BLOCK * NP / 64;  // tokens a lane holds
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
     const int cap = kvp_capacity(c, r);
-    const int limit = rp.cosc != nullptr ? min(cap, rp.rows) : cap;  // positions from here on are dropped
-    const int tab = rp.type == 2 ? rp.dim : HD;                      // row of a table
+    int limit = cap;  // positions from here on are dropped
+    int tab = HD;     // row of a table
+    if constexpr (!NORM) {
+        if (rp.cosc != nullptr) limit = min(cap, rp.rows);
+        if (rp.type == 2) tab = rp.dim;
+    }
 
     if ((int)blockIdx.x >= seq_blocks) {  // q: one pair a thread, or eight
         constexpr int NU = WIDE ? NP / 8 : NP;
@@ -135,7 +109,37 @@ __global__ __launch_bounds__(WIDE ? 2 * HD : 128) void kv_pages_append_kernel(Kv
         const int pos = s.pos + at;
         const T* src = q + row * q_stride + h * HD;
         T* dst = q_out + ((size_t)row * n_q + h) * HD;
-        if constexpr (WIDE) {
+        if constexpr (NORM && WIDE) {
+            int d0, d1;
+            ht_runs(rp, i, d0, d1);
+            float x[8], y[8];
+            kvp_ld8(src + d0, x);
+            kvp_ld8(src + d1, y);
+            if (rp.q_norm != nullptr) ht_norm16<HD>(rp.q_norm, rp.eps, d0, d1, x, y);
+            if (rp.freq != nullptr) {
+                float c8[8], s8[8];
+                ht_angles16(rp, i, pos, c8, s8);
+                ht_turn16(rp, i, c8, s8, x, y);
+            }
+            kvp_st8(dst + d0, x);
+            kvp_st8(dst + d1, y);
+        } else if constexpr (NORM) {
+            int d0, d1;
+            const bool turns = ht_pair(rp, i, d0, d1);
+            float x = ld_act<T>(src + d0), y = ld_act<T>(src + d1);
+            if (rp.q_norm != nullptr) {
+                const float inv = rsqrtf(ht_sum_lanes<NP>(fmaf(x, x, y * y)) * (1.f / HD) + rp.eps);
+                x *= inv * h2f(rp.q_norm[d0]);
+                y *= inv * h2f(rp.q_norm[d1]);
+            }
+            if (turns) {
+                float c1, s1;
+                ht_angle((double)pos, rp.freq[i], rp.amplitude, c1, s1);
+                ht_turn(x, y, c1, s1);
+            }
+            st_act<T>(dst + d0, x);
+            st_act<T>(dst + d1, y);
+        } else if constexpr (WIDE) {
             const int d0 = rp.type == 1 ? 16 * i : 8 * i, d1 = rp.type == 1 ? 16 * i + 8 : 8 * i + NP;
             float x[8], y[8], c8[8], s8[8];
             kvp_ld8(src + d0, x);
@@ -187,7 +191,13 @@ __global__ __launch_bounds__(WIDE ? 2 * HD : 128) void kv_pages_append_kernel(Kv
         __shared__ __align__(16) uint8_t turned[HD][KVP_BLOCK];  // V: a dim's tokens together
         const int id = threadIdx.x % HD, i = id % (HD / 16), p = id / (HD / 16);  // unit of 16 dims, place
         const bool in = p >= j0 && p < j1, old = p < j0;
-        const int d0 = is_v || rp.type == 1 ? 16 * i : 8 * i, d1 = is_v || rp.type == 1 ? 16 * i + 8 : 8 * i + NP;
+        int d0 = 16 * i, d1 = 16 * i + 8;
+        if constexpr (NORM) {
+            if (!is_v) ht_runs(rp, i, d0, d1);
+        } else if (!is_v && rp.type != 1) {
+            d0 = 8 * i;
+            d1 = 8 * i + NP;
+        }
         float x[8], y[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = y[e] = 0.f;
@@ -196,7 +206,16 @@ __global__ __launch_bounds__(WIDE ? 2 * HD : 128) void kv_pages_append_kernel(Kv
                            h * HD;
             kvp_ld8(src + d0, x);
             kvp_ld8(src + d1, y);
-            if (!is_v && rp.cosc != nullptr) {
+            if constexpr (NORM) {
+                if (!is_v) {
+                    if (rp.k_norm != nullptr) ht_norm16<HD>(rp.k_norm, rp.eps, d0, d1, x, y);
+                    if (rp.freq != nullptr) {
+                        float c8[8], s8[8];
+                        ht_angles16(rp, i, t0 + p, c8, s8);
+                        ht_turn16(rp, i, c8, s8, x, y);
+                    }
+                }
+            } else if (!is_v && rp.cosc != nullptr) {
                 float c8[8], s8[8];
                 kvp_ld8(rp.cosc + (size_t)(t0 + p) * HD + 8 * i, c8);
                 kvp_ld8(rp.sinc + (size_t)(t0 + p) * HD + 8 * i, s8);
@@ -290,7 +309,9 @@ __global__ __launch_bounds__(WIDE ? 2 * HD : 128) void kv_pages_append_kernel(Kv
 
     const int i = lane & (NP - 1), jb = (lane / NP) * TOK;  // pair, first place
     int d0, d1;
-    const bool turns = kvp_pair<HD>(i, rp, d0, d1) && !is_v && rp.cosc != nullptr;
+    bool turns;
+    if constexpr (NORM) turns = ht_pair(rp, i, d0, d1) && !is_v;
+    else turns = kvp_pair<HD>(i, rp, d0, d1) && !is_v && rp.cosc != nullptr;
     const T* src = (is_v ? v : k) + (long long)(s.first + t0 - s.pos) * (is_v ? v_stride : k_stride) + h * HD;
     const long long stride = is_v ? v_stride : k_stride;
     float x[TOK], y[TOK];
@@ -306,7 +327,18 @@ __global__ __launch_bounds__(WIDE ? 2 * HD : 128) void kv_pages_append_kernel(Kv
 #pragma unroll
     for (int j = 0; j < TOK; ++j) {
         const int p = jb + j;
-        if (turns && p >= j0 && p < j1) {
+        if constexpr (NORM) {
+            if (!is_v && rp.k_norm != nullptr) {
+                const float inv = rsqrtf(ht_sum_lanes<NP>(fmaf(x[j], x[j], y[j] * y[j])) * (1.f / HD) + rp.eps);
+                x[j] *= inv * h2f(rp.k_norm[d0]);
+                y[j] *= inv * h2f(rp.k_norm[d1]);
+            }
+            if (turns && p >= j0 && p < j1) {
+                float c1, s1;
+                ht_angle((double)(t0 + p), rp.freq[i], rp.amplitude, c1, s1);
+                ht_turn(x[j], y[j], c1, s1);
+            }
+        } else if (turns && p >= j0 && p < j1) {
             const size_t row = (size_t)(t0 + p) * tab + i;
             kvp_rotate(x[j], y[j], h2f(rp.cosc[row]), h2f(rp.sinc[row]));
         }
@@ -414,35 +446,50 @@ __global__ __launch_bounds__(256) void kv_pages_read_kernel(KvPages c, KvRows r,
 // ---------------------------------------------------------------------------
 namespace vte {
 
-template <typename T, int HD>
-static hipError_t append_hd(const KvPages& c, const KvRows& r, const KvRope& rp, const void* k, const void* v,
+static bool fits16(const void* p, long long bytes) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && bytes % 16 == 0; }
+static bool rope_fits(const KvRope& rp) {
+    return rp.cosc == nullptr || (rp.type != 2 && fits16(rp.cosc, 0) && fits16(rp.sinc, 0));
+}
+static bool rope_fits(const HeadForm& f) {
+    return fits16(f.q_norm, 0) && fits16(f.k_norm, 0) && (f.freq == nullptr || f.inter || f.rot % 16 == 0);
+}
+template <typename T, int HD, class R>
+static hipError_t append_hd(const KvPages& c, const KvRows& r, const R& rp, const void* k, const void* v,
                             const void* q, void* q_out, int n_q, long long ks, long long vs, long long qs,
                             hipStream_t st) {
     // a run of max_rows tokens touches at most this many blocks of 16
     const int seq_blocks = r.max_rows == 1 ? 1 : (r.max_rows + KVP_BLOCK - 1) / KVP_BLOCK + 1;
     const long long grid_yz = (long long)c.n_kv * r.batch;
-    auto fits = [](const void* p, long long stride) {
-        return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride * (long long)sizeof(T) % 16 == 0;
-    };
-    const bool wide = (rp.cosc == nullptr || (rp.type != 2 && fits(rp.cosc, 0) && fits(rp.sinc, 0))) && fits(k, ks) &&
-                      fits(v, vs) && (!q || (fits(q, qs) && fits(q_out, 0)));
+    const long long size = sizeof(T);
+    const bool wide = rope_fits(rp) && fits16(k, ks * size) && fits16(v, vs * size) &&
+                      (!q || (fits16(q, qs * size) && fits16(q_out, 0)));
     const int nt = wide ? 2 * HD : 128;
     const long long q_blocks = q ? ((long long)r.rows * n_q * (HD / (wide ? 16 : 2)) + nt - 1) / nt : 0;
     const int qx = (int)((q_blocks + grid_yz - 1) / grid_yz);
-    auto kernel = wide ? kv_pages_append_kernel<T, HD, true> : kv_pages_append_kernel<T, HD, false>;
+    auto kernel = wide ? kv_pages_append_kernel<T, HD, true, R> : kv_pages_append_kernel<T, HD, false, R>;
     hipLaunchKernelGGL(kernel, dim3(seq_blocks + qx, c.n_kv, r.batch), dim3(nt), 0, st, c, r,
                        rp, (const T*)k, (const T*)v, (const T*)q, (T*)q_out, n_q, ks, vs, qs, seq_blocks);
     return hipGetLastError();
+}
+template <class R>
+static hipError_t append_any(const KvPages& c, const KvRows& r, int hd, bool f16, const R& rp, const void* k, const void* v,
+                             const void* q, void* q_out, int n_q, long long ks, long long vs, long long qs, hipStream_t st) {
+#define KVP_APPEND(T, HD) append_hd<T, HD, R>(c, r, rp, k, v, q, q_out, n_q, ks, vs, qs, st)
+    if (hd == 128) return f16 ? KVP_APPEND(__half, 128) : KVP_APPEND(float, 128);
+    return f16 ? KVP_APPEND(__half, 64) : KVP_APPEND(float, 64);
+#undef KVP_APPEND
 }
 hipError_t kv_pages_append(const KvPages& c, const KvRows& r, int hd, bool f16, const void* k, const void* v,
                            const void* q, void* q_out, int n_q, long long ks, long long vs, long long qs,
                            const void* cosc, const void* sinc, int rope_rows, int rope_type, int rotary_dim,
                            hipStream_t st) {
-    const KvRope rp{(const __half*)cosc, (const __half*)sinc, rope_rows, rope_type, rotary_dim};
-#define KVP_APPEND(T, HD) append_hd<T, HD>(c, r, rp, k, v, q, q_out, n_q, ks, vs, qs, st)
-    if (hd == 128) return f16 ? KVP_APPEND(__half, 128) : KVP_APPEND(float, 128);
-    return f16 ? KVP_APPEND(__half, 64) : KVP_APPEND(float, 64);
-#undef KVP_APPEND
+    return append_any(c, r, hd, f16, KvRope{(const __half*)cosc, (const __half*)sinc, rope_rows, rope_type, rotary_dim}, k, v, q,
+                      q_out, n_q, ks, vs, qs, st);
+}
+hipError_t kv_pages_append_norm(const KvPages& c, const KvRows& r, int hd, bool f16, const HeadForm& f, const void* k,
+                                const void* v, const void* q, void* q_out, int n_q, long long ks, long long vs, long long qs,
+                                hipStream_t st) {
+    return append_any(c, r, hd, f16, f, k, v, q, q_out, n_q, ks, vs, qs, st);
 }
 
 template <typename T, int HD>

@@ -1,0 +1,127 @@
+// Queries and keys normed head by head and rotated by their positions (head_turn.h), gfx950.
+// The reference has the two steps apart, for heads that are not normed:
+// vte/compiler/templates/rdna/rope.hip.template:17-137.
+#include "head_turn.h"
+
+// q and k of one call: rows of heads.
+template <typename T>
+struct QkRows {
+    const T* x;
+    T* y;
+    int heads;
+    long long in, out;  // elements between rows
+};
+
+// A thread takes 16 dims of a head, HD / 16 threads a head; q heads of a row, then its k heads.
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void qk_norm_rope_kernel(HeadForm f, QkRows<T> q, QkRows<T> k, int rows,
+                                                           const int* __restrict__ positions) {
+    constexpr int NU = HD / 16;
+    const int per_row = (q.heads + k.heads) * NU;
+    const long long gid = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (gid >= (long long)rows * per_row) return;
+    const int row = (int)(gid / per_row), hu = (int)(gid - (long long)row * per_row), u = hu % NU;
+    const int pos = positions != nullptr ? positions[row] : 0;
+    if (pos < 0) return;
+    const bool is_q = hu / NU < q.heads;
+    const int h = is_q ? hu / NU : hu / NU - q.heads;
+    const QkRows<T>& r = is_q ? q : k;
+    const T* src = r.x + row * r.in + h * HD;
+    T* dst = r.y + row * r.out + h * HD;
+    int d0, d1;
+    ht_runs(f, u, d0, d1);
+    float x[8], y[8];
+    kvp_ld8(src + d0, x);
+    kvp_ld8(src + d1, y);
+    const __half* w = is_q ? f.q_norm : f.k_norm;
+    if (w != nullptr) ht_norm16<HD>(w, f.eps, d0, d1, x, y);
+    if (f.freq != nullptr) {
+        float c[8], s[8];
+        ht_angles16(f, u, pos, c, s);
+        ht_turn16(f, u, c, s, x, y);
+    }
+    kvp_st8(dst + d0, x);
+    kvp_st8(dst + d1, y);
+}
+
+// Any alignment and rotation: a wave takes a head, a lane one pair of dims (heads of 256: two).
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void qk_norm_rope_pairs_kernel(HeadForm f, QkRows<T> q, QkRows<T> k, int rows,
+                                                                 const int* __restrict__ positions) {
+    constexpr int NP = HD / 2, EACH = NP > 64 ? NP / 64 : 1;
+    const int heads = q.heads + k.heads, lane = threadIdx.x & 63;
+    const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (item >= (long long)rows * heads) return;
+    const int row = (int)(item / heads), hh = (int)(item - (long long)row * heads);
+    const int pos = positions != nullptr ? positions[row] : 0;
+    if (pos < 0) return;
+    const bool is_q = hh < q.heads;
+    const int h = is_q ? hh : hh - q.heads;
+    const QkRows<T>& r = is_q ? q : k;
+    const T* src = r.x + row * r.in + h * HD;
+    T* dst = r.y + row * r.out + h * HD;
+    const __half* w = is_q ? f.q_norm : f.k_norm;
+    float a[EACH], b[EACH], sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+        a[e] = b[e] = 0.f;
+        if (lane < NP) {
+            int d0, d1;
+            ht_pair(f, lane + 64 * e, d0, d1);
+            a[e] = ld_act<T>(src + d0);
+            b[e] = ld_act<T>(src + d1);
+        }
+        sum = fmaf(a[e], a[e], fmaf(b[e], b[e], sum));
+    }
+    sum = wave_sum(sum);
+    const float inv = rsqrtf(sum * (1.f / HD) + f.eps);
+    if (lane >= NP) return;
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+        int d0, d1;
+        const bool turns = ht_pair(f, lane + 64 * e, d0, d1);
+        if (w != nullptr) {
+            a[e] *= inv * h2f(w[d0]);
+            b[e] *= inv * h2f(w[d1]);
+        }
+        if (turns) {
+            float c, s;
+            ht_angle((double)pos, f.freq[lane + 64 * e], f.amplitude, c, s);
+            ht_turn(a[e], b[e], c, s);
+        }
+        st_act<T>(dst + d0, a[e]);
+        st_act<T>(dst + d1, b[e]);
+    }
+}
+
+namespace vte {
+
+template <typename T, int HD>
+static hipError_t norm_hd(const HeadForm& f, const void* q, void* q_out, int n_q, long long qs, const void* k, void* k_out,
+                          int n_kv, long long ks, int rows, const int* positions, hipStream_t st) {
+    const QkRows<T> Q{(const T*)q, (T*)q_out, n_q, qs, q == q_out ? qs : (long long)n_q * HD};
+    const QkRows<T> K{(const T*)k, (T*)k_out, n_kv, ks, k == k_out ? ks : (long long)n_kv * HD};
+    auto fits = [](const void* p, long long stride) {
+        return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride * (long long)sizeof(T) % 16 == 0;
+    };
+    const bool wide = fits(q, qs) && fits(q_out, 0) && fits(k, ks) && fits(k_out, 0) && fits(f.q_norm, 0) &&
+                      fits(f.k_norm, 0) && (f.freq == nullptr || f.inter || f.rot % 16 == 0);
+    const long long items = (long long)rows * (n_q + n_kv);
+    if (wide)
+        hipLaunchKernelGGL((qk_norm_rope_kernel<T, HD>), dim3((unsigned)((items * (HD / 16) + 255) / 256)), dim3(256), 0, st,
+                           f, Q, K, rows, positions);
+    else
+        hipLaunchKernelGGL((qk_norm_rope_pairs_kernel<T, HD>), dim3((unsigned)((items + 3) / 4)), dim3(256), 0, st, f, Q, K,
+                           rows, positions);
+    return hipGetLastError();
+}
+hipError_t qk_norm_rope(const HeadForm& f, int hd, bool f16, const void* q, void* q_out, int n_q, long long qs, const void* k,
+                        void* k_out, int n_kv, long long ks, int rows, const int* positions, hipStream_t st) {
+#define QK_NORM(T, HD) norm_hd<T, HD>(f, q, q_out, n_q, qs, k, k_out, n_kv, ks, rows, positions, st)
+    if (hd == 64) return f16 ? QK_NORM(__half, 64) : QK_NORM(float, 64);
+    if (hd == 128) return f16 ? QK_NORM(__half, 128) : QK_NORM(float, 128);
+    return f16 ? QK_NORM(__half, 256) : QK_NORM(float, 256);
+#undef QK_NORM
+}
+
+}  // namespace vte

@@ -63,13 +63,25 @@ SIGNATURES = {
     "vte_kv_pages_read": [_vp, _vp, _i, _vp, _vp, _i, _vp],
     "vte_attn_pages_scratch_bytes": [_vp, _vp, _i],
     "vte_attn_pages": [_vp, _vp, _i, _vp, _vp, _i, _f, _vp, _ll, _vp],
+    "vte_attn_pages_window_scratch_bytes": [_vp, _vp, _i, _i, _i],
+    "vte_attn_pages_window": [_vp, _vp, _i, _vp, _vp, _i, _f, _i, _i, _vp, _ll, _vp],
+    "vte_qk_norm_rope": [_vp, _i, _i, _i, _vp, _vp, _vp, _i, _ll, _vp, _vp, _i, _ll, _vp],
+    "vte_kv_pages_append_norm": [_vp, _vp, _vp, _i, _vp, _vp, _ll, _ll, _vp, _vp, _i, _ll, _vp],
+    "vte_kv_pages_copy": [_vp, _i, _vp, _vp, _i, _vp],
+    "vte_kv_pages_free": [_vp, _i, _vp, _i, _vp, _i, _vp],
+    "vte_kv_pages_reserve": [_vp, _i, _vp, _vp, _vp, _i, _vp, _vp],
+    "vte_kv_pages_fork_scratch_bytes": [_i],
+    "vte_kv_pages_fork": [_vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _ll, _vp],
+    "vte_kv_pages_compact_scratch_bytes": [_vp],
+    "vte_kv_pages_compact": [_vp, _i, _vp, _vp, _vp, _vp, _ll, _vp],
     "vte_sample_scratch_bytes": [_i],
     "vte_sample": [_vp, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
     "vte_last_error": [],
 }
 RESTYPES = {"vte_last_error": ctypes.c_char_p, "vte_attn_scratch_floats": _ll, "vte_topk_scratch_bytes": _ll,
             "vte_decode_workspace_bytes": _ll, "vte_decode_batch_workspace_bytes": _ll, "vte_attn_pages_scratch_bytes": _ll,
-            "vte_sample_scratch_bytes": _ll}
+            "vte_attn_pages_window_scratch_bytes": _ll, "vte_kv_pages_fork_scratch_bytes": _ll,
+            "vte_kv_pages_compact_scratch_bytes": _ll, "vte_sample_scratch_bytes": _ll}
 
 
 class DecodeLayer(ctypes.Structure):
@@ -106,6 +118,28 @@ class KVRows(ctypes.Structure):
     def of(cls, batch: int, rows: int, max_rows: int, row_start, kv_offset, page_table, max_pages: int) -> "KVRows":
         """From device pointers; ``row_start`` None: one row per sequence, or none (rows = max_rows = 0)."""
         return cls(batch, rows, max_rows, max_pages, _p(row_start), _p(kv_offset), _p(page_table))
+
+
+class KVTables(ctypes.Structure):
+    """vte_kv_tables (include/vte_amd.h): the sequences' page tables and every page's number of users."""
+    _fields_ = [(n, _vp) for n in ("page_table", "refs")] + [(n, _i) for n in ("batch", "max_pages", "n_pages", "page_tokens")]
+
+    @classmethod
+    def of(cls, page_table, refs, batch: int, max_pages: int, n_pages: int, page_tokens: int) -> "KVTables":
+        """From device pointers (ints or objects with ``.ptr``)."""
+        return cls(_p(page_table), _p(refs), batch, max_pages, n_pages, page_tokens)
+
+
+class HeadForm(ctypes.Structure):
+    """vte_head_form (include/vte_amd.h): how a model's q and k heads are normed and rotated."""
+    _fields_ = [(n, _vp) for n in ("q_norm", "k_norm", "freq")] + [("eps", _f), ("amplitude", _f)] + \
+               [(n, _i) for n in ("rotary_dim", "interleaved")]
+
+    @classmethod
+    def of(cls, freq=None, rotary_dim: int = 0, interleaved: bool = False, amplitude: float = 1.0, q_norm=None,
+           k_norm=None, eps: float = 1e-6) -> "HeadForm":
+        """From device pointers: ``freq`` float64 (``rope_frequencies`` makes them; None: no rotation), norms fp16."""
+        return cls(_p(q_norm), _p(k_norm), _p(freq), eps, amplitude, rotary_dim, int(interleaved))
 
 
 def _p(x) -> Optional[int]:
@@ -336,6 +370,72 @@ class VTEKernels:
         """Attention of the new rows (decoded tokens, prompt chunks) over the 8-bit paged cache."""
         self._check(self.lib.vte_attn_pages(ctypes.byref(pages), ctypes.byref(rows), DT[dtype], _p(q), _p(out), n_q,
                                             scale, _p(scratch), scratch_bytes, self._st(stream)), "vte_attn_pages")
+
+    def attn_pages_window_scratch_bytes(self, pages: KVPages, rows: KVRows, n_q: int, window: int, sinks: int) -> int:
+        n = int(self.lib.vte_attn_pages_window_scratch_bytes(ctypes.byref(pages), ctypes.byref(rows), n_q, window, sinks))
+        if n < 0:
+            self._check(-1, "vte_attn_pages_window_scratch_bytes")
+        return n
+
+    def attn_pages_window(self, pages: KVPages, rows: KVRows, q, out, n_q: int, scale: float, window: int, sinks: int,
+                          scratch, scratch_bytes: int, dtype="f16", stream=None) -> None:
+        """As ``attn_pages``, of rows that see the last ``window`` tokens (themselves among them) and the first ``sinks``."""
+        self._check(self.lib.vte_attn_pages_window(ctypes.byref(pages), ctypes.byref(rows), DT[dtype], _p(q), _p(out), n_q,
+                                                   scale, window, sinks, _p(scratch), scratch_bytes, self._st(stream)),
+                    "vte_attn_pages_window")
+
+    def qk_norm_rope(self, form: HeadForm, rows: int, positions, q=None, q_out=None, n_q=0, k=None, k_out=None, n_kv=0,
+                     head_dim=128, dtype="f16", q_stride=0, k_stride=0, stream=None) -> None:
+        """q_out, k_out = the rows' q and k heads normed and rotated by ``positions`` (device int [rows])."""
+        self._check(self.lib.vte_qk_norm_rope(ctypes.byref(form), DT[dtype], head_dim, rows, _p(positions), _p(q), _p(q_out),
+                                              n_q, q_stride, _p(k), _p(k_out), n_kv, k_stride, self._st(stream)),
+                    "vte_qk_norm_rope")
+
+    def kv_pages_append_norm(self, pages: KVPages, rows: KVRows, form: HeadForm, k, v, q=None, q_out=None, n_q=0,
+                             dtype="f16", k_stride=0, v_stride=0, q_stride=0, stream=None) -> None:
+        """As ``kv_pages_append``, with k and q normed and rotated as ``form`` says."""
+        self._check(self.lib.vte_kv_pages_append_norm(ctypes.byref(pages), ctypes.byref(rows), ctypes.byref(form), DT[dtype],
+                                                      _p(k), _p(v), k_stride, v_stride, _p(q), _p(q_out), n_q, q_stride,
+                                                      self._st(stream)), "vte_kv_pages_append_norm")
+
+    def kv_pages_copy(self, layers, src, dst, n: int, stream=None) -> None:
+        """Pages src[i] -> dst[i] (device ints) of every layer; ``layers``: a ctypes array of KVPages."""
+        self._check(self.lib.vte_kv_pages_copy(layers, len(layers), _p(src), _p(dst), n, self._st(stream)),
+                    "vte_kv_pages_copy")
+
+    def kv_pages_free(self, tables: KVTables, n: int, seqs=None, keep=0, end=None, behind=0, stream=None) -> None:
+        """Give back the pages of sequences seqs[i] (None: 0 .. n - 1) that hold only tokens keep .. end[i] - behind - 1
+        (``end`` None: all from ``keep`` on)."""
+        self._check(self.lib.vte_kv_pages_free(ctypes.byref(tables), n, _p(seqs), keep, _p(end), behind, self._st(stream)),
+                    "vte_kv_pages_free")
+
+    def kv_pages_reserve(self, tables: KVTables, n: int, start, count: int, missing=None, seqs=None, stop=None,
+                         stream=None) -> None:
+        """A page wherever sequences seqs[i] have none for tokens start[i] .. start[i] + count - 1 (below stop[i] if given);
+        missing[0] = pages that there were not."""
+        self._check(self.lib.vte_kv_pages_reserve(ctypes.byref(tables), n, _p(seqs), _p(start), _p(stop), count, _p(missing),
+                                                  self._st(stream)), "vte_kv_pages_reserve")
+
+    def kv_pages_fork_scratch_bytes(self, n: int) -> int:
+        return int(self.lib.vte_kv_pages_fork_scratch_bytes(n))
+
+    def kv_pages_fork(self, layers, tables: KVTables, n: int, parents, children, lengths, missing, scratch,
+                      scratch_bytes: int, stream=None) -> None:
+        """children[i] becomes the first lengths[i] tokens of parents[i]: whole pages shared, the begun one copied."""
+        self._check(self.lib.vte_kv_pages_fork(layers, len(layers), ctypes.byref(tables), n, _p(parents), _p(children),
+                                               _p(lengths), _p(missing), _p(scratch), scratch_bytes, self._st(stream)),
+                    "vte_kv_pages_fork")
+
+    def kv_pages_compact_scratch_bytes(self, tables: KVTables) -> int:
+        n = int(self.lib.vte_kv_pages_compact_scratch_bytes(ctypes.byref(tables)))
+        if n < 0:
+            self._check(-1, "vte_kv_pages_compact_scratch_bytes")
+        return n
+
+    def kv_pages_compact(self, layers, tables: KVTables, where, used, scratch, scratch_bytes: int, stream=None) -> None:
+        """The used pages become the pool's first ones; where[p] = the place page p went to (-1: free), used[0] = how many."""
+        self._check(self.lib.vte_kv_pages_compact(layers, len(layers), ctypes.byref(tables), _p(where), _p(used),
+                                                  _p(scratch), scratch_bytes, self._st(stream)), "vte_kv_pages_compact")
 
     def sample_scratch_bytes(self, rows: int) -> int:
         """For calls of at most ``rows`` rows."""
