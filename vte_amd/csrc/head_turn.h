@@ -106,26 +106,34 @@ __device__ __forceinline__ void ht_norm16(const __half* w, float eps, int d0, in
         y[e] *= inv * b[e];
     }
 }
-// cos and sin of the thread's eight pairs (those that do not rotate: 1 and 0).
-__device__ __forceinline__ void ht_angles16(const HeadForm& f, int u, int position, float (&c)[8], float (&s)[8]) {
-    const double p = (double)position;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        c[e] = 1.f;
-        s[e] = 0.f;
-        if (8 * u + e < f.rot / 2) ht_angle(p, f.freq[8 * u + e], f.amplitude, c[e], s[e]);
+// Cosines and sines of a block's rows, once for all their heads: turn[row][pair], rows at positions pos(row).  (By each
+// thread for its own eight pairs they cost as much time as the bytes: see the kernels.)
+template <int NT, int NP, class Pos>
+__device__ __forceinline__ void ht_fill(const HeadForm& f, float2 (*turn)[NP], int rows, Pos pos) {
+    const int pairs = f.rot / 2;
+    for (int i = threadIdx.x; i < rows * pairs; i += NT) {
+        const int r = i / pairs, p = i - r * pairs;
+        float2 t;
+        ht_angle((double)pos(r), f.freq[p], f.amplitude, t.x, t.y);
+        turn[r][p] = t;
     }
 }
+// A barrier for what stands in LDS only: loads from memory stay under way.
+__device__ __forceinline__ void ht_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
 // (Pairs that do not rotate are left alone: times 0 an infinite neighbour would make NaN of them.)
-__device__ __forceinline__ void ht_turn16(const HeadForm& f, int u, const float (&c)[8], const float (&s)[8], float (&x)[8],
-                                          float (&y)[8]) {
+__device__ __forceinline__ void ht_turn16(const HeadForm& f, int u, const float2* turn, float (&x)[8], float (&y)[8]) {
     const int n = f.rot / 2 - 8 * u;  // pairs from here on rotate
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         if (e >= n) continue;
-        if (!f.inter) ht_turn(x[e], y[e], c[e], s[e]);
-        else if (e < 4) ht_turn(x[2 * e], x[2 * e + 1], c[e], s[e]);  // pairs lie side by side
-        else ht_turn(y[2 * e - 8], y[2 * e - 7], c[e], s[e]);
+        const float2 t = turn[8 * u + e];
+        if (!f.inter) ht_turn(x[e], y[e], t.x, t.y);
+        else if (e < 4) ht_turn(x[2 * e], x[2 * e + 1], t.x, t.y);  // pairs lie side by side
+        else ht_turn(y[2 * e - 8], y[2 * e - 7], t.x, t.y);
     }
 }
 

@@ -93,6 +93,52 @@ __global__ __launch_bounds__(WIDE ? 2 * HD : 128) void kv_pages_append_kernel(Kv
         if (rp.type == 2) tab = rp.dim;
     }
 
+    // Of NORM && WIDE: cosines and sines of a block's rows, for all their heads.
+    constexpr bool TURN = NORM && WIDE;
+    constexpr int NT = WIDE ? 2 * HD : 128, ROWS = TURN ? 2 * HD / (HD / 16) : 1;
+    __shared__ __align__(16) float2 turn[ROWS][TURN ? NP : 1];
+    if constexpr (TURN) {
+        if ((int)blockIdx.x >= seq_blocks) {  // q: 16 dims a thread
+            constexpr int NU = HD / 16;
+            __shared__ int pos_sh[ROWS];
+            const int tid = threadIdx.x, u = tid % NU;
+            const long long first = ((long long)(blockIdx.x - seq_blocks) + (long long)(gridDim.x - seq_blocks) *
+                                     (blockIdx.y + (long long)gridDim.y * blockIdx.z)) * ROWS;
+            const long long all = (long long)r.rows * n_q, item = first + tid / NU;
+            if (first >= all) return;
+            const int row0 = (int)(first / n_q), row_n = (int)((min(first + ROWS, all) - 1) / n_q) - row0 + 1;
+            const bool in = item < all;
+            const int row = (int)((in ? item : first) / n_q), h = (int)((in ? item : first) - (long long)row * n_q);
+            const T* src = q + row * q_stride + h * HD;
+            T* dst = q_out + ((size_t)row * n_q + h) * HD;
+            int d0, d1;
+            ht_runs(rp, u, d0, d1);
+            float x[8], y[8];
+            kvp_ld8(src + d0, x);
+            kvp_ld8(src + d1, y);
+            if (tid < row_n) {
+                const int b = kvp_row_seq(r, row0 + tid);
+                int pos = -1;  // (a row of nobody, or without a place)
+                if (b >= 0) {
+                    const KvSeq s = kvp_seq(r, b);
+                    const int at = row0 + tid - s.first;
+                    if (at >= 0 && at < s.n && s.pos < limit - at) pos = s.pos + at;
+                }
+                pos_sh[tid] = pos;
+            }
+            ht_barrier();
+            if (rp.freq != nullptr) {
+                ht_fill<NT, NP>(rp, turn, row_n, [&](int i) { return pos_sh[i]; });
+                ht_barrier();
+            }
+            if (!in || pos_sh[row - row0] < 0) return;
+            if (rp.q_norm != nullptr) ht_norm16<HD>(rp.q_norm, rp.eps, d0, d1, x, y);
+            if (rp.freq != nullptr) ht_turn16(rp, u, turn[row - row0], x, y);
+            kvp_st8(dst + d0, x);
+            kvp_st8(dst + d1, y);
+            return;
+        }
+    }
     if ((int)blockIdx.x >= seq_blocks) {  // q: one pair a thread, or eight
         constexpr int NU = WIDE ? NP / 8 : NP;
         const int per_row = n_q * NU;
@@ -109,21 +155,7 @@ __global__ __launch_bounds__(WIDE ? 2 * HD : 128) void kv_pages_append_kernel(Kv
         const int pos = s.pos + at;
         const T* src = q + row * q_stride + h * HD;
         T* dst = q_out + ((size_t)row * n_q + h) * HD;
-        if constexpr (NORM && WIDE) {
-            int d0, d1;
-            ht_runs(rp, i, d0, d1);
-            float x[8], y[8];
-            kvp_ld8(src + d0, x);
-            kvp_ld8(src + d1, y);
-            if (rp.q_norm != nullptr) ht_norm16<HD>(rp.q_norm, rp.eps, d0, d1, x, y);
-            if (rp.freq != nullptr) {
-                float c8[8], s8[8];
-                ht_angles16(rp, i, pos, c8, s8);
-                ht_turn16(rp, i, c8, s8, x, y);
-            }
-            kvp_st8(dst + d0, x);
-            kvp_st8(dst + d1, y);
-        } else if constexpr (NORM) {
+        if constexpr (NORM) {
             int d0, d1;
             const bool turns = ht_pair(rp, i, d0, d1);
             float x = ld_act<T>(src + d0), y = ld_act<T>(src + d1);
@@ -207,14 +239,7 @@ __global__ __launch_bounds__(WIDE ? 2 * HD : 128) void kv_pages_append_kernel(Kv
             kvp_ld8(src + d0, x);
             kvp_ld8(src + d1, y);
             if constexpr (NORM) {
-                if (!is_v) {
-                    if (rp.k_norm != nullptr) ht_norm16<HD>(rp.k_norm, rp.eps, d0, d1, x, y);
-                    if (rp.freq != nullptr) {
-                        float c8[8], s8[8];
-                        ht_angles16(rp, i, t0 + p, c8, s8);
-                        ht_turn16(rp, i, c8, s8, x, y);
-                    }
-                }
+                if (!is_v && rp.k_norm != nullptr) ht_norm16<HD>(rp.k_norm, rp.eps, d0, d1, x, y);
             } else if (!is_v && rp.cosc != nullptr) {
                 float c8[8], s8[8];
                 kvp_ld8(rp.cosc + (size_t)(t0 + p) * HD + 8 * i, c8);
@@ -229,6 +254,13 @@ __global__ __launch_bounds__(WIDE ? 2 * HD : 128) void kv_pages_append_kernel(Kv
 #pragma unroll
                     for (int e = 0; e < 8; ++e) kvp_rotate(x[e], y[e], c8[e], s8[e]);
                 }
+            }
+        }
+        if constexpr (NORM) {
+            if (rp.freq != nullptr) {
+                ht_fill<NT, NP>(rp, turn, j1 - j0, [&](int i_row) { return t0 + j0 + i_row; });
+                ht_barrier();
+                if (!is_v && in) ht_turn16(rp, i, turn[p - j0], x, y);
             }
         }
         // old tokens' bytes: K this thread's own, V those of dim id

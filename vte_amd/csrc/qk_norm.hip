@@ -12,19 +12,21 @@ struct QkRows {
     long long in, out;  // elements between rows
 };
 
-// A thread takes 16 dims of a head, HD / 16 threads a head; q heads of a row, then its k heads.
+// A thread takes 16 dims of a head, HD / 16 threads a head; q heads of a row, then its k heads.  A block's rows share
+// their cosines and sines.
 template <typename T, int HD>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(HeadForm f, QkRows<T> q, QkRows<T> k, int rows,
                                                            const int* __restrict__ positions) {
-    constexpr int NU = HD / 16;
-    const int per_row = (q.heads + k.heads) * NU;
-    const long long gid = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (gid >= (long long)rows * per_row) return;
-    const int row = (int)(gid / per_row), hu = (int)(gid - (long long)row * per_row), u = hu % NU;
-    const int pos = positions != nullptr ? positions[row] : 0;
-    if (pos < 0) return;
-    const bool is_q = hu / NU < q.heads;
-    const int h = is_q ? hu / NU : hu / NU - q.heads;
+    constexpr int NU = HD / 16, HEADS = 256 / NU;
+    __shared__ __align__(16) float2 turn[HEADS][HD / 2];
+    __shared__ int pos_sh[HEADS];
+    const int heads = q.heads + k.heads, tid = threadIdx.x, u = tid % NU;
+    const long long first = (long long)blockIdx.x * HEADS, all = (long long)rows * heads, item = first + tid / NU;
+    const int row0 = (int)(first / heads), row_n = (int)((min(first + HEADS, all) - 1) / heads) - row0 + 1;
+    const bool in = item < all;
+    const int row = (int)((in ? item : first) / heads), hh = (int)((in ? item : first) - (long long)row * heads);
+    const bool is_q = hh < q.heads;
+    const int h = is_q ? hh : hh - q.heads;
     const QkRows<T>& r = is_q ? q : k;
     const T* src = r.x + row * r.in + h * HD;
     T* dst = r.y + row * r.out + h * HD;
@@ -33,13 +35,19 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(HeadForm f, QkRows<T>
     float x[8], y[8];
     kvp_ld8(src + d0, x);
     kvp_ld8(src + d1, y);
+    if (positions != nullptr) {
+        if (tid < row_n) pos_sh[tid] = positions[row0 + tid];
+        ht_barrier();
+        if (f.freq != nullptr) {
+            ht_fill<256, HD / 2>(f, turn, row_n, [&](int i) { return pos_sh[i]; });
+            ht_barrier();
+        }
+        if (pos_sh[row - row0] < 0) return;
+    }
+    if (!in) return;
     const __half* w = is_q ? f.q_norm : f.k_norm;
     if (w != nullptr) ht_norm16<HD>(w, f.eps, d0, d1, x, y);
-    if (f.freq != nullptr) {
-        float c[8], s[8];
-        ht_angles16(f, u, pos, c, s);
-        ht_turn16(f, u, c, s, x, y);
-    }
+    if (f.freq != nullptr) ht_turn16(f, u, turn[row - row0], x, y);
     kvp_st8(dst + d0, x);
     kvp_st8(dst + d1, y);
 }
@@ -108,7 +116,7 @@ static hipError_t norm_hd(const HeadForm& f, const void* q, void* q_out, int n_q
                       fits(f.k_norm, 0) && (f.freq == nullptr || f.inter || f.rot % 16 == 0);
     const long long items = (long long)rows * (n_q + n_kv);
     if (wide)
-        hipLaunchKernelGGL((qk_norm_rope_kernel<T, HD>), dim3((unsigned)((items * (HD / 16) + 255) / 256)), dim3(256), 0, st,
+        hipLaunchKernelGGL((qk_norm_rope_kernel<T, HD>), dim3((unsigned)((items + 4096 / HD - 1) / (4096 / HD))), dim3(256), 0, st,
                            f, Q, K, rows, positions);
     else
         hipLaunchKernelGGL((qk_norm_rope_pairs_kernel<T, HD>), dim3((unsigned)((items + 3) / 4)), dim3(256), 0, st, f, Q, K,
