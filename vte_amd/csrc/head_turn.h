@@ -72,38 +72,60 @@ __device__ __forceinline__ void ht_turn(float& a, float& b, float c, float s) {
     b = fmaf(x, s, y * c);
 }
 
-// ---- 16 dims a thread: HD / 16 neighbouring lanes hold a head.  Needs rot % 16 = 0 or neighbouring pairs.
-// The two runs of 8 dims that thread u holds.
-__device__ __forceinline__ void ht_runs(const HeadForm& f, int u, int& d0, int& d1) {
-    if (f.freq != nullptr && !f.inter && 16 * u < f.rot) {
-        d0 = 8 * u;
-        d1 = d0 + f.rot / 2;
-    } else {  // (behind the rotated dims the rest in order)
-        d0 = 16 * u;
-        d1 = d0 + 8;
+// N consecutive elements, 8 or 4.
+template <typename T, int N>
+__device__ __forceinline__ void ht_ld(const T* p, float (&v)[N]) {
+    if constexpr (N == 8) {
+        kvp_ld8(p, v);
+    } else {
+        static_assert(N == 4 && sizeof(T) == 4, "");
+        const float4 a = *reinterpret_cast<const float4*>(p);
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
     }
 }
-// Sum over N neighbouring lanes (4, 8 or 16).
+template <typename T, int N>
+__device__ __forceinline__ void ht_st(T* p, const float (&v)[N]) {
+    if constexpr (N == 8) kvp_st8(p, v);
+    else *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+}
+
+// ---- Two runs of V dims a thread: HD / (2 V) neighbouring lanes hold a head.  Needs rot % (2 V) = 0 or neighbouring pairs.
+// A run of the neighbouring lane begins where the lane's ends, so that a load touches whole lines.
+template <int HD, int V>
+__device__ __forceinline__ void ht_runs(const HeadForm& f, int u, int& d0, int& d1) {
+    const int n = f.inter ? 0 : f.rot;  // dims whose pairs lie half of them apart
+    d0 = V * u;
+    d1 = d0 + (V * u < n / 2 ? n : HD) / 2;
+    if (d0 >= n / 2) d0 += n / 2;  // (behind them the rest in two halves: d1 - d0 = (HD - n) / 2)
+}
+// Sum over N neighbouring lanes (4, 8, 16 or 32).
 template <int N>
 __device__ __forceinline__ float ht_sum(float v) {
     v += VTE_DPP_F(v, 0xB1);
     v += VTE_DPP_F(v, 0x4E);
     if constexpr (N >= 8) v += VTE_DPP_F(v, 0x141);
     if constexpr (N >= 16) v += VTE_DPP_F(v, 0x140);
+    if constexpr (N >= 32) v += __shfl_xor(v, 16, 64);
     return v;
 }
-template <int HD>
-__device__ __forceinline__ void ht_norm16(const __half* w, float eps, int d0, int d1, float (&x)[8], float (&y)[8]) {
-    float a[8], b[8], sum = 0.f;
-    kvp_ld8(w + d0, a);
-    kvp_ld8(w + d1, b);
+template <int HD, int V>
+__device__ __forceinline__ void ht_norm(const __half* w, float eps, int d0, int d1, float (&x)[V], float (&y)[V]) {
+    __half a[V], b[V];
+    if constexpr (V == 8) {
+        *reinterpret_cast<uint4*>(a) = *reinterpret_cast<const uint4*>(w + d0);
+        *reinterpret_cast<uint4*>(b) = *reinterpret_cast<const uint4*>(w + d1);
+    } else {
+        *reinterpret_cast<uint2*>(a) = *reinterpret_cast<const uint2*>(w + d0);
+        *reinterpret_cast<uint2*>(b) = *reinterpret_cast<const uint2*>(w + d1);
+    }
+    float sum = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sum = fmaf(x[e], x[e], fmaf(y[e], y[e], sum));
-    const float inv = rsqrtf(ht_sum<HD / 16>(sum) * (1.f / HD) + eps);
+    for (int e = 0; e < V; ++e) sum = fmaf(x[e], x[e], fmaf(y[e], y[e], sum));
+    const float inv = rsqrtf(ht_sum<HD / (2 * V)>(sum) * (1.f / HD) + eps);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        x[e] *= inv * a[e];
-        y[e] *= inv * b[e];
+    for (int e = 0; e < V; ++e) {
+        x[e] *= inv * h2f(a[e]);
+        y[e] *= inv * h2f(b[e]);
     }
 }
 // Cosines and sines of a block's rows, once for all their heads: turn[row][pair], rows at positions pos(row).  (By each
@@ -125,15 +147,17 @@ __device__ __forceinline__ void ht_barrier() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 // (Pairs that do not rotate are left alone: times 0 an infinite neighbour would make NaN of them.)
-__device__ __forceinline__ void ht_turn16(const HeadForm& f, int u, const float2* turn, float (&x)[8], float (&y)[8]) {
-    const int n = f.rot / 2 - 8 * u;  // pairs from here on rotate
+template <int V>
+__device__ __forceinline__ void ht_turn_runs(const HeadForm& f, int d0, int d1, const float2* turn, float (&x)[V], float (&y)[V]) {
+    if (f.inter) {  // each run holds pairs
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        if (e >= n) continue;
-        const float2 t = turn[8 * u + e];
-        if (!f.inter) ht_turn(x[e], y[e], t.x, t.y);
-        else if (e < 4) ht_turn(x[2 * e], x[2 * e + 1], t.x, t.y);  // pairs lie side by side
-        else ht_turn(y[2 * e - 8], y[2 * e - 7], t.x, t.y);
+        for (int e = 0; e < V; e += 2) {
+            if (d0 + e < f.rot) ht_turn(x[e], x[e + 1], turn[(d0 + e) / 2].x, turn[(d0 + e) / 2].y);
+            if (d1 + e < f.rot) ht_turn(y[e], y[e + 1], turn[(d1 + e) / 2].x, turn[(d1 + e) / 2].y);
+        }
+    } else if (d0 < f.rot / 2) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) ht_turn(x[e], y[e], turn[d0 + e].x, turn[d0 + e].y);
     }
 }
 

@@ -102,17 +102,19 @@ __global__ __launch_bounds__(WIDE ? 2 * HD : 128) void kv_pages_append_kernel(Kv
             constexpr int NU = HD / 16;
             __shared__ int pos_sh[ROWS];
             const int tid = threadIdx.x, u = tid % NU;
-            const long long first = ((long long)(blockIdx.x - seq_blocks) + (long long)(gridDim.x - seq_blocks) *
-                                     (blockIdx.y + (long long)gridDim.y * blockIdx.z)) * ROWS;
-            const long long all = (long long)r.rows * n_q, item = first + tid / NU;
-            if (first >= all) return;
-            const int row0 = (int)(first / n_q), row_n = (int)((min(first + ROWS, all) - 1) / n_q) - row0 + 1;
-            const bool in = item < all;
-            const int row = (int)((in ? item : first) / n_q), h = (int)((in ? item : first) - (long long)row * n_q);
+            const long long block = (long long)(blockIdx.x - seq_blocks) + (long long)(gridDim.x - seq_blocks) *
+                                    (blockIdx.y + (long long)gridDim.y * blockIdx.z);
+            const int all = r.rows * n_q;  // (2^25 at most)
+            if (block * ROWS >= all) return;
+            const int first = (int)block * ROWS;
+            const bool in = first + tid / NU < all;
+            const int item = in ? first + tid / NU : first;
+            const int row0 = first / n_q, row_n = (min(first + ROWS, all) - 1) / n_q - row0 + 1;
+            const int row = item / n_q, h = item - row * n_q;
             const T* src = q + row * q_stride + h * HD;
             T* dst = q_out + ((size_t)row * n_q + h) * HD;
             int d0, d1;
-            ht_runs(rp, u, d0, d1);
+            ht_runs<HD, 8>(rp, u, d0, d1);
             float x[8], y[8];
             kvp_ld8(src + d0, x);
             kvp_ld8(src + d1, y);
@@ -132,8 +134,8 @@ __global__ __launch_bounds__(WIDE ? 2 * HD : 128) void kv_pages_append_kernel(Kv
                 ht_barrier();
             }
             if (!in || pos_sh[row - row0] < 0) return;
-            if (rp.q_norm != nullptr) ht_norm16<HD>(rp.q_norm, rp.eps, d0, d1, x, y);
-            if (rp.freq != nullptr) ht_turn16(rp, u, turn[row - row0], x, y);
+            if (rp.q_norm != nullptr) ht_norm<HD, 8>(rp.q_norm, rp.eps, d0, d1, x, y);
+            if (rp.freq != nullptr) ht_turn_runs<8>(rp, d0, d1, turn[row - row0], x, y);
             kvp_st8(dst + d0, x);
             kvp_st8(dst + d1, y);
             return;
@@ -225,7 +227,7 @@ __global__ __launch_bounds__(WIDE ? 2 * HD : 128) void kv_pages_append_kernel(Kv
         const bool in = p >= j0 && p < j1, old = p < j0;
         int d0 = 16 * i, d1 = 16 * i + 8;
         if constexpr (NORM) {
-            if (!is_v) ht_runs(rp, i, d0, d1);
+            if (!is_v) ht_runs<HD, 8>(rp, i, d0, d1);
         } else if (!is_v && rp.type != 1) {
             d0 = 8 * i;
             d1 = 8 * i + NP;
@@ -239,7 +241,7 @@ __global__ __launch_bounds__(WIDE ? 2 * HD : 128) void kv_pages_append_kernel(Kv
             kvp_ld8(src + d0, x);
             kvp_ld8(src + d1, y);
             if constexpr (NORM) {
-                if (!is_v && rp.k_norm != nullptr) ht_norm16<HD>(rp.k_norm, rp.eps, d0, d1, x, y);
+                if (!is_v && rp.k_norm != nullptr) ht_norm<HD, 8>(rp.k_norm, rp.eps, d0, d1, x, y);
             } else if (!is_v && rp.cosc != nullptr) {
                 float c8[8], s8[8];
                 kvp_ld8(rp.cosc + (size_t)(t0 + p) * HD + 8 * i, c8);
@@ -260,7 +262,7 @@ __global__ __launch_bounds__(WIDE ? 2 * HD : 128) void kv_pages_append_kernel(Kv
             if (rp.freq != nullptr) {
                 ht_fill<NT, NP>(rp, turn, j1 - j0, [&](int i_row) { return t0 + j0 + i_row; });
                 ht_barrier();
-                if (!is_v && in) ht_turn16(rp, i, turn[p - j0], x, y);
+                if (!is_v && in) ht_turn_runs<8>(rp, d0, d1, turn[p - j0], x, y);
             }
         }
         // old tokens' bytes: K this thread's own, V those of dim id

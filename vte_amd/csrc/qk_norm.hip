@@ -12,29 +12,30 @@ struct QkRows {
     long long in, out;  // elements between rows
 };
 
-// A thread takes 16 dims of a head, HD / 16 threads a head; q heads of a row, then its k heads.  A block's rows share
-// their cosines and sines.
+// A thread takes two 16-byte runs of a head; q heads of a row, then its k heads.  A block's rows share their cosines and
+// sines.
 template <typename T, int HD>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(HeadForm f, QkRows<T> q, QkRows<T> k, int rows,
                                                            const int* __restrict__ positions) {
-    constexpr int NU = HD / 16, HEADS = 256 / NU;
+    constexpr int V = 16 / sizeof(T), NU = HD / (2 * V), HEADS = 256 / NU;
     __shared__ __align__(16) float2 turn[HEADS][HD / 2];
     __shared__ int pos_sh[HEADS];
     const int heads = q.heads + k.heads, tid = threadIdx.x, u = tid % NU;
-    const long long first = (long long)blockIdx.x * HEADS, all = (long long)rows * heads, item = first + tid / NU;
-    const int row0 = (int)(first / heads), row_n = (int)((min(first + HEADS, all) - 1) / heads) - row0 + 1;
-    const bool in = item < all;
-    const int row = (int)((in ? item : first) / heads), hh = (int)((in ? item : first) - (long long)row * heads);
+    const int first = blockIdx.x * HEADS, all = rows * heads;  // (2^27 at most)
+    const bool in = first + tid / NU < all;
+    const int item = in ? first + tid / NU : first;
+    const int row0 = first / heads, row_n = (min(first + HEADS, all) - 1) / heads - row0 + 1;
+    const int row = item / heads, hh = item - row * heads;
     const bool is_q = hh < q.heads;
     const int h = is_q ? hh : hh - q.heads;
     const QkRows<T>& r = is_q ? q : k;
     const T* src = r.x + row * r.in + h * HD;
     T* dst = r.y + row * r.out + h * HD;
     int d0, d1;
-    ht_runs(f, u, d0, d1);
-    float x[8], y[8];
-    kvp_ld8(src + d0, x);
-    kvp_ld8(src + d1, y);
+    ht_runs<HD, V>(f, u, d0, d1);
+    float x[V], y[V];
+    ht_ld(src + d0, x);
+    ht_ld(src + d1, y);
     if (positions != nullptr) {
         if (tid < row_n) pos_sh[tid] = positions[row0 + tid];
         ht_barrier();
@@ -46,10 +47,10 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(HeadForm f, QkRows<T>
     }
     if (!in) return;
     const __half* w = is_q ? f.q_norm : f.k_norm;
-    if (w != nullptr) ht_norm16<HD>(w, f.eps, d0, d1, x, y);
-    if (f.freq != nullptr) ht_turn16(f, u, turn[row - row0], x, y);
-    kvp_st8(dst + d0, x);
-    kvp_st8(dst + d1, y);
+    if (w != nullptr) ht_norm<HD, V>(w, f.eps, d0, d1, x, y);
+    if (f.freq != nullptr) ht_turn_runs<V>(f, d0, d1, turn[row - row0], x, y);
+    ht_st(dst + d0, x);
+    ht_st(dst + d1, y);
 }
 
 // Any alignment and rotation: a wave takes a head, a lane one pair of dims (heads of 256: two).
@@ -113,10 +114,10 @@ static hipError_t norm_hd(const HeadForm& f, const void* q, void* q_out, int n_q
         return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride * (long long)sizeof(T) % 16 == 0;
     };
     const bool wide = fits(q, qs) && fits(q_out, 0) && fits(k, ks) && fits(k_out, 0) && fits(f.q_norm, 0) &&
-                      fits(f.k_norm, 0) && (f.freq == nullptr || f.inter || f.rot % 16 == 0);
-    const long long items = (long long)rows * (n_q + n_kv);
+                      fits(f.k_norm, 0) && (f.freq == nullptr || f.inter || f.rot % (32 / (int)sizeof(T)) == 0);
+    const long long items = (long long)rows * (n_q + n_kv), per = 8192 / (HD * (int)sizeof(T));  // heads of a block
     if (wide)
-        hipLaunchKernelGGL((qk_norm_rope_kernel<T, HD>), dim3((unsigned)((items + 4096 / HD - 1) / (4096 / HD))), dim3(256), 0, st,
+        hipLaunchKernelGGL((qk_norm_rope_kernel<T, HD>), dim3((unsigned)((items + per - 1) / per)), dim3(256), 0, st,
                            f, Q, K, rows, positions);
     else
         hipLaunchKernelGGL((qk_norm_rope_pairs_kernel<T, HD>), dim3((unsigned)((items + 3) / 4)), dim3(256), 0, st, f, Q, K,
