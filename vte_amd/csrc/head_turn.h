@@ -51,10 +51,11 @@ __device__ __forceinline__ void kvp_st8(T* p, const float (&v)[8]) {
     }
 }
 
-// amplitude * (cos, sin) of position * freq.  The angle in quarter turns is n + r, |r| <= 1/2; Taylor series of
-// sin(pi/2 r) and cos(pi/2 r) to r^9 and r^10 (what is left out is below 2^-28 of either).
-__device__ __forceinline__ void ht_angle(double position, double freq, float amplitude, float& c, float& s) {
-    double t = position * (freq * 0.15915494309189533577);  // turns
+// amplitude * (cos, sin) of position * freq, with `turns` = freq / (2 pi).  The angle in quarter turns is n + r, |r| <= 1/2;
+// Taylor series of sin(pi/2 r) and cos(pi/2 r) to r^9 and r^10 (what is left out is below 2^-28 of either).
+__device__ __forceinline__ double ht_turns(double freq) { return freq * 0.15915494309189533577; }
+__device__ __forceinline__ void ht_angle(double position, double turns, float amplitude, float& c, float& s) {
+    double t = position * turns;
     t = 4.0 * (t - rint(t));
     const double n = rint(t);
     const float r = (float)(t - n), x = r * r;
@@ -129,17 +130,31 @@ __device__ __forceinline__ void ht_norm(const __half* w, float eps, int d0, int 
     }
 }
 // Cosines and sines of a block's rows, once for all their heads: turn[row][pair], rows at positions pos(row).  (By each
-// thread for its own eight pairs they cost as much time as the bytes: see the kernels.)
-template <int NT, int NP, class Pos>
-__device__ __forceinline__ void ht_fill(const HeadForm& f, float2 (*turn)[NP], int rows, Pos pos) {
-    const int pairs = f.rot / 2;
-    for (int i = threadIdx.x; i < rows * pairs; i += NT) {
-        const int r = i / pairs, p = i - r * pairs;
-        float2 t;
-        ht_angle((double)pos(r), f.freq[p], f.amplitude, t.x, t.y);
-        turn[r][p] = t;
+// thread for its own eight pairs they cost as much time as the bytes: see the kernels.)  A thread keeps to one pair,
+// whose frequency it asks for before the positions are there.
+template <int NT>
+struct HtPair {
+    int row, pair, step;  // its first row, and the rows between its rows
+    double freq;
+    __device__ __forceinline__ explicit HtPair(const HeadForm& f) : row(0), pair(0), step(0), freq(0.) {
+        if (f.freq == nullptr) return;
+        const int pairs = f.rot / 2, tid = threadIdx.x;
+        step = NT / pairs;
+        row = tid / pairs;
+        pair = tid - row * pairs;
+        if (row < step) freq = f.freq[pair];
     }
-}
+    template <int NP, class Pos>
+    __device__ __forceinline__ void fill(const HeadForm& f, float2 (*turn)[NP], int rows, Pos pos) const {
+        if (row >= step) return;
+        const double turns = ht_turns(freq);
+        for (int r = row; r < rows; r += step) {
+            float2 t;
+            ht_angle((double)pos(r), turns, f.amplitude, t.x, t.y);
+            turn[r][pair] = t;
+        }
+    }
+};
 // A barrier for what stands in LDS only: loads from memory stay under way.
 __device__ __forceinline__ void ht_barrier() {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");

@@ -113,24 +113,20 @@ __global__ __launch_bounds__(WIDE ? 2 * HD : 128) void kv_pages_append_kernel(Kv
             const int row = item / n_q, h = item - row * n_q;
             const T* src = q + row * q_stride + h * HD;
             T* dst = q_out + ((size_t)row * n_q + h) * HD;
+            const HtPair<NT> mine(rp);
             int d0, d1;
             ht_runs<HD, 8>(rp, u, d0, d1);
             float x[8], y[8];
             kvp_ld8(src + d0, x);
             kvp_ld8(src + d1, y);
-            if (tid < row_n) {
-                const int b = kvp_row_seq(r, row0 + tid);
-                int pos = -1;  // (a row of nobody, or without a place)
-                if (b >= 0) {
-                    const KvSeq s = kvp_seq(r, b);
-                    const int at = row0 + tid - s.first;
-                    if (at >= 0 && at < s.n && s.pos < limit - at) pos = s.pos + at;
-                }
-                pos_sh[tid] = pos;
+            if (tid < 64) {  // (rows of a block are 32 at most)
+                const int at_row = row0 + min(tid, row_n - 1);
+                const int pos = kvp_row_pos(r, at_row, limit);
+                if (tid < row_n) pos_sh[tid] = pos;
             }
             ht_barrier();
             if (rp.freq != nullptr) {
-                ht_fill<NT, NP>(rp, turn, row_n, [&](int i) { return pos_sh[i]; });
+                mine.fill(rp, turn, row_n, [&](int i) { return pos_sh[i]; });
                 ht_barrier();
             }
             if (!in || pos_sh[row - row0] < 0) return;
@@ -168,7 +164,7 @@ __global__ __launch_bounds__(WIDE ? 2 * HD : 128) void kv_pages_append_kernel(Kv
             }
             if (turns) {
                 float c1, s1;
-                ht_angle((double)pos, rp.freq[i], rp.amplitude, c1, s1);
+                ht_angle((double)pos, ht_turns(rp.freq[i]), rp.amplitude, c1, s1);
                 ht_turn(x, y, c1, s1);
             }
             st_act<T>(dst + d0, x);
@@ -260,7 +256,7 @@ __global__ __launch_bounds__(WIDE ? 2 * HD : 128) void kv_pages_append_kernel(Kv
         }
         if constexpr (NORM) {
             if (rp.freq != nullptr) {
-                ht_fill<NT, NP>(rp, turn, j1 - j0, [&](int i_row) { return t0 + j0 + i_row; });
+                HtPair<NT>(rp).fill(rp, turn, j1 - j0, [&](int i_row) { return t0 + j0 + i_row; });
                 ht_barrier();
                 if (!is_v && in) ht_turn_runs<8>(rp, d0, d1, turn[p - j0], x, y);
             }
@@ -369,7 +365,7 @@ __global__ __launch_bounds__(WIDE ? 2 * HD : 128) void kv_pages_append_kernel(Kv
             }
             if (turns && p >= j0 && p < j1) {
                 float c1, s1;
-                ht_angle((double)(t0 + p), rp.freq[i], rp.amplitude, c1, s1);
+                ht_angle((double)(t0 + p), ht_turns(rp.freq[i]), rp.amplitude, c1, s1);
                 ht_turn(x[j], y[j], c1, s1);
             }
         } else if (turns && p >= j0 && p < j1) {

@@ -31,6 +31,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(HeadForm f, QkRows<T>
     const QkRows<T>& r = is_q ? q : k;
     const T* src = r.x + row * r.in + h * HD;
     T* dst = r.y + row * r.out + h * HD;
+    const HtPair<256> mine(f);
     int d0, d1;
     ht_runs<HD, V>(f, u, d0, d1);
     float x[V], y[V];
@@ -40,7 +41,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(HeadForm f, QkRows<T>
         if (tid < row_n) pos_sh[tid] = positions[row0 + tid];
         ht_barrier();
         if (f.freq != nullptr) {
-            ht_fill<256, HD / 2>(f, turn, row_n, [&](int i) { return pos_sh[i]; });
+            mine.fill(f, turn, row_n, [&](int i) { return pos_sh[i]; });
             ht_barrier();
         }
         if (pos_sh[row - row0] < 0) return;
@@ -95,7 +96,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_pairs_kernel(HeadForm f, QkR
         }
         if (turns) {
             float c, s;
-            ht_angle((double)pos, f.freq[lane + 64 * e], f.amplitude, c, s);
+            ht_angle((double)pos, ht_turns(f.freq[lane + 64 * e]), f.amplitude, c, s);
             ht_turn(a[e], b[e], c, s);
         }
         st_act<T>(dst + d0, a[e]);
