@@ -13,6 +13,8 @@
 #define KVM_LAYERS 64    // of a copy launch: 2 KB of arguments
 #define KVM_CHUNK 1024   // pages a block counts
 #define KVM_PIECE 1024   // 16-byte words that a block copies
+#define KVM_FEW 8192     // pages that every block of a compaction counts itself
+#define KVM_BLOCKS 128   // of a CU, at most, where the number of pairs is not known
 
 struct KvLayers {
     uint8_t *k[KVM_LAYERS], *v[KVM_LAYERS];
@@ -31,30 +33,42 @@ __device__ __forceinline__ void kvm_set(const KvTables& t, int row, int j, int p
 }
 
 // ---------------------------------------------------------------------------
-// Copies: pages src[i] -> dst[i] of every layer, i < n (n_dev: read on the device); pairs of which one is no page are
-// skipped.  An item is KVM_PIECE words of K then V of one pair and layer, its first one takes the exponents along.
+// Copies: pages src[i] -> dst[i] of every layer, i < n; pairs of which one is no page are skipped.  grid (pieces, layers,
+// pairs, or as many of them as there are blocks for): a block copies KVM_PIECE words of K then V, the first piece takes
+// the exponents along.
+//
+// Stores pass the caches by, whose lines they would fill for nobody; loads too (ONCE) where the pools are larger than the
+// memory-side cache, so that the pages are not in it: 470 MB read and written by a compaction in us, stores / loads past
+// the caches: neither 114.3, stores 114.9, both 103.6; 59 MB of a smaller pool 11.9, 11.5, 13.0, 117 MB of forks (whose
+// pages are in the cache) 30.4, 29.6, 34.4.
 // ---------------------------------------------------------------------------
-__device__ __forceinline__ void kvm_copy(const KvLayers& L, int n_layers, int layer_words, int exps, int n_pages,
-                                         const int* src, const int* dst, int n) {
-    const int words = 2 * layer_words;  // 16-byte words of a page, K and V
-    const int pieces = (words + KVM_PIECE - 1) / KVM_PIECE;
-    const long long items = (long long)n * n_layers * pieces;
-    for (long long it = blockIdx.x; it < items; it += gridDim.x) {
-        const int piece = (int)(it % pieces), i = (int)(it / pieces / n_layers), l = (int)(it / pieces % n_layers);
+template <bool ONCE>
+__device__ __forceinline__ uint4 kvm_load(const uint8_t* p) {
+    if constexpr (!ONCE) return ldg_g16(p);
+    const vte_u32x4 v = __builtin_nontemporal_load((vte_g_u32x4*)p);
+    return make_uint4(v.x, v.y, v.z, v.w);
+}
+template <bool ONCE>
+__device__ __forceinline__ void kvm_copy(const KvLayers& L, int layer_words, int exps, int n_pages, const int* src,
+                                         const int* dst, int n) {
+    const int words = 2 * layer_words, piece = blockIdx.x, l = blockIdx.y;  // 16-byte words of a page, K and V
+    for (int i = blockIdx.z; i < n; i += gridDim.z) {
         const int a = src[i], b = dst[i];
         if ((unsigned)a >= (unsigned)n_pages || (unsigned)b >= (unsigned)n_pages) continue;
         uint4 x[KVM_PIECE / 256];
 #pragma unroll
         for (int u = 0; u < KVM_PIECE / 256; ++u) {
             const int w = piece * KVM_PIECE + u * 256 + threadIdx.x;
-            if (w < words) x[u] = ldg_g16(w < layer_words ? L.k[l] + ((size_t)a * layer_words + w) * 16
+            if (w < words) x[u] = kvm_load<ONCE>(w < layer_words ? L.k[l] + ((size_t)a * layer_words + w) * 16
                                                           : L.v[l] + ((size_t)a * layer_words + w - layer_words) * 16);
         }
 #pragma unroll
         for (int u = 0; u < KVM_PIECE / 256; ++u) {
             const int w = piece * KVM_PIECE + u * 256 + threadIdx.x;
-            if (w < words) *reinterpret_cast<uint4*>(w < layer_words ? L.k[l] + ((size_t)b * layer_words + w) * 16
-                                                                     : L.v[l] + ((size_t)b * layer_words + w - layer_words) * 16) = x[u];
+            if (w < words)
+                __builtin_nontemporal_store(vte_u32x4{x[u].x, x[u].y, x[u].z, x[u].w},
+                                            reinterpret_cast<vte_u32x4*>(w < layer_words ? L.k[l] + ((size_t)b * layer_words + w) * 16
+                                                                                         : L.v[l] + ((size_t)b * layer_words + w - layer_words) * 16));
         }
         if (piece == 0)
             for (int e = threadIdx.x; e < exps; e += 256) {
@@ -63,9 +77,9 @@ __device__ __forceinline__ void kvm_copy(const KvLayers& L, int n_layers, int la
             }
     }
 }
-__global__ __launch_bounds__(256) void kv_copy_kernel(KvLayers L, int n_layers, int layer_words, int exps, int n_pages,
+__global__ __launch_bounds__(256) void kv_copy_kernel(KvLayers L, int layer_words, int exps, int n_pages,
                                                       const int* __restrict__ src, const int* __restrict__ dst, int n) {
-    kvm_copy(L, n_layers, layer_words, exps, n_pages, src, dst, n);
+    kvm_copy<false>(L, layer_words, exps, n_pages, src, dst, n);
 }
 
 // ---------------------------------------------------------------------------
@@ -84,11 +98,15 @@ __global__ __launch_bounds__(256) void kv_free_kernel(KvTables t, const int* __r
 }
 
 // ---------------------------------------------------------------------------
-// New pages, by one block of 1024 threads.  `want(slot)` says whether a slot of 0 .. slots - 1 needs one, `give(slot, rank,
-// page)` takes it (page -1: there are no more).  The result: slots that got none.
+// New pages, by one block of 1024 threads.  `want(slot)` says whether a slot of 0 .. slots - 1 needs one, `give(slot,
+// page)`, called by the same thread right after, takes it (page -1: there are no more).  The result: slots that got none.
 // Free pages are found 4096 at a time into a ring in LDS, only when a slot needs them.
 // ---------------------------------------------------------------------------
 #define KVM_RING 8192
+// (refs are read past the first cache: users may have been counted in the same launch)
+__device__ __forceinline__ int kvm_users(const KvTables& t, int p) {
+    return __hip_atomic_load(&t.refs[p], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
 template <class Want, class Give>
 __device__ __forceinline__ int kvm_new_pages(const KvTables& t, int slots, Want want, Give give) {
     __shared__ int ring[KVM_RING];
@@ -113,7 +131,10 @@ __device__ __forceinline__ int kvm_new_pages(const KvTables& t, int slots, Want 
         }
         return before + incl - v;
     };
-    int head = 0, have = 0, next = 0, missing = 0, done = 0;  // of the ring; the first page not looked at; slots served
+    int ahead[4];  // the first pages, asked for while it is not known yet whether a slot needs one
+#pragma unroll
+    for (int u = 0; u < 4; ++u) ahead[u] = 4 * tid + u < t.n_pages && kvm_users(t, 4 * tid + u) <= 0;
+    int head = 0, have = 0, next = 0, missing = 0;  // of the ring; the first page not looked at
     for (int s0 = 0; s0 < slots; s0 += 1024) {
         const bool w = s0 + tid < slots && want(s0 + tid);
         int n;
@@ -123,7 +144,7 @@ __device__ __forceinline__ int kvm_new_pages(const KvTables& t, int slots, Want 
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 const int p = next + 4 * tid + u;
-                r[u] = p < t.n_pages && t.refs[p] <= 0;
+                r[u] = next == 0 ? ahead[u] : p < t.n_pages && kvm_users(t, p) <= 0;
                 count += r[u];
             }
             int found;
@@ -141,13 +162,12 @@ __device__ __forceinline__ int kvm_new_pages(const KvTables& t, int slots, Want 
                 atomicExch(&t.refs[page], 1);
                 __threadfence_block();  // (before the entry that shows it to others, which may release it)
             }
-            give(s0 + tid, done + rank, page);
+            give(s0 + tid, page);
         }
         const int got = min(n, have);
         head += got;
         have -= got;
         missing += n - got;
-        done += n;
         __syncthreads();
     }
     return missing;
@@ -157,7 +177,8 @@ __device__ __forceinline__ int kvm_new_pages(const KvTables& t, int slots, Want 
 __global__ __launch_bounds__(1024) void kv_reserve_kernel(KvTables t, int n, const int* __restrict__ seqs,
                                                           const int* __restrict__ start, const int* __restrict__ stop,
                                                           int count, int per, int* missing) {
-    auto entry = [&](int slot, int& row, int& j) {
+    int row = 0, j = 0;  // of the slot at hand
+    auto entry = [&](int slot) {
         const int i = slot / per;
         row = seqs != nullptr ? seqs[i] : i;
         if ((unsigned)row >= (unsigned)t.batch || start[i] < 0) return false;
@@ -169,13 +190,9 @@ __global__ __launch_bounds__(1024) void kv_reserve_kernel(KvTables t, int n, con
     };
     const int short_of = kvm_new_pages(
         t, n * per,
-        [&](int slot) {
-            int row, j;
-            return entry(slot, row, j) && !kvm_is_page(t, t.table[(size_t)row * t.max_pages + j]);
-        },
-        [&](int slot, int, int page) {
-            int row, j;
-            if (page >= 0 && entry(slot, row, j)) kvm_set(t, row, j, page);
+        [&](int slot) { return entry(slot) && !kvm_is_page(t, t.table[(size_t)row * t.max_pages + j]); },
+        [&](int, int page) {
+            if (page >= 0) kvm_set(t, row, j, page);
         });
     if (missing != nullptr && threadIdx.x == 0) *missing = short_of;
 }
@@ -183,6 +200,8 @@ __global__ __launch_bounds__(1024) void kv_reserve_kernel(KvTables t, int n, con
 // ---------------------------------------------------------------------------
 // Forks.  First the whole pages of a parent's first tokens are shared with the child, whose own go (grid (entries,
 // children)); then one block finds a page for each child whose last page is begun, and lists what is to be copied.
+// Up to an entry a thread of the one block, it does both: a launch less (a fork of 1020 entries between a free and a
+// reserve, a graph 14.9 against 15.2 us, calls 19.8 against 22.7; of 2108 entries the graph is slower, 17.4 against 16.3).
 // A child that is its own parent stays as it is.
 // ---------------------------------------------------------------------------
 struct KvFork {
@@ -195,10 +214,7 @@ __device__ __forceinline__ bool kvm_fork(const KvTables& t, const KvFork& f, int
     length = f.lengths[i];
     return (unsigned)parent < (unsigned)t.batch && (unsigned)child < (unsigned)t.batch && parent != child && length >= 0;
 }
-__global__ __launch_bounds__(256) void kv_fork_kernel(KvTables t, KvFork f) {
-    const int j = blockIdx.x * 256 + threadIdx.x;
-    int parent, child, length;
-    if (!kvm_fork(t, f, blockIdx.y, parent, child, length) || j >= t.max_pages) return;
+__device__ __forceinline__ void kvm_fork_entry(const KvTables& t, int parent, int child, int length, int j) {
     int p = -1;
     if (j < length >> t.page_log2) {
         p = t.table[(size_t)parent * t.max_pages + j];
@@ -207,30 +223,36 @@ __global__ __launch_bounds__(256) void kv_fork_kernel(KvTables t, KvFork f) {
     }
     kvm_set(t, child, j, p);
 }
-__global__ __launch_bounds__(1024) void kv_fork_last_kernel(KvTables t, KvFork f, int* src, int* dst, int* missing) {
-    auto begun = [&](int i, int& child, int& j, int& page) {
-        int parent, length;
-        if (!kvm_fork(t, f, i, parent, child, length)) return false;
-        j = length >> t.page_log2;
-        if ((length & ((1 << t.page_log2) - 1)) == 0 || j >= t.max_pages) return false;
-        page = t.table[(size_t)parent * t.max_pages + j];
-        return kvm_is_page(t, page);
-    };
+__global__ __launch_bounds__(256) void kv_fork_kernel(KvTables t, KvFork f) {
+    const int j = blockIdx.x * 256 + threadIdx.x;
+    int parent, child, length;
+    if (kvm_fork(t, f, blockIdx.y, parent, child, length) && j < t.max_pages) kvm_fork_entry(t, parent, child, length, j);
+}
+// `all`: the entries that kv_fork_kernel takes, too.
+__global__ __launch_bounds__(1024) void kv_fork_last_kernel(KvTables t, KvFork f, bool all, int* src, int* dst, int* missing) {
+    if (all) {
+        for (int e = threadIdx.x; e < f.n * t.max_pages; e += 1024) {
+            const int i = e / t.max_pages;
+            int parent, child, length;
+            if (kvm_fork(t, f, i, parent, child, length)) kvm_fork_entry(t, parent, child, length, e - i * t.max_pages);
+        }
+    }
     for (int i = threadIdx.x; i < f.n; i += 1024) src[i] = dst[i] = -1;
+    __builtin_amdgcn_s_waitcnt(0);  // (atomics that return nothing, too: the counts are read next)
     __syncthreads();
+    int child = 0, j = 0, page = -1;  // of the slot at hand
     const int short_of = kvm_new_pages(
         t, f.n,
         [&](int i) {
-            int child, j, page;
-            return begun(i, child, j, page);
+            int parent, length;
+            if (!kvm_fork(t, f, i, parent, child, length)) return false;
+            j = length >> t.page_log2;
+            if ((length & ((1 << t.page_log2) - 1)) == 0 || j >= t.max_pages) return false;
+            page = t.table[(size_t)parent * t.max_pages + j];
+            return kvm_is_page(t, page);
         },
-        [&](int i, int rank, int to) {
-            int child, j, page;
+        [&](int i, int to) {
             if (to < 0) return;
-            if (!begun(i, child, j, page)) {  // (a parent that is a child as well and lost it just now)
-                kvm_release(t, to);
-                return;
-            }
             src[i] = page;
             dst[i] = to;
             kvm_set(t, child, j, to);
@@ -239,9 +261,11 @@ __global__ __launch_bounds__(1024) void kv_fork_last_kernel(KvTables t, KvFork f
 }
 
 // ---------------------------------------------------------------------------
-// Compaction: with U used pages, the k-th used page from U on moves to the k-th free one below U.  Counts per chunk; then
-// every block knows U and what lies before its chunk, lists its pages' places and writes where each page goes, those
-// that move as -2 - k until the copies' launch, which knows the lists.
+// Compaction: with U used pages, the k-th used page from U on moves to the k-th free one below U.  Counts per chunk (of
+// up to KVM_FEW pages every block counts them all itself, a launch less, a graph's us: 1000 pages 10.4 against 11.9, 8192 13.8
+// against 14.8, 16384 17.9 against 16.4); then every block knows U and what
+// lies before its chunk, lists its pages' places and writes where each page goes, those that move as -2 - k until the
+// copies' launch, which knows the lists.
 // ---------------------------------------------------------------------------
 struct KvMoves {
     int *counts, *src, *dst, *moves;  // used pages of each chunk; pairs; how many
@@ -257,10 +281,11 @@ __global__ __launch_bounds__(256) void kv_count_kernel(KvTables t, int* __restri
     __syncthreads();
     if (threadIdx.x == 0) counts[blockIdx.x] = sums[0] + sums[1] + sums[2] + sums[3];
 }
+template <bool COUNTED>
 __global__ __launch_bounds__(256) void kv_place_kernel(KvTables t, KvMoves m, int chunks, int* __restrict__ where,
                                                        int* __restrict__ used) {
     __shared__ int sums[3][4];
-    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, chunk0 = blockIdx.x * KVM_CHUNK;
     auto all = [&](int row, int v) {  // the block's sum
 #pragma unroll
         for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d, 64);
@@ -268,16 +293,32 @@ __global__ __launch_bounds__(256) void kv_place_kernel(KvTables t, KvMoves m, in
         __syncthreads();
         return sums[row][0] + sums[row][1] + sums[row][2] + sums[row][3];
     };
-    int v = 0;
-    for (int c = tid; c < chunks; c += 256) v += m.counts[c];
-    const int U = all(0, v), cut = U / KVM_CHUNK;  // (U is in chunk `cut`, which may be one behind the last)
+    int v = 0, first = 0;  // used pages: all of them, and those before the chunk
+    if constexpr (COUNTED) {
+        for (int c = tid; c < chunks; c += 256) {
+            v += m.counts[c];
+            first += c < (int)blockIdx.x ? m.counts[c] : 0;
+        }
+    } else {
+#pragma unroll 8
+        for (int p = tid; p < t.n_pages; p += 256) {
+            const int n = t.refs[p] > 0;
+            v += n;
+            first += p < chunk0 ? n : 0;
+        }
+    }
+    const int U = all(0, v);
+    int before = all(1, first);
     v = 0;
-    for (int c = tid; c < chunks; c += 256) v += c < cut ? m.counts[c] : 0;
-    for (int p = cut * KVM_CHUNK + tid; p < U; p += 256) v += t.refs[p] > 0;
-    const int below = all(1, v);  // used pages below U
-    v = 0;
-    for (int c = tid; c < (int)blockIdx.x; c += 256) v += m.counts[c];
-    int before = all(2, v);       // used pages before the chunk
+    int p0 = 0;
+    if constexpr (COUNTED) {
+        const int cut = U / KVM_CHUNK;  // (U is in chunk `cut`, which may be one behind the last)
+        for (int c = tid; c < cut; c += 256) v += m.counts[c];
+        p0 = cut * KVM_CHUNK;
+    }
+#pragma unroll 8
+    for (int p = p0 + tid; p < U; p += 256) v += t.refs[p] > 0;
+    const int below = all(2, v);  // used pages below U
     if (blockIdx.x == 0 && tid == 0) {
         *used = U;
         *m.moves = U - below;
@@ -286,14 +327,14 @@ __global__ __launch_bounds__(256) void kv_place_kernel(KvTables t, KvMoves m, in
     uint64_t bits[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-        const int p = blockIdx.x * KVM_CHUNK + u * 256 + tid;
+        const int p = chunk0 + u * 256 + tid;
         bits[u] = __ballot(p < t.n_pages && t.refs[p] > 0);
         if (lane == 0) row_sums[u][wv] = __popcll(bits[u]);
     }
     __syncthreads();
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-        const int p = blockIdx.x * KVM_CHUNK + u * 256 + tid;
+        const int p = chunk0 + u * 256 + tid;
         int n = before + __popcll(bits[u] & ((1ull << lane) - 1));  // used pages before p
         for (int w = 0; w < 4; ++w) {
             n += w < wv ? row_sums[u][w] : 0;
@@ -311,11 +352,13 @@ __global__ __launch_bounds__(256) void kv_place_kernel(KvTables t, KvMoves m, in
     }
 }
 // (first: the launch that also rewrites tables, counts and `where`)
-__global__ __launch_bounds__(256) void kv_move_kernel(KvLayers L, int n_layers, int layer_words, int exps, KvTables t, KvMoves m,
-                                                      int* where, bool first) {
+template <bool ONCE>
+__global__ __launch_bounds__(256) void kv_move_kernel(KvLayers L, int layer_words, int exps, KvTables t, KvMoves m, int* where,
+                                                      bool first) {
     const int n = *m.moves;
     if (first) {
-        const long long step = (long long)gridDim.x * 256, at = (long long)blockIdx.x * 256 + threadIdx.x;
+        const long long step = (long long)gridDim.x * gridDim.y * gridDim.z * 256;
+        const long long at = (blockIdx.x + (long long)gridDim.x * (blockIdx.y + gridDim.y * blockIdx.z)) * 256 + threadIdx.x;
         for (long long e = at; e < (long long)t.batch * t.max_pages; e += step) {
             const int p = t.table[e];
             if (!kvm_is_page(t, p)) continue;
@@ -329,7 +372,7 @@ __global__ __launch_bounds__(256) void kv_move_kernel(KvLayers L, int n_layers, 
             t.refs[a] = 0;
         }
     }
-    kvm_copy(L, n_layers, layer_words, exps, t.n_pages, m.src, m.dst, n);
+    kvm_copy<ONCE>(L, layer_words, exps, t.n_pages, m.src, m.dst, n);
 }
 
 // ---------------------------------------------------------------------------
@@ -357,14 +400,19 @@ static CopyShape copy_shape(const KvPages& c, int hd) {
     s.pieces = (2 * s.words + KVM_PIECE - 1) / KVM_PIECE;
     return s;
 }
-static unsigned copy_blocks(long long items) { return (unsigned)std::max(1LL, std::min<long long>(items, 16 * device_cus())); }
+// One block for each piece of n pairs, KVM_BLOCKS a CU at most; at least `least` in all.
+static dim3 copy_grid(const CopyShape& s, int n_layers, long long n, long long least) {
+    const long long each = (long long)s.pieces * n_layers;
+    const long long z = std::max(std::min(n, (KVM_BLOCKS * device_cus() + each - 1) / each), (least + each - 1) / each);
+    return dim3(s.pieces, n_layers, (unsigned)std::min(std::max(z, 1LL), 65535LL));
+}
 
 hipError_t kv_pages_copy(const KvPages* layers, int n_layers, int hd, const int* src, const int* dst, int n, hipStream_t st) {
     const CopyShape s = copy_shape(layers[0], hd);
     for (int l = 0; l < n_layers; l += KVM_LAYERS) {
         const int m = std::min(KVM_LAYERS, n_layers - l);
-        hipLaunchKernelGGL(kv_copy_kernel, dim3(copy_blocks((long long)n * m * s.pieces)), dim3(256), 0, st,
-                           layers_of(layers + l, m), m, s.words, s.exps, layers[0].n_pages, src, dst, n);
+        hipLaunchKernelGGL(kv_copy_kernel, copy_grid(s, m, n, 1), dim3(256), 0, st, layers_of(layers + l, m), s.words, s.exps,
+                           layers[0].n_pages, src, dst, n);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
@@ -376,7 +424,7 @@ hipError_t kv_pages_free(const KvTables& t, int n, const int* seqs, int keep, co
 }
 // Slots of a sequence: pages that `count` tokens touch at most.
 int kv_pages_reserve_slots(const KvTables& t, int count) {
-    return (int)std::min<long long>(t.max_pages, ((long long)count - 1 >> t.page_log2) + 2);
+    return (int)std::min<long long>(t.max_pages, (((long long)count - 1) >> t.page_log2) + 2);
 }
 hipError_t kv_pages_reserve(const KvTables& t, int n, const int* seqs, const int* start, const int* stop, int count,
                             int* missing, hipStream_t st) {
@@ -389,10 +437,14 @@ hipError_t kv_pages_fork(const KvPages* layers, int n_layers, int hd, const KvTa
                          const int* children, const int* lengths, int* missing, void* scratch, hipStream_t st) {
     const KvFork f{parents, children, lengths, n};
     int* src = static_cast<int*>(scratch);
-    hipLaunchKernelGGL(kv_fork_kernel, dim3((t.max_pages + 255) / 256, n), dim3(256), 0, st, t, f);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(kv_fork_last_kernel, dim3(1), dim3(1024), 0, st, t, f, src, src + n, missing);
+    const bool all = (long long)n * t.max_pages <= 1024;
+    hipError_t e = hipSuccess;
+    if (!all) {
+        hipLaunchKernelGGL(kv_fork_kernel, dim3((t.max_pages + 255) / 256, n), dim3(256), 0, st, t, f);
+        e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    hipLaunchKernelGGL(kv_fork_last_kernel, dim3(1), dim3(1024), 0, st, t, f, all, src, src + n, missing);
     e = hipGetLastError();
     return e != hipSuccess ? e : kv_pages_copy(layers, n_layers, hd, src, src + n, n, st);
 }
@@ -405,17 +457,24 @@ hipError_t kv_pages_compact(const KvPages* layers, int n_layers, int hd, const K
     m.counts = m.moves + 4;
     m.src = m.counts + chunks_of(t);
     m.dst = m.src + t.n_pages;
-    hipLaunchKernelGGL(kv_count_kernel, dim3(chunks_of(t)), dim3(256), 0, st, t, m.counts);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(kv_place_kernel, dim3(chunks_of(t)), dim3(256), 0, st, t, m, chunks_of(t), where, used);
+    hipError_t e = hipSuccess;
+    if (t.n_pages <= KVM_FEW) {
+        hipLaunchKernelGGL(kv_place_kernel<false>, dim3(chunks_of(t)), dim3(256), 0, st, t, m, chunks_of(t), where, used);
+    } else {
+        hipLaunchKernelGGL(kv_count_kernel, dim3(chunks_of(t)), dim3(256), 0, st, t, m.counts);
+        e = hipGetLastError();
+        if (e != hipSuccess) return e;
+        hipLaunchKernelGGL(kv_place_kernel<true>, dim3(chunks_of(t)), dim3(256), 0, st, t, m, chunks_of(t), where, used);
+    }
     e = hipGetLastError();
     const CopyShape s = copy_shape(layers[0], hd);
     for (int l = 0; l < n_layers && e == hipSuccess; l += KVM_LAYERS) {
         const int n = std::min(KVM_LAYERS, n_layers - l);
-        const long long items = std::max((long long)(t.n_pages / 2) * n * s.pieces, (long long)t.batch * t.max_pages / 256 + 1);
-        hipLaunchKernelGGL(kv_move_kernel, dim3(copy_blocks(items)), dim3(256), 0, st, layers_of(layers + l, n), n, s.words,
-                           s.exps, t, m, where, l == 0);
+        const long long entries = std::min<long long>((long long)t.batch * t.max_pages / 256 + 1, 4 * device_cus());
+        // (256 MB: the memory-side cache)
+        const bool once = 32LL * s.words * t.n_pages * n > (256LL << 20);
+        hipLaunchKernelGGL(once ? kv_move_kernel<true> : kv_move_kernel<false>, copy_grid(s, n, t.n_pages / 2, l == 0 ? entries : 1), dim3(256), 0, st,
+                           layers_of(layers + l, n), s.words, s.exps, t, m, where, l == 0);
         e = hipGetLastError();
     }
     return e;
