@@ -1049,6 +1049,7 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
         // Sums: a block's probabilities are formed, and the one's V behind it read, under its products.
         const float shift = (float)PA_Q_LOG2 - m_run;
         const pa_h2 ones = {(_Float16)1.f, (_Float16)1.f};
+        float l_odd = 0.f;
         float minus = -1.f;  // (a value that the compiler does not know: p - h as one mixed operation instead of two)
         asm("" : "+v"(minus));
         union Probs {
@@ -1064,10 +1065,15 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
                 const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[kb >> 1][j + 1], kf, shift));
                 Probs(&f)[PA_P_PARTS] = pf[kb & 1];
                 f[0].h[i] = __builtin_convertvector(pa_f2{p0, p1}, pa_h2);
-                l_run = __builtin_amdgcn_fdot2(f[0].h[i], ones, l_run, false);
                 const pa_h2 h = f[0].h[i];
                 f[1].h[i] = __builtin_convertvector(pa_f2{fmaf((float)h[0], minus, p0), fmaf((float)h[1], minus, p1)}, pa_h2);
-                l_run = __builtin_amdgcn_fdot2(f[1].h[i], ones, l_run, false);
+                if constexpr (WIN) {
+                    l_run += p0;
+                    l_odd += p1;
+                } else {
+                    l_run = __builtin_amdgcn_fdot2(f[0].h[i], ones, l_run, false);
+                    l_run = __builtin_amdgcn_fdot2(f[1].h[i], ones, l_run, false);
+                }
             }
         };
         auto read_v = [&](int kb) {
@@ -1097,6 +1103,7 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
             }
         }
         __builtin_amdgcn_sched_barrier(0);
+        if constexpr (WIN) l_run += l_odd;
     };
 
     scales();
