@@ -1009,7 +1009,12 @@ __global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, Kv
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const int i = 8 * (kb & 1) + j;
-                    sc[kb >> 1][i] = (WIN ? (bits >> j & 1) != 0 : j < n) ? sc[kb >> 1][i] : -INFINITY;
+                    if constexpr (WIN) {  // (the bit as a mask: two operations a score)
+                        const uint32_t m = (uint32_t)__builtin_amdgcn_sbfe((int)bits, j, 1);
+                        sc[kb >> 1][i] = __uint_as_float((m & __float_as_uint(sc[kb >> 1][i])) | (~m & 0xFF800000u));
+                    } else {
+                        sc[kb >> 1][i] = j < n ? sc[kb >> 1][i] : -INFINITY;
+                    }
                 }
             }
         }
@@ -1253,6 +1258,10 @@ static long long most_tiles(const KvPages& c, const KvRows& r, long long rows, c
     if (w.window == 0) return all;
     return std::min(all, (w.window + rows + PA_TILE - 2) / PA_TILE + 1 + ((long long)w.sinks + PA_TILE - 1) / PA_TILE);
 }
+// Whether the window is shorter than the table, so that row blocks see about as many tokens each.
+static bool limited(const KvPages& c, const KvRows& r, const PaWindow& w) {
+    return w.window != 0 && 2LL * w.window < (long long)r.max_pages << c.page_log2;
+}
 // Blocks of the few-rows form: two per CU (their registers allow no more), and
 // no more than the table's capacity, or the window, has shares of four tiles.
 static PaPlan rows_plan(const KvPages& c, const KvRows& r, int hd, int G, const PaWindow& w, void* scratch, long long* bytes) {
@@ -1294,6 +1303,17 @@ static PromptForm prompt_form(const KvPages& c, const KvRows& r, int hd, int G, 
     PromptForm f;
     auto blocks = [&](int rows) { return ((long long)r.rows * G + rows - 1) / rows + r.batch - 1; };
     f.groups = blocks(256) * c.n_kv * 4 >= 9 * device_cus() ? 1 : 2;
+    // Short windows: row blocks see about as many tokens each, and start and end weigh on them, so what counts is rounds of
+    // blocks times a block's time, in half steps, of which start and end take four.  us by the rule above / by this one:
+    // four ragged prompts of up to 1500 tokens, window 300, fp32 heads of 64 55.1 / 48.7, fp16 ones of 128 37.7 / 29.5; two
+    // of 2048, window 256 32.5 / 27.0; 4000 tokens, window 2000 103.3 / 91.2; four of 2048, window 256 50.0 / 50.7.
+    if (limited(c, r, w) && blocks(128) * c.n_kv >= device_cus()) {  // (else shares: two groups)
+        auto time = [&](int rows) {
+            const long long rounds = (blocks(rows) * c.n_kv + device_cus() - 1) / device_cus();
+            return rounds * (4 + most_tiles(c, r, std::min(r.max_rows, rows / G + 2), w) * (rows == 256 ? 2 : 1));
+        };
+        f.groups = time(256) <= time(128) ? 1 : 2;
+    }
     f.rbs = blocks(f.groups == 1 ? 256 : 128);
     const long long steps = most_tiles(c, r, std::min(r.max_rows, 128 / G + 2), w);
     const long long most = std::max(std::min(16LL, steps / 2), std::min<long long>(PA_SHARES, steps / 4));
