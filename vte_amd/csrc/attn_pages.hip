@@ -571,7 +571,8 @@ __global__ __launch_bounds__(256) void attn_pages_combine_kernel(KvPages c, KvRo
 // of threads takes a row block, or while these are fewer than the CUs one of nsp
 // equal shares of its steps (joined by a second launch).
 //
-// The block's eight waves hold 32 rows each (GROUPS = 1), or are two groups of
+// The block's eight waves hold 32 rows each (GROUPS = 1; with short windows also
+// four of them, blocks of which share a CU), or are two groups of
 // four that take every other step and whose sums meet in LDS at the end (GROUPS =
 // 2: half as many rows, so twice as many blocks or half as many shares).  The bytes
 // of a step become fp16 once per group on their way into LDS, times 2^(e - ref)
@@ -756,12 +757,12 @@ __device__ __forceinline__ void pa_apart(const KvPages& c, const int* table, int
 
 // grid (row blocks * n_kv, nsp), the last row blocks (which see most) first, whatever their head: with the heads one after
 // the other some started long ones late (four ragged fp32 prompts 65 -> 53 us).  nsp > 1 with two groups only.
-template <typename T, int HD, int GROUPS, bool WIN>
-__global__ __launch_bounds__(512, 2) void attn_pages_prompt_kernel(KvPages c, KvRows r, PaPrompt pp,
+template <typename T, int HD, int GROUPS, int WAVES, bool WIN>
+__global__ __launch_bounds__(64 * GROUPS * WAVES, GROUPS * WAVES == 4 && HD == 64 ? 3 : 2) void attn_pages_prompt_kernel(KvPages c, KvRows r, PaPrompt pp,
                                                                    const T* q, T* out,
                                                                    int n_q, float scale, PaWindow win) {
     constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;  // fp16 parts of q
-    constexpr int WAVES = 8 / GROUPS, ROWS = 32 * WAVES;  // of a group
+    constexpr int ROWS = 32 * WAVES;  // of a group
     constexpr int KS = HD / 16, DT = HD / 32;              // 16-dim steps of a score, 32-dim tiles
     constexpr int NP = 8 * HD / (64 * WAVES);              // 16-byte pieces of K and V a thread stages (1: waves 0..3 K, 4..7 V)
     // A lane's operand is 16 bytes of one token (K) or dim (V); those of neighbouring tokens or dims lie side by side, so
@@ -1294,7 +1295,7 @@ static PaPlan rows_plan(const KvPages& c, const KvRows& r, int hd, int G, const 
 // heads, 16 / 32 / 64 / 128 shares, us: after 8192 tokens 23.0 / 19.8 / 21.8 / 22.0, after 32768 57 / 37 / 30 / 34; after
 // 2048 8 / 16 shares 16.0 / 14.4.
 struct PromptForm {
-    int groups;
+    int groups;  // 0: one of four waves
     long long rbs;
     PaPrompt p;
     long long bytes;
@@ -1303,16 +1304,20 @@ static PromptForm prompt_form(const KvPages& c, const KvRows& r, int hd, int G, 
     PromptForm f;
     auto blocks = [&](int rows) { return ((long long)r.rows * G + rows - 1) / rows + r.batch - 1; };
     f.groups = blocks(256) * c.n_kv * 4 >= 9 * device_cus() ? 1 : 2;
-    // Short windows: row blocks see about as many tokens each, and start and end weigh on them, so what counts is rounds of
-    // blocks times a block's time, in half steps, of which start and end take four.  us by the rule above / by this one:
-    // four ragged prompts of up to 1500 tokens, window 300, fp32 heads of 64 55.1 / 48.7, fp16 ones of 128 37.7 / 29.5; two
-    // of 2048, window 256 32.5 / 27.0; 4000 tokens, window 2000 103.3 / 91.2; four of 2048, window 256 50.0 / 50.7.
+    // Short windows: row blocks see about as many tokens each, and their starts and ends, some two steps' time, weigh on
+    // them.  With heads of 64 blocks of four waves, three of which share a CU, so that one's start lies under another's
+    // steps; with heads of 128 the form that takes the least: whole rounds of eight waves, or of four, two blocks a CU, which
+    // follow each other without rounds but whose steps take 8 % longer.  us by the rule above / wide / of four waves: four
+    // ragged prompts of up to 1500 tokens, window 300, heads of 64 fp32 55.1 / 48.4 / 39.8, fp16 47.6 / 40.7 / 34.3, of 128
+    // 37.7 / 29.4 / 29.9; eight of 300 to 1000, window 128 28.8 / 28.6 / 22.6; four of 2048, window 256 50.0 / 50.0 / 43.2;
+    // 4000 tokens, window 2000 103.3 / 90.2 / 98.2; two of 2400, window 1000 53.6 wide, 55.8 of four.
     if (limited(c, r, w) && blocks(128) * c.n_kv >= device_cus()) {  // (else shares: two groups)
-        auto time = [&](int rows) {
-            const long long rounds = (blocks(rows) * c.n_kv + device_cus() - 1) / device_cus();
-            return rounds * (4 + most_tiles(c, r, std::min(r.max_rows, rows / G + 2), w) * (rows == 256 ? 2 : 1));
-        };
-        f.groups = time(256) <= time(128) ? 1 : 2;
+        const long long cus = device_cus();
+        auto steps = [&](int rows) { return most_tiles(c, r, std::min(r.max_rows, rows / G + 2), w); };
+        auto rounds = [&](int rows) { return (blocks(rows) * c.n_kv + cus - 1) / cus; };
+        const long long wide = rounds(256) * (200 + 100 * steps(256)), two = rounds(128) * (200 + 50 * steps(128));
+        const long long four = std::max(2 * cus, blocks(128) * c.n_kv) * (200 + 108 * steps(128)) / (2 * cus);
+        f.groups = hd == 64 || four < std::min(wide, two) ? 0 : wide <= two ? 1 : 2;
     }
     f.rbs = blocks(f.groups == 1 ? 256 : 128);
     const long long steps = most_tiles(c, r, std::min(r.max_rows, 128 / G + 2), w);
@@ -1364,8 +1369,15 @@ static hipError_t attn_hd(const KvPages& c, const KvRows& r, const void* q, void
         return hipGetLastError();
     }
     const PromptForm f = prompt_form(c, r, HD, G, w, scratch);
-    auto kernel = f.groups == 1 ? attn_pages_prompt_kernel<T, HD, 1, WIN> : attn_pages_prompt_kernel<T, HD, 2, WIN>;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(f.rbs * c.n_kv), f.p.nsp), dim3(512), 0, st, c, r, f.p, (const T*)q, (T*)out,
+    auto kernel = f.groups == 1 ? attn_pages_prompt_kernel<T, HD, 1, 8, WIN> : attn_pages_prompt_kernel<T, HD, 2, 4, WIN>;
+    int threads = 512;
+    if constexpr (WIN) {
+        if (f.groups == 0) {
+            kernel = attn_pages_prompt_kernel<T, HD, 1, 4, WIN>;
+            threads = 256;
+        }
+    }
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(f.rbs * c.n_kv), f.p.nsp), dim3(threads), 0, st, c, r, f.p, (const T*)q, (T*)out,
                        n_q, scale, w);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || f.p.nsp == 1) return e;
