@@ -470,13 +470,13 @@ int vte_attn_pages_window(const vte_kv_pages* cache, const vte_kv_rows* rows, in
 typedef struct vte_head_form {
     const void *q_norm, *k_norm;
     const double* freq;
-    float eps, amplitude; /* eps in (0, 1] where there is a norm */
+    float eps, amplitude; /* eps 1e-30..1 where there is a norm; amplitude finite */
     int rotary_dim, interleaved;
 } vte_head_form;
 
 /* q_out, k_out = the rows' heads as `form` has them, row i at positions[i] (device int
- * [rows]; below 0: the row is left as it is in q_out and k_out; NULL without a
- * rotation).  q [rows][n_q][head_dim], k [rows][n_kv][head_dim] (dtype fp16 or fp32),
+ * [rows]; below 0: the row is left as it is in q_out and k_out; may be NULL without
+ * a rotation).  q [rows][n_q][head_dim], k [rows][n_kv][head_dim] (dtype fp16 or fp32),
  * rows q_stride / k_stride elements apart (0: contiguous); q_out and k_out contiguous,
  * or q and k themselves, with their strides.  q or k may be NULL.  head_dim 64, 128 or
  * 256; rows <= 2^24, rows * (n_q + n_kv) <= 2^27.  Rows and norms that are 16-byte

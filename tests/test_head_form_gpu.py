@@ -262,6 +262,93 @@ def test_append_token_by_token(hip, K, hd, dtype, rot):
             assert (off <= step + (np.array(want[b]["t"]) if n == "k" else 0)).all()  # 1/2 + 1/4 + ... of the last step
 
 
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_append_with_an_empty_form(hip, K, dtype):
+    """No norms and no rotation: the plain append's bytes, and q as it was; 200 sequences of none to three rows, in place."""
+    rng = np.random.default_rng(20)
+    new = [int(x) for x in rng.integers(0, 4, 200)]
+    pos = [int(p) if b % 7 else -1 for b, p in enumerate(rng.integers(0, 40, 200))]
+    lens = [max(p, 0) + n for p, n in zip(pos, new)]
+    a = Batch(hip, K, rng, lens, 1, 64, 16, width=3)
+    R = sum(new)
+    q, k, v = normal(rng, (R, 2, 64), dtype), up(hip, normal(rng, (R, 1, 64), dtype)), up(hip, normal(rng, (R, 1, 64), dtype))
+    r = a.rows(pos, new)
+    K.kv_pages_append(a.pages, r, k, v, dtype=dtype, stream=hip.stream)
+    want = [down(a.d[n]).copy() for n in ("k", "v", "ke", "ve")]
+    a.upload()
+    r = a.rows(pos, new)
+    f, dq = Form(hip, rng, 64, None, norms=(False, False)), up(hip, q)
+    K.kv_pages_append_norm(a.pages, r, f.c, k, v, q=dq, q_out=dq, n_q=2, dtype=dtype, stream=hip.stream)
+    assert all(np.array_equal(down(a.d[n]), w) for n, w in zip(("k", "v", "ke", "ve"), want))
+    assert np.array_equal(down(dq), q)
+
+
+@pytest.mark.parametrize("batch", [3, 64, 65, 200])
+def test_append_to_many_sequences(hip, K, batch):
+    """A few rows of each of many sequences, some of none, some that do not run, rows of nobody before the first one's."""
+    rng = np.random.default_rng(batch)
+    new = [int(n) for n in rng.integers(0, 4, batch)]
+    new[1] = 3
+    pos = [int(p) if b % 7 else -1 for b, p in enumerate(rng.integers(0, 40, batch))]
+    bt = Batch(hip, K, rng, [max(p, 0) + n for p, n in zip(pos, new)], 2, 64, 16, width=3)
+    r = bt.rows(pos, new, pad=2)
+    start = (2 + np.concatenate([[0], np.cumsum(new)])).astype(np.int32)
+    bt.d["start"] = up(hip, start)
+    r.row_start = bt.d["start"].ptr
+    R = int(start[-1])
+    for n_q in (1, 6):
+        f = Form(hip, rng, 64, 64)
+        q, k, v = normal(rng, (R, n_q, 64), "f16"), normal(rng, (R, 2, 64), "f16"), normal(rng, (R, 2, 64), "f16")
+        do = up(hip, np.full(q.shape, 9, np.float16))
+        K.kv_pages_append_norm(bt.pages, r, f.c, up(hip, k), up(hip, v), q=up(hip, q), q_out=do, n_q=n_q, stream=hip.stream)
+        got = down(do)
+        assert (got[:2] == 9).all()
+        for b, n in enumerate(new):
+            mine = slice(int(start[b]), int(start[b + 1]))
+            if pos[b] < 0:
+                assert (got[mine] == 9).all()
+            elif n:
+                at = pos[b] + np.arange(n)
+                check("f16", got[mine], *f.of(q[mine], at, False), f"{n_q} heads, sequence {b}")
+                kk, tol = f.of(k[mine], at, True)
+                check_pages_of(bt, b, pos[b], kk, tol, "k")
+                check_pages_of(bt, b, pos[b], v[mine].astype(np.float64), 0 * tol, "v")
+
+
+def test_captured_heads_follow_staged_positions(hip, K):
+    """Rows in place and an append as one graph, replayed with other positions, eager work between."""
+    rng = np.random.default_rng(22)
+    bt = Batch(hip, K, rng, [60, 60], 2, 128, 32)
+    f = Form(hip, rng, 128, 64, True)
+    q, k, v = (normal(rng, (2, h, 128), "f16") for h in (4, 2, 2))
+    dq, do, dk, dv, ko = up(hip, q), empty(hip, q.shape, np.float16), up(hip, k), up(hip, v), empty(hip, k.shape, np.float16)
+    r = bt.rows([0, 0])
+    off = bt.d["off"]
+    hip.stream_synchronize()
+    hip.stream_begin_capture()
+    K.kv_pages_append_norm(bt.pages, r, f.c, dk, dv, q=dq, q_out=do, n_q=4, stream=hip.stream)
+    K.qk_norm_rope(f.c, 2, off, k=dk, k_out=ko, n_kv=2, stream=hip.stream)
+    g = hip.stream_end_capture()
+    ge = hip.graph_instantiate(g)
+    try:
+        for pos in ([0, 3], [17, 40], [33, 0], [59, 48]):
+            off.upload(np.array(pos, np.int32))
+            hip.graph_launch(ge)
+            hip.synchronize()
+            check("f16", down(do), *f.of(q, pos, False))
+            kk, tol = f.of(k, pos, True)
+            check("f16", down(ko), kk, tol)
+            eager = empty(hip, k.shape, np.float16)
+            K.qk_norm_rope(f.c, 2, off, k=dk, k_out=eager, n_kv=2, stream=hip.stream)
+            assert np.array_equal(down(eager), down(ko))
+            for b in range(2):
+                if pos[b] % 16 == 0:
+                    check_pages_of(bt, b, pos[b], kk[b:b + 1], tol[b:b + 1], "k")
+    finally:
+        hip.graph_exec_destroy(ge)
+        hip.graph_destroy(g)
+
+
 def test_append_not_finite(hip, K):
     """A row of k with an Inf or a NaN makes its block read as NaN, and no other."""
     rng = np.random.default_rng(6)

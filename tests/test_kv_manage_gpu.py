@@ -178,6 +178,26 @@ def test_fork(hip, K, page, n_layers, n_kv, hd):
     p.check()
 
 
+def test_forks_of_more_entries_than_a_block_has_threads(hip, K):
+    """60 children of 3 parents in tables of 24 pages, a launch that shares before the one that finds pages; then the number
+    of missing pages is not asked for."""
+    rng = np.random.default_rng(19)
+    table = np.full((70, 24), -1)
+    order = rng.permutation(300)
+    table[0, :20], table[1, :3], table[2, :24] = order[:20], order[20:23], order[23:47]
+    table[5, 3:9], table[60, ::2] = order[50:56], order[60:72]
+    p = Pools(hip, K, rng, table, 300, page=32, n_layers=2, n_kv=1)
+    par = [i % 3 for i in range(60)]
+    p.fork(par, list(range(3, 63)), [int(x) for x in rng.integers(0, 800, 60)])
+    p.check()
+    p.ref.fork([3, 0], [65, 66], [40, 639])
+    K.kv_pages_fork(p.layers, p.t, 2, p.ints([3, 0]), p.ints([65, 66]), p.ints([40, 639]), None, empty(hip, 16, np.uint8), 16,
+                    stream=hip.stream)
+    p.ref.reserve([64], [5], 70)
+    K.kv_pages_reserve(p.t, 1, p.ints([5]), 70, None, seqs=p.ints([64]), stream=hip.stream)
+    p.check()
+
+
 def test_forks_without_free_pages(hip, K):
     """The first children of the list get the pages there are; the others' last entry is none."""
     rng = np.random.default_rng(11)
@@ -190,10 +210,10 @@ def test_forks_without_free_pages(hip, K):
 
 
 @pytest.mark.parametrize("n_pages,used", [(1, 0), (1, 1), (10, 4), (300, 150), (1024, 1024), (1025, 700), (5000, 2048), (5000, 4999),
-                                          (4096, 1024)])
+                                          (4096, 1024), (8192, 5000), (8193, 1024), (20001, 15000)])
 def test_compact(hip, K, n_pages, used):
     """Pools from empty to full, their sizes and numbers of used pages at and beside the chunks' borders, shared pages,
-    users that no table names."""
+    users that no table names; every block counting all pages, and a launch of counts before."""
     rng = np.random.default_rng(n_pages + used)
     rows = 1 + used // 13
     table = scattered(rng, rows, 14, n_pages, used - used // 9)

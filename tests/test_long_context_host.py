@@ -66,7 +66,7 @@ def test_window_scratch_goes_by_the_window():
     assert K.attn_pages_window_scratch_bytes(c, r, 4, 2 ** 31 - 1, 2 ** 31 - 1) == K.attn_pages_scratch_bytes(c, r, 4)
 
 
-BAD_FORMS = [dict(freq=P + 4), dict(q_norm=P + 1), dict(k_norm=P + 1), dict(eps=0.0), dict(eps=-1.0), dict(eps=float("nan")),
+BAD_FORMS = [dict(freq=P + 4), dict(q_norm=P + 1), dict(k_norm=P + 1), dict(eps=0.0), dict(eps=9e-31), dict(eps=-1.0), dict(eps=float("nan")),
              dict(eps=2.0), dict(rotary_dim=3), dict(rotary_dim=-2), dict(rotary_dim=130), dict(amplitude=float("inf")),
              dict(amplitude=float("nan"))]
 

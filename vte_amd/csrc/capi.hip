@@ -970,7 +970,7 @@ static int check_form(const char* who, const vte_head_form* f, int hd, HeadForm*
     REQUIRE(f, "%s: null form", who);
     REQUIRE(aligned(f->q_norm, 2) && aligned(f->k_norm, 2) && aligned(f->freq, 8),
             "%s: norms must be 2-byte and frequencies 8-byte aligned", who);
-    REQUIRE(!(f->q_norm || f->k_norm) || (f->eps > 0.f && f->eps <= 1.f), "%s: eps outside (0, 1]", who);
+    REQUIRE(!(f->q_norm || f->k_norm) || (f->eps >= 1e-30f && f->eps <= 1.f), "%s: eps outside 1e-30..1", who);
     const int rot = f->rotary_dim ? f->rotary_dim : hd;
     if (f->freq) {
         REQUIRE(rot >= 2 && rot <= hd && rot % 2 == 0, "%s: bad rotary_dim %d", who, f->rotary_dim);
