@@ -147,6 +147,24 @@ def test_reserve_for_more_slots_than_a_block_has_threads(hip, K):
     p.check()
 
 
+@pytest.mark.parametrize("n_pages", [16383, 16386, 50003])
+@pytest.mark.parametrize("shift", [1, 2, 3])
+def test_reserve_from_unaligned_users(hip, K, n_pages, shift):
+    """Users at any 4-byte address, pools around the pages that are looked at together, the last pages among the free."""
+    rng = np.random.default_rng(n_pages + shift)
+    refs = np.ones(n_pages, np.int32)
+    free = np.sort(np.concatenate([rng.permutation(n_pages - 3)[:30], [n_pages - 1, n_pages - 2]]))
+    refs[free] = 0
+    refs[free[3]] = -7  # (counts below 0 are none)
+    d = up(hip, np.concatenate([np.zeros(shift, np.int32), refs]))
+    table, missing = up(hip, np.full((40, 2), -1, np.int32)), up(hip, np.zeros(1, np.int32))
+    t = KVTables.of(table, d.ptr + 4 * shift, 40, 2, n_pages, 16)
+    K.kv_pages_reserve(t, 40, up(hip, np.full(40, 20, np.int32)), 1, missing, stream=hip.stream)
+    got, now = down(table), down(d)[shift:]
+    assert np.array_equal(got[:32, 1], free) and (got[32:] == -1).all() and (got[:, 0] == -1).all() and down(missing)[0] == 8
+    assert (now == 1).all() and not down(d)[:shift].any()
+
+
 def test_the_same_sequence_twice_costs_no_page(hip, K):
     rng = np.random.default_rng(9)
     p = Pools(hip, K, rng, np.full((3, 4), -1), 40)

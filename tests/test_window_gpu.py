@@ -256,3 +256,50 @@ def test_captured_windows_follow_staged_lengths(hip, K, new):
     finally:
         hip.graph_exec_destroy(ge)
         hip.graph_destroy(g)
+
+
+def test_two_streams_at_once(hip, K):
+    """Windows over a prompt chunk, windows of decoded tokens, heads and a pool's calls on three streams that are not the
+    runtime's, each with memory of its own, together: the results of each alone."""
+    import ctypes
+    from tests.test_head_form_gpu import Form
+    from tests.test_kv_manage_gpu import Pools
+    rng = np.random.default_rng(41)
+    streams = []
+    for _ in range(3):
+        s = ctypes.c_void_p()
+        hip._check_error(hip._lib.hipStreamCreate(ctypes.byref(s)), "hipStreamCreate")
+        streams.append(s)
+    jobs, outs = [], []
+    for new, s in zip((1, 150), streams):
+        bt = filled(hip, K, rng, [900, 333], 2, 128, 64)
+        q, r = up(hip, normal(rng, (2 * new, 8, 128), "f16")), bt.rows([900 - new, 333 - new], [new, new])
+        n = K.attn_pages_window_scratch_bytes(bt.pages, r, 8, 200, 4)
+        o, sc = empty(hip, (2 * new, 8, 128), np.float16), empty(hip, n, np.uint8)
+        jobs.append(lambda bt=bt, r=r, q=q, o=o, sc=sc, n=n, s=s: K.attn_pages_window(bt.pages, r, q, o, 8, 0.1, 200, 4, sc, n, stream=s))
+        outs.append(o)
+    f, x, y = Form(hip, rng, 128, 128), up(hip, normal(rng, (200, 8, 128), "f16")), empty(hip, (200, 8, 128), np.float16)
+    pos = up(hip, np.arange(200, dtype=np.int32))
+    jobs.append(lambda: K.qk_norm_rope(f.c, 200, pos, q=x, q_out=y, n_q=8, stream=streams[2]))
+    p = Pools(hip, K, rng, np.full((8, 6), -1), 60)
+    start = p.ints([10] * 8)
+
+    def pool():
+        K.kv_pages_free(p.t, 8, stream=streams[2])
+        K.kv_pages_reserve(p.t, 8, start, 60, None, stream=streams[2])
+    jobs.append(pool)
+    outs += [y, p.table, p.refs]
+    try:
+        for job in jobs:
+            job()
+            hip.synchronize()
+        alone = [down(o).copy() for o in outs]
+        for _ in range(10):
+            for job in jobs:
+                job()
+        hip.synchronize()
+        for o, a in zip(outs, alone):
+            assert np.array_equal(down(o), a)
+    finally:
+        for s in streams:
+            hip._lib.hipStreamDestroy(s)

@@ -83,7 +83,8 @@ __global__ __launch_bounds__(256) void kv_copy_kernel(KvLayers L, int layer_word
 }
 
 // ---------------------------------------------------------------------------
-// Pages given back: entries of whole pages of tokens keep .. end[i] - behind - 1.  grid (entries, sequences).
+// Pages given back: entries of whole pages of tokens keep .. end[i] - behind - 1.  grid (entries, sequences); a chain of
+// loads and atomics, 2.6 to 3 us.
 // ---------------------------------------------------------------------------
 __global__ __launch_bounds__(256) void kv_free_kernel(KvTables t, const int* __restrict__ seqs, int keep,
                                                       const int* __restrict__ end, int behind) {
@@ -98,15 +99,18 @@ __global__ __launch_bounds__(256) void kv_free_kernel(KvTables t, const int* __r
 }
 
 // ---------------------------------------------------------------------------
-// New pages, by one block of 1024 threads.  `want(slot)` says whether a slot of 0 .. slots - 1 needs one, `give(slot,
-// page)`, called by the same thread right after, takes it (page -1: there are no more).  The result: slots that got none.
-// Free pages are found 4096 at a time into a ring in LDS, only when a slot needs them.
+// New pages, by one block of 1024 threads, so that they are the lowest free ones in the slots' order without a wait between
+// blocks.  `want(slot)` says whether a slot of 0 .. slots - 1 needs one, `give(slot, page)`, called by the same thread right
+// after, takes it (page -1: there are no more).  The result: slots that got none.
+//
+// Pages are looked at 16384 at a time, the next ones asked for meanwhile, and free ones put into a ring in LDS, 4096 pages'
+// at a time while slots need them.  Bound by latency: a chain of five loads and atomics, 2.8 us of eight sequences, 4.2 of
+// 64; a reserve and a free where the last 70 of 4096, 65536 or 2^20 pages are free 6.8, 14 to 17 and 83 us (4096 pages at a
+// time and none ahead: 6.9, 30 and 410).  (refs of pages that were not looked at yet do not change in the call: what it takes or gives back lies
+// before them.)
 // ---------------------------------------------------------------------------
 #define KVM_RING 8192
-// (refs are read past the first cache: users may have been counted in the same launch)
-__device__ __forceinline__ int kvm_users(const KvTables& t, int p) {
-    return __hip_atomic_load(&t.refs[p], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
+#define KVM_LOOK 16384
 template <class Want, class Give>
 __device__ __forceinline__ int kvm_new_pages(const KvTables& t, int slots, Want want, Give give) {
     __shared__ int ring[KVM_RING];
@@ -131,27 +135,51 @@ __device__ __forceinline__ int kvm_new_pages(const KvTables& t, int slots, Want 
         }
         return before + incl - v;
     };
-    int ahead[4];  // the first pages, asked for while it is not known yet whether a slot needs one
+    uint4 ahead[4];
+    auto ask = [&](int base) {  // for this thread's four pages of every 4096 from base on
 #pragma unroll
-    for (int u = 0; u < 4; ++u) ahead[u] = 4 * tid + u < t.n_pages && kvm_users(t, 4 * tid + u) <= 0;
+        for (int g = 0; g < 4; ++g) {
+            const int p = base + 4096 * g + 4 * tid;
+            ahead[g] = make_uint4(1, 1, 1, 1);
+            if (p + 4 <= t.n_pages) {
+                ahead[g] = ldg_g16(t.refs + p);
+            } else if (p < t.n_pages) {
+                ahead[g].x = t.refs[p];
+                if (p + 1 < t.n_pages) ahead[g].y = t.refs[p + 1];
+                if (p + 2 < t.n_pages) ahead[g].z = t.refs[p + 2];
+            }
+        }
+    };
+    uint32_t free_bits = 0;  // of the pages at hand: bit 4 g + u
+    auto look = [&] {
+        free_bits = 0;
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            free_bits |= (uint32_t)((int)ahead[g].x <= 0) << (4 * g) | (uint32_t)((int)ahead[g].y <= 0) << (4 * g + 1) |
+                         (uint32_t)((int)ahead[g].z <= 0) << (4 * g + 2) | (uint32_t)((int)ahead[g].w <= 0) << (4 * g + 3);
+    };
+    ask(0);  // (while it is not known yet whether a slot needs one)
     int head = 0, have = 0, next = 0, missing = 0;  // of the ring; the first page not looked at
     for (int s0 = 0; s0 < slots; s0 += 1024) {
         const bool w = s0 + tid < slots && want(s0 + tid);
         int n;
         const int rank = scan(w, n);
         while (have < n && next < t.n_pages) {
-            int r[4], count = 0;
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int p = next + 4 * tid + u;
-                r[u] = next == 0 ? ahead[u] : p < t.n_pages && kvm_users(t, p) <= 0;
-                count += r[u];
+            const int group = next / 4096 % (KVM_LOOK / 4096);
+            if (group == 0) {
+                look();
+                if (next + KVM_LOOK < t.n_pages) ask(next + KVM_LOOK);
+                if (next > 0 && !__syncthreads_or(free_bits != 0)) {  // (the lowest pages: with the scan)
+                    next += KVM_LOOK;
+                    continue;
+                }
             }
+            const uint32_t mine = free_bits >> (4 * group) & 15;
             int found;
-            int at = head + have + scan(count, found);
+            int at = head + have + scan(__popc(mine), found);
 #pragma unroll
             for (int u = 0; u < 4; ++u)
-                if (r[u]) ring[at++ & (KVM_RING - 1)] = next + 4 * tid + u;
+                if (mine >> u & 1) ring[at++ & (KVM_RING - 1)] = next + 4 * tid + u;
             have += found;
             next += 4096;
         }

@@ -26,6 +26,10 @@
 // for one token.  Prompts: bytes, 41 MB of four chunks of 700 to 2048 tokens with
 // their q in 10.7 us, 3.9 TB/s (a large copy reaches 5.0).  With the read-back of the
 // chunks, us: 14.7 WIDE, 44.0 otherwise; one token each of 64 sequences 12.6 / 13.9.
+//
+// R says how heads are turned: KvRope by tables, HeadForm normed and by frequencies (head_turn.h), whose WIDE form needs
+// pairs that are neighbours or a rotary_dim that is a multiple of 16, and has a block's rows share their cosines: the same
+// chunks 16.4 with their read-back (20.1 with cosines by each thread), one token each of 64 sequences 12.5 (13.7).
 // ---------------------------------------------------------------------------
 struct KvRope {
     const __half *cosc, *sinc;
