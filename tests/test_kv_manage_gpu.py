@@ -354,6 +354,19 @@ def test_pages_beyond_32_bits(hip, K):
         assert np.abs(want[0][0].astype(np.float64) - rows[0]).max() < 0.1
         K.kv_pages_copy(L, up(hip, np.array([n_pages - 1], np.int32)), up(hip, np.array([2], np.int32)), 1, stream=hip.stream)
         assert all(np.array_equal(a, b) for a, b in zip(read(2), want))
+
+        def attend(entry):
+            table.upload(np.array([[entry]], np.int32))
+            out = []
+            for new in (1, 20):
+                rr = KVRows.of(1, new, new, up(hip, np.array([0, new], np.int32)), up(hip, np.array([33 - new], np.int32)), table, 1)
+                n, o = K.attn_pages_window_scratch_bytes(pages, rr, 4, 9, 2), empty(hip, (new, 4, hd), np.float16)
+                K.attn_pages_window(pages, rr, up(hip, q[:new]), o, 4, 0.1, 9, 2, empty(hip, n, np.uint8), n, stream=hip.stream)
+                out.append(down(o).copy())
+            return out
+        q = normal(rng, (20, 4, hd), "f16")
+        far, near = attend(n_pages - 1), attend(2)
+        assert all(np.array_equal(a, b) and np.abs(a).max() > 0 for a, b in zip(far, near))
         table.upload(np.array([[n_pages - 1]], np.int32))
         refs = np.zeros(n_pages, np.int32)
         refs[-1] = 1

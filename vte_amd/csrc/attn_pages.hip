@@ -772,9 +772,8 @@ __device__ __forceinline__ void pa_apart(const KvPages& c, const int* table, int
 // grid (row blocks * n_kv, nsp), the last row blocks (which see most) first, whatever their head: with the heads one after
 // the other some started long ones late (four ragged fp32 prompts 65 -> 53 us).  nsp > 1 with two groups only.
 template <typename T, int HD, int GROUPS, int WAVES, bool WIN>
-__global__ __launch_bounds__(64 * GROUPS * WAVES, GROUPS * WAVES == 4 && HD == 64 ? 3 : 2) void attn_pages_prompt_kernel(KvPages c, KvRows r, PaPrompt pp,
-                                                                   const T* q, T* out,
-                                                                   int n_q, float scale, PaWindow win) {
+__global__ __launch_bounds__(64 * GROUPS * WAVES, GROUPS * WAVES == 4 && HD == 64 ? 3 : 2) void attn_pages_prompt_kernel(
+    KvPages c, KvRows r, PaPrompt pp, const T* q, T* out, int n_q, float scale, PaWindow win) {
     constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;  // fp16 parts of q
     constexpr int ROWS = 32 * WAVES;  // of a group
     constexpr int KS = HD / 16, DT = HD / 32;              // 16-dim steps of a score, 32-dim tiles

@@ -52,6 +52,10 @@ template <bool ONCE>
 __device__ __forceinline__ void kvm_copy(const KvLayers& L, int layer_words, int exps, int n_pages, const int* src,
                                          const int* dst, int n) {
     const int words = 2 * layer_words, piece = blockIdx.x, l = blockIdx.y;  // 16-byte words of a page, K and V
+    auto at = [&](int page, int w) {
+        return w < layer_words ? L.k[l] + ((size_t)page * layer_words + w) * 16
+                               : L.v[l] + ((size_t)page * layer_words + w - layer_words) * 16;
+    };
     for (int i = blockIdx.z; i < n; i += gridDim.z) {
         const int a = src[i], b = dst[i];
         if ((unsigned)a >= (unsigned)n_pages || (unsigned)b >= (unsigned)n_pages) continue;
@@ -59,16 +63,13 @@ __device__ __forceinline__ void kvm_copy(const KvLayers& L, int layer_words, int
 #pragma unroll
         for (int u = 0; u < KVM_PIECE / 256; ++u) {
             const int w = piece * KVM_PIECE + u * 256 + threadIdx.x;
-            if (w < words) x[u] = kvm_load<ONCE>(w < layer_words ? L.k[l] + ((size_t)a * layer_words + w) * 16
-                                                          : L.v[l] + ((size_t)a * layer_words + w - layer_words) * 16);
+            if (w < words) x[u] = kvm_load<ONCE>(at(a, w));
         }
 #pragma unroll
         for (int u = 0; u < KVM_PIECE / 256; ++u) {
             const int w = piece * KVM_PIECE + u * 256 + threadIdx.x;
             if (w < words)
-                __builtin_nontemporal_store(vte_u32x4{x[u].x, x[u].y, x[u].z, x[u].w},
-                                            reinterpret_cast<vte_u32x4*>(w < layer_words ? L.k[l] + ((size_t)b * layer_words + w) * 16
-                                                                                         : L.v[l] + ((size_t)b * layer_words + w - layer_words) * 16));
+                __builtin_nontemporal_store(vte_u32x4{x[u].x, x[u].y, x[u].z, x[u].w}, reinterpret_cast<vte_u32x4*>(at(b, w)));
         }
         if (piece == 0)
             for (int e = threadIdx.x; e < exps; e += 256) {
@@ -106,8 +107,8 @@ __global__ __launch_bounds__(256) void kv_free_kernel(KvTables t, const int* __r
 // Pages are looked at 16384 at a time, the next ones asked for meanwhile, and free ones put into a ring in LDS, 4096 pages'
 // at a time while slots need them.  Bound by latency: a chain of five loads and atomics, 2.8 us of eight sequences, 4.2 of
 // 64; a reserve and a free where the last 70 of 4096, 65536 or 2^20 pages are free 6.8, 14 to 17 and 83 us (4096 pages at a
-// time and none ahead: 6.9, 30 and 410).  (refs of pages that were not looked at yet do not change in the call: what it takes or gives back lies
-// before them.)
+// time and none ahead: 6.9, 30 and 410).  (refs of pages that were not looked at yet do not change in the call: what it
+// takes or gives back lies before them.)
 // ---------------------------------------------------------------------------
 #define KVM_RING 8192
 #define KVM_LOOK 16384
@@ -290,10 +291,9 @@ __global__ __launch_bounds__(1024) void kv_fork_last_kernel(KvTables t, KvFork f
 
 // ---------------------------------------------------------------------------
 // Compaction: with U used pages, the k-th used page from U on moves to the k-th free one below U.  Counts per chunk (of
-// up to KVM_FEW pages every block counts them all itself, a launch less, a graph's us: 1000 pages 10.4 against 11.9, 8192 13.8
-// against 14.8, 16384 17.9 against 16.4); then every block knows U and what
-// lies before its chunk, lists its pages' places and writes where each page goes, those that move as -2 - k until the
-// copies' launch, which knows the lists.
+// up to KVM_FEW pages every block counts them all itself, a launch less, a graph's us: 1000 pages 10.4 against 11.9, 8192
+// 13.8 against 14.8, 16384 17.9 against 16.4); then every block knows U and what lies before its chunk, lists its pages'
+// places and writes where each page goes, those that move as -2 - k until the copies' launch, which knows the lists.
 // ---------------------------------------------------------------------------
 struct KvMoves {
     int *counts, *src, *dst, *moves;  // used pages of each chunk; pairs; how many
