@@ -176,6 +176,21 @@ def test_the_same_sequence_twice_costs_no_page(hip, K):
     assert down(p.refs).sum() == 4 and (down(p.refs) >= 0).all()
 
 
+@pytest.mark.parametrize("times", [300, 1500])
+def test_a_sequence_many_times_keeps_its_lowest_pages(hip, K, times):
+    """Two entries of one sequence asked for over and over, then those of others: the same pages every time.  (1024 slots
+    are served together; later ones see what the earlier ones were given.)"""
+    rng = np.random.default_rng(times)
+    first = min(2 * times, 1024)  # pages taken for sequence 1
+    for _ in range(5):
+        p = Pools(hip, K, rng, [[-1, -1], [10 ** 6, -9], [-1, -1]], 4000, n_layers=1, n_kv=1)
+        seqs = [1] * times + [2, 0]
+        p.K.kv_pages_reserve(p.t, len(seqs), p.ints([0] * len(seqs)), 32, p.missing, seqs=p.ints(seqs), stream=hip.stream)
+        assert np.array_equal(down(p.table), [[first + 2, first + 3], [0, 1], [first, first + 1]])
+        refs = down(p.refs)
+        assert refs.sum() == 6 and (refs[down(p.table)] == 1).all() and down(p.missing)[0] == 0
+
+
 @pytest.mark.parametrize("page,n_layers,n_kv,hd", [(16, 1, 1, 64), (64, 3, 2, 128), (32, 66, 1, 64)])
 def test_fork(hip, K, page, n_layers, n_kv, hd):
     """One parent and several, lengths of whole pages, of none, inside pages, past the parent's pages and the table's end,

@@ -6,7 +6,7 @@
 // one refs array serve the pools of all layers: only copies touch bytes.  New pages are always the lowest free ones, in
 // the order of the call's list, so what a call does depends on its inputs alone and not on which block came first; users
 // are counted by integer atomics, whose order does not matter.  Entries are exchanged, not written, and what stood there
-// loses a user: a sequence listed twice costs no page.
+// loses a user; new pages of one entry (of a sequence listed twice) are compared, and the lowest stays.
 #include <algorithm>
 #include "kv_pages.h"
 
@@ -30,6 +30,12 @@ __device__ __forceinline__ void kvm_release(const KvTables& t, int p) {
 // Entry j of a row becomes p, whose user it already counts as.
 __device__ __forceinline__ void kvm_set(const KvTables& t, int row, int j, int p) {
     kvm_release(t, atomicExch(&t.table[(size_t)row * t.max_pages + j], p));
+}
+// Entry j of a row, which is no page (above all of them without a sign), becomes p, whose user it already counts as, or
+// keeps the lower page that it was given meanwhile.
+__device__ __forceinline__ void kvm_set_lowest(const KvTables& t, int row, int j, int p) {
+    const unsigned old = atomicMin(reinterpret_cast<unsigned*>(&t.table[(size_t)row * t.max_pages + j]), (unsigned)p);
+    kvm_release(t, (int)max(old, (unsigned)p));
 }
 
 // ---------------------------------------------------------------------------
@@ -219,9 +225,12 @@ __global__ __launch_bounds__(1024) void kv_reserve_kernel(KvTables t, int n, con
     };
     const int short_of = kvm_new_pages(
         t, n * per,
-        [&](int slot) { return entry(slot) && !kvm_is_page(t, t.table[(size_t)row * t.max_pages + j]); },
+        [&](int slot) {  // (not from the cache of this CU: the entry may have been given a page by an earlier slot)
+            return entry(slot) && !kvm_is_page(t, __hip_atomic_load(&t.table[(size_t)row * t.max_pages + j], __ATOMIC_RELAXED,
+                                                                    __HIP_MEMORY_SCOPE_AGENT));
+        },
         [&](int, int page) {
-            if (page >= 0) kvm_set(t, row, j, page);
+            if (page >= 0) kvm_set_lowest(t, row, j, page);
         });
     if (missing != nullptr && threadIdx.x == 0) *missing = short_of;
 }
