@@ -442,7 +442,8 @@ long long vte_attn_pages_scratch_bytes(const vte_kv_pages* cache, const vte_kv_r
 int vte_attn_pages(const vte_kv_pages* cache, const vte_kv_rows* rows, int dtype, const void* q, void* out, int n_q,
                    float scale, void* scratch, long long scratch_bytes, void* stream);
 
-/* Scratch bytes of vte_attn_pages_window (-1: rejected arguments); as those of vte_attn_pages. */
+/* Scratch bytes of vte_attn_pages_window (-1: rejected arguments); as those of
+ * vte_attn_pages: ask for each shape and window. */
 long long vte_attn_pages_window_scratch_bytes(const vte_kv_pages* cache, const vte_kv_rows* rows, int n_q, int window,
                                               int sinks);
 
@@ -539,7 +540,8 @@ long long vte_kv_pages_fork_scratch_bytes(int n);
  * layer.  Entries that are no page stay so.  Where no page is free the last entry is -1;
  * missing (device int, may be NULL) counts those.  A child must be in the list once, and
  * not be a parent in it; a child that is its own parent, or a length below 0, is passed
- * over. */
+ * over.  scratch: 16-byte aligned, need not be cleared; calls that may overlap need one
+ * each. */
 int vte_kv_pages_fork(const vte_kv_pages* layers, int n_layers, const vte_kv_tables* tables, int n, const int* parents,
                       const int* children, const int* lengths, int* missing, void* scratch, long long scratch_bytes,
                       void* stream);
@@ -550,7 +552,8 @@ long long vte_kv_pages_compact_scratch_bytes(const vte_kv_tables* tables);
 /* The pool's used pages (refs above 0) become its first ones: with U of them, the k-th
  * used page from U on moves to the k-th free one below U, in every layer; entries and
  * refs follow (an entry that names a free page becomes -1).  used (device int) = U;
- * where (device int [n_pages]) = the place each used page has now, -1 of free ones. */
+ * where (device int [n_pages]) = the place each used page has now, -1 of free ones.
+ * Pages moved from keep their bytes.  scratch as that of the fork. */
 int vte_kv_pages_compact(const vte_kv_pages* layers, int n_layers, const vte_kv_tables* tables, int* where, int* used,
                          void* scratch, long long scratch_bytes, void* stream);
 

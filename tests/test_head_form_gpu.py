@@ -263,6 +263,32 @@ def test_append_token_by_token(hip, K, hd, dtype, rot):
 
 
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("rot,inter", [(128, False), (64, True), (24, False)])
+def test_append_from_unaligned_rows(hip, K, dtype, rot, inter):
+    """q, k and v inside rows of an odd length, an element off 16-byte alignment, weights 2 bytes off."""
+    rng = np.random.default_rng(rot)
+    n_q, n_kv, hd, n = 5, 2, 128, 37
+    bt = Batch(hip, K, rng, [n + 11], n_kv, hd, 32)
+    f = Form(hip, rng, hd, rot, inter)
+    w = [up(hip, np.concatenate([np.zeros(1, np.float16), x])) for x in f.w]
+    f.c.q_norm, f.c.k_norm = w[0].ptr + 2, w[1].ptr + 2
+    ld = (n_q + 2 * n_kv) * hd + 3
+    flat = normal(rng, n * ld + 1, dtype)
+    d, do = up(hip, flat), empty(hip, (n, n_q, hd), NP[dtype])
+    size = flat.itemsize
+    K.kv_pages_append_norm(bt.pages, bt.rows([11], [n]), f.c, d.ptr + size * (1 + n_q * hd), d.ptr + size * (1 + (n_q + n_kv) * hd),
+                           q=d.ptr + size, q_out=do, n_q=n_q, dtype=dtype, k_stride=ld, v_stride=ld, q_stride=ld,
+                           stream=hip.stream)
+    x = flat[1:].reshape(n, ld)[:, :-3].reshape(n, n_q + 2 * n_kv, hd)
+    at = 11 + np.arange(n)
+    check(dtype, down(do), *f.of(x[:, :n_q], at, False))
+    k, tol = f.of(x[:, n_q:n_q + n_kv], at, True)
+    # (what stood in the first block's pages before has a say in its scale)
+    check_pages_of(bt, 0, 16, k[5:], tol[5:], "k")
+    check_pages_of(bt, 0, 16, x[5:, n_q + n_kv:].astype(np.float64), 0 * tol[5:], "v")
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
 def test_append_with_an_empty_form(hip, K, dtype):
     """No norms and no rotation: the plain append's bytes, and q as it was; 200 sequences of none to three rows, in place."""
     rng = np.random.default_rng(20)
