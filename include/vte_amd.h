@@ -527,9 +527,23 @@ int vte_kv_pages_free(const vte_kv_tables* tables, int n, const int* seqs, int k
  * that is no page gets one.  n * (pages of count tokens + 1) <= 2^24.  missing (device
  * int, may be NULL) = how many entries got none because no page was free.  A sequence in
  * the list twice is given pages twice: an entry keeps the lowest, the others are free
- * again after the call. */
+ * again after the call.
+ * A page comes with the bytes that its former user left.  Where one is given to an entry
+ * that start[i] lies inside, the tokens before start[i] count as being there from then on:
+ * the program has to append them too before anything reads the sequence, or call
+ * vte_kv_pages_extend. */
 int vte_kv_pages_reserve(const vte_kv_tables* tables, int n, const int* seqs, const int* start, const int* stop,
                          int count, int* missing, void* stream);
+
+/* The same for tokens that follow those before them, as in a loop of decoded tokens or
+ * prompt chunks: an entry that is no page and begins before start[i] stays so, and missing
+ * counts it, too.  Its tokens were dropped when there was no page for them (by this call,
+ * the reserve or the fork), and those that come after them in it are dropped likewise, so
+ * that nothing of a page's former user is ever seen; the sequence goes on with the next
+ * entry, without them.  To have them after all, append them again from the entry's
+ * first token on. */
+int vte_kv_pages_extend(const vte_kv_tables* tables, int n, const int* seqs, const int* start, const int* stop,
+                        int count, int* missing, void* stream);
 
 /* Scratch bytes of vte_kv_pages_fork for n children (0: n outside 1..65535). */
 long long vte_kv_pages_fork_scratch_bytes(int n);
@@ -537,8 +551,9 @@ long long vte_kv_pages_fork_scratch_bytes(int n);
 /* Sequence children[i] becomes the first lengths[i] tokens of parents[i]: its former
  * pages are given back, whole pages are shared with the parent (which neither may write
  * again below lengths[i]), the page in which they end is copied to a new one in every
- * layer.  Entries that are no page stay so.  Where no page is free the last entry is -1;
- * missing (device int, may be NULL) counts those.  A child must be in the list once, and
+ * layer.  Entries that are no page stay so.  Where no page is free the last entry is -1
+ * (the child has none of its tokens: go on with vte_kv_pages_extend); missing (device int,
+ * may be NULL) counts those.  A child must be in the list once, and
  * not be a parent in it; a child that is its own parent, or a length below 0, is passed
  * over.  scratch: 16-byte aligned, need not be cleared; calls that may overlap need one
  * each. */

@@ -69,8 +69,9 @@ class Pool:
                     self.release(self.table[b, j])
                     self.table[b, j] = -1
 
-    def reserve(self, seqs, start, count, stop=None):
-        """Entries are served in order; users change at the end only (a page given back is none of this call's)."""
+    def reserve(self, seqs, start, count, stop=None, follow=False):
+        """Entries are served in order; users change at the end only (a page given back is none of this call's).  ``follow``:
+        an entry that begins before its start gets no page."""
         missing = 0
         for i, b in enumerate(seqs):
             if not 0 <= b < len(self.table) or start[i] < 0:
@@ -79,7 +80,7 @@ class Pool:
             end = end if stop is None else min(end, stop[i])
             for j in range(start[i] // self.page, -(-end // self.page) if end > start[i] else 0):
                 if not self.is_page(self.table[b, j]):
-                    p = self.new_page()
+                    p = -1 if follow and j * self.page < start[i] else self.new_page()
                     missing += p < 0
                     if p >= 0:
                         self.table[b, j] = p

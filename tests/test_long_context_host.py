@@ -201,3 +201,26 @@ def test_pool_oracle_counts_users():
     where, used = p.compact()
     assert used == 2 and where.tolist() == [-1, -1, 0, 1, -1] and p.table.tolist() == [[0, -1, 1], [-1] * 3, [0, -1, -1]]
     assert p.content[:2] == ["c", "d"] and p.refs.tolist() == [2, 1, 0, 0, 0]
+
+
+def test_pool_oracle_leaves_begun_entries():
+    p = olc.Pool([[-1, 0, -1], [-1, -1, -1]], [1, 0, 0, 0], 16, "abcd")
+    assert p.reserve([0, 1, 1], [20, 7, 16], 20, follow=True) == 1
+    assert p.table.tolist() == [[-1, 0, 1], [-1, 2, 3]] and p.refs.tolist() == [1, 1, 1, 1]
+    assert p.reserve([1], [15], 1, follow=True) == 1 and p.reserve([0], [0], 16, follow=True) == 1
+
+
+# ---------------------------------------------------------------------------- room for tokens that follow others
+@pytest.mark.parametrize("bad", BAD_TABLES, ids=str)
+def test_extend_refuses_bad_tables(bad):
+    refused(lambda: kernels().kv_pages_extend(tables(**bad), 1, P, 1, P))
+
+
+def test_extend_refusals():
+    K, t = kernels(), tables()
+    refused(lambda: K.kv_pages_extend(t, 1, None, 1, P), lambda: K.kv_pages_extend(t, 1, P, 0, P),
+            lambda: K.kv_pages_extend(t, 4, P, 1, P), lambda: K.kv_pages_extend(t, 0, P, 1, P),
+            lambda: K.kv_pages_extend(t, 1, P, 1, P + 2), lambda: K.kv_pages_extend(t, 1, P + 1, 1, P),
+            lambda: K.kv_pages_extend(t, 1, P, 1, P, seqs=P + 2), lambda: K.kv_pages_extend(t, 1, P, 1, P, stop=P + 3),
+            lambda: K.kv_pages_extend(tables(max_pages=1 << 12), 65535, P, 1 << 30, P, seqs=P))
+    assert K.lib.vte_kv_pages_extend(None, 1, None, P, None, 1, P, None) == -1

@@ -95,7 +95,7 @@ hipError_t kv_pages_free(const KvTables& t, int n, const int* seqs, int keep, co
                          hipStream_t st);
 int kv_pages_reserve_slots(const KvTables& t, int count);
 hipError_t kv_pages_reserve(const KvTables& t, int n, const int* seqs, const int* start, const int* stop, int count,
-                            int* missing, hipStream_t st);
+                            bool follow, int* missing, hipStream_t st);
 long long kv_pages_fork_scratch_bytes(int n);
 hipError_t kv_pages_fork(const KvPages* layers, int n_layers, int hd, const KvTables& t, int n, const int* parents,
                          const int* children, const int* lengths, int* missing, void* scratch, hipStream_t st);
@@ -1090,18 +1090,28 @@ int vte_kv_pages_free(const vte_kv_tables* tables, int n, const int* seqs, int k
     return hip_status(vte::kv_pages_free(t, n, seqs, keep, end, behind, (hipStream_t)stream), "vte_kv_pages_free launch");
 }
 
+static int reserve_pages(const char* who, const vte_kv_tables* tables, int n, const int* seqs, const int* start,
+                         const int* stop, int count, bool follow, int* missing, void* stream) {
+    KvTables t;
+    if (int rc = check_tables(who, tables, n, &t)) return rc;
+    REQUIRE(start && aligned(start, 4) && aligned(seqs, 4) && aligned(stop, 4) && aligned(missing, 4),
+            "%s: start must be there, all 4-byte aligned", who);
+    REQUIRE(seqs || n <= t.batch, "%s: %d sequences of %d", who, n, t.batch);
+    REQUIRE(count >= 1, "%s: count %d", who, count);
+    REQUIRE((long long)n * vte::kv_pages_reserve_slots(t, count) <= (1 << 24),
+            "%s: %d sequences x pages of %d tokens above 2^24", who, n, count);
+    return hip_status(vte::kv_pages_reserve(t, n, seqs, start, stop, count, follow, missing, (hipStream_t)stream),
+                      follow ? "vte_kv_pages_extend launch" : "vte_kv_pages_reserve launch");
+}
+
 int vte_kv_pages_reserve(const vte_kv_tables* tables, int n, const int* seqs, const int* start, const int* stop,
                          int count, int* missing, void* stream) {
-    KvTables t;
-    if (int rc = check_tables("kv_pages_reserve", tables, n, &t)) return rc;
-    REQUIRE(start && aligned(start, 4) && aligned(seqs, 4) && aligned(stop, 4) && aligned(missing, 4),
-            "kv_pages_reserve: start must be there, all 4-byte aligned");
-    REQUIRE(seqs || n <= t.batch, "kv_pages_reserve: %d sequences of %d", n, t.batch);
-    REQUIRE(count >= 1, "kv_pages_reserve: count %d", count);
-    REQUIRE((long long)n * vte::kv_pages_reserve_slots(t, count) <= (1 << 24),
-            "kv_pages_reserve: %d sequences x pages of %d tokens above 2^24", n, count);
-    return hip_status(vte::kv_pages_reserve(t, n, seqs, start, stop, count, missing, (hipStream_t)stream),
-                      "vte_kv_pages_reserve launch");
+    return reserve_pages("kv_pages_reserve", tables, n, seqs, start, stop, count, false, missing, stream);
+}
+
+int vte_kv_pages_extend(const vte_kv_tables* tables, int n, const int* seqs, const int* start, const int* stop,
+                        int count, int* missing, void* stream) {
+    return reserve_pages("kv_pages_extend", tables, n, seqs, start, stop, count, true, missing, stream);
 }
 
 long long vte_kv_pages_fork_scratch_bytes(int n) { return n >= 1 && n <= 65535 ? vte::kv_pages_fork_scratch_bytes(n) : 0; }

@@ -208,11 +208,17 @@ __device__ __forceinline__ int kvm_new_pages(const KvTables& t, int slots, Want 
     return missing;
 }
 
-// Entries of tokens start[i] .. start[i] + count - 1 (below stop[i]) of each sequence; `per` slots a sequence.
+// Entries of tokens start[i] .. start[i] + count - 1 (below stop[i]) of each sequence; `per` slots a sequence.  `follow`: the
+// tokens follow others, which are in the cache or were dropped; an entry that begins before start[i] and is no page stays
+// so, because a page given now would show what it held as the tokens before.
 __global__ __launch_bounds__(1024) void kv_reserve_kernel(KvTables t, int n, const int* __restrict__ seqs,
                                                           const int* __restrict__ start, const int* __restrict__ stop,
-                                                          int count, int per, int* missing) {
-    int row = 0, j = 0;  // of the slot at hand
+                                                          int count, int per, bool follow, int* missing) {
+    __shared__ int all_begun;
+    if (threadIdx.x == 0) all_begun = 0;
+    int row = 0, j = 0;   // of the slot at hand
+    bool inside = false;  // its entry begins before start[i]
+    int begun = 0;        // entries that stay without a page for that
     auto entry = [&](int slot) {
         const int i = slot / per;
         row = seqs != nullptr ? seqs[i] : i;
@@ -221,18 +227,28 @@ __global__ __launch_bounds__(1024) void kv_reserve_kernel(KvTables t, int n, con
         if (stop != nullptr) end = min(end, (long long)stop[i]);
         const long long at = (start[i] >> t.page_log2) + (long long)(slot - i * per);
         j = (int)at;
+        inside = at << t.page_log2 < start[i];
         return at << t.page_log2 < end && end > start[i];
     };
     const int short_of = kvm_new_pages(
         t, n * per,
         [&](int slot) {  // (not from the cache of this CU: the entry may have been given a page by an earlier slot)
-            return entry(slot) && !kvm_is_page(t, __hip_atomic_load(&t.table[(size_t)row * t.max_pages + j], __ATOMIC_RELAXED,
-                                                                    __HIP_MEMORY_SCOPE_AGENT));
+            if (!entry(slot) || kvm_is_page(t, __hip_atomic_load(&t.table[(size_t)row * t.max_pages + j], __ATOMIC_RELAXED,
+                                                                 __HIP_MEMORY_SCOPE_AGENT)))
+                return false;
+            if (!follow || !inside) return true;
+            ++begun;
+            return false;
         },
         [&](int, int page) {
             if (page >= 0) kvm_set_lowest(t, row, j, page);
         });
-    if (missing != nullptr && threadIdx.x == 0) *missing = short_of;
+    if (missing == nullptr) return;
+    if (follow) {
+        if (begun != 0) atomicAdd(&all_begun, begun);
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) *missing = short_of + all_begun;
 }
 
 // ---------------------------------------------------------------------------
@@ -464,9 +480,9 @@ int kv_pages_reserve_slots(const KvTables& t, int count) {
     return (int)std::min<long long>(t.max_pages, (((long long)count - 1) >> t.page_log2) + 2);
 }
 hipError_t kv_pages_reserve(const KvTables& t, int n, const int* seqs, const int* start, const int* stop, int count,
-                            int* missing, hipStream_t st) {
+                            bool follow, int* missing, hipStream_t st) {
     hipLaunchKernelGGL(kv_reserve_kernel, dim3(1), dim3(1024), 0, st, t, n, seqs, start, stop, count,
-                       kv_pages_reserve_slots(t, count), missing);
+                       kv_pages_reserve_slots(t, count), follow, missing);
     return hipGetLastError();
 }
 long long kv_pages_fork_scratch_bytes(int n) { return 8LL * n; }

@@ -70,6 +70,7 @@ SIGNATURES = {
     "vte_kv_pages_copy": [_vp, _i, _vp, _vp, _i, _vp],
     "vte_kv_pages_free": [_vp, _i, _vp, _i, _vp, _i, _vp],
     "vte_kv_pages_reserve": [_vp, _i, _vp, _vp, _vp, _i, _vp, _vp],
+    "vte_kv_pages_extend": [_vp, _i, _vp, _vp, _vp, _i, _vp, _vp],
     "vte_kv_pages_fork_scratch_bytes": [_i],
     "vte_kv_pages_fork": [_vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _ll, _vp],
     "vte_kv_pages_compact_scratch_bytes": [_vp],
@@ -415,6 +416,12 @@ class VTEKernels:
         missing[0] = pages that there were not."""
         self._check(self.lib.vte_kv_pages_reserve(ctypes.byref(tables), n, _p(seqs), _p(start), _p(stop), count, _p(missing),
                                                   self._st(stream)), "vte_kv_pages_reserve")
+
+    def kv_pages_extend(self, tables: KVTables, n: int, start, count: int, missing=None, seqs=None, stop=None,
+                        stream=None) -> None:
+        """As ``kv_pages_reserve``, but an entry without a page that begins before start[i] stays so (``missing`` counts it)."""
+        self._check(self.lib.vte_kv_pages_extend(ctypes.byref(tables), n, _p(seqs), _p(start), _p(stop), count, _p(missing),
+                                                 self._st(stream)), "vte_kv_pages_extend")
 
     def kv_pages_fork_scratch_bytes(self, n: int) -> int:
         return int(self.lib.vte_kv_pages_fork_scratch_bytes(n))
