@@ -525,9 +525,10 @@ int vte_kv_pages_free(const vte_kv_tables* tables, int n, const int* seqs, int k
 /* Room: of sequences seqs[i] (NULL: 0 .. n - 1) every entry of tokens start[i] ..
  * start[i] + count - 1 (those below stop[i], where stop is given; start below 0: none)
  * that is no page gets one.  n * (pages of count tokens + 1) <= 2^24.  missing (device
- * int, may be NULL) = how many entries got none because no page was free.  A sequence in
- * the list twice is given pages twice: an entry keeps the lowest, the others are free
- * again after the call.
+ * int, may be NULL) = how many entries got none because no page was free (one that the list
+ * asks for twice counts twice).  A sequence in the list twice is given pages twice: an entry
+ * keeps the lowest, the others are free again after the call, or go to entries that would get
+ * none.
  * A page comes with the bytes that its former user left.  Where one is given to an entry
  * that start[i] lies inside, the tokens before start[i] count as being there from then on:
  * the program has to append them too before anything reads the sequence, or call

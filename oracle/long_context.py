@@ -72,19 +72,21 @@ class Pool:
     def reserve(self, seqs, start, count, stop=None, follow=False):
         """Entries are served in order; users change at the end only (a page given back is none of this call's).  ``follow``:
         an entry that begins before its start gets no page."""
-        missing = 0
+        missing, begun = 0, []
         for i, b in enumerate(seqs):
             if not 0 <= b < len(self.table) or start[i] < 0:
                 continue
             end = min(start[i] + count, self.table.shape[1] * self.page)
             end = end if stop is None else min(end, stop[i])
             for j in range(start[i] // self.page, -(-end // self.page) if end > start[i] else 0):
-                if not self.is_page(self.table[b, j]):
-                    p = -1 if follow and j * self.page < start[i] else self.new_page()
+                if follow and j * self.page < start[i]:
+                    begun.append((b, j))
+                elif not self.is_page(self.table[b, j]):
+                    p = self.new_page()
                     missing += p < 0
                     if p >= 0:
                         self.table[b, j] = p
-        return missing
+        return missing + sum(not self.is_page(self.table[e]) for e in begun)
 
     def fork(self, parents, children, lengths):
         todo = [(p, c, n) for p, c, n in zip(parents, children, lengths)

@@ -115,3 +115,35 @@ def test_a_former_users_tokens_are_never_seen(hip, K, left, chunk):
                 assert matches("f16", got[i], want, tol).all(), (pos, i, win)
         pos += n
     assert given.sum() == 130 - 32
+
+
+# ---------------------------------------------------------------------------- a sequence twice in the list
+@pytest.mark.parametrize("call", ["kv_pages_reserve", "kv_pages_extend"])
+@pytest.mark.parametrize("free", [0, 1, 2, 3, 4, 8, 9, 40])
+def test_a_sequence_twice_takes_no_page_from_others(hip, K, call, free):
+    """With some ten entries to fill, one sequence many times over, those first in the list get the pages there are; the rest is
+    missing, once for each time it is asked for."""
+    rng = np.random.default_rng(free)
+    seqs = [1, 1, 1, 2, 1, 3, 2, 2, 4, 1, 5, 5, 4, 0]
+    start = [0, 5, 16, 0, 0, 20, 0, 16, 7, 16, 0, 0, 0, 33]
+    p = Pools(hip, K, rng, np.full((6, 4), -1), 50, n_layers=1, n_kv=1, more=rng.permutation(50)[:50 - free])
+    want = p.ref.reserve(seqs, start, 17, follow=call == "kv_pages_extend")
+    getattr(K, call)(p.t, len(seqs), p.ints(start), 17, p.missing, seqs=p.ints(seqs), stream=hip.stream)
+    table, refs = down(p.table), down(p.refs)
+    assert np.array_equal(table >= 0, p.ref.table >= 0) and down(p.missing)[0] == want
+    held = table[table >= 0]
+    assert len(np.unique(held)) == len(held) == (p.ref.table >= 0).sum() and refs.sum() == 50 - free + len(held)
+    assert (refs[held] == 1).all() and refs.max() == 1
+
+
+@pytest.mark.parametrize("times,free", [(700, 3), (1500, 2), (3000, 700)])
+def test_many_times_the_same_sequence_before_others(hip, K, times, free):
+    """More repeats than a block has threads, and than there are free pages; the others come last."""
+    rng = np.random.default_rng(times)
+    seqs = [1] * times + [2, 0, 3]
+    p = Pools(hip, K, rng, np.full((4, 2), -1), 900, n_layers=1, n_kv=1, more=rng.permutation(900)[:900 - free])
+    want = p.ref.reserve(seqs, [0] * len(seqs), 32)
+    p.K.kv_pages_reserve(p.t, len(seqs), p.ints([0] * len(seqs)), 32, p.missing, seqs=p.ints(seqs), stream=hip.stream)
+    table, refs = down(p.table), down(p.refs)
+    assert np.array_equal(table >= 0, p.ref.table >= 0) and down(p.missing)[0] == want
+    assert refs.sum() == 900 - free + (table >= 0).sum() and (refs[table[table >= 0]] == 1).all()

@@ -32,10 +32,11 @@ __device__ __forceinline__ void kvm_set(const KvTables& t, int row, int j, int p
     kvm_release(t, atomicExch(&t.table[(size_t)row * t.max_pages + j], p));
 }
 // Entry j of a row, which is no page (above all of them without a sign), becomes p, whose user it already counts as, or
-// keeps the lower page that it was given meanwhile.
-__device__ __forceinline__ void kvm_set_lowest(const KvTables& t, int row, int j, int p) {
+// keeps the lower page that it was given meanwhile.  Whether a page is free again by that.
+__device__ __forceinline__ bool kvm_set_lowest(const KvTables& t, int row, int j, int p) {
     const unsigned old = atomicMin(reinterpret_cast<unsigned*>(&t.table[(size_t)row * t.max_pages + j]), (unsigned)p);
     kvm_release(t, (int)max(old, (unsigned)p));
+    return kvm_is_page(t, (int)max(old, (unsigned)p));
 }
 
 // ---------------------------------------------------------------------------
@@ -107,8 +108,9 @@ __global__ __launch_bounds__(256) void kv_free_kernel(KvTables t, const int* __r
 
 // ---------------------------------------------------------------------------
 // New pages, by one block of 1024 threads, so that they are the lowest free ones in the slots' order without a wait between
-// blocks.  `want(slot)` says whether a slot of 0 .. slots - 1 needs one, `give(slot, page)`, called by the same thread right
-// after, takes it (page -1: there are no more).  The result: slots that got none.
+// blocks.  `want(slot)` says whether a slot of 0 .. slots - 1 needs one (1), is to have none (KVM_LEFT) or has one (0),
+// `give(slot, page)`, called by the same thread right after, takes it (page -1: there are no more).  The result: slots that got
+// none, and those that were to have none (counted in one sum with the others, which holds 1024 of both).
 //
 // Pages are looked at 16384 at a time, the next ones asked for meanwhile, and free ones put into a ring in LDS, 4096 pages'
 // at a time while slots need them.  Bound by latency: a chain of five loads and atomics, 2.8 us of eight sequences, 4.2 of
@@ -118,8 +120,12 @@ __global__ __launch_bounds__(256) void kv_free_kernel(KvTables t, const int* __r
 // ---------------------------------------------------------------------------
 #define KVM_RING 8192
 #define KVM_LOOK 16384
+#define KVM_LEFT (1 << 16)
+struct KvmNone {
+    int missing, left;
+};
 template <class Want, class Give>
-__device__ __forceinline__ int kvm_new_pages(const KvTables& t, int slots, Want want, Give give) {
+__device__ __forceinline__ KvmNone kvm_new_pages(const KvTables& t, int slots, Want want, Give give) {
     __shared__ int ring[KVM_RING];
     __shared__ int sums[16];
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
@@ -166,11 +172,14 @@ __device__ __forceinline__ int kvm_new_pages(const KvTables& t, int slots, Want 
                          (uint32_t)((int)ahead[g].z <= 0) << (4 * g + 2) | (uint32_t)((int)ahead[g].w <= 0) << (4 * g + 3);
     };
     ask(0);  // (while it is not known yet whether a slot needs one)
-    int head = 0, have = 0, next = 0, missing = 0;  // of the ring; the first page not looked at
+    KvmNone none = {0, 0};
+    int head = 0, have = 0, next = 0;  // of the ring; the first page not looked at
     for (int s0 = 0; s0 < slots; s0 += 1024) {
-        const bool w = s0 + tid < slots && want(s0 + tid);
+        const int w = s0 + tid < slots ? want(s0 + tid) : 0;
         int n;
-        const int rank = scan(w, n);
+        const int rank = scan(w, n) & (KVM_LEFT - 1);
+        none.left += n / KVM_LEFT;
+        n &= KVM_LEFT - 1;
         while (have < n && next < t.n_pages) {
             const int group = next / 4096 % (KVM_LOOK / 4096);
             if (group == 0) {
@@ -191,7 +200,7 @@ __device__ __forceinline__ int kvm_new_pages(const KvTables& t, int slots, Want 
             next += 4096;
         }
         __syncthreads();
-        if (w) {
+        if (w == 1) {
             const int page = rank < have ? ring[(head + rank) & (KVM_RING - 1)] : -1;
             if (page >= 0) {
                 atomicExch(&t.refs[page], 1);
@@ -202,10 +211,10 @@ __device__ __forceinline__ int kvm_new_pages(const KvTables& t, int slots, Want 
         const int got = min(n, have);
         head += got;
         have -= got;
-        missing += n - got;
+        none.missing += n - got;
         __syncthreads();
     }
-    return missing;
+    return none;
 }
 
 // Entries of tokens start[i] .. start[i] + count - 1 (below stop[i]) of each sequence; `per` slots a sequence.  `follow`: the
@@ -214,11 +223,8 @@ __device__ __forceinline__ int kvm_new_pages(const KvTables& t, int slots, Want 
 __global__ __launch_bounds__(1024) void kv_reserve_kernel(KvTables t, int n, const int* __restrict__ seqs,
                                                           const int* __restrict__ start, const int* __restrict__ stop,
                                                           int count, int per, bool follow, int* missing) {
-    __shared__ int all_begun;
-    if (threadIdx.x == 0) all_begun = 0;
     int row = 0, j = 0;   // of the slot at hand
     bool inside = false;  // its entry begins before start[i]
-    int begun = 0;        // entries that stay without a page for that
     auto entry = [&](int slot) {
         const int i = slot / per;
         row = seqs != nullptr ? seqs[i] : i;
@@ -230,25 +236,36 @@ __global__ __launch_bounds__(1024) void kv_reserve_kernel(KvTables t, int n, con
         inside = at << t.page_log2 < start[i];
         return at << t.page_log2 < end && end > start[i];
     };
-    const int short_of = kvm_new_pages(
-        t, n * per,
-        [&](int slot) {  // (not from the cache of this CU: the entry may have been given a page by an earlier slot)
-            if (!entry(slot) || kvm_is_page(t, __hip_atomic_load(&t.table[(size_t)row * t.max_pages + j], __ATOMIC_RELAXED,
-                                                                 __HIP_MEMORY_SCOPE_AGENT)))
-                return false;
-            if (!follow || !inside) return true;
-            ++begun;
-            return false;
-        },
-        [&](int, int page) {
-            if (page >= 0) kvm_set_lowest(t, row, j, page);
-        });
-    if (missing == nullptr) return;
-    if (follow) {
-        if (begun != 0) atomicAdd(&all_begun, begun);
-        __syncthreads();
+    auto page_at_entry = [&] {  // (not from the cache of this CU: it may have been given a page by an earlier slot)
+        return kvm_is_page(t, __hip_atomic_load(&t.table[(size_t)row * t.max_pages + j], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+    };
+    bool back = false;  // a page that an entry was given twice is free again
+    auto want = [&](int slot) { return !entry(slot) || page_at_entry() ? 0 : follow && inside ? KVM_LEFT : 1; };
+    auto give = [&](int, int page) {
+        if (page >= 0 && kvm_set_lowest(t, row, j, page)) back = true;
+    };
+    KvmNone none = kvm_new_pages(t, n * per, want, give);
+    if (none.missing + none.left == 0) {
+        if (missing != nullptr && threadIdx.x == 0) *missing = 0;
+        return;
     }
-    if (threadIdx.x == 0) *missing = short_of + all_begun;
+    // Pages that came back go to the entries that got none.  (A search of its own: with the first one inside the loop every
+    // call took 0.6 us more.)
+    while (none.missing != 0) {
+        __threadfence();  // users as they are now: what was counted here is in memory,
+        if (!__syncthreads_or(back)) break;
+        __threadfence();  // and nothing older is left in the cache of this CU
+        back = false;
+        none = kvm_new_pages(t, n * per, want, give);
+    }
+    // Entries as they are now: one that the list asks for twice may have got a page by the other slot.
+    __shared__ int without;
+    if (threadIdx.x == 0) without = 0;
+    __syncthreads();
+    for (int slot = threadIdx.x; slot < n * per; slot += 1024)
+        if (entry(slot) && !page_at_entry()) atomicAdd(&without, 1);
+    __syncthreads();
+    if (missing != nullptr && threadIdx.x == 0) *missing = without;
 }
 
 // ---------------------------------------------------------------------------
@@ -295,15 +312,15 @@ __global__ __launch_bounds__(1024) void kv_fork_last_kernel(KvTables t, KvFork f
     __builtin_amdgcn_s_waitcnt(0);  // (atomics that return nothing, too: the counts are read next)
     __syncthreads();
     int child = 0, j = 0, page = -1;  // of the slot at hand
-    const int short_of = kvm_new_pages(
+    const KvmNone none = kvm_new_pages(
         t, f.n,
         [&](int i) {
             int parent, length;
-            if (!kvm_fork(t, f, i, parent, child, length)) return false;
+            if (!kvm_fork(t, f, i, parent, child, length)) return 0;
             j = length >> t.page_log2;
-            if ((length & ((1 << t.page_log2) - 1)) == 0 || j >= t.max_pages) return false;
+            if ((length & ((1 << t.page_log2) - 1)) == 0 || j >= t.max_pages) return 0;
             page = t.table[(size_t)parent * t.max_pages + j];
-            return kvm_is_page(t, page);
+            return kvm_is_page(t, page) ? 1 : 0;
         },
         [&](int i, int to) {
             if (to < 0) return;
@@ -311,7 +328,7 @@ __global__ __launch_bounds__(1024) void kv_fork_last_kernel(KvTables t, KvFork f
             dst[i] = to;
             kvm_set(t, child, j, to);
         });
-    if (missing != nullptr && threadIdx.x == 0) *missing = short_of;
+    if (missing != nullptr && threadIdx.x == 0) *missing = none.missing;
 }
 
 // ---------------------------------------------------------------------------
