@@ -115,6 +115,39 @@ def test_rows_in_place_strided_and_misaligned(hip, K, dtype, rot, inter):
             check(dtype, y[:, part].reshape(rows, n, hd), *f.of(x[:, part].reshape(rows, n, hd), pos, is_k), f"shift {shift}")
 
 
+@pytest.mark.parametrize("dtype,hd,rot,rows", [("f16", 64, 24, 2 ** 23 + 1), ("f32", 256, 64, 2 ** 20 + 3)])
+def test_rows_of_more_heads_than_a_launch_has_in_one_dimension(hip, K, dtype, hd, rot, rows):
+    """8 GiB of heads in place: 2^26 of a pair a lane, 2^23 of 16-byte runs; the rows at the ends, and around where blocks
+    begin a second time."""
+    rng = np.random.default_rng(rot)
+    n_q = 8
+    f, size = Form(hip, rng, hd, rot), np.dtype(NP[dtype]).itemsize
+    row = n_q * hd * size
+    per = 4 if rot == 24 else 8192 // (hd * size)
+    again = 2 ** 20 * per // n_q  # (the row at which block 2^20 begins)
+    at = sorted({0, 1, rows // 3, again - 1, again, again + 1, min(4 * again, rows - 3), rows - 2, rows - 1})
+    assert at[-1] * n_q > 2 ** 20 * per
+    d = hip.safe_malloc(rows * row, "rows")
+    try:
+        x = normal(rng, (len(at), n_q, hd), dtype, 3.0)
+        pos = np.full(rows, -1, np.int32)
+        pos[at] = rng.integers(0, 1 << 20, len(at))
+        pos[at[2]] = -1
+        for i, r in enumerate(at):
+            hip.safe_memcpy_host_to_device(d.value + r * row, x[i])
+        K.qk_norm_rope(f.c, rows, up(hip, pos), q=d, q_out=d, n_q=n_q, head_dim=hd, dtype=dtype, stream=hip.stream)
+        hip.synchronize()
+        got = np.empty_like(x)
+        for i, r in enumerate(at):
+            hip.safe_memcpy_device_to_host(got[i], d.value + r * row)
+    finally:
+        hip.synchronize()
+        hip.safe_free(d)
+    assert np.array_equal(got[2], x[2])
+    live = np.arange(len(at)) != 2
+    check(dtype, got[live], *f.of(x[live], pos[at][live], False))
+
+
 @pytest.mark.parametrize("rot,inter", [(64, False), (64, True), (40, False)])
 def test_not_finite_values_stay_in_their_pairs(hip, K, rot, inter):
     """Without a norm an Inf or a NaN reaches its partner in a pair that turns, and nothing else; a row of zeros stays zero

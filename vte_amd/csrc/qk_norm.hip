@@ -2,6 +2,7 @@
 // The reference has the two steps apart, for heads that are not normed:
 // vte/compiler/templates/rdna/rope.hip.template:17-137.
 #include "head_turn.h"
+#include "launch.h"
 
 // q and k of one call: rows of heads.
 template <typename T>
@@ -22,11 +23,13 @@ struct QkRows {
 template <typename T, int HD>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(HeadForm f, QkRows<T> q, QkRows<T> k, int rows,
                                                            const int* __restrict__ positions) {
-    constexpr int V = 16 / sizeof(T), NU = HD / (2 * V), HEADS = 256 / NU;
+    constexpr int V = 16 / sizeof(T), NU = HD / (2 * V), HEADS = vte::qk_norm_heads(true, HD, sizeof(T));
+    static_assert(HEADS * NU == 256, "");
     __shared__ __align__(16) float2 turn[HEADS][HD / 2];
     __shared__ int pos_sh[HEADS];
     const int heads = q.heads + k.heads, tid = threadIdx.x, u = tid % NU;
-    const int first = blockIdx.x * HEADS, all = rows * heads;  // (2^27 at most)
+    const int first = (blockIdx.x + gridDim.x * blockIdx.y) * HEADS, all = rows * heads;  // (2^27 at most, and a row of blocks more)
+    if (first >= all) return;
     const bool in = first + tid / NU < all;
     const int item = in ? first + tid / NU : first;
     const int row0 = first / heads, row_n = (min(first + HEADS, all) - 1) / heads - row0 + 1;
@@ -65,9 +68,9 @@ __global__ __launch_bounds__(256) void qk_norm_rope_pairs_kernel(HeadForm f, QkR
                                                                  const int* __restrict__ positions) {
     constexpr int NP = HD / 2, EACH = NP > 64 ? NP / 64 : 1;
     const int heads = q.heads + k.heads, lane = threadIdx.x & 63;
-    const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (item >= (long long)rows * heads) return;
-    const int row = (int)(item / heads), hh = (int)(item - (long long)row * heads);
+    const int item = (blockIdx.x + gridDim.x * blockIdx.y) * 4 + (threadIdx.x >> 6);
+    if (item >= rows * heads) return;  // (2^27 at most, and a row of blocks more)
+    const int row = item / heads, hh = item - row * heads;
     const int pos = positions != nullptr ? positions[row] : 0;
     if (pos < 0) return;
     const bool is_q = hh < q.heads;
@@ -121,13 +124,12 @@ static hipError_t norm_hd(const HeadForm& f, const void* q, void* q_out, int n_q
     };
     const bool wide = fits(q, qs) && fits(q_out, 0) && fits(k, ks) && fits(k_out, 0) && fits(f.q_norm, 0) &&
                       fits(f.k_norm, 0) && (f.freq == nullptr || f.inter || f.rot % (32 / (int)sizeof(T)) == 0);
-    const long long items = (long long)rows * (n_q + n_kv), per = 8192 / (HD * (int)sizeof(T));  // heads of a block
+    const long long items = (long long)rows * (n_q + n_kv), per = qk_norm_heads(wide, HD, sizeof(T));
+    const BlockGrid g = block_grid((items + per - 1) / per);
     if (wide)
-        hipLaunchKernelGGL((qk_norm_rope_kernel<T, HD>), dim3((unsigned)((items + per - 1) / per)), dim3(256), 0, st,
-                           f, Q, K, rows, positions);
+        hipLaunchKernelGGL((qk_norm_rope_kernel<T, HD>), dim3(g.x, g.y), dim3(256), 0, st, f, Q, K, rows, positions);
     else
-        hipLaunchKernelGGL((qk_norm_rope_pairs_kernel<T, HD>), dim3((unsigned)((items + 3) / 4)), dim3(256), 0, st, f, Q, K,
-                           rows, positions);
+        hipLaunchKernelGGL((qk_norm_rope_pairs_kernel<T, HD>), dim3(g.x, g.y), dim3(256), 0, st, f, Q, K, rows, positions);
     return hipGetLastError();
 }
 hipError_t qk_norm_rope(const HeadForm& f, int hd, bool f16, const void* q, void* q_out, int n_q, long long qs, const void* k,
