@@ -147,3 +147,41 @@ def test_many_times_the_same_sequence_before_others(hip, K, times, free):
     table, refs = down(p.table), down(p.refs)
     assert np.array_equal(table >= 0, p.ref.table >= 0) and down(p.missing)[0] == want
     assert refs.sum() == 900 - free + (table >= 0).sum() and (refs[table[table >= 0]] == 1).all()
+
+
+def test_captured_extend_follows_staged_starts(hip, K):
+    """A graph of one extend, replayed a token a time while pages run out, come back and are wanted twice; eager calls and
+    synchronizations between."""
+    rng = np.random.default_rng(31)
+    p = Pools(hip, K, rng, np.full((6, 5), -1), 13, page=16, n_layers=1, n_kv=1)
+    seqs = [4, 0, 1, 2, 0, 3]
+    start, listed = p.ints([0] * 6), p.ints(seqs)
+    at = {b: int(x) for b, x in enumerate(rng.integers(0, 16, 6))}
+    hip.stream_synchronize()
+    hip.stream_begin_capture()
+    K.kv_pages_extend(p.t, 6, start, 9, p.missing, seqs=listed, stream=hip.stream)
+    g = hip.stream_end_capture()
+    ge = hip.graph_instantiate(g)
+    short = 0
+    try:
+        for step in range(24):
+            now = [at[b] for b in seqs]
+            start.upload(np.array(now, np.int32))
+            hip.graph_launch(ge)
+            hip.synchronize()
+            want = p.ref.reserve(seqs, now, 9, follow=True)
+            table, refs = down(p.table), down(p.refs)
+            assert down(p.missing)[0] == want and np.array_equal(table >= 0, p.ref.table >= 0)
+            assert np.array_equal(np.bincount(table[table >= 0], minlength=13), refs)
+            p.ref.table, p.ref.refs = np.array(table), np.array(refs)  # (which pages they are goes by the searches)
+            short += want > 0
+            for b in at:
+                at[b] += 3
+            if step % 6 == 5:
+                gone = int(rng.integers(0, 6))
+                p.free([gone])
+                at[gone] = int(rng.integers(0, 8))
+    finally:
+        hip.graph_exec_destroy(ge)
+        hip.graph_destroy(g)
+    assert 0 < short < 24
