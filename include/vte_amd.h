@@ -451,7 +451,8 @@ long long vte_attn_pages_window_scratch_bytes(const vte_kv_pages* cache, const v
  * of sequence b, at position p = kv_offset[b] + i, sees tokens t <= p with
  * t > p - window or t < sinks (window >= 1, the row's own token among them; sinks
  * >= 0).  Pages of which no row of the call sees a token are not read: their entries
- * may be -1.  Time and scratch go by the window, not by the sequence's length.
+ * may be -1.  Time and scratch go by the window, not by the sequence's length.  Which
+ * form of the kernel runs, and so the last bits of a result, can also go by max_pages.
  * No counterpart in the reference. */
 int vte_attn_pages_window(const vte_kv_pages* cache, const vte_kv_rows* rows, int dtype, const void* q, void* out,
                           int n_q, float scale, int window, int sinks, void* scratch, long long scratch_bytes,
@@ -554,10 +555,10 @@ long long vte_kv_pages_fork_scratch_bytes(int n);
  * again below lengths[i]), the page in which they end is copied to a new one in every
  * layer.  Entries that are no page stay so.  Where no page is free the last entry is -1
  * (the child has none of its tokens: go on with vte_kv_pages_extend); missing (device int,
- * may be NULL) counts those.  A child must be in the list once, and
- * not be a parent in it; a child that is its own parent, or a length below 0, is passed
- * over.  scratch: 16-byte aligned, need not be cleared; calls that may overlap need one
- * each. */
+ * may be NULL) counts those.  A child must be in the list once, and not be a parent in it
+ * (else whose tokens it holds goes by chance); a child that is its own parent, or a length
+ * below 0, is passed over.  scratch: 16-byte aligned, need not be cleared; calls that may
+ * overlap need one each. */
 int vte_kv_pages_fork(const vte_kv_pages* layers, int n_layers, const vte_kv_tables* tables, int n, const int* parents,
                       const int* children, const int* lengths, int* missing, void* scratch, long long scratch_bytes,
                       void* stream);

@@ -121,8 +121,9 @@ __device__ __forceinline__ int pa_tokens(const KvSeq& s, int cap) {
 // that none of the rows at hand sees are left out: those that are walked are numbered through, `head` at the front and from
 // there on those `skip` further.  (WIN false: all of them, and the kernels are those of the attention without windows.)
 // A tile that some see whole costs as before, one at a window's edge two operations a score more.  64 sequences of 1000 to
-// 65000 tokens, window 4096, 28 and 4 heads: 264 MB in 53.5 us, 4.9 TB/s (a copy 5.1); one sequence 12.4 us in two
-// launches, whatever its length; a chunk of 512 tokens after 32256, window 4096, 33 us, 390 TFLOP/s.
+// 65000 tokens, window 4096, 28 and 4 heads: 264 MB in 53.4 (two inputs in turn) to 58.1 us, 4.6 to 4.9 TB/s (a copy 5.1);
+// one sequence 12.3 us in two launches, whatever its length; a chunk of 512 tokens after 32256, window 4096, 33 us, 392
+// TFLOP/s.
 struct PaWindow {
     int window, sinks;
 };

@@ -6,7 +6,9 @@
 // one refs array serve the pools of all layers: only copies touch bytes.  New pages are always the lowest free ones, in
 // the order of the call's list, so what a call does depends on its inputs alone and not on which block came first; users
 // are counted by integer atomics, whose order does not matter.  Entries are exchanged, not written, and what stood there
-// loses a user; new pages of one entry (of a sequence listed twice) are compared, and the lowest stays.
+// loses a user; new pages of one entry (of a sequence listed twice) are compared, and the lowest stays.  (A fork's lists may
+// not have a child twice, or as a parent too: whose pages such a child shows, and whether a begun page is copied before or
+// after it was filled, would go by the threads' order.  Users are counted right all the same.)
 #include <algorithm>
 #include "kv_pages.h"
 
@@ -45,9 +47,9 @@ __device__ __forceinline__ bool kvm_set_lowest(const KvTables& t, int row, int j
 // the exponents along.
 //
 // Stores pass the caches by, whose lines they would fill for nobody; loads too (ONCE) where the pools are larger than the
-// memory-side cache, so that the pages are not in it: 470 MB read and written by a compaction in us, stores / loads past
-// the caches: neither 114.3, stores 114.9, both 103.6; 59 MB of a smaller pool 11.9, 11.5, 13.0, 117 MB of forks (whose
-// pages are in the cache) 30.4, 29.6, 34.4.
+// memory-side cache, so that the pages are not in it.  us of two inputs in turn with neither past the caches, stores, both:
+// 470 MB read and written by a compaction 112.0, 104.4, 101.9 (98.3 of more inputs); one of a smaller pool, a graph, 10.2,
+// 10.0, 11.5; 117 MB of forks, whose pages are in the cache, 30.5, 29.8, 36.6.
 // ---------------------------------------------------------------------------
 template <bool ONCE>
 __device__ __forceinline__ uint4 kvm_load(const uint8_t* p) {
@@ -113,10 +115,10 @@ __global__ __launch_bounds__(256) void kv_free_kernel(KvTables t, const int* __r
 // none, and those that were to have none (counted in one sum with the others, which holds 1024 of both).
 //
 // Pages are looked at 16384 at a time, the next ones asked for meanwhile, and free ones put into a ring in LDS, 4096 pages'
-// at a time while slots need them.  Bound by latency: a chain of five loads and atomics, 2.8 us of eight sequences, 4.2 of
-// 64; a reserve and a free where the last 70 of 4096, 65536 or 2^20 pages are free 6.8, 14 to 17 and 83 us (4096 pages at a
-// time and none ahead: 6.9, 30 and 410).  (refs of pages that were not looked at yet do not change in the call: what it
-// takes or gives back lies before them.)
+// at a time while slots need them.  Bound by latency: a chain of five loads and atomics, 2.9 us where no page is needed (a
+// graph), 3.1 traced of eight sequences, 4.6 of 64; a reserve and a free where the last 70 of 4096, 65536 or 2^20 pages are
+// free 6.8, 14 to 17 and 82 us (4096 pages at a time and none ahead: 6.9, 30 and 410).  (refs of pages that were not looked
+// at yet do not change in a search: what it takes or gives back lies before them.)
 // ---------------------------------------------------------------------------
 #define KVM_RING 8192
 #define KVM_LOOK 16384

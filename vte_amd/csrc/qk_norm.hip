@@ -17,8 +17,8 @@ struct QkRows {
 // sines.
 //
 // A value is read once and written once: bound by bytes where there are many rows, 134 MB of 4096 fp32 rows of 32 heads of
-// 128 in 24 to 28 us, 4.7 to 5.6 TB/s (a large copy reaches 5.1; part of it is in the memory-side cache), by latency where
-// there are few (one row 2.8 us).  With cosines by each thread 39.1, with a thread's dims side by side (half a line a load
+// 128 in 27.7 to 28.7 us, 4.7 to 4.8 TB/s (a large copy reaches 5.1 to 5.2; 24 where two inputs take turns, which the
+// memory-side cache holds in part), by latency where there are few (one row 2.6 to 2.9 us).  With cosines by each thread 39.1, with a thread's dims side by side (half a line a load
 // in fp32) 33.5; stores past the caches, of which such a load's are parts of lines, took 84.
 template <typename T, int HD>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(HeadForm f, QkRows<T> q, QkRows<T> k, int rows,
@@ -62,7 +62,9 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(HeadForm f, QkRows<T>
     ht_st(dst + d1, y);
 }
 
-// Any alignment and rotation: a wave takes a head, a lane one pair of dims (heads of 256: two).
+// Any alignment and rotation: a wave takes a head, a lane one pair of dims (heads of 256: two).  Values are loaded one by
+// one and every head forms its row's angles again, which bound it: 4096 rows of 32 heads of 128, the first 40 dims rotated in
+// halves (fp32: 20), 38.7 us fp16 and 41.6 fp32, against 13.8 and 22.9 of the kernel above with 64 (two inputs in turn).
 template <typename T, int HD>
 __global__ __launch_bounds__(256) void qk_norm_rope_pairs_kernel(HeadForm f, QkRows<T> q, QkRows<T> k, int rows,
                                                                  const int* __restrict__ positions) {
